@@ -245,6 +245,124 @@ int tl_xent_backward_rows(const float *logits, const uint32_t *targets,
                           const float *row_scale, float *dlogits,
                           uint32_t rows, uint32_t vocab, void *stream);
 
+/* ------------------------------------- token scoring and distillation rows */
+/* Operators on rows of next-token logits beside tl_xent_rows.  No
+ * counterpart in the reference, whose cross entropy (src/my_metal/
+ * runtime.cpp:768-841) is its only operator on logits.  Logits are fp32,
+ * fp16 or bf16, row r at logits + r * row_stride (elements; 0 = vocab), of
+ * any alignment of the type's own; all sums, statistics and per-row results
+ * are fp32, and a gradient has the logits' type, rounded once.  A logit of
+ * -inf is a token that cannot occur (probability 0, gradient 0); a row of
+ * nothing else has log probabilities -inf, entropy 0 and a zero gradient.
+ * A NaN or +inf logit makes its row's statistics NaN.  The calls allocate
+ * nothing, need no workspace, keep no state between calls and are
+ * deterministic; calls on different streams may overlap. */
+enum tl_float_type { TL_FLOAT32 = 0, TL_FLOAT16 = 1, TL_BFLOAT16 = 2 };
+/* A row without a given token (padding): log probability 0, no gradient
+ * from it.  Any other id >= vocab is treated alike and sets
+ * TL_FLAG_INDEX_RANGE. */
+#define TL_NO_TOKEN 0xffffffffu
+#define TL_TOKEN_MAX_TOP 128u
+
+/*
+ * With x_j = z_j / temperature and log q_j = x_j - log sum_i e^(x_i):
+ *   logprob[r]     = log q_t, t = targets[r]
+ *   entropy[r]     = -sum_j q_j log q_j
+ *   stats[r]       = { max_j z_j, sum_j e^(x_j - max x) } (0 in the second
+ *                    place for a row of -inf), what the backward needs
+ *   top_ids[r, i], top_logprob[r, i] = the `top` most likely tokens in
+ *                    order, the lower id first among equals, and their
+ *                    log q; NaN logits rank last
+ * Every output is optional (NULL), except that targets and logprob go
+ * together, top > 0 needs both top arrays, and something must be asked for.
+ * top <= min(vocab, TL_TOKEN_MAX_TOP).
+ */
+typedef struct tl_token_logprob_desc {
+  const void *logits;
+  uint64_t row_stride;
+  uint32_t rows, vocab, top;
+  int32_t type;      /* tl_float_type                                     */
+  float temperature; /* > 0, finite                                       */
+  uint32_t reserved;
+  const uint32_t *targets; /* [rows]                                      */
+  float *logprob;          /* [rows]                                      */
+  float *entropy;          /* [rows]; the backward reads it               */
+  float *stats;            /* [rows, 2]; the backward reads it            */
+  float *top_logprob;      /* [rows, top]                                 */
+  uint32_t *top_ids;       /* [rows, top]                                 */
+  /* backward only */
+  const float *d_logprob; /* [rows], optional: the gradient of logprob    */
+  const float *d_entropy; /* [rows], optional: the gradient of entropy    */
+  void *dlogits;          /* row r at dlogits + r * d_row_stride          */
+  uint64_t d_row_stride;  /* elements; 0 = vocab                          */
+} tl_token_logprob_desc;
+int tl_token_logprob_rows(const tl_token_logprob_desc *desc, void *stream);
+/*
+ * dz_j = (d_logprob ([j = t] - q_j) - d_entropy q_j (log q_j + H)) /
+ * temperature from logits, targets, stats and entropy (each of the last
+ * three only where its gradient is given; stats always).  A row whose
+ * gradients are both 0 gets zeros whatever its logits.  dlogits may be
+ * logits itself (with the same stride), otherwise they do not overlap.
+ */
+int tl_token_logprob_backward_rows(const tl_token_logprob_desc *desc, void *stream);
+
+/*
+ * The loss of a student against the top tokens of a teacher, row by row:
+ * slot k of row r is the token teacher_ids[r, k] with the teacher's value
+ * u_k = teacher[r, k] / teacher_temperature.  A slot whose id is
+ * TL_NO_TOKEN or whose value is -inf is empty; the ids of a row's other
+ * slots are distinct.  q is the student's softmax of z / temperature.
+ *   TL_DISTILL_RENORM: p = softmax of u over the slots (any row constant in
+ *     the teacher's values cancels: logits or log probabilities),
+ *     KL = sum_k p_k (log p_k - log q_k)
+ *   TL_DISTILL_TAIL: p_k = e^(u_k): the values are log probabilities (what
+ *     tl_token_logprob_rows gives at this temperature), and the tokens
+ *     outside the slots share the rest, p_r = max(0, 1 - sum_k p_k) against
+ *     q_r = sum of their q: KL gains p_r (log p_r - log q_r) (dropped in a
+ *     row where the student has no token outside the slots)
+ *   loss[r] = kd_weight KL + ce_weight (-log softmax(z)_t), t = targets[r]
+ * A row without slots has no KL term, a row whose target is TL_NO_TOKEN (or
+ * a call without targets) no second term.  1 <= top <= min(vocab,
+ * TL_TOKEN_MAX_TOP); TL_DISTILL_TAIL takes vocab <= TL_DISTILL_MAX_VOCAB
+ * (a bit per token in shared memory).
+ */
+enum tl_distill_tail { TL_DISTILL_RENORM = 0, TL_DISTILL_TAIL = 1 };
+#define TL_DISTILL_STATS 8u
+#define TL_DISTILL_MAX_VOCAB (1u << 20)
+typedef struct tl_distill_desc {
+  const void *logits; /* the student's                                    */
+  uint64_t row_stride;
+  uint32_t rows, vocab, top;
+  int32_t type; /* tl_float_type                                          */
+  float temperature, teacher_temperature; /* > 0, finite                  */
+  float kd_weight, ce_weight;             /* finite                       */
+  int32_t tail;                           /* tl_distill_tail              */
+  uint32_t reserved;
+  const uint32_t *teacher_ids; /* [rows, top]                             */
+  const float *teacher;        /* [rows, top]                             */
+  const uint32_t *targets;     /* [rows], optional                        */
+  float *loss;                 /* [rows]                                  */
+  float *kl;                   /* [rows], optional: the KL term, unweighted */
+  /* [rows, TL_DISTILL_STATS], optional in the forward, read by the
+   * backward: { m = max z, sum e^((z - m) / temperature), sum e^(z - m) (0
+   * without a second term), g, a, h, b, 0 } with the slots' p_k = b e^(u_k
+   * - h) and, outside the slots, dKL/dz_j = a e^((z_j - g) / temperature) /
+   * temperature */
+  float *stats;
+  const float *row_scale; /* [rows], optional: the gradient of loss (1)   */
+  void *dlogits;          /* row r at dlogits + r * d_row_stride          */
+  uint64_t d_row_stride;  /* elements; 0 = vocab                          */
+} tl_distill_desc;
+/* logits, teacher, targets -> loss, kl, stats */
+int tl_distill_rows(const tl_distill_desc *desc, void *stream);
+/* logits, teacher, targets, stats, row_scale -> dlogits = row_scale[r] *
+ * d loss[r] / d z.  A row whose scale is 0 gets zeros whatever its logits.
+ * dlogits may be logits itself (with the same stride). */
+int tl_distill_backward_rows(const tl_distill_desc *desc, void *stream);
+/* Both in one call, for a caller that knows row_scale beforehand (1 /
+ * tokens for a mean loss): the logits are read from memory once. */
+int tl_distill_train_rows(const tl_distill_desc *desc, void *stream);
+
 /* -------------------------------------------------------------- embedding */
 /* out[i,:] = weights[ids[i],:].  Replaces Runtime::embedding_lookup /
  * gather_rows (src/my_metal/runtime.cpp:920-950; math.metal:778-793).

@@ -32,6 +32,12 @@ TL_SIGMOID, TL_SQRT, TL_EXP, TL_GELU, TL_GELU_DERIVATIVE = range(5)
 TL_REDUCE_SUM, TL_REDUCE_MAX = range(2)
 TL_REDUCE_MAX_GROUPS = 4
 TL_GEMM_TF32, TL_GEMM_FP32, TL_GEMM_3XTF32 = range(3)
+TL_FLOAT32, TL_FLOAT16, TL_BFLOAT16 = range(3)
+TL_NO_TOKEN = 0xFFFFFFFF
+TL_TOKEN_MAX_TOP = 128
+TL_DISTILL_RENORM, TL_DISTILL_TAIL = range(2)
+TL_DISTILL_STATS = 8
+TL_DISTILL_MAX_VOCAB = 1 << 20
 
 
 class TlParamSlot(Structure):
@@ -80,6 +86,26 @@ class TlFlashDesc(Structure):
                 ("d_o", TlAttnView), ("dq", TlAttnView), ("dk", TlAttnView), ("dv", TlAttnView),
                 ("divisor", c_void_p), ("mask", c_void_p), ("mask_flag", c_void_p),
                 ("lse", c_void_p), ("delta", c_void_p)]
+
+
+class TlTokenLogprobDesc(Structure):
+    _fields_ = [("logits", c_void_p), ("row_stride", c_uint64), ("rows", c_uint32),
+                ("vocab", c_uint32), ("top", c_uint32), ("type", c_int32),
+                ("temperature", c_float), ("reserved", c_uint32), ("targets", c_void_p),
+                ("logprob", c_void_p), ("entropy", c_void_p), ("stats", c_void_p),
+                ("top_logprob", c_void_p), ("top_ids", c_void_p), ("d_logprob", c_void_p),
+                ("d_entropy", c_void_p), ("dlogits", c_void_p), ("d_row_stride", c_uint64)]
+
+
+class TlDistillDesc(Structure):
+    _fields_ = [("logits", c_void_p), ("row_stride", c_uint64), ("rows", c_uint32),
+                ("vocab", c_uint32), ("top", c_uint32), ("type", c_int32),
+                ("temperature", c_float), ("teacher_temperature", c_float),
+                ("kd_weight", c_float), ("ce_weight", c_float), ("tail", c_int32),
+                ("reserved", c_uint32), ("teacher_ids", c_void_p), ("teacher", c_void_p),
+                ("targets", c_void_p), ("loss", c_void_p), ("kl", c_void_p),
+                ("stats", c_void_p), ("row_scale", c_void_p), ("dlogits", c_void_p),
+                ("d_row_stride", c_uint64)]
 
 
 class TlgConfig(Structure):
@@ -168,6 +194,11 @@ CUDA_ABI = {
     "tl_xent_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_void_p]),
     "tl_xent_backward_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint32,
                                       c_uint32, c_void_p]),
+    "tl_token_logprob_rows": (c_int, [POINTER(TlTokenLogprobDesc), c_void_p]),
+    "tl_token_logprob_backward_rows": (c_int, [POINTER(TlTokenLogprobDesc), c_void_p]),
+    "tl_distill_rows": (c_int, [POINTER(TlDistillDesc), c_void_p]),
+    "tl_distill_backward_rows": (c_int, [POINTER(TlDistillDesc), c_void_p]),
+    "tl_distill_train_rows": (c_int, [POINTER(TlDistillDesc), c_void_p]),
     "tl_embedding_gather": (c_int, [c_void_p, c_uint32, c_uint32, c_void_p, c_uint32,
                                     c_void_p, c_void_p]),
     "tl_embedding_scatter_add": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_void_p,
