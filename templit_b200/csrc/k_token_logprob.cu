@@ -3,6 +3,8 @@
 // (tl_token_logprob_rows, tl_token_logprob_backward_rows).
 #include "token_rows.cuh"
 
+#include <cooperative_groups.h>
+
 namespace tl {
 namespace token {
 
@@ -46,6 +48,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kBatch = 4;          // vectors of a thread in flight
+constexpr uint32_t kSegments = 32; // most segments that have their own maximum
+constexpr uint32_t kList = 1024;   // candidates, and segments that hold some
 
 struct ScoreArgs {
   const void *logits;
@@ -59,66 +65,300 @@ struct ScoreArgs {
   const float *d_logprob, *d_entropy;
   void *dlogits;
   uint64_t d_row_stride;
+  uint32_t segment_shift;  // a segment is 2^shift batches of a thread's vectors
   uint32_t *status;
 };
 
-// log q of a logit from its row's sums; -inf in a row of -inf.
-__device__ __forceinline__ float log_q(float z, const Sums &r, float log_s, float inv_t) {
+// A row's statistics.
+struct RowSums {
+  float m, s;       // largest logit, sum of e^((z - m) / temperature)
+  float log_s, entropy;
+};
+
+// log q of a logit; -inf in a row of -inf.
+__device__ __forceinline__ float log_q(float z, const RowSums &r, float inv_t) {
   if (r.m == -INFINITY) return r.s != r.s ? r.s : -INFINITY;
-  return (z - r.m) * inv_t - log_s;
+  return (z - r.m) * inv_t - r.log_s;
 }
 
-// One CTA per row.
+__device__ __forceinline__ uint64_t key_of(float z, uint32_t id) {
+  return (static_cast<uint64_t>(order_of(z)) << 32) | ~id;
+}
+__device__ __forceinline__ float logit_of(uint64_t key) {
+  const uint32_t o = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+
+struct ScoreShared {
+  Sums scratch[kWarps];
+  Pow2Sums sums[kMaxCluster * kWarps];
+  float largest[kMaxCluster * kWarps];
+  alignas(16) float group[kThreads];  // maxima of the row's 256 groups of threads
+  uint32_t entries, candidates, least, count[kWarps];
+  uint32_t entry[kList];
+  alignas(16) uint64_t candidate[kList];
+};
+
+// The sums of a row by add_logit, for rows that Pow2Sums cannot hold.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) score_kernel(const ScoreArgs a) {
-  __shared__ Sums scratch[kWarps];
-  __shared__ uint64_t best[kWarps];
+__device__ __noinline__ Sums careful_sums(const T *z, uint32_t vocab, float c, Sums *scratch) {
+  Sums v = empty_sums();
+  for (uint32_t j = threadIdx.x; j < vocab; j += kThreads) add_logit(v, to_float(z[j]), c);
+  return block_merge<kWarps>(v, c, scratch);
+}
+
+// The `top` largest (logit, lowest id) of a row whatever the data: bisects
+// the order of the logits for the top-th largest value v (32 counts of the
+// row at most; rows of many equals end at the first), takes the logits
+// above v and the first ids at v.  For rows where a threshold leaves too
+// many candidates (long runs of equal logits, masks that leave fewer tokens
+// than alternatives, NaN).
+template <typename T>
+__device__ __noinline__ void careful_top(const T *z, uint32_t vocab, uint32_t top, uint32_t least,
+                                         ScoreShared &sh) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const auto count_from = [&](uint32_t from) {
+    uint32_t n = 0;
+    for (uint32_t j = threadIdx.x; j < vocab; j += kThreads) n += order_of(to_float(z[j])) >= from;
+    n = __reduce_add_sync(0xffffffffu, n);
+    __syncthreads();
+    if (lane == 0) sh.count[warp] = n;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < kWarps; ++w) n += sh.count[w];
+    return n;
+  };
+  // count_from(lo) >= top > count_from(hi)
+  uint32_t lo = count_from(least) >= top ? least : 0u, hi = 0xffffffffu;
+  if (count_from(lo + 1) < top) hi = lo + 1;
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (count_from(mid) >= top) lo = mid;
+    else hi = mid;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sh.candidates = 0;
+  __syncthreads();
+  for (uint32_t j = threadIdx.x; j < vocab; j += kThreads) {
+    const float x = to_float(z[j]);
+    if (order_of(x) > lo) sh.candidate[atomicAdd(&sh.candidates, 1u)] = key_of(x, j);
+  }
+  __syncthreads();
+  uint32_t have = sh.candidates;
+  for (uint32_t at = 0; have < top; at += kThreads) {
+    const uint32_t j = at + threadIdx.x;
+    const float x = j < vocab ? to_float(z[j]) : 0.0f;
+    const bool equal = j < vocab && order_of(x) == lo;
+    const uint32_t mask = __ballot_sync(0xffffffffu, equal);
+    __syncthreads();
+    if (lane == 0) sh.count[warp] = __popc(mask);
+    __syncthreads();
+    uint32_t before = have + __popc(mask & ((1u << lane) - 1));
+    for (uint32_t w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sh.count[w];
+      have += sh.count[w];
+    }
+    if (equal && before < top) sh.candidate[before] = key_of(x, j);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sh.candidates = top;
+  __syncthreads();
+}
+
+// One CTA per row, or a cluster of CTAs that share a row (CLUSTER).  One
+// pass over the row: every thread keeps its sums in powers of two and the
+// largest logit of each segment of its vectors.  Alternatives: the top-th
+// largest of the maxima of 256 groups of threads is a logit that at least
+// `top` others reach, so the alternatives are among the logits from there
+// on, and only segments whose maximum reaches it are looked at again; their
+// ranks among one another order the few candidates.
+template <typename T, bool ENTROPY, bool TOP, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, 4) score_kernel(const ScoreArgs a) {
+  extern __shared__ float segment[];  // [segments][kThreads] maxima (TOP)
+  __shared__ ScoreShared sh;
+  constexpr uint32_t E = Vec<T>::kElems;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t parts = CLUSTER ? cluster.num_blocks() : 1, part = CLUSTER ? cluster.block_rank() : 0;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const auto everyone = [&] {
+    if (CLUSTER) cluster.sync();
+    else __syncthreads();
+  };
+  if (CLUSTER) cluster.sync();  // every CTA runs before its memory is written to
   pdl_enter();
-  for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (size_t row = blockIdx.x / parts; row < a.rows; row += gridDim.x / parts) {
     const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
-    Sums v = empty_sums();
-    for (uint32_t j = threadIdx.x; j < a.vocab; j += kThreads) add_logit(v, to_float(z[j]), a.c);
-    v = block_merge<kWarps>(v, a.c, scratch);
-    const float log_s = logf(v.s);
-    if (threadIdx.x == 0) {
-      if (a.targets) {
-        const uint32_t t = a.targets[row];
-        float out = 0.0f;
-        if (t < a.vocab) out = log_q(to_float(z[t]), v, log_s, a.inv_t);
-        else if (t != TL_NO_TOKEN) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
-        a.logprob[row] = out;
-      }
-      if (a.entropy) a.entropy[row] = v.s == 0.0f ? 0.0f : log_s - v.h * a.inv_t / v.s;
-      if (a.stats) {
-        a.stats[2 * row] = v.m;
-        a.stats[2 * row + 1] = v.s;
-      }
+    const Part p = part_of(z, a.vocab, part, parts);
+    if (TOP && tid == 0) sh.entries = sh.candidates = 0;
+    uint32_t t = TL_NO_TOKEN;
+    float zt = 0.0f;
+    if (tid == 32 && part == 0 && a.targets) {
+      t = a.targets[row];
+      if (t < a.vocab) zt = to_float(z[t]);
     }
-    // the i-th alternative: the largest (logit, lowest id) below the last
-    uint64_t last = ~0ull;
-    for (uint32_t i = 0; i < a.top; ++i) {
-      uint64_t mine = 0;
-      for (uint32_t j = threadIdx.x; j < a.vocab; j += kThreads) {
-        const uint64_t key = (static_cast<uint64_t>(order_of(to_float(z[j]))) << 32) | ~j;
-        if (key < last && key > mine) mine = key;
-      }
+    const uint4 *vec = reinterpret_cast<const uint4 *>(z + p.head);
+    Pow2Sums v = {-kFar, 0.0f, 0.0f};
+    float largest = -INFINITY, in_segment = -INFINITY;
+    uint32_t batch = 0;
+    for (uint32_t at = p.begin; at < p.end; at += kThreads * kBatch, ++batch) {
+      uint4 r[kBatch];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t other = __shfl_xor_sync(0xffffffffu, mine, o);
-        if (other > mine) mine = other;
+      for (int u = 0; u < kBatch; ++u) {
+        const uint32_t i = at + u * kThreads + tid;
+        r[u] = i < p.end ? vec[i] : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
       }
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = mine;
-      __syncthreads();
-      for (int w = 0; w < kWarps; ++w)
-        if (best[w] > mine) mine = best[w];
-      last = mine;
-      if (threadIdx.x == 0) {
-        const uint32_t id = ~static_cast<uint32_t>(mine);
-        a.top_ids[row * a.top + i] = id;
-        a.top_logprob[row * a.top + i] = log_q(to_float(z[id]), v, log_s, a.inv_t);
+      float most = Vec<T>::largest(r[0]);
+#pragma unroll
+      for (int u = 1; u < kBatch; ++u) most = fmaxf(most, Vec<T>::largest(r[u]));
+      largest = fmaxf(largest, most);
+      if (TOP) {
+        in_segment = batch & ((1u << a.segment_shift) - 1) ? fmaxf(in_segment, most) : most;
+        segment[(batch >> a.segment_shift) * kThreads + tid] = in_segment;
+      }
+      move_to<ENTROPY>(v, fmaxf(v.n, shift_of(most, a.c)));
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        float f[E];
+        Vec<T>::unpack(r[u], f);
+#pragma unroll
+        for (uint32_t e = 0; e < E; ++e) add_term<ENTROPY>(v, f[e], a.c);
       }
     }
+    float loose = -INFINITY;
+    if (tid < p.loose) {
+      loose = to_float(z[loose_at(p, tid)]);
+      largest = fmaxf(largest, loose);
+      move_to<ENTROPY>(v, fmaxf(v.n, shift_of(loose, a.c)));
+      add_term<ENTROPY>(v, loose, a.c);
+    }
+    // join the row's sums in every CTA of it
+    warp_join<ENTROPY>(v);
+    const float warp_largest = warp_max(largest);
+    float group = largest;
+    if (TOP && CLUSTER)
+      for (uint32_t o = 1; o < parts; o <<= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
+    for (uint32_t c = 0; c < parts; ++c) {
+      ScoreShared *to = CLUSTER ? cluster.map_shared_rank(&sh, c) : &sh;
+      if (lane == 0) {
+        to->sums[part * kWarps + warp] = v;
+        to->largest[part * kWarps + warp] = warp_largest;
+      }
+      if (TOP && tid % parts == 0) to->group[(part * kThreads + tid) / parts] = group;
+    }
+    everyone();
+    v = {-kFar, 0.0f, 0.0f};
+    RowSums r;
+    r.m = -INFINITY;
+    for (uint32_t i = lane; i < parts * kWarps; i += 32) {
+      Pow2Sums w = sh.sums[i];
+      const float n = fmaxf(v.n, w.n);
+      move_to<ENTROPY>(v, n);
+      move_to<ENTROPY>(w, n);
+      v.s += w.s;
+      v.h += w.h;
+      r.m = fmaxf(r.m, sh.largest[i]);
+    }
+    warp_join<ENTROPY>(v);
+    r.m = warp_max(r.m);
+    r.s = sum_at(v.s, v.n, r.m, a.c);
+    r.log_s = logf(r.s);
+    if (ENTROPY)
+      r.entropy = v.s == 0.0f ? 0.0f : (log2f(v.s) - v.h / v.s) * 0.6931471805599453f;
+    if (far_out(r.m, a.c)) {
+      const Sums w = careful_sums(z, a.vocab, a.c, sh.scratch);
+      r.s = w.s;
+      r.log_s = logf(r.s);
+      r.entropy = r.log_s - w.h * a.inv_t / w.s;
+    }
+    if (tid == 32 && part == 0) {
+      if (a.targets) {
+        a.logprob[row] = t < a.vocab ? log_q(zt, r, a.inv_t) : 0.0f;
+        if (t >= a.vocab && t != TL_NO_TOKEN) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
+      }
+      if (ENTROPY) a.entropy[row] = r.entropy;
+      if (a.stats) {
+        a.stats[2 * row] = r.m;
+        a.stats[2 * row + 1] = r.s;
+      }
+    }
+    if (TOP) {
+      if (warp == 0) {
+        // bisect for a value that `top` to a few more of the 256 maxima reach
+        uint32_t key[kThreads / 32];
+        uint32_t hi = 0;
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i) {
+          key[i] = order_of(sh.group[i * 32 + lane]);
+          hi = max(hi, key[i]);
+        }
+        uint32_t lo = order_of(-INFINITY);
+        hi = __reduce_max_sync(0xffffffffu, hi) + 1;
+        while (hi - lo > 1) {
+          const uint32_t mid = lo + (hi - lo) / 2;
+          uint32_t n = 0;
+#pragma unroll
+          for (int i = 0; i < kThreads / 32; ++i) n += key[i] >= mid;
+          n = __reduce_add_sync(0xffffffffu, n);
+          if (n >= a.top) lo = mid;
+          else hi = mid;
+          if (n >= a.top && n <= a.top + a.top / 8) break;
+        }
+        if (lane == 0) sh.least = lo;
+      }
+      __syncthreads();
+      const uint32_t least = sh.least;
+      const float from = logit_of(static_cast<uint64_t>(least) << 32);
+      ScoreShared *first = CLUSTER ? cluster.map_shared_rank(&sh, 0) : &sh;
+      const auto candidate = [&](float x, uint32_t id) {
+        const uint32_t i = atomicAdd(&first->candidates, 1u);
+        if (i < kList) first->candidate[i] = key_of(x, id);
+      };
+      if (largest >= from) {
+        const uint32_t segments = (batch + (1u << a.segment_shift) - 1) >> a.segment_shift;
+        for (uint32_t s = 0; s < segments; ++s)
+          if (segment[s * kThreads + tid] >= from) {
+            const uint32_t i = atomicAdd(&sh.entries, 1u);
+            if (i < kList) sh.entry[i] = s * kThreads + tid;
+          }
+        if (tid < p.loose && loose >= from) candidate(loose, loose_at(p, tid));
+      }
+      __syncthreads();
+      const uint32_t entries = sh.entries;
+      if (entries <= kList) {
+        const uint32_t each = kBatch << a.segment_shift;  // vectors of a segment
+        for (uint32_t i = tid; i < entries * each; i += kThreads) {
+          const uint32_t en = sh.entry[i / each];
+          const uint32_t at = p.begin + (en / kThreads * each + i % each) * kThreads + en % kThreads;
+          if (at >= p.end) continue;
+          const uint4 r4 = vec[at];
+          if (!(Vec<T>::largest(r4) >= from)) continue;
+          float f[E];
+          Vec<T>::unpack(r4, f);
+#pragma unroll
+          for (uint32_t e = 0; e < E; ++e)
+            if (f[e] >= from) candidate(f[e], p.head + at * E + e);
+        }
+      } else if (tid == 0) {
+        atomicAdd(&first->candidates, kList + 1);
+      }
+      everyone();
+      if (part == 0) {
+        if (sh.candidates > kList || sh.candidates < a.top)
+          careful_top(z, a.vocab, a.top, least, sh);
+        const uint32_t n = sh.candidates;
+        for (uint32_t i = tid; i < n; i += kThreads) {
+          const uint64_t key = sh.candidate[i];
+          uint32_t rank = 0;
+          for (uint32_t j = 0; j < n; ++j) rank += sh.candidate[j] > key;
+          if (rank < a.top) {
+            a.top_ids[row * a.top + rank] = ~static_cast<uint32_t>(key);
+            a.top_logprob[row * a.top + rank] = log_q(logit_of(key), r, a.inv_t);
+          }
+        }
+      }
+    }
+    everyone();  // shared memory is free for the next row
   }
 }
 
@@ -159,6 +399,37 @@ __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArg
 unsigned grid_of(uint32_t rows) {
   const uint32_t most = kNumSMs * 64u;
   return rows < most ? rows : most;
+}
+
+// CTAs that share a row.
+uint32_t parts_for(uint32_t rows, uint32_t vecs) {
+  uint32_t parts = 1;
+  while (parts < kMaxCluster && rows * parts * 2ull <= 2 * kNumSMs && vecs / parts > 2 * kThreads) parts *= 2;
+  return parts;
+}
+
+template <typename T, bool ENTROPY, bool TOP>
+void launch_score_form(ScoreArgs &a, cudaStream_t s) {
+  const uint32_t vecs = a.vocab / Vec<T>::kElems;
+  const uint32_t parts = parts_for(a.rows, vecs);
+  size_t smem = 0;
+  if (TOP) {
+    const uint32_t batches = ((vecs + parts - 1) / parts + kThreads * kBatch - 1) / (kThreads * kBatch);
+    a.segment_shift = 0;
+    while ((batches + (1u << a.segment_shift) - 1) >> a.segment_shift > kSegments) ++a.segment_shift;
+    smem = ((batches + (1u << a.segment_shift) - 1) >> a.segment_shift) * kThreads * sizeof(float);
+  }
+  const uint32_t most = kNumSMs * 64u;
+  const unsigned teams = a.rows < most ? a.rows : most;
+  if (parts == 1)
+    launch_pdl(score_kernel<T, ENTROPY, TOP, false>, teams, kThreads, smem, s, a);
+  else
+    launch_pdl_cluster(score_kernel<T, ENTROPY, TOP, true>, teams * parts, kThreads, smem, s, parts, a);
+}
+
+template <typename T> void launch_score(ScoreArgs &a, cudaStream_t s) {
+  if (a.entropy) a.top ? launch_score_form<T, true, true>(a, s) : launch_score_form<T, true, false>(a, s);
+  else a.top ? launch_score_form<T, false, true>(a, s) : launch_score_form<T, false, false>(a, s);
 }
 
 int score_args(const char *who, const tl_token_logprob_desc *d, ScoreArgs &a) {
@@ -213,7 +484,7 @@ int tl_token_logprob_rows(const tl_token_logprob_desc *desc, void *stream) {
   if (!a.logprob && !a.entropy && !a.stats && !a.top) return bad(who, "no output");
   a.status = device_status_ptr();
   if (!a.status) return fail(TL_ERR_CUDA, std::string(who) + ": no status word");
-#define L(T) launch_pdl(score_kernel<T>, grid_of(a.rows), kThreads, 0, as_stream(stream), a)
+#define L(T) launch_score<T>(a, as_stream(stream))
   TL_BY_TYPE(desc->type, L)
 #undef L
   return launch_status(who);

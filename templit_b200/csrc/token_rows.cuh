@@ -99,6 +99,176 @@ __device__ __forceinline__ Sums block_merge(Sums v, float c, Sums *scratch) {
   return v;
 }
 
+// ---- rows in 16-byte vectors -------------------------------------------
+// A CTA reads its part of a row (the whole row, or its slice of one that
+// several CTAs share) as aligned 16-byte vectors; the elements before the
+// first and after the last vector (fewer than two vectors' worth) belong to
+// the first part and take one thread each.
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int kElems = 4;
+  static constexpr uint32_t kNone = 0xff800000u;  // -inf
+  static __device__ __forceinline__ void unpack(const uint4 &v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  }
+  // largest element (NaN ignored)
+  static __device__ __forceinline__ float largest(const uint4 &v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                 fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                      __float_as_uint(f[3]));
+  }
+};
+template <> struct Vec<__half> {
+  static constexpr int kElems = 8;
+  static constexpr uint32_t kNone = 0xfc00fc00u;
+  static __device__ __forceinline__ void unpack(const uint4 &v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      f[2 * i] = p.x, f[2 * i + 1] = p.y;
+    }
+  }
+  static __device__ __forceinline__ float largest(const uint4 &v) {
+    const __half2 *p = reinterpret_cast<const __half2 *>(&v);
+    const __half2 a = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(__low2float(a), __high2float(a));
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&p);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int kElems = 8;
+  static constexpr uint32_t kNone = 0xff80ff80u;
+  static __device__ __forceinline__ void unpack(const uint4 &v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ float largest(const uint4 &v) {
+    const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(&v);
+    const __nv_bfloat162 a = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(__low2float(a), __high2float(a));
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&p);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// One CTA's part of a row: vectors [begin, end) of those that start at
+// element `head`, and in the first part the elements outside the vectors.
+struct Part {
+  uint32_t head, begin, end, tail;  // tail: first element after the vectors
+  uint32_t loose;                   // elements outside the vectors (first part)
+};
+
+template <typename T>
+__device__ __forceinline__ Part part_of(const T *row, uint32_t vocab, uint32_t part, uint32_t parts) {
+  constexpr uint32_t E = Vec<T>::kElems;
+  const uint32_t past = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T);
+  const uint32_t head = min(vocab, (E - past) % E);
+  const uint32_t vecs = (vocab - head) / E;
+  const uint32_t each = (vecs + parts - 1) / parts;
+  Part p;
+  p.head = head;
+  p.begin = min(vecs, part * each);
+  p.end = min(vecs, p.begin + each);
+  p.tail = head + vecs * E;
+  p.loose = part == 0 ? head + (vocab - p.tail) : 0;
+  return p;
+}
+
+// Element of loose index i (< part.loose), and whether a part holds element j.
+__device__ __forceinline__ uint32_t loose_at(const Part &p, uint32_t i) {
+  return i < p.head ? i : p.tail + (i - p.head);
+}
+template <typename T> __device__ __forceinline__ bool holds(const Part &p, uint32_t j) {
+  constexpr uint32_t E = Vec<T>::kElems;
+  if (j < p.head || j >= p.tail) return p.loose != 0;
+  const uint32_t v = (j - p.head) / E;
+  return v >= p.begin && v < p.end;
+}
+
+// x or lo, whichever is larger; NaN stays.
+__device__ __forceinline__ float max_nan(float x, float lo) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(lo));
+  return y;
+}
+
+// ---- sums in powers of two ---------------------------------------------
+// The streaming form of the sums: the shift is a whole number n of powers
+// of two, so that z c - n is one rounded operation (no error from a rounded
+// shift, which would scale one thread's terms against another's), and sums
+// with different shifts join by exact factors.  h = sum of e x with x = z c
+// - n.  n never leaves +-kFar; a row whose largest logit does (all logits
+// at the type's lowest value, say) is summed by add_logit instead.
+constexpr float kFar = 1e30f;
+
+struct Pow2Sums {
+  float n, s, h;
+};
+
+__device__ __forceinline__ float shift_of(float max, float c) {
+  return fminf(fmaxf(rintf(max * c), -kFar), kFar);
+}
+
+template <bool ENTROPY>
+__device__ __forceinline__ void move_to(Pow2Sums &a, float n) {
+  const float f = ex2_approx(a.n - n);
+  if (ENTROPY) a.h = f * fmaf(a.n - n, a.s, a.h);
+  a.s *= f;
+  a.n = n;
+}
+
+template <bool ENTROPY>
+__device__ __forceinline__ void add_term(Pow2Sums &a, float z, float c) {
+  float x = fmaf(z, c, -a.n);
+  if (ENTROPY) x = max_nan(x, -1e4f);  // -inf: 0 times a number
+  const float e = ex2_approx(x);
+  a.s += e;
+  if (ENTROPY) a.h = fmaf(e, x, a.h);
+}
+
+// The warp's sums, in every lane.
+template <bool ENTROPY>
+__device__ __forceinline__ void warp_join(Pow2Sums &a) {
+  move_to<ENTROPY>(a, warp_max(a.n));
+  a.s = warp_sum(a.s);
+  if (ENTROPY) a.h = warp_sum(a.h);
+}
+
+// Whether a row of largest logit m is outside what Pow2Sums hold.
+__device__ __forceinline__ bool far_out(float m, float c) {
+  return m != -INFINITY && !(fabsf(m * c) < kFar);
+}
+
+// Sums relative to the largest logit itself.
+__device__ __forceinline__ float sum_at(float s, float n, float m, float c) {
+  return m == -INFINITY ? s : s * ex2_approx(-fmaf(m, c, -n));
+}
+
 inline size_t type_size(int32_t type) { return type == TL_FLOAT32 ? 4 : 2; }
 
 // Checks the fields that both descriptors have; fills in the default
