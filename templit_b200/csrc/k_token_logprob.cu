@@ -44,6 +44,12 @@ int check_gradient(const char *who, const void *logits, uint64_t row_stride, voi
   return TL_OK;
 }
 
+dim3 gradient_grid(uint32_t rows, uint32_t vecs) {
+  uint32_t parts = 1;
+  while (static_cast<uint64_t>(rows) * parts < 4 * kNumSMs && vecs / parts > 4 * 256) ++parts;
+  return dim3(rows < kNumSMs * 64u ? rows : kNumSMs * 64u, parts);
+}
+
 namespace {
 
 constexpr int kThreads = 256;
@@ -362,8 +368,13 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const ScoreArgs a) {
   }
 }
 
-template <typename T>
+// The gradient of part of a row: dz = -e (A + B x) with e = 2^x, x = z c -
+// n, n a whole number at the row's largest logit: q = e k, log q = x ln 2 +
+// const fold into A and B.  The target's element is written again at the
+// end by the part that holds it.
+template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArgs a) {
+  const uint32_t tid = threadIdx.x, parts = gridDim.y, part = blockIdx.y;
   pdl_enter();
   for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
@@ -373,32 +384,44 @@ __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArg
     float gl = 0.0f, ge = 0.0f, entropy = 0.0f;
     if (a.d_logprob) {
       t = a.targets[row];
-      if (t < a.vocab) gl = a.d_logprob[row] * a.inv_t;
-      else if (t != TL_NO_TOKEN && threadIdx.x == 0) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
+      if (t < a.vocab) {
+        gl = a.d_logprob[row] * a.inv_t;
+      } else {
+        if (t != TL_NO_TOKEN && tid == 0) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
+        t = TL_NO_TOKEN;
+      }
     }
-    if (a.d_entropy) {
+    if (ENTROPY) {
       ge = a.d_entropy[row] * a.inv_t;
       if (ge != 0.0f) entropy = a.entropy[row];
     }
+    const Part p = part_of(z, a.vocab, part, parts);
     const bool none = s == 0.0f || (gl == 0.0f && ge == 0.0f);
-    // dz = q (-gl - ge (log q + H)) + gl [j = t]
-    const float inv_s = 1.0f / s, log_s = logf(s), base = entropy - log_s;
-    for (uint32_t j = threadIdx.x; j < a.vocab; j += kThreads) {
-      float g = 0.0f;
-      if (!none) {
-        const float d = to_float(z[j]) - m;
-        const float q = ex2_approx(d * a.c) * inv_s;
-        g = q == 0.0f ? 0.0f : -q * fmaf(ge, fmaf(d, a.inv_t, base), gl);
-        if (j == t) g += gl;
-      }
-      dz[j] = from_float<T>(g);
-    }
+    const float inv_s = 1.0f / s, base = entropy - logf(s);
+    const float n = rintf(m * a.c), off = fmaf(m, a.c, -n);  // x of the largest logit
+    const float k = ex2_approx(-off) * inv_s;                // q = 2^x k
+    const float B = k * ge * 0.6931471805599453f;
+    const float A = k * fmaf(ge, fmaf(-off, 0.6931471805599453f, base), gl);
+    const auto gradient = [&](float x) {
+      float y = fmaf(x, a.c, -n);
+      if (ENTROPY) y = max_nan(y, -1e4f);  // -inf: 0 times a number
+      return -ex2_approx(y) * (ENTROPY ? fmaf(B, y, A) : A);
+    };
+    const auto careful = [&](float x) {
+      const float d = x - m, q = ex2_approx(d * a.c) * inv_s;
+      return q == 0.0f ? 0.0f : -q * fmaf(ge, fmaf(d, a.inv_t, base), gl);
+    };
+    const bool far = far_out(m, a.c);
+    float zt = 0.0f;
+    const bool mine = tid == 0 && t != TL_NO_TOKEN && !none && holds<T>(p, t);
+    if (mine) zt = to_float(z[t]);
+    __syncthreads();  // dz may be z
+    if (none) write_elements<kThreads>(z, dz, p, [](float) { return 0.0f; });
+    else if (far) write_elements<kThreads>(z, dz, p, careful);
+    else write_vectors<kThreads, kBatch>(z, dz, p, gradient);
+    __syncthreads();
+    if (mine) dz[t] = from_float<T>((far ? careful(zt) : gradient(zt)) + gl);
   }
-}
-
-unsigned grid_of(uint32_t rows) {
-  const uint32_t most = kNumSMs * 64u;
-  return rows < most ? rows : most;
 }
 
 // CTAs that share a row.
@@ -430,6 +453,12 @@ void launch_score_form(ScoreArgs &a, cudaStream_t s) {
 template <typename T> void launch_score(ScoreArgs &a, cudaStream_t s) {
   if (a.entropy) a.top ? launch_score_form<T, true, true>(a, s) : launch_score_form<T, true, false>(a, s);
   else a.top ? launch_score_form<T, false, true>(a, s) : launch_score_form<T, false, false>(a, s);
+}
+
+template <typename T> void launch_score_backward(const ScoreArgs &a, cudaStream_t s) {
+  const dim3 grid = gradient_grid(a.rows, a.vocab / Vec<T>::kElems);
+  if (a.d_entropy) launch_pdl(score_backward_kernel<T, true>, grid, kThreads, 0, s, a);
+  else launch_pdl(score_backward_kernel<T, false>, grid, kThreads, 0, s, a);
 }
 
 int score_args(const char *who, const tl_token_logprob_desc *d, ScoreArgs &a) {
@@ -504,7 +533,7 @@ int tl_token_logprob_backward_rows(const tl_token_logprob_desc *desc, void *stre
   if (a.d_entropy && !a.entropy) return bad(who, "d_entropy without entropy");
   a.status = device_status_ptr();
   if (!a.status) return fail(TL_ERR_CUDA, std::string(who) + ": no status word");
-#define L(T) launch_pdl(score_backward_kernel<T>, grid_of(a.rows), kThreads, 0, as_stream(stream), a)
+#define L(T) launch_score_backward<T>(a, as_stream(stream))
   TL_BY_TYPE(desc->type, L)
 #undef L
   return launch_status(who);

@@ -210,6 +210,51 @@ template <typename T> __device__ __forceinline__ bool holds(const Part &p, uint3
   return v >= p.begin && v < p.end;
 }
 
+// dz_j = f(z_j) over a CTA's part, element by element.
+template <int THREADS, typename T, typename F>
+__device__ __forceinline__ void write_elements(const T *z, T *dz, const Part &p, F f) {
+  constexpr uint32_t E = Vec<T>::kElems;
+  for (uint32_t j = p.head + p.begin * E + threadIdx.x; j < p.head + p.end * E; j += THREADS)
+    dz[j] = from_float<T>(f(to_float(z[j])));
+  if (threadIdx.x < p.loose) {
+    const uint32_t j = loose_at(p, threadIdx.x);
+    dz[j] = from_float<T>(f(to_float(z[j])));
+  }
+}
+
+// The same by vectors, BATCH of a thread's in flight, where logits and
+// gradient are aligned alike.  dz may be z: a thread reads what it writes.
+template <int THREADS, int BATCH, typename T, typename F>
+__device__ __forceinline__ void write_vectors(const T *z, T *dz, const Part &p, F f) {
+  constexpr uint32_t E = Vec<T>::kElems;
+  if ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u)
+    return write_elements<THREADS>(z, dz, p, f);
+  const uint4 *vec = reinterpret_cast<const uint4 *>(z + p.head);
+  uint4 *out = reinterpret_cast<uint4 *>(dz + p.head);
+  for (uint32_t at = p.begin; at < p.end; at += THREADS * BATCH) {
+    uint4 r[BATCH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const uint32_t i = at + u * THREADS + threadIdx.x;
+      if (i < p.end) r[u] = vec[i];
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const uint32_t i = at + u * THREADS + threadIdx.x;
+      if (i >= p.end) continue;
+      float x[E];
+      Vec<T>::unpack(r[u], x);
+#pragma unroll
+      for (uint32_t e = 0; e < E; ++e) x[e] = f(x[e]);
+      out[i] = Vec<T>::pack(x);
+    }
+  }
+  if (threadIdx.x < p.loose) {
+    const uint32_t j = loose_at(p, threadIdx.x);
+    dz[j] = from_float<T>(f(to_float(z[j])));
+  }
+}
+
 // x or lo, whichever is larger; NaN stays.
 __device__ __forceinline__ float max_nan(float x, float lo) {
   float y;
@@ -278,6 +323,10 @@ int check_rows(const char *who, const void *logits, int32_t type, uint32_t rows,
 // The same for the gradient of a backward call.
 int check_gradient(const char *who, const void *logits, uint64_t row_stride, void *dlogits,
                    int32_t type, uint32_t rows, uint32_t vocab, uint64_t &d_row_stride);
+
+// Grid of a gradient without a reduction, CTAs of 256: rows x parts, more
+// than one part where the rows alone would leave SMs idle.
+dim3 gradient_grid(uint32_t rows, uint32_t vecs);
 
 }  // namespace token
 }  // namespace tl
