@@ -50,11 +50,17 @@ dim3 gradient_grid(uint32_t rows, uint32_t vecs) {
   return dim3(rows < kNumSMs * 64u ? rows : kNumSMs * 64u, parts);
 }
 
+uint32_t cluster_parts(uint32_t rows, uint32_t vecs) {
+  uint32_t parts = 1;
+  while (parts < kMaxCluster && static_cast<uint64_t>(rows) * parts <= kNumSMs && vecs / parts > 2 * 256)
+    parts *= 2;
+  return parts;
+}
+
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxCluster = 8;
 constexpr int kBatch = 4;          // vectors of a thread in flight
 constexpr uint32_t kSegments = 32; // most segments that have their own maximum
 constexpr uint32_t kList = 1024;   // candidates, and segments that hold some
@@ -171,7 +177,7 @@ __device__ __noinline__ void careful_top(const T *z, uint32_t vocab, uint32_t to
   __syncthreads();
 }
 
-// One CTA per row, or a cluster of CTAs that share a row (CLUSTER).  One
+// One CTA per row, or a cluster of CTAs that share a row.  One
 // pass over the row: every thread keeps its sums in powers of two and the
 // largest logit of each segment of its vectors.  Alternatives: the top-th
 // largest of the maxima of 256 groups of threads is a logit that at least
@@ -424,17 +430,10 @@ __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArg
   }
 }
 
-// CTAs that share a row.
-uint32_t parts_for(uint32_t rows, uint32_t vecs) {
-  uint32_t parts = 1;
-  while (parts < kMaxCluster && rows * parts * 2ull <= 2 * kNumSMs && vecs / parts > 2 * kThreads) parts *= 2;
-  return parts;
-}
-
 template <typename T, bool ENTROPY, bool TOP>
 void launch_score_form(ScoreArgs &a, cudaStream_t s) {
   const uint32_t vecs = a.vocab / Vec<T>::kElems;
-  const uint32_t parts = parts_for(a.rows, vecs);
+  const uint32_t parts = cluster_parts(a.rows, vecs);
   size_t smem = 0;
   if (TOP) {
     const uint32_t batches = ((vecs + parts - 1) / parts + kThreads * kBatch - 1) / (kThreads * kBatch);
@@ -444,10 +443,8 @@ void launch_score_form(ScoreArgs &a, cudaStream_t s) {
   }
   const uint32_t most = kNumSMs * 64u;
   const unsigned teams = a.rows < most ? a.rows : most;
-  if (parts == 1)
-    launch_pdl(score_kernel<T, ENTROPY, TOP, false>, teams, kThreads, smem, s, a);
-  else
-    launch_pdl_cluster(score_kernel<T, ENTROPY, TOP, true>, teams * parts, kThreads, smem, s, parts, a);
+  if (parts == 1) launch_pdl(score_kernel<T, ENTROPY, TOP, false>, teams, kThreads, smem, s, a);
+  else launch_pdl_cluster(score_kernel<T, ENTROPY, TOP, true>, teams * parts, kThreads, smem, s, parts, a);
 }
 
 template <typename T> void launch_score(ScoreArgs &a, cudaStream_t s) {

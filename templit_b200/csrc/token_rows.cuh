@@ -113,6 +113,13 @@ template <> struct Vec<float> {
     f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
     f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
   }
+  // makes the elements whose bit is set in m -inf
+  static __device__ __forceinline__ void drop(uint4 &v, uint32_t m) {
+    if (m & 1) v.x = kNone;
+    if (m & 2) v.y = kNone;
+    if (m & 4) v.z = kNone;
+    if (m & 8) v.w = kNone;
+  }
   // largest element (NaN ignored)
   static __device__ __forceinline__ float largest(const uint4 &v) {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
@@ -133,6 +140,15 @@ template <> struct Vec<__half> {
       const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
       f[2 * i] = p.x, f[2 * i + 1] = p.y;
     }
+  }
+  static __device__ __forceinline__ void drop(uint4 &v, uint32_t m) {
+    v.x = drop_pair(v.x, m), v.y = drop_pair(v.y, m >> 2);
+    v.z = drop_pair(v.z, m >> 4), v.w = drop_pair(v.w, m >> 6);
+  }
+  static __device__ __forceinline__ uint32_t drop_pair(uint32_t w, uint32_t m) {
+    if (m & 1) w = (w & 0xffff0000u) | (kNone & 0xffffu);
+    if (m & 2) w = (w & 0xffffu) | (kNone & 0xffff0000u);
+    return w;
   }
   static __device__ __forceinline__ float largest(const uint4 &v) {
     const __half2 *p = reinterpret_cast<const __half2 *>(&v);
@@ -159,6 +175,15 @@ template <> struct Vec<__nv_bfloat16> {
       f[2 * i] = __uint_as_float(w[i] << 16);
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
+  }
+  static __device__ __forceinline__ void drop(uint4 &v, uint32_t m) {
+    v.x = drop_pair(v.x, m), v.y = drop_pair(v.y, m >> 2);
+    v.z = drop_pair(v.z, m >> 4), v.w = drop_pair(v.w, m >> 6);
+  }
+  static __device__ __forceinline__ uint32_t drop_pair(uint32_t w, uint32_t m) {
+    if (m & 1) w = (w & 0xffff0000u) | (kNone & 0xffffu);
+    if (m & 2) w = (w & 0xffffu) | (kNone & 0xffff0000u);
+    return w;
   }
   static __device__ __forceinline__ float largest(const uint4 &v) {
     const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(&v);
@@ -324,6 +349,10 @@ int check_rows(const char *who, const void *logits, int32_t type, uint32_t rows,
 int check_gradient(const char *who, const void *logits, uint64_t row_stride, void *dlogits,
                    int32_t type, uint32_t rows, uint32_t vocab, uint64_t &d_row_stride);
 
+// CTAs of 256 (a cluster) that share a row: more than one where the rows
+// alone leave SMs idle and each still has two vectors a thread.
+constexpr uint32_t kMaxCluster = 8;
+uint32_t cluster_parts(uint32_t rows, uint32_t vecs);
 // Grid of a gradient without a reduction, CTAs of 256: rows x parts, more
 // than one part where the rows alone would leave SMs idle.
 dim3 gradient_grid(uint32_t rows, uint32_t vecs);
