@@ -1,0 +1,225 @@
+// Distillation rows: what the kernels share (k_distill.cu for a CTA or a
+// cluster per row, k_distill_short.cu for a warp per row).
+//
+// With the student's q = softmax(z / tau) and the teacher's p over the slots
+// (and p_r over the tokens outside, TL_DISTILL_TAIL), the gradient of
+// KL(p || q) is (q_j - p_j) / tau in a slot and, outside the slots, q_j (1 -
+// p_r / q_r) / tau.  The second is evaluated as e^((z_j - g) / tau) a / tau
+// with g the largest logit outside the slots, s_r the sum there and a =
+// (q_r - p_r) / s_r: neither q_r nor q_j / q_r can leave the range of fp32,
+// however small the student's mass outside the slots is.
+#pragma once
+
+#include "token_rows.cuh"
+
+namespace tl {
+namespace token {
+
+constexpr int kPerLane = TL_TOKEN_MAX_TOP / 32;  // slots of a lane where a warp has them all
+
+struct DistillArgs {
+  const void *logits;
+  uint64_t row_stride;
+  uint32_t rows, vocab, top;
+  float c, inv_t;   // log2(e) / temperature, 1 / temperature
+  float u_scale;    // 1 / teacher_temperature
+  float kd, ce;
+  const uint32_t *teacher_ids;
+  const float *teacher;
+  const uint32_t *targets;
+  float *loss, *kl, *stats;
+  const float *row_scale;
+  void *dlogits;
+  uint64_t d_row_stride;
+  uint32_t *status;
+};
+
+// What the gradient of a row needs.
+struct RowStats {
+  float m, s, s1;  // largest logit, sums at the temperature and at 1
+  float g, a;      // outside the slots
+  float h, b;      // the slots' p
+};
+
+// Slot k of a row: its id and value, empty ones as TL_NO_TOKEN.
+__device__ __forceinline__ void read_slot(const DistillArgs &a, size_t row, uint32_t k, uint32_t &id,
+                                          float &u) {
+  id = TL_NO_TOKEN;
+  u = -INFINITY;
+  if (k >= a.top) return;
+  id = a.teacher_ids[row * a.top + k];
+  u = a.teacher[row * a.top + k] * a.u_scale;
+  if (id >= a.vocab) {
+    if (id != TL_NO_TOKEN) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
+    id = TL_NO_TOKEN;
+  }
+  if (u == -INFINITY) id = TL_NO_TOKEN;
+  if (id == TL_NO_TOKEN) u = -INFINITY;
+}
+
+// The coefficients of a row's gradient.
+struct DistillGradient {
+  float k, n, k1, n1;            // dz = k 2^(z c - n) + k1 2^(z log2(e) - n1)
+  float coef, coef1, kd, ce;     // the weights with the row's scale
+  bool none, far;                // no gradient; outside Pow2Sums' range
+};
+
+// Outside the slots dz = kd/tau a e^((z - g) / tau) + ce e^(z - m) / s1, by
+// whole powers of two n: e^((z - g) / tau) = 2^(z c - n) 2^(n - g c).  At a
+// temperature of 1 (not DUAL) both terms are one exponential.
+template <bool DUAL>
+__device__ __forceinline__ DistillGradient distill_gradient(const DistillArgs &a, const RowStats &r,
+                                                            uint32_t t, float scale) {
+  DistillGradient g;
+  g.none = scale == 0.0f || r.s == 0.0f;
+  g.far = far_out(r.m, a.c) || far_out(r.g, a.c) || far_out(r.m, kLog2e);
+  g.kd = a.kd * a.inv_t * scale;
+  g.ce = t == TL_NO_TOKEN ? 0.0f : a.ce * scale;
+  g.coef = g.kd * r.a;
+  g.coef1 = g.ce == 0.0f ? 0.0f : g.ce / r.s1;
+  g.n = shift_of(r.g, a.c);
+  g.n1 = shift_of(r.m, kLog2e);
+  g.k = g.coef * ex2_approx(-fmaf(r.g, a.c, -g.n));
+  g.k1 = g.coef1 == 0.0f ? 0.0f : g.coef1 * ex2_approx(-fmaf(r.m, kLog2e, DUAL ? -g.n1 : -g.n));
+  if (!DUAL) g.k += g.k1;
+  return g;
+}
+
+template <bool DUAL>
+__device__ __forceinline__ float distill_dz(const DistillGradient &g, float c, float z) {
+  const float d = g.k * ex2_approx(fmaf(z, c, -g.n));
+  return DUAL ? fmaf(g.k1, ex2_approx(fmaf(z, kLog2e, -g.n1)), d) : d;
+}
+
+// The same for rows far out.
+__device__ __forceinline__ float careful_distill_dz(const DistillGradient &g, const RowStats &r,
+                                                    float c, float z) {
+  const float d = g.coef * ex2_approx((z - r.g) * c);
+  return g.coef1 == 0.0f ? d : fmaf(g.coef1, ex2_approx((z - r.m) * kLog2e), d);
+}
+
+// In a slot with the teacher's p and the student's logit z.
+__device__ __forceinline__ float slot_dz(const DistillGradient &g, const RowStats &r, float c, float p,
+                                         float z, bool target) {
+  const float d = g.kd * (ex2_approx((z - r.m) * c) / r.s - p);
+  return g.ce == 0.0f ? d : d + fmaf(g.coef1, ex2_approx((z - r.m) * kLog2e), target ? -g.ce : 0.0f);
+}
+
+// What a warp makes of a row's slots and of the sums over the logits
+// outside them (TAIL) or over all of them: lane l holds slots l + 32 i.
+struct SlotLane {
+  bool slot[kPerLane];
+  float u[kPerLane], z[kPerLane];
+};
+
+// Relative to its largest logit m: s = sum of e^((z - m) / tau), s1 = sum of
+// e^(z - m).
+struct Outside {
+  float m, s, s1;
+};
+
+template <bool TAIL>
+__device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotLane &l,
+                                               const Outside &o, bool target, float zt, float &loss,
+                                               float &kl) {
+  RowStats r;
+  uint32_t slots = 0;
+  float u_max = -INFINITY, z_max = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    slots += l.slot[i];
+    if (l.slot[i]) u_max = fmaxf(u_max, l.u[i]), z_max = fmaxf(z_max, l.z[i]);
+  }
+  slots = __reduce_add_sync(0xffffffffu, slots);
+  r.m = o.m, r.s = o.s, r.s1 = o.s1;
+  if (TAIL) {
+    // the whole row: the sums outside the slots and the slots' terms
+    r.m = fmaxf(o.m, warp_max(z_max));
+    float s = 0.0f, s1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i)
+      if (l.slot[i] && l.z[i] != -INFINITY) {
+        s += ex2_approx((l.z[i] - r.m) * a.c);
+        if (target) s1 += ex2_approx((l.z[i] - r.m) * kLog2e);
+      }
+    r.s = o.s * rescale(o.m, r.m, a.c) + warp_sum(s);
+    if (target) r.s1 = o.s1 * rescale(o.m, r.m, kLog2e) + warp_sum(s1);
+  }
+  if (!target) r.s1 = 0.0f;
+  // the teacher's p.  Their sum is taken in 64 bits: what is left of 1 may
+  // be far smaller than the sum
+  r.h = 0.0f, r.b = slots ? 1.0f : 0.0f;
+  float p[kPerLane], log_sum = 0.0f, rest = 0.0f;
+  if (!TAIL) r.h = slots ? warp_max(u_max) : 0.0f;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    p[i] = l.slot[i] ? expf(l.u[i] - r.h) : 0.0f;
+    sum += p[i];
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if (TAIL) {
+    rest = slots ? fmaxf(0.0f, static_cast<float>(1.0 - sum)) : 0.0f;
+  } else if (slots) {
+    r.b = static_cast<float>(1.0 / sum);
+    log_sum = logf(static_cast<float>(sum));
+  }
+  const float log_s = logf(r.s);
+  kl = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    p[i] *= r.b;
+    if (p[i] != p[i]) {
+      kl = p[i];
+    } else if (l.slot[i] && p[i] > 0.0f) {
+      // a row of -inf has q = 0 everywhere
+      const float log_q = r.s == 0.0f ? -INFINITY : (l.z[i] - r.m) * a.inv_t - log_s;
+      kl += p[i] * ((l.u[i] - r.h) - log_sum - log_q);
+    }
+  }
+  kl = warp_sum(kl);
+  if (TAIL) {
+    r.g = o.m == -INFINITY ? 0.0f : o.m;
+    r.a = 0.0f;
+    if (o.m != -INFINITY) {
+      const float log_left = (o.m - r.m) * a.inv_t + logf(o.s) - log_s;  // log q_r
+      if (rest > 0.0f) kl += rest * (logf(rest) - log_left);
+      r.a = slots ? (expf(log_left) - rest) / o.s : 0.0f;
+    }
+  } else {
+    r.g = r.m == -INFINITY ? 0.0f : r.m;
+    r.a = slots && r.s != 0.0f ? 1.0f / r.s : 0.0f;
+  }
+  loss = a.kd == 0.0f ? 0.0f : a.kd * kl;  // a KL of +inf without weight
+  if (target) {
+    const float log_q1 = r.s1 == 0.0f ? -INFINITY : (zt - r.m) - logf(r.s1);
+    loss -= a.ce * log_q1;
+  }
+  return r;
+}
+
+// Bits of the tokens in slots, so placed that a vector's are whole bytes
+// (or half bytes): element j of a row at bit j + elements of a vector -
+// head.
+template <typename T> __device__ __forceinline__ uint32_t vector_marks(const uint32_t *marks, uint32_t v) {
+  const uint8_t *b = reinterpret_cast<const uint8_t *>(marks);
+  if (Vec<T>::kElems == 8) return b[v + 1];
+  return b[(v + 1) / 2] >> (4 * ((v + 1) & 1)) & 15u;
+}
+
+__device__ __forceinline__ void write_stats(float *st, const RowStats &r) {
+  st[0] = r.m, st[1] = r.s, st[2] = r.s1, st[3] = r.g;
+  st[4] = r.a, st[5] = r.h, st[6] = r.b, st[7] = 0.0f;
+}
+
+// Whether the target's term needs exponentials of its own.
+inline bool dual(const DistillArgs &a) { return a.targets && a.ce != 0.0f && a.inv_t != 1.0f; }
+
+// Launch the warp-per-row kernels for rows that suit them (false: not
+// launched).
+bool distill_short(const DistillArgs &a, int32_t type, bool tail, bool gradient, cudaStream_t s);
+bool distill_backward_short(const DistillArgs &a, int32_t type, cudaStream_t s);
+
+}  // namespace token
+}  // namespace tl

@@ -1,15 +1,7 @@
 // Distillation from a teacher's top tokens: loss rows, their gradient, and
 // both in one call (tl_distill_rows, tl_distill_backward_rows,
 // tl_distill_train_rows).
-//
-// With the student's q = softmax(z / tau) and the teacher's p over the slots
-// (and p_r over the tokens outside, TL_DISTILL_TAIL), the gradient of
-// KL(p || q) is (q_j - p_j) / tau in a slot and, outside the slots, q_j (1 -
-// p_r / q_r) / tau.  The second is evaluated as e^((z_j - g) / tau) a / tau
-// with g the largest logit outside the slots, s_r the sum there and a =
-// (q_r - p_r) / s_r: neither q_r nor q_j / q_r can leave the range of fp32,
-// however small the student's mass outside the slots is.
-#include "token_rows.cuh"
+#include "distill_rows.cuh"
 
 #include <cooperative_groups.h>
 
@@ -20,96 +12,33 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;  // vectors of a thread in flight
-constexpr int kPerLane = TL_TOKEN_MAX_TOP / 32;
-
-struct DistillArgs {
-  const void *logits;
-  uint64_t row_stride;
-  uint32_t rows, vocab, top;
-  float c, inv_t;   // log2(e) / temperature, 1 / temperature
-  float u_scale;    // 1 / teacher_temperature
-  float kd, ce;
-  const uint32_t *teacher_ids;
-  const float *teacher;
-  const uint32_t *targets;
-  float *loss, *kl, *stats;
-  const float *row_scale;
-  void *dlogits;
-  uint64_t d_row_stride;
-  uint32_t *status;
-};
-
-// What the gradient of a row needs.
-struct RowStats {
-  float m, s, s1;  // largest logit, sums at the temperature and at 1
-  float g, a;      // outside the slots
-  float h, b;      // the slots' p
-};
-
-// Whether the row's logits are outside what whole powers of two hold.
-__device__ __forceinline__ bool row_far(const RowStats &r, float c) {
-  return far_out(r.m, c) || far_out(r.g, c) || far_out(r.m, kLog2e);
-}
-
 // The gradient of one row's part.  Thread k < top has slot k: id
 // (TL_NO_TOKEN if empty or in another part), its p and its logit, read
-// before anything is written (dlogits may be logits); t is the target (or
-// TL_NO_TOKEN), `target_here` its logit zt in the thread that writes it.
-// Outside the slots dz = kd/tau a e^((z - g) / tau) + ce e^(z - m) / s1; with
-// a temperature of 1 (not DUAL) both are one exponential.  The slots and
-// the target are written a second time.
+// before anything is written (dlogits may be logits); `target_here` has the
+// target's logit zt in the thread that writes it.  The slots and the target
+// are written a second time.
 template <typename T, bool DUAL>
 __device__ __forceinline__ void gradient_part(const DistillArgs &a, size_t row, const Part &part,
                                               const RowStats &r, uint32_t id, float p, float zk,
                                               uint32_t t, bool target_here, float zt) {
   const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
   T *dz = static_cast<T *>(a.dlogits) + row * a.d_row_stride;
-  const float scale = a.row_scale ? a.row_scale[row] : 1.0f;
-  const bool none = scale == 0.0f || r.s == 0.0f;
-  const float kd = a.kd * a.inv_t * scale, ce = t == TL_NO_TOKEN ? 0.0f : a.ce * scale;
-  const float coef = kd * r.a, coef1 = ce == 0.0f ? 0.0f : ce / r.s1;
-  const bool far = row_far(r, a.c);
-  // e^((z - g) / tau) = 2^(z c - n) 2^(n - g c), n whole: see Pow2Sums
-  const float n = shift_of(r.g, a.c), n1 = shift_of(r.m, kLog2e);
-  float k = coef * ex2_approx(-fmaf(r.g, a.c, -n));
-  const float k1 = coef1 == 0.0f ? 0.0f : coef1 * ex2_approx(-fmaf(r.m, kLog2e, DUAL ? -n1 : -n));
-  if (!DUAL) k += k1;
-  const auto fast = [&](float x) {
-    float g = k * ex2_approx(fmaf(x, a.c, -n));
-    if (DUAL) g = fmaf(k1, ex2_approx(fmaf(x, kLog2e, -n1)), g);
-    return g;
-  };
-  const auto careful = [&](float x) {
-    const float g = coef * ex2_approx((x - r.g) * a.c);
-    return coef1 == 0.0f ? g : fmaf(coef1, ex2_approx((x - r.m) * kLog2e), g);
-  };
-  if (none) write_elements<kThreads>(z, dz, part, [](float) { return 0.0f; });
-  else if (far) write_elements<kThreads>(z, dz, part, careful);
+  const DistillGradient g = distill_gradient<DUAL>(a, r, t, a.row_scale ? a.row_scale[row] : 1.0f);
+  const auto fast = [&](float x) { return distill_dz<DUAL>(g, a.c, x); };
+  const auto careful = [&](float x) { return careful_distill_dz(g, r, a.c, x); };
+  if (g.none) write_elements<kThreads>(z, dz, part, [](float) { return 0.0f; });
+  else if (g.far) write_elements<kThreads>(z, dz, part, careful);
   else write_vectors<kThreads, kBatch>(z, dz, part, fast);
   __syncthreads();
-  if (none) return;
-  if (target_here && ce != 0.0f) dz[t] = from_float<T>((far ? careful(zt) : fast(zt)) - ce);
+  if (g.none) return;
+  if (target_here && g.ce != 0.0f) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) - g.ce);
   __syncthreads();  // a target in a slot: the slot's value stands
-  if (id != TL_NO_TOKEN) {
-    float g = kd * (ex2_approx((zk - r.m) * a.c) / r.s - p);
-    if (ce != 0.0f) g += fmaf(coef1, ex2_approx((zk - r.m) * kLog2e), id == t ? -ce : 0.0f);
-    dz[id] = from_float<T>(g);
-  }
+  if (id != TL_NO_TOKEN) dz[id] = from_float<T>(slot_dz(g, r, a.c, p, zk, id == t));
 }
 
-// Slot k of a row in thread k: its id and value, empty ones as TL_NO_TOKEN.
+// Slot k of a row in thread k.
 __device__ __forceinline__ void read_slot(const DistillArgs &a, size_t row, uint32_t &id, float &u) {
-  id = TL_NO_TOKEN;
-  u = -INFINITY;
-  if (threadIdx.x >= a.top) return;
-  id = a.teacher_ids[row * a.top + threadIdx.x];
-  u = a.teacher[row * a.top + threadIdx.x] * a.u_scale;
-  if (id >= a.vocab) {
-    if (id != TL_NO_TOKEN) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
-    id = TL_NO_TOKEN;
-  }
-  if (u == -INFINITY) id = TL_NO_TOKEN;
-  if (id == TL_NO_TOKEN) u = -INFINITY;
+  read_slot(a, row, threadIdx.x, id, u);
 }
 
 __device__ __forceinline__ uint32_t read_target(const DistillArgs &a, size_t row) {
@@ -118,100 +47,6 @@ __device__ __forceinline__ uint32_t read_target(const DistillArgs &a, size_t row
   if (t < a.vocab) return t;
   if (t != TL_NO_TOKEN && threadIdx.x == 0) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
   return TL_NO_TOKEN;
-}
-
-// What a warp makes of a row's slots and of the sums over the logits
-// outside them (TAIL) or over all of them: lane l holds slots l + 32 i.
-struct SlotLane {
-  bool slot[kPerLane];
-  float u[kPerLane], z[kPerLane];
-};
-
-// Relative to its largest logit m: s = sum of e^((z - m) / tau), s1 = sum of
-// e^(z - m).
-struct Outside {
-  float m, s, s1;
-};
-
-template <bool TAIL>
-__device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotLane &l,
-                                               const Outside &o, bool target, float zt, float &loss,
-                                               float &kl) {
-  RowStats r;
-  uint32_t slots = 0;
-  float u_max = -INFINITY, z_max = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    slots += l.slot[i];
-    if (l.slot[i]) u_max = fmaxf(u_max, l.u[i]), z_max = fmaxf(z_max, l.z[i]);
-  }
-  slots = __reduce_add_sync(0xffffffffu, slots);
-  r.m = o.m, r.s = o.s, r.s1 = o.s1;
-  if (TAIL) {
-    // the whole row: the sums outside the slots and the slots' terms
-    r.m = fmaxf(o.m, warp_max(z_max));
-    float s = 0.0f, s1 = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i)
-      if (l.slot[i] && l.z[i] != -INFINITY) {
-        s += ex2_approx((l.z[i] - r.m) * a.c);
-        if (target) s1 += ex2_approx((l.z[i] - r.m) * kLog2e);
-      }
-    r.s = o.s * rescale(o.m, r.m, a.c) + warp_sum(s);
-    if (target) r.s1 = o.s1 * rescale(o.m, r.m, kLog2e) + warp_sum(s1);
-  }
-  if (!target) r.s1 = 0.0f;
-  // the teacher's p.  Their sum is taken in 64 bits: what is left of 1 may
-  // be far smaller than the sum
-  r.h = 0.0f, r.b = slots ? 1.0f : 0.0f;
-  float p[kPerLane], log_sum = 0.0f, rest = 0.0f;
-  if (!TAIL) r.h = slots ? warp_max(u_max) : 0.0f;
-  double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    p[i] = l.slot[i] ? expf(l.u[i] - r.h) : 0.0f;
-    sum += p[i];
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-  if (TAIL) {
-    rest = slots ? fmaxf(0.0f, static_cast<float>(1.0 - sum)) : 0.0f;
-  } else if (slots) {
-    r.b = static_cast<float>(1.0 / sum);
-    log_sum = logf(static_cast<float>(sum));
-  }
-  const float log_s = logf(r.s);
-  kl = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    p[i] *= r.b;
-    if (p[i] != p[i]) {
-      kl = p[i];
-    } else if (l.slot[i] && p[i] > 0.0f) {
-      // a row of -inf has q = 0 everywhere
-      const float log_q = r.s == 0.0f ? -INFINITY : (l.z[i] - r.m) * a.inv_t - log_s;
-      kl += p[i] * ((l.u[i] - r.h) - log_sum - log_q);
-    }
-  }
-  kl = warp_sum(kl);
-  if (TAIL) {
-    r.g = o.m == -INFINITY ? 0.0f : o.m;
-    r.a = 0.0f;
-    if (o.m != -INFINITY) {
-      const float log_left = (o.m - r.m) * a.inv_t + logf(o.s) - log_s;  // log q_r
-      if (rest > 0.0f) kl += rest * (logf(rest) - log_left);
-      r.a = slots ? (expf(log_left) - rest) / o.s : 0.0f;
-    }
-  } else {
-    r.g = r.m == -INFINITY ? 0.0f : r.m;
-    r.a = slots && r.s != 0.0f ? 1.0f / r.s : 0.0f;
-  }
-  loss = a.kd == 0.0f ? 0.0f : a.kd * kl;  // a KL of +inf without weight
-  if (target) {
-    const float log_q1 = r.s1 == 0.0f ? -INFINITY : (zt - r.m) - logf(r.s1);
-    loss -= a.ce * log_q1;
-  }
-  return r;
 }
 
 struct DistillShared {
@@ -224,15 +59,6 @@ struct DistillShared {
   uint32_t t;
   RowStats r;
 };
-
-// Bits of the tokens in slots, so placed that a vector's are whole bytes
-// (or half bytes): element j of a row at bit j + elements of a vector -
-// head.
-template <typename T> __device__ __forceinline__ uint32_t vector_marks(const uint32_t *marks, uint32_t v) {
-  const uint8_t *b = reinterpret_cast<const uint8_t *>(marks);
-  if (Vec<T>::kElems == 8) return b[v + 1];
-  return b[(v + 1) / 2] >> (4 * ((v + 1) & 1)) & 15u;
-}
 
 // The sums outside the slots by add_logit, for rows that Pow2Sums cannot
 // hold.
@@ -384,11 +210,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_kernel(const DistillArgs 
         if (part == 0) {
           a.loss[row] = loss;
           if (a.kl) a.kl[row] = kl;
-          if (a.stats) {
-            float *st = a.stats + row * TL_DISTILL_STATS;
-            st[0] = r.m, st[1] = r.s, st[2] = r.s1, st[3] = r.g;
-            st[4] = r.a, st[5] = r.h, st[6] = r.b, st[7] = 0.0f;
-          }
+          if (a.stats) write_stats(a.stats + row * TL_DISTILL_STATS, r);
         }
       }
     }
@@ -500,9 +322,6 @@ int launch_form(const char *who, const DistillArgs &a, cudaStream_t s) {
   return launch_status(who);
 }
 
-// Whether the target's term needs exponentials of its own.
-bool dual(const DistillArgs &a) { return a.targets && a.ce != 0.0f && a.inv_t != 1.0f; }
-
 template <typename T, bool TAIL, bool GRAD>
 int launch_distill(const char *who, const DistillArgs &a, cudaStream_t s) {
   return dual(a) ? launch_form<T, TAIL, true, GRAD>(who, a, s)
@@ -522,6 +341,7 @@ int distill_forward(const char *who, const tl_distill_desc *d, DistillArgs &a, v
   if (int rc = with_status(who, a)) return rc;
   cudaStream_t s = as_stream(stream);
   const bool tail = d->tail == TL_DISTILL_TAIL;
+  if (distill_short(a, d->type, tail, GRAD, s)) return launch_status(who);
   switch (d->type) {
     case TL_FLOAT32:
       return tail ? launch_distill<float, true, GRAD>(who, a, s)
@@ -574,6 +394,7 @@ int tl_distill_backward_rows(const tl_distill_desc *desc, void *stream) {
   if (!a.stats) return bad(who, "null stats");
   if (int rc = with_status(who, a)) return rc;
   cudaStream_t s = as_stream(stream);
+  if (distill_backward_short(a, desc->type, s)) return launch_status(who);
   switch (desc->type) {
     case TL_FLOAT32: return launch_backward<float>(who, a, s);
     case TL_FLOAT16: return launch_backward<__half>(who, a, s);

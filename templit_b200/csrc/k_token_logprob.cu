@@ -1,7 +1,7 @@
 // Token scoring: log probability of given tokens, entropy and top
 // alternatives of rows of logits, and their gradient
 // (tl_token_logprob_rows, tl_token_logprob_backward_rows).
-#include "token_rows.cuh"
+#include "token_score.cuh"
 
 #include <cooperative_groups.h>
 
@@ -64,42 +64,6 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;          // vectors of a thread in flight
 constexpr uint32_t kSegments = 32; // most segments that have their own maximum
 constexpr uint32_t kList = 1024;   // candidates, and segments that hold some
-
-struct ScoreArgs {
-  const void *logits;
-  uint64_t row_stride;
-  uint32_t rows, vocab, top;
-  float c;      // log2(e) / temperature
-  float inv_t;  // 1 / temperature
-  const uint32_t *targets;
-  float *logprob, *entropy, *stats, *top_logprob;
-  uint32_t *top_ids;
-  const float *d_logprob, *d_entropy;
-  void *dlogits;
-  uint64_t d_row_stride;
-  uint32_t segment_shift;  // a segment is 2^shift batches of a thread's vectors
-  uint32_t *status;
-};
-
-// A row's statistics.
-struct RowSums {
-  float m, s;       // largest logit, sum of e^((z - m) / temperature)
-  float log_s, entropy;
-};
-
-// log q of a logit; -inf in a row of -inf.
-__device__ __forceinline__ float log_q(float z, const RowSums &r, float inv_t) {
-  if (r.m == -INFINITY) return r.s != r.s ? r.s : -INFINITY;
-  return (z - r.m) * inv_t - r.log_s;
-}
-
-__device__ __forceinline__ uint64_t key_of(float z, uint32_t id) {
-  return (static_cast<uint64_t>(order_of(z)) << 32) | ~id;
-}
-__device__ __forceinline__ float logit_of(uint64_t key) {
-  const uint32_t o = static_cast<uint32_t>(key >> 32);
-  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
-}
 
 struct ScoreShared {
   Sums scratch[kWarps];
@@ -374,9 +338,7 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const ScoreArgs a) {
   }
 }
 
-// The gradient of part of a row: dz = -e (A + B x) with e = 2^x, x = z c -
-// n, n a whole number at the row's largest logit: q = e k, log q = x ln 2 +
-// const fold into A and B.  The target's element is written again at the
+// The gradient of part of a row.  The target's element is written again at the
 // end by the part that holds it.
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArgs a) {
@@ -402,31 +364,18 @@ __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArg
       if (ge != 0.0f) entropy = a.entropy[row];
     }
     const Part p = part_of(z, a.vocab, part, parts);
-    const bool none = s == 0.0f || (gl == 0.0f && ge == 0.0f);
-    const float inv_s = 1.0f / s, base = entropy - logf(s);
-    const float n = rintf(m * a.c), off = fmaf(m, a.c, -n);  // x of the largest logit
-    const float k = ex2_approx(-off) * inv_s;                // q = 2^x k
-    const float B = k * ge * 0.6931471805599453f;
-    const float A = k * fmaf(ge, fmaf(-off, 0.6931471805599453f, base), gl);
-    const auto gradient = [&](float x) {
-      float y = fmaf(x, a.c, -n);
-      if (ENTROPY) y = max_nan(y, -1e4f);  // -inf: 0 times a number
-      return -ex2_approx(y) * (ENTROPY ? fmaf(B, y, A) : A);
-    };
-    const auto careful = [&](float x) {
-      const float d = x - m, q = ex2_approx(d * a.c) * inv_s;
-      return q == 0.0f ? 0.0f : -q * fmaf(ge, fmaf(d, a.inv_t, base), gl);
-    };
-    const bool far = far_out(m, a.c);
+    const ScoreGradient g = score_gradient(a, m, s, entropy, gl, ge);
+    const auto fast = [&](float x) { return score_dz<ENTROPY>(g, a.c, x); };
+    const auto careful = [&](float x) { return careful_score_dz(g, a, x); };
     float zt = 0.0f;
-    const bool mine = tid == 0 && t != TL_NO_TOKEN && !none && holds<T>(p, t);
+    const bool mine = tid == 0 && t != TL_NO_TOKEN && !g.none && holds<T>(p, t);
     if (mine) zt = to_float(z[t]);
     __syncthreads();  // dz may be z
-    if (none) write_elements<kThreads>(z, dz, p, [](float) { return 0.0f; });
-    else if (far) write_elements<kThreads>(z, dz, p, careful);
-    else write_vectors<kThreads, kBatch>(z, dz, p, gradient);
+    if (g.none) write_elements<kThreads>(z, dz, p, [](float) { return 0.0f; });
+    else if (g.far) write_elements<kThreads>(z, dz, p, careful);
+    else write_vectors<kThreads, kBatch>(z, dz, p, fast);
     __syncthreads();
-    if (mine) dz[t] = from_float<T>((far ? careful(zt) : gradient(zt)) + gl);
+    if (mine) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) + gl);
   }
 }
 
@@ -489,13 +438,6 @@ int score_args(const char *who, const tl_token_logprob_desc *d, ScoreArgs &a) {
 using namespace tl;
 using namespace tl::token;
 
-#define TL_BY_TYPE(TYPE, LAUNCH)                   \
-  switch (TYPE) {                                  \
-    case TL_FLOAT32: LAUNCH(float); break;         \
-    case TL_FLOAT16: LAUNCH(__half); break;        \
-    default: LAUNCH(__nv_bfloat16); break;         \
-  }
-
 extern "C" {
 
 int tl_token_logprob_rows(const tl_token_logprob_desc *desc, void *stream) {
@@ -510,6 +452,7 @@ int tl_token_logprob_rows(const tl_token_logprob_desc *desc, void *stream) {
   if (!a.logprob && !a.entropy && !a.stats && !a.top) return bad(who, "no output");
   a.status = device_status_ptr();
   if (!a.status) return fail(TL_ERR_CUDA, std::string(who) + ": no status word");
+  if (score_short(a, desc->type, as_stream(stream))) return launch_status(who);
 #define L(T) launch_score<T>(a, as_stream(stream))
   TL_BY_TYPE(desc->type, L)
 #undef L
@@ -530,6 +473,7 @@ int tl_token_logprob_backward_rows(const tl_token_logprob_desc *desc, void *stre
   if (a.d_entropy && !a.entropy) return bad(who, "d_entropy without entropy");
   a.status = device_status_ptr();
   if (!a.status) return fail(TL_ERR_CUDA, std::string(who) + ": no status word");
+  if (score_backward_short(a, desc->type, as_stream(stream))) return launch_status(who);
 #define L(T) launch_score_backward<T>(a, as_stream(stream))
   TL_BY_TYPE(desc->type, L)
 #undef L

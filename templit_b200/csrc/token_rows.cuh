@@ -339,6 +339,56 @@ __device__ __forceinline__ float sum_at(float s, float n, float m, float c) {
   return m == -INFINITY ? s : s * ex2_approx(-fmaf(m, c, -n));
 }
 
+// Fewest rows that take a warp each; fewer leave the SMs to a CTA per row.
+constexpr uint32_t kShortRows = 512;
+
+// ---- short rows: a warp holds a row in registers -------------------------
+// Vectors of a lane: 4 or 16, lane l has vectors l + 32 i.  Rows of up to
+// 8 KB; the caller sees to it that they fit.
+constexpr int kShortWarps = 4;  // warps (rows) of a CTA
+inline uint32_t short_vectors(uint32_t vocab, size_t type_bytes) {
+  const uint64_t vecs = static_cast<uint64_t>(vocab) * type_bytes / 16;
+  return vecs <= 4 * 32 ? 4 : vecs <= 16 * 32 ? 16 : 0;
+}
+inline unsigned short_grid(uint32_t rows) {
+  const uint32_t ctas = (rows + kShortWarps - 1) / kShortWarps, most = kNumSMs * 64u;
+  return ctas < most ? ctas : most;
+}
+
+template <typename T, int NV>
+__device__ __forceinline__ void load_row(const T *z, const Part &p, uint32_t lane, uint4 (&r)[NV]) {
+  const uint4 *vec = reinterpret_cast<const uint4 *>(z + p.head);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t j = i * 32 + lane;
+    r[i] = j < p.end ? vec[j] : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+  }
+}
+
+// dz_j = f(z_j) for the row in registers and the lane's loose element.
+template <typename T, int NV, typename F>
+__device__ __forceinline__ void store_row(T *dz, const Part &p, uint32_t lane, const uint4 (&r)[NV],
+                                          float loose, F f) {
+  constexpr int E = Vec<T>::kElems;
+  const bool aligned = aligned16(dz + p.head);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t j = i * 32 + lane;
+    if (j >= p.end) break;
+    float x[E];
+    Vec<T>::unpack(r[i], x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = f(x[e]);
+    if (aligned) {
+      reinterpret_cast<uint4 *>(dz + p.head)[j] = Vec<T>::pack(x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) dz[p.head + j * E + e] = from_float<T>(x[e]);
+    }
+  }
+  if (lane < p.loose) dz[loose_at(p, lane)] = from_float<T>(f(loose));
+}
+
 inline size_t type_size(int32_t type) { return type == TL_FLOAT32 ? 4 : 2; }
 
 // Checks the fields that both descriptors have; fills in the default
@@ -359,3 +409,10 @@ dim3 gradient_grid(uint32_t rows, uint32_t vecs);
 
 }  // namespace token
 }  // namespace tl
+
+#define TL_BY_TYPE(TYPE, LAUNCH)                   \
+  switch (TYPE) {                                  \
+    case TL_FLOAT32: LAUNCH(float); break;         \
+    case TL_FLOAT16: LAUNCH(__half); break;        \
+    default: LAUNCH(__nv_bfloat16); break;         \
+  }

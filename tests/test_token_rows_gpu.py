@@ -159,6 +159,14 @@ def logits(rng, rows, vocab, sharp=3.0):
 SIZES = [(1, 1), (3, 2), (2, 7), (5, 31), (4, 33), (3, 200), (7, 511), (5, 1023), (6, 2047), (300, 2048), (5, 2049),
          (3, 4096), (4, 4100), (3, 6001), (3, 8192), (4, 8193), (2, 16411), (3, 32768), (3, 50001), (2, 65536),
          (2, 131072), (1, 200003), (1, 2048), (160, 40000)]
+# many rows, some of them short enough for a warp each
+SIZES += [(700, v) for v in (1, 6, 30, 129, 511, 512, 1000, 1026, 2047, 2048, 2050, 4095, 4096, 4099)]
+
+
+def repeat(many, *arrays):
+    """The rows many times over: enough of them to take a warp each."""
+    out = [a if a is None or not many else np.concatenate([a] * (-(-700 // len(a)))) for a in arrays]
+    return out if len(out) > 1 else out[0]
 
 
 @pytest.mark.parametrize("type", list(TYPES))
@@ -172,12 +180,14 @@ def test_scoring_sizes(dev, type, rows, vocab):
 
 
 @pytest.mark.parametrize("type", list(TYPES))
+@pytest.mark.parametrize("rows", [9, 700])
 @pytest.mark.parametrize("vocab,pad,offset", [(2048, 8, 0), (2048, 1, 3), (50001, 0, 1), (50001, 7, 5), (777, 3, 2),
                                               (9001, 0, 1), (40, 2, 1), (131075, 0, 3)])
-def test_scoring_strides_and_alignment(dev, type, vocab, pad, offset):
+def test_scoring_strides_and_alignment(dev, type, vocab, pad, offset, rows):
+    rows = min(rows, 9 if vocab > 4200 else rows)
     rng = np.random.default_rng(vocab + pad)
-    z = Rows(dev, logits(rng, 9, vocab), type, pad, offset)
-    targets = rng.integers(0, vocab, 9)
+    z = Rows(dev, logits(rng, rows, vocab), type, pad, offset)
+    targets = rng.integers(0, vocab, rows)
     check_score(z, score(dev, z, targets, 20, 0.7), targets, 20, 0.7)
     assert z.untouched()
 
@@ -191,8 +201,9 @@ def test_scoring_alternatives(dev, top, vocab):
 
 
 @pytest.mark.parametrize("type", list(TYPES))
-@pytest.mark.parametrize("vocab", [130, 2048, 5000, 70001])
-def test_scoring_ties_and_order(dev, type, vocab):
+@pytest.mark.parametrize("vocab,many", [(130, False), (2048, False), (5000, False), (70001, False),
+                                        (130, True), (512, True), (2047, True), (2048, True)])
+def test_scoring_ties_and_order(dev, type, vocab, many):
     """Equal rows, two values, ascending, descending, all in one place, zeros
     of both signs: the lowest ids first among equals, and more candidates
     than any buffer of a fast path can expect."""
@@ -207,13 +218,16 @@ def test_scoring_ties_and_order(dev, type, vocab):
     z[6] = np.where(rng.integers(0, 2, vocab), 0.0, -0.0)
     z[7, ::64] = 2.0
     z[8] = np.floor(rng.standard_normal(vocab) * 2)
-    z = Rows(dev, z, type)
-    check_score(z, score(dev, z, np.full(9, vocab - 1), 128), np.full(9, vocab - 1), 128, 1.0)
+    z = Rows(dev, repeat(many, z), type)
+    targets = np.full(len(z.host), vocab - 1)
+    for top in (128, 40):
+        check_score(z, score(dev, z, targets, top), targets, top, 1.0)
 
 
 @pytest.mark.parametrize("type", list(TYPES))
-@pytest.mark.parametrize("vocab", [129, 2048, 20001, 100000])
-def test_scoring_masks(dev, type, vocab):
+@pytest.mark.parametrize("vocab,many", [(129, False), (2048, False), (20001, False), (100000, False),
+                                        (129, True), (1030, True), (2048, True)])
+def test_scoring_masks(dev, type, vocab, many):
     """Masked tokens: -inf, the type's lowest value, rows with one token, and
     with none."""
     rng = np.random.default_rng(6)
@@ -228,23 +242,24 @@ def test_scoring_masks(dev, type, vocab):
     z[5, 1:] = low
     z[6, :-1] = -np.inf
     z[7, :vocab // 2] = -np.inf
+    z, targets = repeat(many, z, np.array([0, 1, 2, 3, vocab // 2, 0, vocab - 1, 5]))
     z = Rows(dev, z, type)
-    targets = np.array([0, 1, 2, 3, vocab // 2, 0, vocab - 1, 5])
     top = min(vocab, 64)
     got = score(dev, z, targets, top)
     check_score(z, got, targets, top, 1.0)
     assert got["entropy"][2] == 0 and got["logprob"][2] == -np.inf
 
 
-@pytest.mark.parametrize("vocab", [100, 2048, 30001])
-def test_scoring_nan_and_infinity(dev, vocab):
+@pytest.mark.parametrize("vocab,many", [(100, False), (2048, False), (30001, False), (100, True), (2048, True)])
+def test_scoring_nan_and_infinity(dev, vocab, many):
     rng = np.random.default_rng(7)
     z = logits(rng, 4, vocab)
     z[0, 3] = np.nan
     z[1, 50] = np.inf
     z[2] = np.nan
+    z, targets = repeat(many, z, np.array([0, 1, 2, 3]))
     zr = Rows(dev, z)
-    got = score(dev, zr, np.array([0, 1, 2, 3]), 100)
+    got = score(dev, zr, targets, 100)
     assert np.isnan(got["logprob"][:3]).all() and np.isnan(got["entropy"][:3]).all()
     assert np.isnan(got["top_logprob"][:3]).all()
     np.testing.assert_array_equal(got["top_ids"], ops.top(zr.host, 100))
@@ -267,7 +282,7 @@ def test_scoring_single_outputs(dev):
     """Each output alone equals the one of a full call, bit for bit, and
     again on a second call."""
     rng = np.random.default_rng(9)
-    for type, vocab, rows in (("f32", 2048, 40), ("bf16", 50001, 5), ("f16", 9000, 2)):
+    for type, vocab, rows in (("f32", 2048, 40), ("bf16", 50001, 5), ("f16", 9000, 2), ("f32", 2048, 700)):
         z = Rows(dev, logits(rng, rows, vocab), type)
         targets = rng.integers(0, vocab, rows)
         full = score(dev, z, targets, 17, 1.3)
@@ -342,14 +357,16 @@ def test_scoring_gradient_sizes(dev, type, rows, vocab):
 
 
 @pytest.mark.parametrize("type", list(TYPES))
+@pytest.mark.parametrize("rows", [9, 700])
 @pytest.mark.parametrize("vocab,pads,offsets", [(2048, (8, 16), (0, 0)), (2048, (1, 0), (3, 0)),
                                                 (50001, (0, 0), (1, 1)), (50001, (7, 0), (5, 2)),
                                                 (777, (3, 3), (2, 2)), (9001, (0, 8), (1, 3))])
-def test_scoring_gradient_strides(dev, type, vocab, pads, offsets):
+def test_scoring_gradient_strides(dev, type, vocab, pads, offsets, rows):
+    rows = min(rows, 9 if vocab > 4200 else rows)
     rng = np.random.default_rng(vocab)
-    z = Rows(dev, logits(rng, 9, vocab), type, pads[0], offsets[0])
-    targets = rng.integers(0, vocab, 9)
-    gl, ge = rng.standard_normal(9).astype(np.float32), rng.standard_normal(9).astype(np.float32)
+    z = Rows(dev, logits(rng, rows, vocab), type, pads[0], offsets[0])
+    targets = rng.integers(0, vocab, rows)
+    gl, ge = rng.standard_normal(rows).astype(np.float32), rng.standard_normal(rows).astype(np.float32)
     out = z.like(pads[1], offsets[1])
     got = score_gradient(dev, z, targets, gl, ge, 1.7, out)
     check_score_gradient(z, got, targets, gl, ge, 1.7)
@@ -361,8 +378,8 @@ def test_scoring_gradient_strides(dev, type, vocab, pads, offsets):
 
 
 @pytest.mark.parametrize("type", list(TYPES))
-@pytest.mark.parametrize("vocab", [130, 2048, 20001])
-def test_scoring_gradient_masks(dev, type, vocab):
+@pytest.mark.parametrize("vocab,many", [(130, False), (2048, False), (20001, False), (130, True), (2048, True)])
+def test_scoring_gradient_masks(dev, type, vocab, many):
     rng = np.random.default_rng(11)
     z = logits(rng, 7, vocab)
     z[0, rng.random(vocab) < 0.5] = -np.inf
@@ -370,13 +387,14 @@ def test_scoring_gradient_masks(dev, type, vocab):
     z[2, 1:] = -np.inf
     z[3, :-2] = {"f32": -3.4028234663852886e38, "f16": -65504.0, "bf16": -3.3895313892515355e38}[type]
     z[4, 7] = np.nan
-    z = Rows(dev, z, type)
-    targets = np.array([int(np.argmax(z.host[0])), 3, 0, vocab - 1, 0, NO, 2], np.uint32)
+    targets = np.array([int(np.argmax(z[0])), 3, 0, vocab - 1, 0, NO, 2], np.uint32)
     gl, ge = rng.standard_normal(7).astype(np.float32), rng.standard_normal(7).astype(np.float32)
     gl[4] = ge[4] = 0  # nothing comes in: zeros, in spite of the NaN
+    z, targets, gl, ge = repeat(many, z, targets, gl, ge)
+    z = Rows(dev, z, type)
     got = score_gradient(dev, z, targets, gl, ge)
-    assert not got[4].any()
-    z.host[4] = 0
+    assert not got[4::7].any()
+    z.host[4::7] = 0
     check_score_gradient(z, got, targets, gl, ge, 1.0)
     for one in (dict(gl=gl, ge=None), dict(gl=None, ge=ge)):
         got = score_gradient(dev, z, targets, **one)
@@ -495,12 +513,13 @@ def test_distillation_sizes(dev, type, tail, rows, vocab):
 @pytest.mark.parametrize("tau", [0.5, 1.0, 3.0])
 def test_distillation_forms(dev, type, tail, hard, tau):
     rng = np.random.default_rng(12)
-    for vocab in (2048, 30011):
+    for vocab, many in ((2048, False), (30011, False), (2048, True)):
         zt, ids, teacher = teacher_of(rng, 6, vocab, 32)
-        z = Rows(dev, zt + rng.standard_normal((6, vocab)), type)
         # a target in a slot, outside the slots, and none
         targets = np.array([ids[0, 5], ids[1, 0], vocab - 1, NO, 0, NO], np.uint32)
-        all_three(dev, z, ids, teacher, np.ones(6, np.float32), tail=tail, tau=tau, kd=tau * tau,
+        zt, ids, teacher, targets = repeat(many, zt, ids, teacher, targets)
+        z = Rows(dev, zt + rng.standard_normal(zt.shape), type)
+        all_three(dev, z, ids, teacher, np.ones(len(zt), np.float32), tail=tail, tau=tau, kd=tau * tau,
                   ce=0.25 if hard else 0.0, targets=targets if hard else None)
     # teacher's raw logits and their own temperature
     raw = np.take_along_axis(zt, ids.astype(np.int64), 1)
@@ -513,10 +532,12 @@ def test_distillation_forms(dev, type, tail, hard, tau):
                                                 (777, (3, 3), (2, 2)), (9001, (0, 8), (1, 3)),
                                                 (131075, (0, 0), (3, 3))])
 @pytest.mark.parametrize("tail", [False, True])
-def test_distillation_strides(dev, type, vocab, pads, offsets, tail):
+@pytest.mark.parametrize("rows", [5, 700])
+def test_distillation_strides(dev, type, vocab, pads, offsets, tail, rows):
+    rows = min(rows, 5 if vocab > 4200 else rows)
     rng = np.random.default_rng(vocab)
-    zt, ids, teacher = teacher_of(rng, 5, vocab, 24)
-    targets = rng.integers(0, vocab, 5)
+    zt, ids, teacher = teacher_of(rng, rows, vocab, 24)
+    targets = rng.integers(0, vocab, rows)
     args = dict(tail=tail, targets=targets, kd=2.0, ce=0.5, tau=1.5)
     zh = zt + 0.5 * rng.standard_normal(zt.shape)
     z = Rows(dev, zh, type, pads[0], offsets[0])
@@ -539,8 +560,8 @@ def test_distillation_strides(dev, type, vocab, pads, offsets, tail):
 
 
 @pytest.mark.parametrize("tail", [False, True])
-@pytest.mark.parametrize("vocab", [100, 2048, 40001])
-def test_distillation_slots_and_masks(dev, tail, vocab):
+@pytest.mark.parametrize("vocab,many", [(100, False), (2048, False), (40001, False), (100, True), (2048, True)])
+def test_distillation_slots_and_masks(dev, tail, vocab, many):
     """Empty slots, rows without slots, values of -inf, a student that cannot
     say a slot's token, nothing outside the slots, nothing at all, a student
     whose mass outside the slots is far below fp32's range."""
@@ -558,8 +579,9 @@ def test_distillation_slots_and_masks(dev, tail, vocab):
     z[7, np.setdiff1d(np.arange(vocab), ids[7])] -= 300          # underflows outside the slots
     z[8, ids[8].astype(np.int64)] -= 300                         # and within
     targets = np.array([0, 1, 2, NO, 3, int(ids[5, 0]), 5, int(ids[7, 1]), 6, NO], np.uint32)
+    z, ids, teacher, targets = repeat(many, z, ids, teacher, targets)
     zr = Rows(dev, z)
-    one, two, both = all_three(dev, zr, ids, teacher, rng.uniform(.5, 1.5, rows).astype(np.float32),
+    one, two, both = all_three(dev, zr, ids, teacher, rng.uniform(.5, 1.5, len(z)).astype(np.float32),
                                tail=tail, targets=targets, ce=0.5)
     assert one["kl"][1] == one["kl"][3] == 0 and np.isposinf(one["kl"][[4, 6]]).all()
     assert np.isfinite(both["grad"]).all() and not both["grad"][6].any()
@@ -567,9 +589,10 @@ def test_distillation_slots_and_masks(dev, tail, vocab):
 
 def test_distillation_every_token_in_a_slot(dev):
     rng = np.random.default_rng(14)
-    zt, ids, teacher = teacher_of(rng, 5, 64, 64)
-    for tail in (False, True):
-        all_three(dev, Rows(dev, rng.standard_normal((5, 64))), ids, teacher, None, tail=tail)
+    for rows in (5, 700):
+        zt, ids, teacher = teacher_of(rng, rows, 64, 64)
+        for tail in (False, True):
+            all_three(dev, Rows(dev, rng.standard_normal((rows, 64))), ids, teacher, None, tail=tail)
 
 
 def test_distillation_ids_out_of_range(dev):
@@ -591,11 +614,11 @@ def test_distillation_ids_out_of_range(dev):
 def test_distillation_rows_without_gradient(dev):
     """A scale of 0 gives zeros, whatever the logits."""
     rng = np.random.default_rng(16)
-    for vocab in (300, 2048, 20001):
+    for vocab, many in ((300, False), (2048, False), (20001, False), (2048, True)):
         zt, ids, teacher = teacher_of(rng, 3, vocab, 4)
         zt[1, 5] = np.nan
+        zt, ids, teacher, scale = repeat(many, zt, ids, teacher, np.array([1, 0, 2], np.float32))
         z = Rows(dev, zt)
-        scale = np.array([1, 0, 2], np.float32)
         got = distill(dev, z, ids, teacher, "tl_distill_train_rows", scale=scale, out=z.like())
         assert not got["grad"][1].any() and np.isnan(got["kl"][1])
         two = distill(dev, z, ids, teacher, "tl_distill_backward_rows", scale=scale, out=z.like(),
@@ -606,7 +629,7 @@ def test_distillation_rows_without_gradient(dev):
 
 def test_distillation_repeats_bit_for_bit(dev):
     rng = np.random.default_rng(17)
-    for type, rows, vocab in (("f32", 50, 2048), ("bf16", 3, 50001), ("f16", 2, 131072)):
+    for type, rows, vocab in (("f32", 50, 2048), ("bf16", 3, 50001), ("f16", 2, 131072), ("f32", 700, 2048)):
         zt, ids, teacher = teacher_of(rng, rows, vocab, 32)
         z = Rows(dev, zt, type)
         args = dict(tail=True, targets=rng.integers(0, vocab, rows), ce=0.5, tau=2.0)
