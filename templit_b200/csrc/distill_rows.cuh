@@ -91,6 +91,13 @@ __device__ __forceinline__ float distill_dz(const DistillGradient &g, float c, f
   return DUAL ? fmaf(g.k1, ex2_approx(fmaf(z, kLog2e, -g.n1)), d) : d;
 }
 
+template <bool DUAL>
+__device__ __forceinline__ Pair distill_dz2(const DistillGradient &g, Pair c, Pair z) {
+  const Pair d = mul2(pair(g.k, g.k), ex2_pair(fma2(z, c, pair(-g.n, -g.n))));
+  if (!DUAL) return d;
+  return fma2(pair(g.k1, g.k1), ex2_pair(fma2(z, pair(kLog2e, kLog2e), pair(-g.n1, -g.n1))), d);
+}
+
 // The same for rows far out.
 __device__ __forceinline__ float careful_distill_dz(const DistillGradient &g, const RowStats &r,
                                                     float c, float z) {

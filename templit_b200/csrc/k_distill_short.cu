@@ -5,14 +5,8 @@ namespace tl {
 namespace token {
 namespace {
 
-// Words of a warp's marks: a bit per token, see vector_marks.
-__host__ __device__ constexpr uint32_t mark_words(int nv, int elems) {
-  return (nv * 32 * elems + 4 * elems + 31) / 32;
-}
-
-// A lane's slots l + 32 i: their ids, values and logits.
-template <typename T>
-__device__ __forceinline__ void read_slots(const DistillArgs &a, size_t row, const T *z, uint32_t lane,
+// A lane's slots l + 32 i: their ids and values.
+__device__ __forceinline__ void read_slots(const DistillArgs &a, size_t row, uint32_t lane,
                                            uint32_t (&id)[kPerLane], SlotLane &l) {
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
@@ -21,9 +15,12 @@ __device__ __forceinline__ void read_slots(const DistillArgs &a, size_t row, con
     if (i * 32 < a.top) read_slot(a, row, lane + 32 * i, id[i], l.u[i]);
     l.slot[i] = id[i] != TL_NO_TOKEN;
   }
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i)
-    if (l.slot[i]) l.z[i] = to_float(z[id[i]]);
+}
+
+// A logit of the row whose vectors are in shared memory.
+template <typename T>
+__device__ __forceinline__ float logit_at(const T *z, const Part &p, const uint4 *buffer, uint32_t j) {
+  return to_float(j >= p.head && j < p.tail ? reinterpret_cast<const T *>(buffer)[j - p.head] : z[j]);
 }
 
 __device__ __forceinline__ uint32_t read_target(const DistillArgs &a, size_t row, uint32_t lane) {
@@ -34,20 +31,21 @@ __device__ __forceinline__ uint32_t read_target(const DistillArgs &a, size_t row
   return TL_NO_TOKEN;
 }
 
-// The gradient of the row in registers; slots and target, read before, are
-// written a second time.
+// The gradient of the row in shared memory; slots and target, read before,
+// are written a second time.
 template <typename T, int NV, bool DUAL>
 __device__ __forceinline__ void gradient_row(const DistillArgs &a, size_t row, const T *z, const Part &p,
-                                             uint32_t lane, const uint4 (&q)[NV], float loose,
+                                             uint32_t lane, const uint4 *buffer, float loose,
                                              const RowStats &r, const uint32_t (&id)[kPerLane],
                                              const SlotLane &l, uint32_t t, float zt, float scale) {
   T *dz = static_cast<T *>(a.dlogits) + row * a.d_row_stride;
   const DistillGradient g = distill_gradient<DUAL>(a, r, t, scale);
+  const Pair c2 = pair(a.c, a.c);
   const auto fast = [&](float x) { return distill_dz<DUAL>(g, a.c, x); };
+  const auto fast2 = [&](Pair x) { return distill_dz2<DUAL>(g, c2, x); };
   const auto careful = [&](float x) { return careful_distill_dz(g, r, a.c, x); };
-  __syncwarp();  // the slots' logits are read: dz may be z
   if (!g.none && !g.far) {
-    store_row<T, NV>(dz, p, lane, q, loose, fast);
+    write_row<T, NV>(dz, p, lane, buffer, loose, fast2, fast);
   } else {
     for (uint32_t j = lane; j < a.vocab; j += 32)
       dz[j] = from_float<T>(g.none ? 0.0f : careful(to_float(z[j])));
@@ -64,62 +62,62 @@ __device__ __forceinline__ void gradient_row(const DistillArgs &a, size_t row, c
     }
 }
 
-// As distill_kernel in k_distill.cu, with the row read once: the gradient
-// is made from the registers.
+// As distill_kernel in k_distill.cu, with the row read once.  The slots'
+// logits are taken out of the row in shared memory (TAIL): no marks.
 template <typename T, int NV, bool TAIL, bool DUAL, bool GRAD>
 __global__ void __launch_bounds__(kShortWarps * 32) distill_short_kernel(const DistillArgs a) {
+  extern __shared__ uint4 shared[];
   constexpr int E = Vec<T>::kElems;
-  constexpr uint32_t kWords = mark_words(NV, E);
-  __shared__ uint32_t all_marks[TAIL ? kShortWarps : 1][kWords];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t *marks = all_marks[TAIL ? warp : 0];
-  if (TAIL) {
-    for (uint32_t w = lane; w < kWords; w += 32) marks[w] = 0;
-    __syncwarp();
-  }
+  uint4 *buffer = shared + warp * NV * 32;
+  const size_t stride = static_cast<size_t>(gridDim.x) * kShortWarps;
   pdl_enter();
-  for (size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp; row < a.rows;
-       row += static_cast<size_t>(gridDim.x) * kShortWarps) {
+  for (size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp; row < a.rows; row += stride) {
     const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
     const Part p = part_of(z, a.vocab, 0, 1);
-    const uint32_t first = E - p.head;
-    uint4 q[NV];
-    load_row<T, NV>(z, p, lane, q);
+    stage_row<T, NV>(z, p, lane, buffer);
     float loose = lane < p.loose ? to_float(z[loose_at(p, lane)]) : -INFINITY;
     uint32_t id[kPerLane];
     SlotLane l;
-    read_slots(a, row, z, lane, id, l);
+    read_slots(a, row, lane, id, l);
     const uint32_t t = read_target(a, row, lane);
     const bool target = t != TL_NO_TOKEN && a.ce != 0.0f;
-    const float zt = target ? to_float(z[t]) : 0.0f;
     const float scale = GRAD && a.row_scale ? a.row_scale[row] : 1.0f;
+    await_row();
+    const float zt = target ? logit_at(z, p, buffer, t) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i)
+      if (l.slot[i]) l.z[i] = logit_at(z, p, buffer, id[i]);
     if (TAIL) {
+      __syncwarp();  // all of them are read
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i)
-        if (l.slot[i]) atomicOr(&marks[(id[i] + first) / 32], 1u << ((id[i] + first) % 32));
-      __syncwarp();
+        if (l.slot[i] && id[i] >= p.head && id[i] < p.tail)
+          reinterpret_cast<T *>(buffer)[id[i] - p.head] = from_float<T>(-INFINITY);
+      if (p.loose) {
+        uint32_t taken = 0;  // a bit per loose logit
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (i * 32 >= p.end) break;
-        const uint32_t m = vector_marks<T>(marks, i * 32 + lane);
-        if (m) Vec<T>::drop(q[i], m);
+        for (int i = 0; i < kPerLane; ++i)
+          if (l.slot[i] && (id[i] < p.head || id[i] >= p.tail))
+            taken |= 1u << (id[i] < p.head ? id[i] : p.head + (id[i] - p.tail));
+        if (__reduce_or_sync(0xffffffffu, taken) >> lane & 1u) loose = -INFINITY;
       }
-      if (lane < p.loose) {
-        const uint32_t j = loose_at(p, lane) + first;
-        if (marks[j / 32] >> (j % 32) & 1u) loose = -INFINITY;
-      }
+      __syncwarp();
     }
     float m = loose;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) m = fmaxf(m, Vec<T>::largest(q[i]));
+#pragma unroll 4
+    for (int i = 0; i < NV; ++i)
+      if (i * 32 + lane < p.end) m = fmaxf(m, Vec<T>::largest(buffer[i * 32 + lane]));
     m = warp_max(m);
     Outside o = {m, 0.0f, 0.0f};
     if (far_out(m, a.c) || far_out(m, kLog2e)) {
       Sums v = empty_sums(), v1 = empty_sums();
-      for (uint32_t j = lane; j < a.vocab; j += 32) {
-        if (TAIL && marks[(j + first) / 32] >> ((j + first) % 32) & 1u) continue;
-        add_logit(v, to_float(z[j]), a.c);
-        add_logit(v1, to_float(z[j]), kLog2e);
+      add_logit(v, loose, a.c);
+      add_logit(v1, loose, kLog2e);
+      for (uint32_t j = lane; j < p.end * E; j += 32) {
+        const float x = to_float(reinterpret_cast<const T *>(buffer)[j]);
+        add_logit(v, x, a.c);
+        add_logit(v1, x, kLog2e);
       }
       o.s = warp_merge(v, a.c).s;
       o.s1 = warp_merge(v1, kLog2e).s;
@@ -127,19 +125,23 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_short_kernel(const D
       Pow2Sums v = {shift_of(m, a.c), 0.0f, 0.0f}, v1 = {shift_of(m, kLog2e), 0.0f, 0.0f};
       add_term<false>(v, loose, a.c);
       if (DUAL) add_term<false>(v1, loose, kLog2e);
-#pragma unroll
+      const Pair c2 = pair(a.c, a.c), n2 = pair(-v.n, -v.n);
+      const Pair c21 = pair(kLog2e, kLog2e), n21 = pair(-v1.n, -v1.n);
+      Pair s = pair(v.s, 0.0f), s1 = pair(v1.s, 0.0f);
+#pragma unroll 4
       for (int i = 0; i < NV; ++i) {
-        if (i * 32 >= p.end) break;
-        float f[E];
-        Vec<T>::unpack(q[i], f);
+        if (i * 32 + lane >= p.end) break;
+        Pair f[E / 2];
+        Vec<T>::pairs(buffer[i * 32 + lane], f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          add_term<false>(v, f[e], a.c);
-          if (DUAL) add_term<false>(v1, f[e], kLog2e);
+        for (int e = 0; e < E / 2; ++e) {
+          s = add2(s, ex2_pair(fma2(f[e], c2, n2)));
+          if (DUAL) s1 = add2(s1, ex2_pair(fma2(f[e], c21, n21)));
         }
       }
-      o.s = sum_at(warp_sum(v.s), v.n, m, a.c);
-      o.s1 = DUAL ? sum_at(warp_sum(v1.s), v1.n, m, kLog2e) : o.s;
+      const float2 y = halves(s), y1 = halves(s1);
+      o.s = sum_at(warp_sum(y.x + y.y), v.n, m, a.c);
+      o.s1 = DUAL ? sum_at(warp_sum(y1.x + y1.y), v1.n, m, kLog2e) : o.s;
     }
     float loss, kl;
     const RowStats r = join_slots<TAIL>(a, l, o, target, zt, loss, kl);
@@ -148,44 +150,49 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_short_kernel(const D
       if (a.kl) a.kl[row] = kl;
       if (a.stats) write_stats(a.stats + row * TL_DISTILL_STATS, r);
     }
-    if (TAIL) {
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i)
-        if (l.slot[i]) marks[(id[i] + first) / 32] = 0;
-      __syncwarp();
-    }
-    if (GRAD) gradient_row<T, NV, DUAL>(a, row, z, p, lane, q, loose, r, id, l, t, zt, scale);
+    if (GRAD) gradient_row<T, NV, DUAL>(a, row, z, p, lane, buffer, loose, r, id, l, t, zt, scale);
+    __syncwarp();  // the buffer is free
   }
 }
 
 template <typename T, int NV, bool DUAL>
 __global__ void __launch_bounds__(kShortWarps * 32) distill_backward_short_kernel(const DistillArgs a) {
+  extern __shared__ uint4 shared[];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint4 *buffer = shared + warp * NV * 32;
+  const size_t stride = static_cast<size_t>(gridDim.x) * kShortWarps;
   pdl_enter();
-  for (size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp; row < a.rows;
-       row += static_cast<size_t>(gridDim.x) * kShortWarps) {
+  for (size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp; row < a.rows; row += stride) {
     const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
     const Part p = part_of(z, a.vocab, 0, 1);
-    uint4 q[NV];
-    load_row<T, NV>(z, p, lane, q);
+    stage_row<T, NV>(z, p, lane, buffer);
     const float loose = lane < p.loose ? to_float(z[loose_at(p, lane)]) : 0.0f;
     const float *st = a.stats + row * TL_DISTILL_STATS;
     const RowStats r = {st[0], st[1], st[2], st[3], st[4], st[5], st[6]};
     uint32_t id[kPerLane];
     SlotLane l;
-    read_slots(a, row, z, lane, id, l);
+    read_slots(a, row, lane, id, l);
     const uint32_t t = read_target(a, row, lane);
-    const float zt = t != TL_NO_TOKEN ? to_float(z[t]) : 0.0f;
-    gradient_row<T, NV, DUAL>(a, row, z, p, lane, q, loose, r, id, l, t, zt,
-                              a.row_scale ? a.row_scale[row] : 1.0f);
+    const float scale = a.row_scale ? a.row_scale[row] : 1.0f;
+    await_row();
+    const float zt = t != TL_NO_TOKEN ? logit_at(z, p, buffer, t) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i)
+      if (l.slot[i]) l.z[i] = logit_at(z, p, buffer, id[i]);
+    __syncwarp();  // loose logits among them are read: dz may be z
+    gradient_row<T, NV, DUAL>(a, row, z, p, lane, buffer, loose, r, id, l, t, zt, scale);
+    __syncwarp();  // the buffer is free
   }
 }
 
+template <typename K> void launch_short(K kernel, const DistillArgs &a, int nv, cudaStream_t s) {
+  const size_t smem = static_cast<size_t>(nv) * 512 * kShortWarps;
+  launch_pdl(kernel, short_grid(a.rows, smem), kShortWarps * 32, smem, s, a);
+}
+
 template <typename T, int NV, bool TAIL, bool GRAD> void launch(const DistillArgs &a, cudaStream_t s) {
-  const unsigned grid = short_grid(a.rows);
-  if (dual(a)) launch_pdl(distill_short_kernel<T, NV, TAIL, true, GRAD>, grid, kShortWarps * 32, 0, s, a);
-  else launch_pdl(distill_short_kernel<T, NV, TAIL, false, GRAD>, grid, kShortWarps * 32, 0, s, a);
+  if (dual(a)) launch_short(distill_short_kernel<T, NV, TAIL, true, GRAD>, a, NV, s);
+  else launch_short(distill_short_kernel<T, NV, TAIL, false, GRAD>, a, NV, s);
 }
 
 template <typename T, int NV>
@@ -195,9 +202,8 @@ void launch_forward(const DistillArgs &a, bool tail, bool gradient, cudaStream_t
 }
 
 template <typename T, int NV> void launch_backward(const DistillArgs &a, cudaStream_t s) {
-  const unsigned grid = short_grid(a.rows);
-  if (dual(a)) launch_pdl(distill_backward_short_kernel<T, NV, true>, grid, kShortWarps * 32, 0, s, a);
-  else launch_pdl(distill_backward_short_kernel<T, NV, false>, grid, kShortWarps * 32, 0, s, a);
+  if (dual(a)) launch_short(distill_backward_short_kernel<T, NV, true>, a, NV, s);
+  else launch_short(distill_backward_short_kernel<T, NV, false>, a, NV, s);
 }
 
 }  // namespace

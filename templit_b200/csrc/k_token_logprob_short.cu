@@ -6,22 +6,27 @@ namespace token {
 namespace {
 
 constexpr uint32_t kHits = 192;        // vectors that hold candidates
-constexpr uint32_t kCandidates = 256;
+constexpr uint32_t kCandidates = 192;  // a multiple of 4
 
-struct WarpList {
-  uint4 hit[kHits];
-  uint32_t at[kHits];
-  uint64_t candidate[kCandidates];
+// A warp's shared memory: the row, and what picks the alternatives.
+template <int NV, bool TOP> struct WarpShared {
+  uint4 row[NV * 32];
+};
+template <int NV> struct WarpShared<NV, true> {
+  uint4 row[NV * 32];
+  uint32_t key[kCandidates], id[kCandidates];  // order_of the logit; 16-byte aligned
+  uint16_t hit[kHits];
 };
 
-// The value that `top` or a few more of the warp's keys (N a lane) reach:
-// bisected from -inf.
+// A value that `top` or a few more of the warp's keys (N a lane) reach,
+// bisected between their least and their largest: at least `top` keys.
 template <int N>
 __device__ __forceinline__ uint32_t threshold(const uint32_t (&key)[N], uint32_t top) {
-  uint32_t hi = 0;
+  uint32_t lo = key[0], hi = key[0];
 #pragma unroll
-  for (int i = 0; i < N; ++i) hi = max(hi, key[i]);
-  uint32_t lo = order_of(-INFINITY);
+  for (int i = 1; i < N; ++i) lo = min(lo, key[i]), hi = max(hi, key[i]);
+  // with no more than a key a lane asked for, the least of the lanes' largest
+  lo = __reduce_min_sync(0xffffffffu, top <= 32 ? hi : lo);
   hi = __reduce_max_sync(0xffffffffu, hi) + 1;
   while (hi - lo > 1) {
     const uint32_t mid = lo + (hi - lo) / 2;
@@ -40,7 +45,7 @@ __device__ __forceinline__ uint32_t threshold(const uint32_t (&key)[N], uint32_t
 // k_token_logprob.cu.
 template <typename T>
 __device__ __noinline__ void careful_warp_top(const T *z, uint32_t vocab, uint32_t top, uint32_t least,
-                                              uint64_t *candidate) {
+                                              uint32_t *key, uint32_t *id) {
   const uint32_t lane = threadIdx.x & 31;
   const auto count_from = [&](uint32_t from) {
     uint32_t n = 0;
@@ -54,161 +59,254 @@ __device__ __noinline__ void careful_warp_top(const T *z, uint32_t vocab, uint32
     if (count_from(mid) >= top) lo = mid;
     else hi = mid;
   }
-  // those above lo first, then the first ids at lo
-  uint32_t have = 0;
-  for (int equal = 0; equal < 2; ++equal)
-    for (uint32_t at = 0; at < vocab && have < top; at += 32) {
-      const uint32_t j = at + lane;
-      const float x = j < vocab ? to_float(z[j]) : 0.0f;
-      const bool take = j < vocab && (equal ? order_of(x) == lo : order_of(x) > lo);
-      const uint32_t mask = __ballot_sync(0xffffffffu, take);
-      const uint32_t i = have + __popc(mask & ((1u << lane) - 1));
-      if (take && i < top) candidate[i] = key_of(x, j);
-      have += __popc(mask);
-    }
+  // by id: those above lo, and as many of those at lo as there is room for
+  uint32_t have = 0, room = top - count_from(lo + 1);
+  for (uint32_t at = 0; at < vocab && have < top; at += 32) {
+    const uint32_t j = at + lane;
+    const uint32_t o = j < vocab ? order_of(to_float(z[j])) : 0;
+    const bool equal = j < vocab && o == lo;
+    const uint32_t equals = __ballot_sync(0xffffffffu, equal);
+    const bool take = (j < vocab && o > lo) || (equal && __popc(equals & ((1u << lane) - 1)) < room);
+    const uint32_t mask = __ballot_sync(0xffffffffu, take);
+    const uint32_t i = have + __popc(mask & ((1u << lane) - 1));
+    if (take) key[i] = o, id[i] = j;
+    have += __popc(mask);
+    room -= min(room, static_cast<uint32_t>(__popc(equals)));
+  }
   __syncwarp();
 }
 
+// The order of the logits a lane ranks: #keys above each of its R candidates
+// lane + 32 i, all of which are in the list.  Equal keys (lists are by id)
+// rank by their place: looked at again only where the ranks' sum tells that
+// there are some.
+template <int R>
+__device__ __forceinline__ void rank_candidates(const uint32_t *key, uint32_t n, uint32_t lane,
+                                                uint32_t (&mine)[R], uint32_t (&rank)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    mine[r] = lane + 32 * r < n ? key[lane + 32 * r] : 0xffffffffu;
+    rank[r] = 0;
+  }
+  const uint4 *four = reinterpret_cast<const uint4 *>(key);
+  for (uint32_t j = 0; j < n; j += 4) {  // the list is filled up with 0
+    const uint4 k = four[j / 4];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      rank[r] += (k.x > mine[r]) + (k.y > mine[r]) + (k.z > mine[r]) + (k.w > mine[r]);
+  }
+  uint32_t sum = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) sum += rank[r];
+  if (__reduce_add_sync(0xffffffffu, sum) == n * (n - 1) / 2) return;
+  for (uint32_t j = 0; j < n; ++j) {
+    const uint32_t k = key[j];
+#pragma unroll
+    for (int r = 0; r < R; ++r) rank[r] += k == mine[r] && j < lane + 32 * r;
+  }
+}
+
+// Sums of the row in shared memory; CLAMP: safe where a logit is -inf.
+template <typename T, int NV, bool ENTROPY, bool CLAMP>
+__device__ __forceinline__ void sum_row(const uint4 *row, uint32_t end, uint32_t lane, float c,
+                                        Pow2Sums &v) {
+  constexpr int E = Vec<T>::kElems;
+  const Pair c2 = pair(c, c), n2 = pair(-v.n, -v.n);
+  Pair s = pair(v.s, 0.0f), h = pair(v.h, 0.0f);
+#pragma unroll 4
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t j = i * 32 + lane;
+    if (j >= end) break;
+    Pair z[E / 2];
+    Vec<T>::pairs(row[j], z);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      Pair x = fma2(z[e], c2, n2);
+      if (CLAMP) {
+        const float2 f = halves(x);
+        x = pair(max_nan(f.x, -1e4f), max_nan(f.y, -1e4f));
+      }
+      const Pair p = ex2_pair(x);
+      s = add2(s, p);
+      if (ENTROPY) h = fma2(p, x, h);
+    }
+  }
+  const float2 a = halves(s), b = halves(h);
+  v.s = warp_sum(a.x + a.y);
+  if (ENTROPY) v.h = warp_sum(b.x + b.y);
+}
+
 // Alternatives: 128 groups of vectors (or every vector, for more than 64)
-// give a threshold that at least `top` logits reach; the vectors that reach
-// it go to shared memory, their candidates are ranked among one another.
+// give a threshold that at least `top` logits reach; the candidates in the
+// vectors that reach it are ranked among one another.
 template <typename T, int NV, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(kShortWarps * 32) score_short_kernel(const ScoreArgs a) {
-  __shared__ WarpList lists[TOP ? kShortWarps : 1];
+  extern __shared__ uint4 shared[];
   constexpr int E = Vec<T>::kElems;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t before = (1u << lane) - 1;
+  WarpShared<NV, TOP> &w = reinterpret_cast<WarpShared<NV, TOP> *>(shared)[warp];
+  const size_t stride = static_cast<size_t>(gridDim.x) * kShortWarps;
+  size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp;
   pdl_enter();
-  for (size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp; row < a.rows;
-       row += static_cast<size_t>(gridDim.x) * kShortWarps) {
-    const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
-    const Part p = part_of(z, a.vocab, 0, 1);
-    uint4 r[NV];
-    load_row<T, NV>(z, p, lane, r);
-    const float loose = lane < p.loose ? to_float(z[loose_at(p, lane)]) : -INFINITY;
+  const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
+  Part p{};
+  float loose = 0.0f;
+  const auto begin_row = [&] {
+    if (row >= a.rows) return;
+    z = static_cast<const T *>(a.logits) + row * a.row_stride;
+    p = part_of(z, a.vocab, 0, 1);
+    stage_row<T, NV>(z, p, lane, w.row);
+    loose = lane < p.loose ? to_float(z[loose_at(p, lane)]) : -INFINITY;
+  };
+  begin_row();
+  while (row < a.rows) {
+    const size_t r = row;
     uint32_t t = TL_NO_TOKEN;
-    float zt = 0.0f;
-    if (lane == 0 && a.targets) {
-      t = a.targets[row];
-      if (t < a.vocab) zt = to_float(z[t]);
-    }
+    if (a.targets) t = a.targets[r];
+    await_row();
+    const float zt = lane == 0 && t < a.vocab ? to_float(z[t]) : 0.0f;
+    float most[NV];  // of each vector
     float group[4] = {loose, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) group[i * 4 / NV] = fmaxf(group[i * 4 / NV], Vec<T>::largest(r[i]));
+    for (int i = 0; i < NV; ++i) {
+      most[i] = i * 32 + lane < p.end ? Vec<T>::largest(w.row[i * 32 + lane]) : -INFINITY;
+      group[i * 4 / NV] = fmaxf(group[i * 4 / NV], most[i]);
+    }
     RowSums s;
     s.m = warp_max(fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3])));
     Pow2Sums v = {shift_of(s.m, a.c), 0.0f, 0.0f};
     add_term<ENTROPY>(v, loose, a.c);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (i * 32 >= p.end) break;
-      float f[E];
-      Vec<T>::unpack(r[i], f);
-#pragma unroll
-      for (int e = 0; e < E; ++e) add_term<ENTROPY>(v, f[e], a.c);
+    const Pow2Sums start = v;
+    sum_row<T, NV, ENTROPY, false>(w.row, p.end, lane, a.c, v);
+    if (ENTROPY && v.h != v.h) {  // 0 times a masked logit's x
+      v = start;
+      sum_row<T, NV, ENTROPY, true>(w.row, p.end, lane, a.c, v);
     }
-    v.s = warp_sum(v.s);
-    if (ENTROPY) v.h = warp_sum(v.h);
     s.s = sum_at(v.s, v.n, s.m, a.c);
     s.log_s = logf(s.s);
     if (ENTROPY) s.entropy = v.s == 0.0f ? 0.0f : (log2f(v.s) - v.h / v.s) * 0.6931471805599453f;
     if (far_out(s.m, a.c)) {
-      Sums w = empty_sums();
-      for (uint32_t j = lane; j < a.vocab; j += 32) add_logit(w, to_float(z[j]), a.c);
-      w = warp_merge(w, a.c);
-      s.s = w.s;
+      Sums y = empty_sums();
+      for (uint32_t j = lane; j < a.vocab; j += 32) add_logit(y, to_float(z[j]), a.c);
+      y = warp_merge(y, a.c);
+      s.s = y.s;
       s.log_s = logf(s.s);
-      s.entropy = s.log_s - w.h * a.inv_t / w.s;
+      s.entropy = s.log_s - y.h * a.inv_t / y.s;
     }
     if (lane == 0) {
       if (a.targets) {
-        a.logprob[row] = t < a.vocab ? log_q(zt, s, a.inv_t) : 0.0f;
+        a.logprob[r] = t < a.vocab ? log_q(zt, s, a.inv_t) : 0.0f;
         if (t >= a.vocab && t != TL_NO_TOKEN) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
       }
-      if (ENTROPY) a.entropy[row] = s.entropy;
+      if (ENTROPY) a.entropy[r] = s.entropy;
       if (a.stats) {
-        a.stats[2 * row] = s.m;
-        a.stats[2 * row + 1] = s.s;
+        a.stats[2 * r] = s.m;
+        a.stats[2 * r + 1] = s.s;
       }
     }
-    if (!TOP) continue;
-    WarpList &list = lists[warp];
-    uint32_t least;
-    if (NV > 4 && a.top > 64) {
-      uint32_t key[NV];
+    if constexpr (TOP) {
+      uint32_t least;
+      if (NV > 4 && a.top > 64) {
+        uint32_t key[NV];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) key[i] = order_of(Vec<T>::largest(r[i]));
-      least = threshold<NV>(key, a.top);
-    } else {
-      uint32_t key[4];
+        for (int i = 0; i < NV; ++i) key[i] = order_of(most[i]);
+        least = threshold<NV>(key, a.top);
+      } else {
+        uint32_t key[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) key[i] = order_of(group[i]);
-      least = threshold<4>(key, a.top);
-    }
-    const float from = logit_of(static_cast<uint64_t>(least) << 32);
-    uint32_t hits = 0, candidates = 0;
-    const auto candidate = [&](bool take, float x, uint32_t id) {
-      const uint32_t mask = __ballot_sync(0xffffffffu, take);
-      if (!mask) return;
-      const uint32_t i = candidates + __popc(mask & before);
-      if (take && i < kCandidates) list.candidate[i] = key_of(x, id);
-      candidates += __popc(mask);
-    };
+        for (int i = 0; i < 4; ++i) key[i] = order_of(group[i]);
+        least = threshold<4>(key, a.top);
+      }
+      const float from = logit_of(static_cast<uint64_t>(least) << 32);
+      uint32_t hits = 0, candidates = 0;
+      // a loose element before the vectors, or (`after`) behind them
+      const auto loose_candidates = [&](bool after) {
+        const bool take = lane < p.loose && (lane >= p.head) == after && loose >= from;
+        const uint32_t mask = __ballot_sync(0xffffffffu, take);
+        const uint32_t i = candidates + __popc(mask & before);
+        if (take && i < kCandidates) w.key[i] = order_of(loose), w.id[i] = loose_at(p, lane);
+        candidates += __popc(mask);
+      };
+      if (p.loose) loose_candidates(false);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (i * 32 >= p.end) break;
-      const bool hit = i * 32 + lane < p.end && Vec<T>::largest(r[i]) >= from;
-      const uint32_t mask = __ballot_sync(0xffffffffu, hit);
-      if (mask) {
+      for (int i = 0; i < NV; ++i) {
+        if (i * 32 >= p.end) break;
+        const bool hit = i * 32 + lane < p.end && most[i] >= from;
+        const uint32_t mask = __ballot_sync(0xffffffffu, hit);
         const uint32_t j = hits + __popc(mask & before);
-        if (hit && j < kHits) {
-          list.hit[j] = r[i];
-          list.at[j] = p.head + (i * 32 + lane) * E;
-        }
+        if (hit && j < kHits) w.hit[j] = i * 32 + lane;
         hits += __popc(mask);
       }
-    }
-    __syncwarp();
-    candidate(lane < p.loose && loose >= from, loose, loose_at(p, lane));
-    if (hits <= kHits)
-      for (uint32_t base = 0; base < hits; base += 32) {
-        const bool some = base + lane < hits;
-        const uint4 q = some ? list.hit[base + lane] : make_uint4(0, 0, 0, 0);
-        const uint32_t at = some ? list.at[base + lane] : 0;
-        float f[E];
-        Vec<T>::unpack(q, f);
+      __syncwarp();
+      if (hits <= kHits)
+        for (uint32_t base = 0; base < hits; base += 32) {
+          const bool some = base + lane < hits;
+          const uint32_t at = some ? w.hit[base + lane] : 0;
+          float f[E];
+          Vec<T>::unpack(w.row[at], f);
+          uint32_t i = candidates;
 #pragma unroll
-        for (int e = 0; e < E; ++e) candidate(some && f[e] >= from, f[e], at + e);
+          for (int e = 0; e < E; ++e) {
+            const uint32_t mask = __ballot_sync(0xffffffffu, some && f[e] >= from);
+            i += __popc(mask & before);
+            candidates += __popc(mask);
+          }
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (some && f[e] >= from) {
+              if (i < kCandidates) w.key[i] = order_of(f[e]), w.id[i] = p.head + at * E + e;
+              ++i;
+            }
+        }
+      if (p.loose) loose_candidates(true);
+      __syncwarp();
+      if (hits > kHits || candidates > kCandidates || candidates < a.top) {
+        careful_warp_top(z, a.vocab, a.top, least, w.key, w.id);
+        candidates = a.top;
       }
-    __syncwarp();
-    if (hits > kHits || candidates > kCandidates || candidates < a.top) {
-      careful_warp_top(z, a.vocab, a.top, least, list.candidate);
-      candidates = a.top;
-    }
-    for (uint32_t i = lane; i < candidates; i += 32) {
-      const uint64_t key = list.candidate[i];
-      uint32_t rank = 0;
-      for (uint32_t j = 0; j < candidates; ++j) rank += list.candidate[j] > key;
-      if (rank < a.top) {
-        a.top_ids[row * a.top + rank] = ~static_cast<uint32_t>(key);
-        a.top_logprob[row * a.top + rank] = log_q(logit_of(key), s, a.inv_t);
+      row += stride;
+      begin_row();
+      if (lane < 4 && candidates + lane < kCandidates) w.key[candidates + lane] = 0;
+      __syncwarp();
+      const auto put = [&](uint32_t i, uint32_t key, uint32_t rank) {
+        if (i >= candidates || rank >= a.top) return;
+        a.top_ids[r * a.top + rank] = w.id[i];
+        a.top_logprob[r * a.top + rank] = log_q(logit_of(static_cast<uint64_t>(key) << 32), s, a.inv_t);
+      };
+      if (candidates <= 64) {
+        uint32_t mine[2], rank[2];
+        rank_candidates<2>(w.key, candidates, lane, mine, rank);
+        put(lane, mine[0], rank[0]);
+        put(lane + 32, mine[1], rank[1]);
+      } else {
+        uint32_t mine[kCandidates / 32], rank[kCandidates / 32];
+        rank_candidates<kCandidates / 32>(w.key, candidates, lane, mine, rank);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(kCandidates) / 32; ++i) put(lane + 32 * i, mine[i], rank[i]);
       }
+      __syncwarp();  // the list is free for the next row
+    } else {
+      __syncwarp();
+      row += stride;
+      begin_row();
     }
-    __syncwarp();  // the list is free for the next row
   }
 }
 
 template <typename T, int NV, bool ENTROPY>
 __global__ void __launch_bounds__(kShortWarps * 32) score_backward_short_kernel(const ScoreArgs a) {
+  extern __shared__ uint4 shared[];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint4 *buffer = shared + warp * NV * 32;
+  const size_t stride = static_cast<size_t>(gridDim.x) * kShortWarps;
+  size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp;
   pdl_enter();
-  for (size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp; row < a.rows;
-       row += static_cast<size_t>(gridDim.x) * kShortWarps) {
+  for (; row < a.rows; row += stride) {
     const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
     T *dz = static_cast<T *>(a.dlogits) + row * a.d_row_stride;
     const Part p = part_of(z, a.vocab, 0, 1);
-    uint4 r[NV];
-    load_row<T, NV>(z, p, lane, r);
+    stage_row<T, NV>(z, p, lane, buffer);
     const float loose = lane < p.loose ? to_float(z[loose_at(p, lane)]) : 0.0f;
     const float m = a.stats[2 * row], s = a.stats[2 * row + 1];
     uint32_t t = TL_NO_TOKEN;
@@ -226,11 +324,13 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_backward_short_kernel(
     const float ge = ENTROPY ? a.d_entropy[row] * a.inv_t : 0.0f;
     const float entropy = ENTROPY ? a.entropy[row] : 0.0f;
     const ScoreGradient g = score_gradient(a, m, s, ge == 0.0f ? 0.0f : entropy, gl, ge);
+    const Pair c2 = pair(a.c, a.c);
     const auto fast = [&](float x) { return score_dz<ENTROPY>(g, a.c, x); };
+    const auto fast2 = [&](Pair x) { return score_dz2<ENTROPY>(g, c2, x); };
     const auto careful = [&](float x) { return careful_score_dz(g, a, x); };
-    __syncwarp();  // the target's logit is read: dz may be z
+    await_row();  // and the target's logit is read: dz may be z
     if (!g.none && !g.far) {
-      store_row<T, NV>(dz, p, lane, r, loose, fast);
+      write_row<T, NV>(dz, p, lane, buffer, loose, fast2, fast);
     } else {
       for (uint32_t j = lane; j < a.vocab; j += 32)
         dz[j] = from_float<T>(g.none ? 0.0f : careful(to_float(z[j])));
@@ -241,21 +341,28 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_backward_short_kernel(
   }
 }
 
+// Launches a kernel whose warps need `warp_bytes` of shared memory each.
+template <typename K> void launch_short(K kernel, const ScoreArgs &a, size_t warp_bytes, cudaStream_t s) {
+  const size_t smem = warp_bytes * kShortWarps;
+  if (smem > 48 * 1024)  // a failure shows in the launch's status
+    (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  launch_pdl(kernel, short_grid(a.rows, smem), kShortWarps * 32, smem, s, a);
+}
+
 template <typename T, int NV> void launch(const ScoreArgs &a, cudaStream_t s) {
-  const unsigned grid = short_grid(a.rows);
+  constexpr size_t with = sizeof(WarpShared<NV, true>), without = sizeof(WarpShared<NV, false>);
   if (a.entropy) {
-    if (a.top) launch_pdl(score_short_kernel<T, NV, true, true>, grid, kShortWarps * 32, 0, s, a);
-    else launch_pdl(score_short_kernel<T, NV, true, false>, grid, kShortWarps * 32, 0, s, a);
+    if (a.top) launch_short(score_short_kernel<T, NV, true, true>, a, with, s);
+    else launch_short(score_short_kernel<T, NV, true, false>, a, without, s);
   } else {
-    if (a.top) launch_pdl(score_short_kernel<T, NV, false, true>, grid, kShortWarps * 32, 0, s, a);
-    else launch_pdl(score_short_kernel<T, NV, false, false>, grid, kShortWarps * 32, 0, s, a);
+    if (a.top) launch_short(score_short_kernel<T, NV, false, true>, a, with, s);
+    else launch_short(score_short_kernel<T, NV, false, false>, a, without, s);
   }
 }
 
 template <typename T, int NV> void launch_backward(const ScoreArgs &a, cudaStream_t s) {
-  const unsigned grid = short_grid(a.rows);
-  if (a.d_entropy) launch_pdl(score_backward_short_kernel<T, NV, true>, grid, kShortWarps * 32, 0, s, a);
-  else launch_pdl(score_backward_short_kernel<T, NV, false>, grid, kShortWarps * 32, 0, s, a);
+  if (a.d_entropy) launch_short(score_backward_short_kernel<T, NV, true>, a, NV * 512, s);
+  else launch_short(score_backward_short_kernel<T, NV, false>, a, NV * 512, s);
 }
 
 }  // namespace

@@ -105,6 +105,39 @@ __device__ __forceinline__ Sums block_merge(Sums v, float c, Sums *scratch) {
 // first and after the last vector (fewer than two vectors' worth) belong to
 // the first part and take one thread each.
 
+// Two fp32 in a register pair: Blackwell's packed arithmetic does both in
+// one issued instruction.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ float2 halves(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair ex2_pair(Pair x) {
+  const float2 f = halves(x);
+  return pair(ex2_approx(f.x), ex2_approx(f.y));
+}
+
 template <typename T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int kElems = 4;
@@ -112,6 +145,15 @@ template <> struct Vec<float> {
   static __device__ __forceinline__ void unpack(const uint4 &v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
     f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ void pairs(const uint4 &v, Pair (&f)[2]) {
+    f[0] = pair(__uint_as_float(v.x), __uint_as_float(v.y));
+    f[1] = pair(__uint_as_float(v.z), __uint_as_float(v.w));
+  }
+  static __device__ __forceinline__ uint4 pack_pairs(const Pair (&f)[2]) {
+    const float2 a = halves(f[0]), b = halves(f[1]);
+    return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x),
+                      __float_as_uint(b.y));
   }
   // makes the elements whose bit is set in m -inf
   static __device__ __forceinline__ void drop(uint4 &v, uint32_t m) {
@@ -155,6 +197,23 @@ template <> struct Vec<__half> {
     const __half2 a = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
     return fmaxf(__low2float(a), __high2float(a));
   }
+  static __device__ __forceinline__ void pairs(const uint4 &v, Pair (&f)[4]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      f[i] = pair(p.x, p.y);
+    }
+  }
+  static __device__ __forceinline__ uint4 pack_pairs(const Pair (&f)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 p = __float22half2_rn(halves(f[i]));
+      w[i] = *reinterpret_cast<const uint32_t *>(&p);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
     uint32_t w[4];
 #pragma unroll
@@ -189,6 +248,21 @@ template <> struct Vec<__nv_bfloat16> {
     const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(&v);
     const __nv_bfloat162 a = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
     return fmaxf(__low2float(a), __high2float(a));
+  }
+  static __device__ __forceinline__ void pairs(const uint4 &v, Pair (&f)[4]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint4 pack_pairs(const Pair (&f)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 p = __float22bfloat162_rn(halves(f[i]));
+      w[i] = *reinterpret_cast<const uint32_t *>(&p);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
   static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
     uint32_t w[4];
@@ -342,51 +416,71 @@ __device__ __forceinline__ float sum_at(float s, float n, float m, float c) {
 // Fewest rows that take a warp each; fewer leave the SMs to a CTA per row.
 constexpr uint32_t kShortRows = 512;
 
-// ---- short rows: a warp holds a row in registers -------------------------
-// Vectors of a lane: 4 or 16, lane l has vectors l + 32 i.  Rows of up to
-// 8 KB; the caller sees to it that they fit.
-constexpr int kShortWarps = 4;  // warps (rows) of a CTA
+// ---- short rows: a warp holds a row in shared memory -----------------------
+// A row's vectors go to shared memory by cp.async, the next row's while the
+// warp finishes the last one; lane l works on vectors l + 32 i, i < NV.
+// Shared memory, not registers: 20 and more rows are in flight on an SM, and
+// single logits can be looked up and taken out.
+constexpr int kShortWarps = 4;  // warps (rows in flight) of a CTA
+
+// Vectors of a lane for a row: 4, 16, or 0 where a row is too long.
 inline uint32_t short_vectors(uint32_t vocab, size_t type_bytes) {
   const uint64_t vecs = static_cast<uint64_t>(vocab) * type_bytes / 16;
   return vecs <= 4 * 32 ? 4 : vecs <= 16 * 32 ? 16 : 0;
 }
-inline unsigned short_grid(uint32_t rows) {
-  const uint32_t ctas = (rows + kShortWarps - 1) / kShortWarps, most = kNumSMs * 64u;
+// CTAs that fill the SMs, given the shared memory of one.
+inline unsigned short_grid(uint32_t rows, size_t smem) {
+  const uint32_t ctas = (rows + kShortWarps - 1) / kShortWarps;
+  size_t per_sm = (227 * 1024) / (smem + 1024);
+  if (per_sm > 8) per_sm = 8;
+  const uint32_t most = kNumSMs * static_cast<uint32_t>(per_sm);
   return ctas < most ? ctas : most;
 }
 
 template <typename T, int NV>
-__device__ __forceinline__ void load_row(const T *z, const Part &p, uint32_t lane, uint4 (&r)[NV]) {
+__device__ __forceinline__ void stage_row(const T *z, const Part &p, uint32_t lane, uint4 *buffer) {
   const uint4 *vec = reinterpret_cast<const uint4 *>(z + p.head);
+  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(buffer));
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const uint32_t j = i * 32 + lane;
-    r[i] = j < p.end ? vec[j] : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+    if (j < p.end)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + j * 16), "l"(vec + j) : "memory");
   }
 }
+// The staged row is in shared memory, for every lane.
+__device__ __forceinline__ void await_row() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
+}
 
-// dz_j = f(z_j) for the row in registers and the lane's loose element.
-template <typename T, int NV, typename F>
-__device__ __forceinline__ void store_row(T *dz, const Part &p, uint32_t lane, const uint4 (&r)[NV],
-                                          float loose, F f) {
+// dz_j = f(z_j) for the row in shared memory, by pairs; the lane's loose
+// element by `one`.
+template <typename T, int NV, typename F, typename G>
+__device__ __forceinline__ void write_row(T *dz, const Part &p, uint32_t lane, const uint4 *buffer,
+                                          float loose, F two, G one) {
   constexpr int E = Vec<T>::kElems;
   const bool aligned = aligned16(dz + p.head);
-#pragma unroll
+#pragma unroll 4
   for (int i = 0; i < NV; ++i) {
     const uint32_t j = i * 32 + lane;
     if (j >= p.end) break;
-    float x[E];
-    Vec<T>::unpack(r[i], x);
+    Pair x[E / 2];
+    Vec<T>::pairs(buffer[j], x);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = f(x[e]);
+    for (int e = 0; e < E / 2; ++e) x[e] = two(x[e]);
     if (aligned) {
-      reinterpret_cast<uint4 *>(dz + p.head)[j] = Vec<T>::pack(x);
+      reinterpret_cast<uint4 *>(dz + p.head)[j] = Vec<T>::pack_pairs(x);
     } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) dz[p.head + j * E + e] = from_float<T>(x[e]);
+      for (int e = 0; e < E / 2; ++e) {
+        const float2 y = halves(x[e]);
+        dz[p.head + j * E + 2 * e] = from_float<T>(y.x);
+        dz[p.head + j * E + 2 * e + 1] = from_float<T>(y.y);
+      }
     }
   }
-  if (lane < p.loose) dz[loose_at(p, lane)] = from_float<T>(f(loose));
+  if (lane < p.loose) dz[loose_at(p, lane)] = from_float<T>(one(loose));
 }
 
 inline size_t type_size(int32_t type) { return type == TL_FLOAT32 ? 4 : 2; }

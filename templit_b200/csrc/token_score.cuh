@@ -75,6 +75,17 @@ __device__ __forceinline__ float score_dz(const ScoreGradient &g, float c, float
   return -ex2_approx(x) * (ENTROPY ? fmaf(g.B, x, g.A) : g.A);
 }
 
+template <bool ENTROPY>
+__device__ __forceinline__ Pair score_dz2(const ScoreGradient &g, Pair c, Pair z) {
+  Pair x = fma2(z, c, pair(-g.n, -g.n));
+  if (ENTROPY) {
+    const float2 f = halves(x);
+    x = pair(max_nan(f.x, -1e4f), max_nan(f.y, -1e4f));
+  }
+  const Pair f = ENTROPY ? fma2(pair(-g.B, -g.B), x, pair(-g.A, -g.A)) : pair(-g.A, -g.A);
+  return mul2(ex2_pair(x), f);
+}
+
 // The same for rows far out.
 __device__ __forceinline__ float careful_score_dz(const ScoreGradient &g, const ScoreArgs &a, float z) {
   const float d = z - g.m, q = ex2_approx(d * a.c) * g.inv_s;
