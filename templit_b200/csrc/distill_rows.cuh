@@ -134,6 +134,7 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
   float u_max = -INFINITY, z_max = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
+    if (i * 32 >= a.top) break;
     slots += l.slot[i];
     if (l.slot[i]) u_max = fmaxf(u_max, l.u[i]), z_max = fmaxf(z_max, l.z[i]);
   }
@@ -144,11 +145,13 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
     r.m = fmaxf(o.m, warp_max(z_max));
     float s = 0.0f, s1 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i)
+    for (int i = 0; i < kPerLane; ++i) {
+      if (i * 32 >= a.top) break;
       if (l.slot[i] && l.z[i] != -INFINITY) {
         s += ex2_approx((l.z[i] - r.m) * a.c);
         if (target) s1 += ex2_approx((l.z[i] - r.m) * kLog2e);
       }
+    }
     r.s = o.s * rescale(o.m, r.m, a.c) + warp_sum(s);
     if (target) r.s1 = o.s1 * rescale(o.m, r.m, kLog2e) + warp_sum(s1);
   }
@@ -161,6 +164,7 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
+    if (i * 32 >= a.top) break;
     p[i] = l.slot[i] ? expf(l.u[i] - r.h) : 0.0f;
     sum += p[i];
   }
@@ -176,6 +180,7 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
   kl = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
+    if (i * 32 >= a.top) break;
     p[i] *= r.b;
     if (p[i] != p[i]) {
       kl = p[i];

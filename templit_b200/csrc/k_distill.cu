@@ -25,10 +25,12 @@ __device__ __forceinline__ void gradient_part(const DistillArgs &a, size_t row, 
   T *dz = static_cast<T *>(a.dlogits) + row * a.d_row_stride;
   const DistillGradient g = distill_gradient<DUAL>(a, r, t, a.row_scale ? a.row_scale[row] : 1.0f);
   const auto fast = [&](float x) { return distill_dz<DUAL>(g, a.c, x); };
+  const Pair c2 = pair(a.c, a.c);
+  const auto fast2 = [&](Pair x) { return distill_dz2<DUAL>(g, c2, x); };
   const auto careful = [&](float x) { return careful_distill_dz(g, r, a.c, x); };
   if (g.none) write_elements<kThreads>(z, dz, part, [](float) { return 0.0f; });
   else if (g.far) write_elements<kThreads>(z, dz, part, careful);
-  else write_vectors<kThreads, kBatch>(z, dz, part, fast);
+  else write_vectors<kThreads, kBatch>(z, dz, part, fast2, fast);
   __syncthreads();
   if (g.none) return;
   if (target_here && g.ce != 0.0f) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) - g.ce);
@@ -84,7 +86,7 @@ __device__ __noinline__ Outside careful_outside(const T *z, uint32_t vocab, floa
 // thing it read) writes the gradient.  DUAL: the target's term has sums of
 // its own, at temperature 1.
 template <typename T, bool TAIL, bool DUAL, bool GRAD, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, 4) distill_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(kThreads, GRAD ? 4 : 5) distill_kernel(const DistillArgs a) {
   extern __shared__ uint32_t marks[];
   __shared__ DistillShared sh;
   constexpr uint32_t E = Vec<T>::kElems;
@@ -139,16 +141,8 @@ __global__ void __launch_bounds__(kThreads, 4) distill_kernel(const DistillArgs 
       largest = fmaxf(largest, most);
       move_to<false>(v, fmaxf(v.n, shift_of(most, a.c)));
       if (DUAL) move_to<false>(v1, fmaxf(v1.n, shift_of(most, kLog2e)));
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        float f[E];
-        Vec<T>::unpack(q[i], f);
-#pragma unroll
-        for (uint32_t e = 0; e < E; ++e) {
-          add_term<false>(v, f[e], a.c);
-          if (DUAL) add_term<false>(v1, f[e], kLog2e);
-        }
-      }
+      add_batch<false, T>(v, q, a.c);
+      if (DUAL) add_batch<false, T>(v1, q, kLog2e);
     }
     if (tid < p.loose) {
       const uint32_t j = loose_at(p, tid);

@@ -55,11 +55,13 @@ __device__ __forceinline__ void gradient_row(const DistillArgs &a, size_t row, c
   if (lane == 0 && g.ce != 0.0f) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) - g.ce);
   __syncwarp();  // a target in a slot: the slot's value stands
 #pragma unroll
-  for (int i = 0; i < kPerLane; ++i)
+  for (int i = 0; i < kPerLane; ++i) {
+    if (i * 32 >= a.top) break;
     if (l.slot[i]) {
       const float pk = expf(l.u[i] - r.h) * r.b;
       dz[id[i]] = from_float<T>(slot_dz(g, r, a.c, pk, l.z[i], id[i] == t));
     }
+  }
 }
 
 // As distill_kernel in k_distill.cu, with the row read once.  The slots'
@@ -105,9 +107,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_short_kernel(const D
       __syncwarp();
     }
     float m = loose;
-#pragma unroll 4
-    for (int i = 0; i < NV; ++i)
-      if (i * 32 + lane < p.end) m = fmaxf(m, Vec<T>::largest(buffer[i * 32 + lane]));
+    for_vectors<NV>(p.end, lane, [&](int, uint32_t j) { m = fmaxf(m, Vec<T>::largest(buffer[j])); });
     m = warp_max(m);
     Outside o = {m, 0.0f, 0.0f};
     if (far_out(m, a.c) || far_out(m, kLog2e)) {
@@ -128,17 +128,15 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_short_kernel(const D
       const Pair c2 = pair(a.c, a.c), n2 = pair(-v.n, -v.n);
       const Pair c21 = pair(kLog2e, kLog2e), n21 = pair(-v1.n, -v1.n);
       Pair s = pair(v.s, 0.0f), s1 = pair(v1.s, 0.0f);
-#pragma unroll 4
-      for (int i = 0; i < NV; ++i) {
-        if (i * 32 + lane >= p.end) break;
+      for_vectors<NV>(p.end, lane, [&](int, uint32_t j) {
         Pair f[E / 2];
-        Vec<T>::pairs(buffer[i * 32 + lane], f);
+        Vec<T>::pairs(buffer[j], f);
 #pragma unroll
         for (int e = 0; e < E / 2; ++e) {
           s = add2(s, ex2_pair(fma2(f[e], c2, n2)));
           if (DUAL) s1 = add2(s1, ex2_pair(fma2(f[e], c21, n21)));
         }
-      }
+      });
       const float2 y = halves(s), y1 = halves(s1);
       o.s = sum_at(warp_sum(y.x + y.y), v.n, m, a.c);
       o.s1 = DUAL ? sum_at(warp_sum(y1.x + y1.y), v1.n, m, kLog2e) : o.s;

@@ -149,7 +149,7 @@ __device__ __noinline__ void careful_top(const T *z, uint32_t vocab, uint32_t to
 // on, and only segments whose maximum reaches it are looked at again; their
 // ranks among one another order the few candidates.
 template <typename T, bool ENTROPY, bool TOP, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, 4) score_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) score_kernel(const ScoreArgs a) {
   extern __shared__ float segment[];  // [segments][kThreads] maxima (TOP)
   __shared__ ScoreShared sh;
   constexpr uint32_t E = Vec<T>::kElems;
@@ -193,13 +193,7 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const ScoreArgs a) {
         segment[(batch >> a.segment_shift) * kThreads + tid] = in_segment;
       }
       move_to<ENTROPY>(v, fmaxf(v.n, shift_of(most, a.c)));
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        float f[E];
-        Vec<T>::unpack(r[u], f);
-#pragma unroll
-        for (uint32_t e = 0; e < E; ++e) add_term<ENTROPY>(v, f[e], a.c);
-      }
+      add_batch<ENTROPY, T>(v, r, a.c);
     }
     float loose = -INFINITY;
     if (tid < p.loose) {
@@ -260,25 +254,27 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const ScoreArgs a) {
     }
     if (TOP) {
       if (warp == 0) {
-        // bisect for a value that `top` to a few more of the 256 maxima reach
-        uint32_t key[kThreads / 32];
-        uint32_t hi = 0;
+        // a value that `top` to a few more of the 256 maxima reach, bisected
+        // between the least and the largest of them (with no more than a
+        // value a lane asked for, between the lanes' largest)
+        uint32_t key[kThreads / 32], lo = 0xffffffffu, hi = 0;
 #pragma unroll
         for (int i = 0; i < kThreads / 32; ++i) {
-          key[i] = order_of(sh.group[i * 32 + lane]);
+          key[i] = order_of_number(sh.group[i * 32 + lane]);
+          lo = min(lo, key[i]);
           hi = max(hi, key[i]);
         }
-        uint32_t lo = order_of(-INFINITY);
+        lo = __reduce_min_sync(0xffffffffu, a.top <= 32 ? hi : lo);
         hi = __reduce_max_sync(0xffffffffu, hi) + 1;
         while (hi - lo > 1) {
           const uint32_t mid = lo + (hi - lo) / 2;
           uint32_t n = 0;
 #pragma unroll
-          for (int i = 0; i < kThreads / 32; ++i) n += key[i] >= mid;
+          for (int i = 0; i < kThreads / 32; ++i) count_from(n, key[i], mid);
           n = __reduce_add_sync(0xffffffffu, n);
           if (n >= a.top) lo = mid;
           else hi = mid;
-          if (n >= a.top && n <= a.top + a.top / 8) break;
+          if (n >= a.top && n <= a.top + a.top / 8 + 1) break;
         }
         if (lane == 0) sh.least = lo;
       }
@@ -292,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const ScoreArgs a) {
       };
       if (largest >= from) {
         const uint32_t segments = (batch + (1u << a.segment_shift) - 1) >> a.segment_shift;
+#pragma unroll 4
         for (uint32_t s = 0; s < segments; ++s)
           if (segment[s * kThreads + tid] >= from) {
             const uint32_t i = atomicAdd(&sh.entries, 1u);
@@ -326,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 4) score_kernel(const ScoreArgs a) {
         for (uint32_t i = tid; i < n; i += kThreads) {
           const uint64_t key = sh.candidate[i];
           uint32_t rank = 0;
+#pragma unroll 8
           for (uint32_t j = 0; j < n; ++j) rank += sh.candidate[j] > key;
           if (rank < a.top) {
             a.top_ids[row * a.top + rank] = ~static_cast<uint32_t>(key);
@@ -366,6 +364,8 @@ __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArg
     const Part p = part_of(z, a.vocab, part, parts);
     const ScoreGradient g = score_gradient(a, m, s, entropy, gl, ge);
     const auto fast = [&](float x) { return score_dz<ENTROPY>(g, a.c, x); };
+    const Pair c2 = pair(a.c, a.c);
+    const auto fast2 = [&](Pair x) { return score_dz2<ENTROPY>(g, c2, x); };
     const auto careful = [&](float x) { return careful_score_dz(g, a, x); };
     float zt = 0.0f;
     const bool mine = tid == 0 && t != TL_NO_TOKEN && !g.none && holds<T>(p, t);
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArg
     __syncthreads();  // dz may be z
     if (g.none) write_elements<kThreads>(z, dz, p, [](float) { return 0.0f; });
     else if (g.far) write_elements<kThreads>(z, dz, p, careful);
-    else write_vectors<kThreads, kBatch>(z, dz, p, fast);
+    else write_vectors<kThreads, kBatch>(z, dz, p, fast2, fast);
     __syncthreads();
     if (mine) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) + gl);
   }

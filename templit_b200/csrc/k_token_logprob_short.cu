@@ -5,8 +5,7 @@ namespace tl {
 namespace token {
 namespace {
 
-constexpr uint32_t kHits = 192;        // vectors that hold candidates
-constexpr uint32_t kCandidates = 192;  // a multiple of 4
+constexpr uint32_t kCandidates = 192;  // a multiple of 32
 
 // A warp's shared memory: the row, and what picks the alternatives.
 template <int NV, bool TOP> struct WarpShared {
@@ -14,9 +13,33 @@ template <int NV, bool TOP> struct WarpShared {
 };
 template <int NV> struct WarpShared<NV, true> {
   uint4 row[NV * 32];
-  uint32_t key[kCandidates], id[kCandidates];  // order_of the logit; 16-byte aligned
-  uint16_t hit[kHits];
+  uint32_t key[kCandidates], id[kCandidates];  // 16-byte aligned
+  uint32_t candidates;
+  uint32_t unused[3];  // warps' parts stay 16-byte aligned
 };
+
+// A candidate's key, larger for what ranks first.  Of 16-bit logits it holds
+// the id too (rows here are shorter than 2^16): no two are equal.
+template <typename T> __device__ __forceinline__ uint32_t list_key(float x, uint32_t id);
+template <> __device__ __forceinline__ uint32_t list_key<float>(float x, uint32_t) { return order_of(x); }
+template <> __device__ __forceinline__ uint32_t list_key<__nv_bfloat16>(float x, uint32_t id) {
+  return (order_of(x) & 0xffff0000u) | (0xffffu - id);
+}
+template <> __device__ __forceinline__ uint32_t list_key<__half>(float x, uint32_t id) {
+  // fp16's own 16 bits in order
+  const uint32_t b = __half_as_ushort(__float2half_rn(x + 0.0f));
+  const uint32_t o = x != x ? 0u : b & 0x8000u ? 0xffffu & ~b : b | 0x8000u;
+  return o << 16 | (0xffffu - id);
+}
+// The logit of a key.
+template <typename T> __device__ __forceinline__ float list_logit(uint32_t key) {
+  if (sizeof(T) == 4) return logit_of(static_cast<uint64_t>(key) << 32);
+  const uint32_t o = key >> 16;
+  const uint16_t b = static_cast<uint16_t>(o & 0x8000u ? o ^ 0x8000u : ~o);
+  T x;
+  memcpy(&x, &b, sizeof(T) < 2 ? sizeof(T) : 2);
+  return to_float(x);
+}
 
 // A value that `top` or a few more of the warp's keys (N a lane) reach,
 // bisected between their least and their largest: at least `top` keys.
@@ -32,7 +55,7 @@ __device__ __forceinline__ uint32_t threshold(const uint32_t (&key)[N], uint32_t
     const uint32_t mid = lo + (hi - lo) / 2;
     uint32_t n = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) n += key[i] >= mid;
+    for (int i = 0; i < N; ++i) token::count_from(n, key[i], mid);
     n = __reduce_add_sync(0xffffffffu, n);
     if (n >= top) lo = mid;
     else hi = mid;
@@ -69,20 +92,22 @@ __device__ __noinline__ void careful_warp_top(const T *z, uint32_t vocab, uint32
     const bool take = (j < vocab && o > lo) || (equal && __popc(equals & ((1u << lane) - 1)) < room);
     const uint32_t mask = __ballot_sync(0xffffffffu, take);
     const uint32_t i = have + __popc(mask & ((1u << lane) - 1));
-    if (take) key[i] = o, id[i] = j;
+    if (take) key[i] = list_key<T>(to_float(z[j]), j), id[i] = j;
     have += __popc(mask);
     room -= min(room, static_cast<uint32_t>(__popc(equals)));
   }
   __syncwarp();
 }
 
-// The order of the logits a lane ranks: #keys above each of its R candidates
-// lane + 32 i, all of which are in the list.  Equal keys (lists are by id)
-// rank by their place: looked at again only where the ranks' sum tells that
+// Ranks and writes out a list of up to 32 R candidates; lane l has those at
+// l + 32 i.  A candidate's rank is the number of keys above its own; equal
+// keys (fp32 only) rank by id, looked at where the ranks' sum tells that
 // there are some.
-template <int R>
-__device__ __forceinline__ void rank_candidates(const uint32_t *key, uint32_t n, uint32_t lane,
-                                                uint32_t (&mine)[R], uint32_t (&rank)[R]) {
+template <typename T, int R>
+__device__ __forceinline__ void rank_candidates(const ScoreArgs &a, size_t row, const RowSums &s,
+                                                const uint32_t *key, const uint32_t *id, uint32_t n,
+                                                uint32_t lane) {
+  uint32_t mine[R], rank[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     mine[r] = lane + 32 * r < n ? key[lane + 32 * r] : 0xffffffffu;
@@ -92,18 +117,32 @@ __device__ __forceinline__ void rank_candidates(const uint32_t *key, uint32_t n,
   for (uint32_t j = 0; j < n; j += 4) {  // the list is filled up with 0
     const uint4 k = four[j / 4];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      rank[r] += (k.x > mine[r]) + (k.y > mine[r]) + (k.z > mine[r]) + (k.w > mine[r]);
+    for (int r = 0; r < R; ++r) {
+      count_above(rank[r], k.x, mine[r]);
+      count_above(rank[r], k.y, mine[r]);
+      count_above(rank[r], k.z, mine[r]);
+      count_above(rank[r], k.w, mine[r]);
+    }
   }
-  uint32_t sum = 0;
+  if (sizeof(T) == 4) {
+    uint32_t sum = 0;
 #pragma unroll
-  for (int r = 0; r < R; ++r) sum += rank[r];
-  if (__reduce_add_sync(0xffffffffu, sum) == n * (n - 1) / 2) return;
-  for (uint32_t j = 0; j < n; ++j) {
-    const uint32_t k = key[j];
+    for (int r = 0; r < R; ++r) sum += rank[r];
+    if (__reduce_add_sync(0xffffffffu, sum) != n * (n - 1) / 2) {
+      for (uint32_t j = 0; j < n; ++j) {
+        const uint32_t k = key[j], i = id[j];
 #pragma unroll
-    for (int r = 0; r < R; ++r) rank[r] += k == mine[r] && j < lane + 32 * r;
+        for (int r = 0; r < R; ++r)
+          if (lane + 32 * r < n) rank[r] += k == mine[r] && i < id[lane + 32 * r];
+      }
+    }
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (lane + 32 * r < n && rank[r] < a.top) {
+      a.top_ids[row * a.top + rank[r]] = id[lane + 32 * r];
+      a.top_logprob[row * a.top + rank[r]] = log_q(list_logit<T>(mine[r]), s, a.inv_t);
+    }
 }
 
 // Sums of the row in shared memory; CLAMP: safe where a logit is -inf.
@@ -113,10 +152,7 @@ __device__ __forceinline__ void sum_row(const uint4 *row, uint32_t end, uint32_t
   constexpr int E = Vec<T>::kElems;
   const Pair c2 = pair(c, c), n2 = pair(-v.n, -v.n);
   Pair s = pair(v.s, 0.0f), h = pair(v.h, 0.0f);
-#pragma unroll 4
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t j = i * 32 + lane;
-    if (j >= end) break;
+  for_vectors<NV>(end, lane, [&](int, uint32_t j) {
     Pair z[E / 2];
     Vec<T>::pairs(row[j], z);
 #pragma unroll
@@ -130,7 +166,7 @@ __device__ __forceinline__ void sum_row(const uint4 *row, uint32_t end, uint32_t
       s = add2(s, p);
       if (ENTROPY) h = fma2(p, x, h);
     }
-  }
+  });
   const float2 a = halves(s), b = halves(h);
   v.s = warp_sum(a.x + a.y);
   if (ENTROPY) v.h = warp_sum(b.x + b.y);
@@ -144,7 +180,6 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_short_kernel(const Sco
   extern __shared__ uint4 shared[];
   constexpr int E = Vec<T>::kElems;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t before = (1u << lane) - 1;
   WarpShared<NV, TOP> &w = reinterpret_cast<WarpShared<NV, TOP> *>(shared)[warp];
   const size_t stride = static_cast<size_t>(gridDim.x) * kShortWarps;
   size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp;
@@ -167,12 +202,12 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_short_kernel(const Sco
     await_row();
     const float zt = lane == 0 && t < a.vocab ? to_float(z[t]) : 0.0f;
     float most[NV];  // of each vector
+#pragma unroll
+    for (int i = 0; i < NV; ++i) most[i] = -INFINITY;
+    for_vectors<NV>(p.end, lane, [&](int i, uint32_t j) { most[i] = Vec<T>::largest(w.row[j]); });
     float group[4] = {loose, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      most[i] = i * 32 + lane < p.end ? Vec<T>::largest(w.row[i * 32 + lane]) : -INFINITY;
-      group[i * 4 / NV] = fmaxf(group[i * 4 / NV], most[i]);
-    }
+    for (int i = 0; i < NV; ++i) group[i * 4 / NV] = fmaxf(group[i * 4 / NV], most[i]);
     RowSums s;
     s.m = warp_max(fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3])));
     Pow2Sums v = {shift_of(s.m, a.c), 0.0f, 0.0f};
@@ -210,58 +245,43 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_short_kernel(const Sco
       if (NV > 4 && a.top > 64) {
         uint32_t key[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) key[i] = order_of(most[i]);
+        for (int i = 0; i < NV; ++i) key[i] = order_of_number(most[i]);
         least = threshold<NV>(key, a.top);
       } else {
         uint32_t key[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) key[i] = order_of(group[i]);
+        for (int i = 0; i < 4; ++i) key[i] = order_of_number(group[i]);
         least = threshold<4>(key, a.top);
       }
       const float from = logit_of(static_cast<uint64_t>(least) << 32);
-      uint32_t hits = 0, candidates = 0;
-      // a loose element before the vectors, or (`after`) behind them
-      const auto loose_candidates = [&](bool after) {
-        const bool take = lane < p.loose && (lane >= p.head) == after && loose >= from;
-        const uint32_t mask = __ballot_sync(0xffffffffu, take);
-        const uint32_t i = candidates + __popc(mask & before);
-        if (take && i < kCandidates) w.key[i] = order_of(loose), w.id[i] = loose_at(p, lane);
-        candidates += __popc(mask);
-      };
-      if (p.loose) loose_candidates(false);
+      // a bit for each of the lane's vectors that hold candidates
+      uint32_t hits = 0;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (i * 32 >= p.end) break;
-        const bool hit = i * 32 + lane < p.end && most[i] >= from;
-        const uint32_t mask = __ballot_sync(0xffffffffu, hit);
-        const uint32_t j = hits + __popc(mask & before);
-        if (hit && j < kHits) w.hit[j] = i * 32 + lane;
-        hits += __popc(mask);
+      for (int i = 0; i < NV; ++i)
+        mark_from(hits, most[i], from, 1u << i);
+      if (lane == 0) w.candidates = 0;
+      __syncwarp();
+      const auto put = [&](uint32_t i, float x, uint32_t id) {
+        if (i < kCandidates) w.key[i] = list_key<T>(x, id), w.id[i] = id;
+      };
+      if (lane < p.loose && loose >= from) put(atomicAdd(&w.candidates, 1u), loose, loose_at(p, lane));
+      while (hits) {
+        const uint32_t at = (__ffs(hits) - 1) * 32 + lane;
+        hits &= hits - 1;
+        if (at >= p.end) break;  // -inf in place of vectors that a row lacks
+        float f[E];
+        Vec<T>::unpack(w.row[at], f);
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) n += f[e] >= from;
+        uint32_t i = atomicAdd(&w.candidates, n);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (f[e] >= from) put(i++, f[e], p.head + at * E + e);
       }
       __syncwarp();
-      if (hits <= kHits)
-        for (uint32_t base = 0; base < hits; base += 32) {
-          const bool some = base + lane < hits;
-          const uint32_t at = some ? w.hit[base + lane] : 0;
-          float f[E];
-          Vec<T>::unpack(w.row[at], f);
-          uint32_t i = candidates;
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const uint32_t mask = __ballot_sync(0xffffffffu, some && f[e] >= from);
-            i += __popc(mask & before);
-            candidates += __popc(mask);
-          }
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (some && f[e] >= from) {
-              if (i < kCandidates) w.key[i] = order_of(f[e]), w.id[i] = p.head + at * E + e;
-              ++i;
-            }
-        }
-      if (p.loose) loose_candidates(true);
-      __syncwarp();
-      if (hits > kHits || candidates > kCandidates || candidates < a.top) {
+      uint32_t candidates = w.candidates;
+      if (candidates > kCandidates || candidates < a.top) {
         careful_warp_top(z, a.vocab, a.top, least, w.key, w.id);
         candidates = a.top;
       }
@@ -269,22 +289,11 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_short_kernel(const Sco
       begin_row();
       if (lane < 4 && candidates + lane < kCandidates) w.key[candidates + lane] = 0;
       __syncwarp();
-      const auto put = [&](uint32_t i, uint32_t key, uint32_t rank) {
-        if (i >= candidates || rank >= a.top) return;
-        a.top_ids[r * a.top + rank] = w.id[i];
-        a.top_logprob[r * a.top + rank] = log_q(logit_of(static_cast<uint64_t>(key) << 32), s, a.inv_t);
-      };
-      if (candidates <= 64) {
-        uint32_t mine[2], rank[2];
-        rank_candidates<2>(w.key, candidates, lane, mine, rank);
-        put(lane, mine[0], rank[0]);
-        put(lane + 32, mine[1], rank[1]);
-      } else {
-        uint32_t mine[kCandidates / 32], rank[kCandidates / 32];
-        rank_candidates<kCandidates / 32>(w.key, candidates, lane, mine, rank);
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(kCandidates) / 32; ++i) put(lane + 32 * i, mine[i], rank[i]);
-      }
+      if (candidates <= 32) rank_candidates<T, 1>(a, r, s, w.key, w.id, candidates, lane);
+      else if (candidates <= 64) rank_candidates<T, 2>(a, r, s, w.key, w.id, candidates, lane);
+      else if (candidates <= 96) rank_candidates<T, 3>(a, r, s, w.key, w.id, candidates, lane);
+      else if (candidates <= 128) rank_candidates<T, 4>(a, r, s, w.key, w.id, candidates, lane);
+      else rank_candidates<T, kCandidates / 32>(a, r, s, w.key, w.id, candidates, lane);
       __syncwarp();  // the list is free for the next row
     } else {
       __syncwarp();

@@ -35,6 +35,28 @@ __device__ __forceinline__ uint32_t order_of(float z) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// order_of for a number that is not NaN.
+__device__ __forceinline__ uint32_t order_of_number(float z) {
+  const int32_t b = __float_as_int(z + 0.0f);
+  return static_cast<uint32_t>(b ^ ((b >> 31) | static_cast<int32_t>(0x80000000u)));
+}
+
+// n += a > b and n += a >= b in two instructions (the compiler's own takes
+// four or five where many are added up).
+__device__ __forceinline__ void count_above(uint32_t &n, uint32_t a, uint32_t b) {
+  asm("{ .reg .pred p; setp.gt.u32 p, %1, %2; @p add.u32 %0, %0, 1; }" : "+r"(n) : "r"(a), "r"(b));
+}
+__device__ __forceinline__ void count_from(uint32_t &n, uint32_t a, uint32_t b) {
+  asm("{ .reg .pred p; setp.ge.u32 p, %1, %2; @p add.u32 %0, %0, 1; }" : "+r"(n) : "r"(a), "r"(b));
+}
+
+// bits |= bit where a >= b
+__device__ __forceinline__ void mark_from(uint32_t &bits, float a, float b, uint32_t bit) {
+  asm("{ .reg .pred p; setp.ge.f32 p, %1, %2; @p or.b32 %0, %0, %3; }"
+      : "+r"(bits)
+      : "f"(a), "f"(b), "r"(bit));
+}
+
 // Running softmax sums of one thread or row: largest logit m, s = sum of
 // 2^((z - m) c), optionally h = sum of 2^((z - m) c) (z - m) (entropy).
 // -inf adds nothing; NaN reaches s through its exponential.
@@ -322,12 +344,13 @@ __device__ __forceinline__ void write_elements(const T *z, T *dz, const Part &p,
 }
 
 // The same by vectors, BATCH of a thread's in flight, where logits and
-// gradient are aligned alike.  dz may be z: a thread reads what it writes.
-template <int THREADS, int BATCH, typename T, typename F>
-__device__ __forceinline__ void write_vectors(const T *z, T *dz, const Part &p, F f) {
+// gradient are aligned alike: two(pair) for the vectors' logits, one(z) for
+// the others.  dz may be z: a thread reads what it writes.
+template <int THREADS, int BATCH, typename T, typename F, typename G>
+__device__ __forceinline__ void write_vectors(const T *z, T *dz, const Part &p, F two, G one) {
   constexpr uint32_t E = Vec<T>::kElems;
   if ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u)
-    return write_elements<THREADS>(z, dz, p, f);
+    return write_elements<THREADS>(z, dz, p, one);
   const uint4 *vec = reinterpret_cast<const uint4 *>(z + p.head);
   uint4 *out = reinterpret_cast<uint4 *>(dz + p.head);
   for (uint32_t at = p.begin; at < p.end; at += THREADS * BATCH) {
@@ -341,16 +364,16 @@ __device__ __forceinline__ void write_vectors(const T *z, T *dz, const Part &p, 
     for (int u = 0; u < BATCH; ++u) {
       const uint32_t i = at + u * THREADS + threadIdx.x;
       if (i >= p.end) continue;
-      float x[E];
-      Vec<T>::unpack(r[u], x);
+      Pair x[E / 2];
+      Vec<T>::pairs(r[u], x);
 #pragma unroll
-      for (uint32_t e = 0; e < E; ++e) x[e] = f(x[e]);
-      out[i] = Vec<T>::pack(x);
+      for (uint32_t e = 0; e < E / 2; ++e) x[e] = two(x[e]);
+      out[i] = Vec<T>::pack_pairs(x);
     }
   }
   if (threadIdx.x < p.loose) {
     const uint32_t j = loose_at(p, threadIdx.x);
-    dz[j] = from_float<T>(f(to_float(z[j])));
+    dz[j] = from_float<T>(one(to_float(z[j])));
   }
 }
 
@@ -395,6 +418,47 @@ __device__ __forceinline__ void add_term(Pow2Sums &a, float z, float c) {
   if (ENTROPY) a.h = fmaf(e, x, a.h);
 }
 
+// Adds the terms of B vectors (shift a.n at their largest logit or above).
+// With ENTROPY a masked logit's 0 times -inf shows as NaN in h: such a batch
+// is summed again with x held above -1e4, rather than every x being held
+// (1 of 8 instructions per pair of logits).
+template <bool ENTROPY, typename T, int B>
+__device__ __forceinline__ void add_batch(Pow2Sums &a, const uint4 (&r)[B], float c) {
+  constexpr int E = Vec<T>::kElems;
+  const Pair c2 = pair(c, c), n2 = pair(-a.n, -a.n);
+  Pair s = pair(a.s, 0.0f), h = pair(0.0f, 0.0f);
+#pragma unroll
+  for (int u = 0; u < B; ++u) {
+    Pair z[E / 2];
+    Vec<T>::pairs(r[u], z);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      const Pair x = fma2(z[e], c2, n2), p = ex2_pair(x);
+      s = add2(s, p);
+      if (ENTROPY) h = fma2(p, x, h);
+    }
+  }
+  const float2 f = halves(s), g = halves(h);
+  if (ENTROPY) {
+    float sum = g.x + g.y;
+    if (sum != sum) {
+      sum = 0.0f;
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        float z[E];
+        Vec<T>::unpack(r[u], z);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float x = max_nan(fmaf(z[e], c, -a.n), -1e4f);
+          sum = fmaf(ex2_approx(x), x, sum);
+        }
+      }
+    }
+    a.h += sum;
+  }
+  a.s = f.x + f.y;
+}
+
 // The warp's sums, in every lane.
 template <bool ENTROPY>
 __device__ __forceinline__ void warp_join(Pow2Sums &a) {
@@ -437,16 +501,27 @@ inline unsigned short_grid(uint32_t rows, size_t smem) {
   return ctas < most ? ctas : most;
 }
 
+// f(i, v) for the vectors v = l + 32 i of a lane; rows that fill all NV have
+// a loop without conditions.
+template <int NV, typename F>
+__device__ __forceinline__ void for_vectors(uint32_t end, uint32_t lane, F f) {
+  if (end == NV * 32) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) f(i, i * 32 + lane);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * 32 + lane < end) f(i, i * 32 + lane);
+  }
+}
+
 template <typename T, int NV>
 __device__ __forceinline__ void stage_row(const T *z, const Part &p, uint32_t lane, uint4 *buffer) {
   const uint4 *vec = reinterpret_cast<const uint4 *>(z + p.head);
   const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(buffer));
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t j = i * 32 + lane;
-    if (j < p.end)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + j * 16), "l"(vec + j) : "memory");
-  }
+  for_vectors<NV>(p.end, lane, [&](int, uint32_t j) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + j * 16), "l"(vec + j) : "memory");
+  });
 }
 // The staged row is in shared memory, for every lane.
 __device__ __forceinline__ void await_row() {
@@ -461,17 +536,22 @@ __device__ __forceinline__ void write_row(T *dz, const Part &p, uint32_t lane, c
                                           float loose, F two, G one) {
   constexpr int E = Vec<T>::kElems;
   const bool aligned = aligned16(dz + p.head);
-#pragma unroll 4
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t j = i * 32 + lane;
-    if (j >= p.end) break;
-    Pair x[E / 2];
+  const auto values = [&](uint32_t j, Pair (&x)[E / 2]) {
     Vec<T>::pairs(buffer[j], x);
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) x[e] = two(x[e]);
-    if (aligned) {
-      reinterpret_cast<uint4 *>(dz + p.head)[j] = Vec<T>::pack_pairs(x);
-    } else {
+  };
+  if (aligned) {
+    uint4 *out = reinterpret_cast<uint4 *>(dz + p.head);
+    for_vectors<NV>(p.end, lane, [&](int, uint32_t j) {
+      Pair x[E / 2];
+      values(j, x);
+      out[j] = Vec<T>::pack_pairs(x);
+    });
+  } else {
+    for (uint32_t j = lane; j < p.end; j += 32) {
+      Pair x[E / 2];
+      values(j, x);
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) {
         const float2 y = halves(x[e]);
