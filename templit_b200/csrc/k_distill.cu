@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(kThreads, GRAD ? 4 : 5) distill_kernel(const D
       largest = fmaxf(largest, most);
       move_to<false>(v, fmaxf(v.n, shift_of(most, a.c)));
       if (DUAL) move_to<false>(v1, fmaxf(v1.n, shift_of(most, kLog2e)));
-      add_batch<false, T>(v, q, a.c);
-      if (DUAL) add_batch<false, T>(v1, q, kLog2e);
+      add_terms<false, false, T>(v, q, a.c);
+      if (DUAL) add_terms<false, false, T>(v1, q, kLog2e);
     }
     if (tid < p.loose) {
       const uint32_t j = loose_at(p, tid);

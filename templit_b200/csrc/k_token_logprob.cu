@@ -52,7 +52,7 @@ dim3 gradient_grid(uint32_t rows, uint32_t vecs) {
 
 uint32_t cluster_parts(uint32_t rows, uint32_t vecs) {
   uint32_t parts = 1;
-  while (parts < kMaxCluster && static_cast<uint64_t>(rows) * parts <= kNumSMs && vecs / parts > 2 * 256)
+  while (parts < kMaxCluster && static_cast<uint64_t>(rows) * parts <= kNumSMs / 2 && vecs / parts > 4 * 256)
     parts *= 2;
   return parts;
 }
@@ -60,18 +60,21 @@ uint32_t cluster_parts(uint32_t rows, uint32_t vecs) {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kGroups = 256;       // of threads of a row that have a maximum each
 constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;          // vectors of a thread in flight
-constexpr uint32_t kSegments = 32; // most segments that have their own maximum
-constexpr uint32_t kList = 1024;   // candidates, and segments that hold some
+constexpr uint32_t kSegments = 16; // most segments that have their own maximum
+constexpr uint32_t kList = 512;    // candidates, and vectors and segments that hold some
 
 struct ScoreShared {
   Sums scratch[kWarps];
   Pow2Sums sums[kMaxCluster * kWarps];
   float largest[kMaxCluster * kWarps];
-  alignas(16) float group[kThreads];  // maxima of the row's 256 groups of threads
-  uint32_t entries, candidates, least, count[kWarps];
-  uint32_t entry[kList];
+  float group[kGroups];  // maxima of the row's groups of threads
+  uint32_t entries, hits, candidates, least, count[kWarps];
+  uint32_t entry[kList];  // segments with candidates
+  uint32_t at[kList];     // vectors with candidates: where they are
+  uint4 hit[kList];       // and what they hold
   alignas(16) uint64_t candidate[kList];
 };
 
@@ -148,8 +151,8 @@ __device__ __noinline__ void careful_top(const T *z, uint32_t vocab, uint32_t to
 // `top` others reach, so the alternatives are among the logits from there
 // on, and only segments whose maximum reaches it are looked at again; their
 // ranks among one another order the few candidates.
-template <typename T, bool ENTROPY, bool TOP, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, 5) score_kernel(const ScoreArgs a) {
+template <typename T, bool ENTROPY, bool TOP, bool CLUSTER, bool ONCE>
+__global__ void __launch_bounds__(kThreads, CLUSTER || ONCE ? 3 : 5) score_kernel(const ScoreArgs a) {
   extern __shared__ float segment[];  // [segments][kThreads] maxima (TOP)
   __shared__ ScoreShared sh;
   constexpr uint32_t E = Vec<T>::kElems;
@@ -161,12 +164,12 @@ __global__ void __launch_bounds__(kThreads, 5) score_kernel(const ScoreArgs a) {
     if (CLUSTER) cluster.sync();
     else __syncthreads();
   };
-  if (CLUSTER) cluster.sync();  // every CTA runs before its memory is written to
+  if (CLUSTER) cluster.barrier_arrive();  // this CTA runs: its memory may be written to
   pdl_enter();
   for (size_t row = blockIdx.x / parts; row < a.rows; row += gridDim.x / parts) {
     const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
     const Part p = part_of(z, a.vocab, part, parts);
-    if (TOP && tid == 0) sh.entries = sh.candidates = 0;
+    if (TOP && tid == 0) sh.entries = sh.hits = sh.candidates = 0;
     uint32_t t = TL_NO_TOKEN;
     float zt = 0.0f;
     if (tid == 32 && part == 0 && a.targets) {
@@ -177,23 +180,29 @@ __global__ void __launch_bounds__(kThreads, 5) score_kernel(const ScoreArgs a) {
     Pow2Sums v = {-kFar, 0.0f, 0.0f};
     float largest = -INFINITY, in_segment = -INFINITY;
     uint32_t batch = 0;
-    for (uint32_t at = p.begin; at < p.end; at += kThreads * kBatch, ++batch) {
-      uint4 r[kBatch];
+    bool masked = false;
+    uint4 q[kBatch];
+    const auto add = [&](uint32_t at) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const uint32_t i = at + u * kThreads + tid;
-        r[u] = i < p.end ? vec[i] : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+        q[u] = i < p.end ? vec[i] : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
       }
-      float most = Vec<T>::largest(r[0]);
+      float most = Vec<T>::largest(q[0]);
 #pragma unroll
-      for (int u = 1; u < kBatch; ++u) most = fmaxf(most, Vec<T>::largest(r[u]));
+      for (int u = 1; u < kBatch; ++u) most = fmaxf(most, Vec<T>::largest(q[u]));
       largest = fmaxf(largest, most);
-      if (TOP) {
+      if (TOP && !ONCE) {
         in_segment = batch & ((1u << a.segment_shift) - 1) ? fmaxf(in_segment, most) : most;
         segment[(batch >> a.segment_shift) * kThreads + tid] = in_segment;
       }
       move_to<ENTROPY>(v, fmaxf(v.n, shift_of(most, a.c)));
-      add_batch<ENTROPY, T>(v, r, a.c);
+      add_batch<ENTROPY, T>(v, q, a.c, masked);
+    };
+    if (ONCE) {
+      add(p.begin);
+    } else {
+      for (uint32_t at = p.begin; at < p.end; at += kThreads * kBatch, ++batch) add(at);
     }
     float loose = -INFINITY;
     if (tid < p.loose) {
@@ -203,18 +212,20 @@ __global__ void __launch_bounds__(kThreads, 5) score_kernel(const ScoreArgs a) {
       add_term<ENTROPY>(v, loose, a.c);
     }
     // join the row's sums in every CTA of it
+    if (CLUSTER && row == blockIdx.x / parts) cluster.barrier_wait();
     warp_join<ENTROPY>(v);
     const float warp_largest = warp_max(largest);
     float group = largest;
-    if (TOP && CLUSTER)
-      for (uint32_t o = 1; o < parts; o <<= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
+    const uint32_t lanes = kThreads * parts / kGroups;  // of a group
+    if (TOP && (CLUSTER || kThreads > kGroups))
+      for (uint32_t o = 1; o < lanes; o <<= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
     for (uint32_t c = 0; c < parts; ++c) {
       ScoreShared *to = CLUSTER ? cluster.map_shared_rank(&sh, c) : &sh;
       if (lane == 0) {
         to->sums[part * kWarps + warp] = v;
         to->largest[part * kWarps + warp] = warp_largest;
       }
-      if (TOP && tid % parts == 0) to->group[(part * kThreads + tid) / parts] = group;
+      if (TOP && tid % lanes == 0) to->group[(part * kThreads + tid) / lanes] = group;
     }
     everyone();
     v = {-kFar, 0.0f, 0.0f};
@@ -257,9 +268,9 @@ __global__ void __launch_bounds__(kThreads, 5) score_kernel(const ScoreArgs a) {
         // a value that `top` to a few more of the 256 maxima reach, bisected
         // between the least and the largest of them (with no more than a
         // value a lane asked for, between the lanes' largest)
-        uint32_t key[kThreads / 32], lo = 0xffffffffu, hi = 0;
+        uint32_t key[kGroups / 32], lo = 0xffffffffu, hi = 0;
 #pragma unroll
-        for (int i = 0; i < kThreads / 32; ++i) {
+        for (int i = 0; i < kGroups / 32; ++i) {
           key[i] = order_of_number(sh.group[i * 32 + lane]);
           lo = min(lo, key[i]);
           hi = max(hi, key[i]);
@@ -270,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 5) score_kernel(const ScoreArgs a) {
           const uint32_t mid = lo + (hi - lo) / 2;
           uint32_t n = 0;
 #pragma unroll
-          for (int i = 0; i < kThreads / 32; ++i) count_from(n, key[i], mid);
+          for (int i = 0; i < kGroups / 32; ++i) count_from(n, key[i], mid);
           n = __reduce_add_sync(0xffffffffu, n);
           if (n >= a.top) lo = mid;
           else hi = mid;
@@ -286,39 +297,54 @@ __global__ void __launch_bounds__(kThreads, 5) score_kernel(const ScoreArgs a) {
         const uint32_t i = atomicAdd(&first->candidates, 1u);
         if (i < kList) first->candidate[i] = key_of(x, id);
       };
-      if (largest >= from) {
-        const uint32_t segments = (batch + (1u << a.segment_shift) - 1) >> a.segment_shift;
-#pragma unroll 4
-        for (uint32_t s = 0; s < segments; ++s)
-          if (segment[s * kThreads + tid] >= from) {
-            const uint32_t i = atomicAdd(&sh.entries, 1u);
-            if (i < kList) sh.entry[i] = s * kThreads + tid;
+      // vectors with candidates go to shared memory: code for one logit does
+      // for all (unrolled, it is the instruction cache that a short call
+      // waits for)
+      const auto keep = [&](const uint4 &r4, uint32_t at) {
+        const uint32_t i = atomicAdd(&sh.hits, 1u);
+        if (i < kList) sh.hit[i] = r4, sh.at[i] = p.head + at * E;
+      };
+      if constexpr (ONCE) {
+        if (largest >= from) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const uint32_t i = p.begin + u * kThreads + tid;
+            if (i < p.end && Vec<T>::largest(q[u]) >= from) keep(q[u], i);
           }
-        if (tid < p.loose && loose >= from) candidate(loose, loose_at(p, tid));
-      }
-      __syncthreads();
-      const uint32_t entries = sh.entries;
-      if (entries <= kList) {
+        }
+      } else {
+        if (largest >= from) {
+          const uint32_t segments = (batch + (1u << a.segment_shift) - 1) >> a.segment_shift;
+          for (uint32_t s = 0; s < segments; ++s)
+            if (segment[s * kThreads + tid] >= from) {
+              const uint32_t i = atomicAdd(&sh.entries, 1u);
+              if (i < kList) sh.entry[i] = s * kThreads + tid;
+            }
+        }
+        __syncthreads();
+        const uint32_t entries = min(sh.entries, kList);
         const uint32_t each = kBatch << a.segment_shift;  // vectors of a segment
         for (uint32_t i = tid; i < entries * each; i += kThreads) {
           const uint32_t en = sh.entry[i / each];
           const uint32_t at = p.begin + (en / kThreads * each + i % each) * kThreads + en % kThreads;
           if (at >= p.end) continue;
           const uint4 r4 = vec[at];
-          if (!(Vec<T>::largest(r4) >= from)) continue;
-          float f[E];
-          Vec<T>::unpack(r4, f);
-#pragma unroll
-          for (uint32_t e = 0; e < E; ++e)
-            if (f[e] >= from) candidate(f[e], p.head + at * E + e);
+          if (Vec<T>::largest(r4) >= from) keep(r4, at);
         }
-      } else if (tid == 0) {
-        atomicAdd(&first->candidates, kList + 1);
       }
+      __syncthreads();
+      const uint32_t hits = sh.hits;
+      const bool over = hits > kList || (!ONCE && sh.entries > kList);
+      const uint32_t logits_in = over ? 0 : hits * E;
+      for (uint32_t i = tid; i < logits_in + p.loose; i += kThreads) {
+        const uint32_t j = i - logits_in;
+        const float x = i < logits_in ? to_float(reinterpret_cast<const T *>(sh.hit)[i]) : to_float(z[loose_at(p, j)]);
+        if (x >= from) candidate(x, i < logits_in ? sh.at[i / E] + i % E : loose_at(p, j));
+      }
+      if (over && tid == 0) atomicAdd(&first->candidates, kList + 1);
       everyone();
       if (part == 0) {
-        if (sh.candidates > kList || sh.candidates < a.top)
-          careful_top(z, a.vocab, a.top, least, sh);
+        if (sh.candidates > kList || sh.candidates < a.top) careful_top(z, a.vocab, a.top, least, sh);
         const uint32_t n = sh.candidates;
         for (uint32_t i = tid; i < n; i += kThreads) {
           const uint64_t key = sh.candidate[i];
@@ -332,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 5) score_kernel(const ScoreArgs a) {
         }
       }
     }
-    everyone();  // shared memory is free for the next row
+    if (row + gridDim.x / parts < a.rows) everyone();  // shared memory is free for the next row
   }
 }
 
@@ -379,21 +405,28 @@ __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArg
   }
 }
 
-template <typename T, bool ENTROPY, bool TOP>
-void launch_score_form(ScoreArgs &a, cudaStream_t s) {
-  const uint32_t vecs = a.vocab / Vec<T>::kElems;
-  const uint32_t parts = cluster_parts(a.rows, vecs);
+template <typename T, bool ENTROPY, bool TOP, bool CLUSTER>
+void launch_score_team(ScoreArgs &a, uint32_t parts, cudaStream_t s) {
+  const uint32_t vecs = a.vocab / Vec<T>::kElems, most = kNumSMs * 64u;
+  const uint32_t batches = ((vecs + parts - 1) / parts + kThreads * kBatch - 1) / (kThreads * kBatch);
   size_t smem = 0;
-  if (TOP) {
-    const uint32_t batches = ((vecs + parts - 1) / parts + kThreads * kBatch - 1) / (kThreads * kBatch);
+  if (TOP && batches > 1) {
     a.segment_shift = 0;
     while ((batches + (1u << a.segment_shift) - 1) >> a.segment_shift > kSegments) ++a.segment_shift;
     smem = ((batches + (1u << a.segment_shift) - 1) >> a.segment_shift) * kThreads * sizeof(float);
   }
-  const uint32_t most = kNumSMs * 64u;
-  const unsigned teams = a.rows < most ? a.rows : most;
-  if (parts == 1) launch_pdl(score_kernel<T, ENTROPY, TOP, false>, teams, kThreads, smem, s, a);
-  else launch_pdl_cluster(score_kernel<T, ENTROPY, TOP, true>, teams * parts, kThreads, smem, s, parts, a);
+  const auto kernel = TOP && batches <= 1 ? score_kernel<T, ENTROPY, TOP, CLUSTER, TOP>
+                                          : score_kernel<T, ENTROPY, TOP, CLUSTER, false>;
+  const unsigned grid = (a.rows < most ? a.rows : most) * parts;
+  if (CLUSTER) launch_pdl_cluster(kernel, grid, kThreads, smem, s, parts, a);
+  else launch_pdl(kernel, grid, kThreads, smem, s, a);
+}
+
+template <typename T, bool ENTROPY, bool TOP>
+void launch_score_form(ScoreArgs &a, cudaStream_t s) {
+  const uint32_t parts = cluster_parts(a.rows, a.vocab / Vec<T>::kElems);
+  if (parts > 1) launch_score_team<T, ENTROPY, TOP, true>(a, parts, s);
+  else launch_score_team<T, ENTROPY, TOP, false>(a, 1, s);
 }
 
 template <typename T> void launch_score(ScoreArgs &a, cudaStream_t s) {

@@ -419,11 +419,11 @@ __device__ __forceinline__ void add_term(Pow2Sums &a, float z, float c) {
 }
 
 // Adds the terms of B vectors (shift a.n at their largest logit or above).
-// With ENTROPY a masked logit's 0 times -inf shows as NaN in h: such a batch
-// is summed again with x held above -1e4, rather than every x being held
-// (1 of 8 instructions per pair of logits).
-template <bool ENTROPY, typename T, int B>
-__device__ __forceinline__ void add_batch(Pow2Sums &a, const uint4 (&r)[B], float c) {
+// With ENTROPY a masked logit's 0 times -inf shows as NaN in h: from the
+// first batch of a warp that has one on (`masked`), x is held above -1e4;
+// rows without masks are spared that instruction, one of 8 per pair.
+template <bool ENTROPY, bool HOLD, typename T, int B>
+__device__ __forceinline__ float add_terms(Pow2Sums &a, const uint4 (&r)[B], float c) {
   constexpr int E = Vec<T>::kElems;
   const Pair c2 = pair(c, c), n2 = pair(-a.n, -a.n);
   Pair s = pair(a.s, 0.0f), h = pair(0.0f, 0.0f);
@@ -433,30 +433,36 @@ __device__ __forceinline__ void add_batch(Pow2Sums &a, const uint4 (&r)[B], floa
     Vec<T>::pairs(r[u], z);
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) {
-      const Pair x = fma2(z[e], c2, n2), p = ex2_pair(x);
+      Pair x = fma2(z[e], c2, n2);
+      if (HOLD) {
+        const float2 f = halves(x);
+        x = pair(max_nan(f.x, -1e4f), max_nan(f.y, -1e4f));
+      }
+      const Pair p = ex2_pair(x);
       s = add2(s, p);
       if (ENTROPY) h = fma2(p, x, h);
     }
   }
   const float2 f = halves(s), g = halves(h);
-  if (ENTROPY) {
-    float sum = g.x + g.y;
-    if (sum != sum) {
-      sum = 0.0f;
-#pragma unroll
-      for (int u = 0; u < B; ++u) {
-        float z[E];
-        Vec<T>::unpack(r[u], z);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float x = max_nan(fmaf(z[e], c, -a.n), -1e4f);
-          sum = fmaf(ex2_approx(x), x, sum);
-        }
-      }
-    }
-    a.h += sum;
-  }
   a.s = f.x + f.y;
+  return g.x + g.y;
+}
+template <bool ENTROPY, typename T, int B>
+__device__ __forceinline__ void add_batch(Pow2Sums &a, const uint4 (&r)[B], float c, bool &masked) {
+  if (!ENTROPY) {
+    add_terms<false, false, T>(a, r, c);
+    return;
+  }
+  if (!masked) {
+    const float s = a.s, h = add_terms<true, false, T>(a, r, c);
+    masked = __any_sync(0xffffffffu, h != h);
+    if (!masked) {
+      a.h += h;
+      return;
+    }
+    a.s = s;
+  }
+  a.h += add_terms<true, true, T>(a, r, c);
 }
 
 // The warp's sums, in every lane.
@@ -574,7 +580,10 @@ int check_gradient(const char *who, const void *logits, uint64_t row_stride, voi
                    int32_t type, uint32_t rows, uint32_t vocab, uint64_t &d_row_stride);
 
 // CTAs of 256 (a cluster) that share a row: more than one where the rows
-// alone leave SMs idle and each still has two vectors a thread.
+// would leave half of the SMs idle and one CTA would have more than four
+// vectors a thread.  A cluster costs about 2.5 us over a CTA (64 x 8192
+// bf16, 20 alternatives: 6.6 us in clusters of 2, 4.3 us without; 8 x
+// 50001: 6.8 and 8.6 us; 128 x 50001: 10.0 and 8.8 us).
 constexpr uint32_t kMaxCluster = 8;
 uint32_t cluster_parts(uint32_t rows, uint32_t vecs);
 // Grid of a gradient without a reduction, CTAs of 256: rows x parts, more
