@@ -10,27 +10,35 @@ namespace token {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;  // vectors of a thread in flight
+// The gradient's second pass finds a row in L2 only as far as L2 holds the
+// rows that all CTAs have under way (a little under half of its 126 MB, next
+// to the gradients).  Above kL2Again bytes of them the pass goes backwards
+// and lets go of what it touches; above kL2Wide CTAs of twice the threads
+// have half as many rows under way.  Measured, bf16, 256 forwards, 256
+// backwards, 512 backwards: 12000 x 32768 (39 MB under way) 336, 346, 454
+// us; 10000 x 40000 (47 MB) 346, 341, 453; 8192 x 65536 (78 MB) 495, 440,
+// 486; 4096 x 128000 (151 MB) 496, 461, 437.
+constexpr size_t kL2Again = 44 << 20, kL2Wide = 110 << 20;
 // The gradient of one row's part.  Thread k < top has slot k: id
 // (TL_NO_TOKEN if empty or in another part), its p and its logit, read
 // before anything is written (dlogits may be logits); `target_here` has the
 // target's logit zt in the thread that writes it.  The slots and the target
 // are written a second time.
-template <typename T, bool DUAL>
-__device__ __forceinline__ void gradient_part(const DistillArgs &a, size_t row, const Part &part,
+template <int THREADS, bool AGAIN, bool DUAL, typename T>
+__device__ __forceinline__ void gradient_part(const DistillArgs &a, size_t row, const T *z,
+                                              const Part &part,
                                               const RowStats &r, uint32_t id, float p, float zk,
                                               uint32_t t, bool target_here, float zt) {
-  const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
   T *dz = static_cast<T *>(a.dlogits) + row * a.d_row_stride;
   const DistillGradient g = distill_gradient<DUAL>(a, r, t, a.row_scale ? a.row_scale[row] : 1.0f);
   const auto fast = [&](float x) { return distill_dz<DUAL>(g, a.c, x); };
   const Pair c2 = pair(a.c, a.c);
   const auto fast2 = [&](Pair x) { return distill_dz2<DUAL>(g, c2, x); };
   const auto careful = [&](float x) { return careful_distill_dz(g, r, a.c, x); };
-  if (g.none) write_elements<kThreads>(z, dz, part, [](float) { return 0.0f; });
-  else if (g.far) write_elements<kThreads>(z, dz, part, careful);
-  else write_vectors<kThreads, kBatch>(z, dz, part, fast2, fast);
+  if (g.none) write_elements<THREADS>(z, dz, part, [](float) { return 0.0f; });
+  else if (g.far) write_elements<THREADS>(z, dz, part, careful);
+  else write_vectors<THREADS, kBatch, AGAIN>(z, dz, part, fast2, fast);
   __syncthreads();
   if (g.none) return;
   if (target_here && g.ce != 0.0f) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) - g.ce);
@@ -51,7 +59,8 @@ __device__ __forceinline__ uint32_t read_target(const DistillArgs &a, size_t row
   return TL_NO_TOKEN;
 }
 
-struct DistillShared {
+template <int THREADS> struct DistillShared {
+  static constexpr int kWarps = THREADS / 32;
   Sums scratch[kWarps];
   Pow2Sums sums[kMaxCluster * kWarps], sums1[kMaxCluster * kWarps];
   float largest[kMaxCluster * kWarps];
@@ -64,18 +73,18 @@ struct DistillShared {
 
 // The sums outside the slots by add_logit, for rows that Pow2Sums cannot
 // hold.
-template <typename T, bool TAIL>
+template <int THREADS, bool TAIL, typename T>
 __device__ __noinline__ Outside careful_outside(const T *z, uint32_t vocab, float c, bool target,
                                                 const uint32_t *marks, uint32_t first, Sums *scratch) {
   Sums v = empty_sums(), v1 = empty_sums();
-  for (uint32_t j = threadIdx.x; j < vocab; j += kThreads) {
+  for (uint32_t j = threadIdx.x; j < vocab; j += THREADS) {
     if (TAIL && marks[(j + first) / 32] >> ((j + first) % 32) & 1u) continue;
     const float x = to_float(z[j]);
     add_logit(v, x, c);
     if (target) add_logit(v1, x, kLog2e);
   }
-  v = block_merge<kWarps>(v, c, scratch);
-  v1 = block_merge<kWarps>(v1, kLog2e, scratch);
+  v = block_merge<THREADS / 32>(v, c, scratch);
+  v1 = block_merge<THREADS / 32>(v1, kLog2e, scratch);
   return {v.m, v.s, v1.s};
 }
 
@@ -85,10 +94,11 @@ __device__ __noinline__ Outside careful_outside(const T *z, uint32_t vocab, floa
 // GRAD a second pass (out of L2: the CTA's part of the row is the last
 // thing it read) writes the gradient.  DUAL: the target's term has sums of
 // its own, at temperature 1.
-template <typename T, bool TAIL, bool DUAL, bool GRAD, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, GRAD ? 4 : 5) distill_kernel(const DistillArgs a) {
+template <typename T, int THREADS, bool TAIL, bool DUAL, bool GRAD, bool AGAIN, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, THREADS > kThreads ? 2 : GRAD ? 4 : 5) distill_kernel(const DistillArgs a) {
   extern __shared__ uint32_t marks[];
-  __shared__ DistillShared sh;
+  __shared__ DistillShared<THREADS> sh;
+  constexpr uint32_t kWarps = THREADS / 32;
   constexpr uint32_t E = Vec<T>::kElems;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -99,7 +109,7 @@ __global__ void __launch_bounds__(kThreads, GRAD ? 4 : 5) distill_kernel(const D
     else __syncthreads();
   };
   if (TAIL)
-    for (uint32_t w = tid; w < (a.vocab + 2 * E + 31) / 32; w += kThreads) marks[w] = 0;
+    for (uint32_t w = tid; w < (a.vocab + 2 * E + 31) / 32; w += THREADS) marks[w] = 0;
   everyone();  // every CTA of the cluster runs; the marks are clear
   pdl_enter();
   for (size_t row = blockIdx.x / parts; row < a.rows; row += gridDim.x / parts) {
@@ -120,17 +130,17 @@ __global__ void __launch_bounds__(kThreads, GRAD ? 4 : 5) distill_kernel(const D
     const uint4 *vec = reinterpret_cast<const uint4 *>(z + p.head);
     Pow2Sums v = {-kFar, 0.0f, 0.0f}, v1 = v;
     float largest = -INFINITY;
-    for (uint32_t at = p.begin; at < p.end; at += kThreads * kBatch) {
+    for (uint32_t at = p.begin; at < p.end; at += THREADS * kBatch) {
       uint4 q[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const uint32_t j = at + i * kThreads + tid;
+        const uint32_t j = at + i * THREADS + tid;
         q[i] = j < p.end ? vec[j] : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
       }
       if (TAIL) {
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-          const uint32_t j = at + i * kThreads + tid;
+          const uint32_t j = at + i * THREADS + tid;
           const uint32_t m = j < p.end ? vector_marks<T>(marks, j) : 0;
           if (m) Vec<T>::drop(q[i], m);
         }
@@ -167,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, GRAD ? 4 : 5) distill_kernel(const D
     largest = warp_max(largest);
     if (lane == 0)
       for (uint32_t c = 0; c < parts; ++c) {
-        DistillShared *to = CLUSTER ? cluster.map_shared_rank(&sh, c) : &sh;
+        DistillShared<THREADS> *to = CLUSTER ? cluster.map_shared_rank(&sh, c) : &sh;
         to->sums[part * kWarps + warp] = v;
         if (DUAL) to->sums1[part * kWarps + warp] = v1;
         to->largest[part * kWarps + warp] = largest;
@@ -178,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, GRAD ? 4 : 5) distill_kernel(const D
     m = warp_max(m);
     Outside o = {m, 0.0f, 0.0f};
     const bool far = far_out(m, a.c) || far_out(m, kLog2e);
-    if (far) o = careful_outside<T, TAIL>(z, a.vocab, a.c, target, marks, first, sh.scratch);
+    if (far) o = careful_outside<THREADS, TAIL>(z, a.vocab, a.c, target, marks, first, sh.scratch);
     if (warp == 0) {
       if (!far) {
         const float n = shift_of(m, a.c), n1 = shift_of(m, kLog2e);
@@ -215,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, GRAD ? 4 : 5) distill_kernel(const D
       const RowStats r = sh.r;
       const float pk = id != TL_NO_TOKEN ? expf(u - r.h) * r.b : 0.0f;
       const bool here = id != TL_NO_TOKEN && holds<T>(p, id);
-      gradient_part<T, DUAL>(a, row, p, r, here ? id : TL_NO_TOKEN, pk, zk, t,
+      gradient_part<THREADS, AGAIN, DUAL>(a, row, z, p, r, here ? id : TL_NO_TOKEN, pk, zk, t,
                              target && tid == 0 && holds<T>(p, t), zt);
     }
     everyone();  // shared memory is free for the next row
@@ -240,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const Distil
     const bool here = t != TL_NO_TOKEN && threadIdx.x == 0 && holds<T>(p, t);
     const float zt = here ? to_float(z[t]) : 0.0f;
     __syncthreads();  // every slot's logit is read
-    gradient_part<T, DUAL>(a, row, p, r, id, pk, zk, t, here, zt);
+    gradient_part<kThreads, false, DUAL>(a, row, z, p, r, id, pk, zk, t, here, zt);
     __syncthreads();
   }
 }
@@ -297,23 +307,34 @@ int with_status(const char *who, DistillArgs &a) {
   return a.status ? TL_OK : fail(TL_ERR_CUDA, std::string(who) + ": no status word");
 }
 
-template <typename T, bool TAIL, bool DUAL, bool GRAD>
-int launch_form(const char *who, const DistillArgs &a, cudaStream_t s) {
-  const uint32_t vecs = a.vocab / Vec<T>::kElems;
-  const uint32_t parts = cluster_parts(a.rows, vecs), most = kNumSMs * 64u;
+template <typename T, int THREADS, bool TAIL, bool DUAL, bool GRAD, bool AGAIN, bool CLUSTER>
+int launch_team(const char *who, const DistillArgs &a, uint32_t parts, cudaStream_t s) {
+  const uint32_t most = kNumSMs * 64u;
   const size_t smem = TAIL ? (static_cast<size_t>(a.vocab) + 2 * Vec<T>::kElems + 31) / 32 * 4 : 0;
-  const unsigned teams = a.rows < most ? a.rows : most;
-  const auto kernel = parts == 1 ? distill_kernel<T, TAIL, DUAL, GRAD, false>
-                                 : distill_kernel<T, TAIL, DUAL, GRAD, true>;
+  const unsigned grid = (a.rows < most ? a.rows : most) * parts;
+  const auto kernel = distill_kernel<T, THREADS, TAIL, DUAL, GRAD, AGAIN, CLUSTER>;
   if (smem > 40 * 1024) {
     if (int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  static_cast<int>(smem)),
                             who))
       return rc;
   }
-  if (parts == 1) launch_pdl(kernel, teams, kThreads, smem, s, a);
-  else launch_pdl_cluster(kernel, teams * parts, kThreads, smem, s, parts, a);
+  if (CLUSTER) launch_pdl_cluster(kernel, grid, THREADS, smem, s, parts, a);
+  else launch_pdl(kernel, grid, THREADS, smem, s, a);
   return launch_status(who);
+}
+
+template <typename T, bool TAIL, bool DUAL, bool GRAD>
+int launch_form(const char *who, const DistillArgs &a, cudaStream_t s) {
+  const uint32_t parts = cluster_parts(a.rows, a.vocab / Vec<T>::kElems);
+  if (parts > 1) return launch_team<T, kThreads, TAIL, DUAL, GRAD, false, true>(who, a, parts, s);
+  if constexpr (GRAD) {
+    const size_t rows = a.rows < 4 * kNumSMs ? a.rows : 4 * kNumSMs;
+    const size_t under_way = rows * a.vocab * sizeof(T);
+    if (under_way > kL2Wide) return launch_team<T, 2 * kThreads, TAIL, DUAL, true, true, false>(who, a, 1, s);
+    if (under_way > kL2Again) return launch_team<T, kThreads, TAIL, DUAL, true, true, false>(who, a, 1, s);
+  }
+  return launch_team<T, kThreads, TAIL, DUAL, GRAD, false, false>(who, a, 1, s);
 }
 
 template <typename T, bool TAIL, bool GRAD>

@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_backward_short_kerne
 
 template <typename K> void launch_short(K kernel, const DistillArgs &a, int nv, cudaStream_t s) {
   const size_t smem = static_cast<size_t>(nv) * 512 * kShortWarps;
-  launch_pdl(kernel, short_grid(a.rows, smem), kShortWarps * 32, smem, s, a);
+  launch_pdl(kernel, short_grid(a.rows, kShortWarps, smem), kShortWarps * 32, smem, s, a);
 }
 
 template <typename T, int NV, bool TAIL, bool GRAD> void launch(const DistillArgs &a, cudaStream_t s) {

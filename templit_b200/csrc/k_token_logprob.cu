@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kThreads) score_backward_kernel(const ScoreArg
     __syncthreads();  // dz may be z
     if (g.none) write_elements<kThreads>(z, dz, p, [](float) { return 0.0f; });
     else if (g.far) write_elements<kThreads>(z, dz, p, careful);
-    else write_vectors<kThreads, kBatch>(z, dz, p, fast2, fast);
+    else write_vectors<kThreads, kBatch, false>(z, dz, p, fast2, fast);
     __syncthreads();
     if (mine) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) + gl);
   }

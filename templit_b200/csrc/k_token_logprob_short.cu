@@ -6,6 +6,7 @@ namespace token {
 namespace {
 
 constexpr uint32_t kCandidates = 192;  // a multiple of 32
+constexpr uint32_t kHits = 192;        // a multiple of 8
 
 // A warp's shared memory: the row, and what picks the alternatives.
 template <int NV, bool TOP> struct WarpShared {
@@ -14,8 +15,9 @@ template <int NV, bool TOP> struct WarpShared {
 template <int NV> struct WarpShared<NV, true> {
   uint4 row[NV * 32];
   uint32_t key[kCandidates], id[kCandidates];  // 16-byte aligned
-  uint32_t candidates;
-  uint32_t unused[3];  // warps' parts stay 16-byte aligned
+  uint32_t hits, candidates;
+  uint32_t unused[2];  // warps' parts stay 16-byte aligned
+  uint16_t hit[kHits];  // vectors with candidates
 };
 
 // A candidate's key, larger for what ranks first.  Of 16-bit logits it holds
@@ -172,17 +174,17 @@ __device__ __forceinline__ void sum_row(const uint4 *row, uint32_t end, uint32_t
   if (ENTROPY) v.h = warp_sum(b.x + b.y);
 }
 
-// Alternatives: 128 groups of vectors (or every vector, for more than 64)
+// Alternatives: 128 groups of vectors (or every vector, for more than 32)
 // give a threshold that at least `top` logits reach; the candidates in the
 // vectors that reach it are ranked among one another.
 template <typename T, int NV, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kShortWarps * 32) score_short_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(kScoreWarps * 32) score_short_kernel(const ScoreArgs a) {
   extern __shared__ uint4 shared[];
   constexpr int E = Vec<T>::kElems;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   WarpShared<NV, TOP> &w = reinterpret_cast<WarpShared<NV, TOP> *>(shared)[warp];
-  const size_t stride = static_cast<size_t>(gridDim.x) * kShortWarps;
-  size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp;
+  const size_t stride = static_cast<size_t>(gridDim.x) * kScoreWarps;
+  size_t row = static_cast<size_t>(blockIdx.x) * kScoreWarps + warp;
   pdl_enter();
   const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
   Part p{};
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_short_kernel(const Sco
     }
     if constexpr (TOP) {
       uint32_t least;
-      if (NV > 4 && a.top > 64) {
+      if (NV > 4 && a.top > 32) {
         uint32_t key[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) key[i] = order_of_number(most[i]);
@@ -259,29 +261,31 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_short_kernel(const Sco
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         mark_from(hits, most[i], from, 1u << i);
-      if (lane == 0) w.candidates = 0;
+      if (lane == 0) w.hits = w.candidates = 0;
       __syncwarp();
-      const auto put = [&](uint32_t i, float x, uint32_t id) {
-        if (i < kCandidates) w.key[i] = list_key<T>(x, id), w.id[i] = id;
-      };
-      if (lane < p.loose && loose >= from) put(atomicAdd(&w.candidates, 1u), loose, loose_at(p, lane));
       while (hits) {
         const uint32_t at = (__ffs(hits) - 1) * 32 + lane;
         hits &= hits - 1;
         if (at >= p.end) break;  // -inf in place of vectors that a row lacks
-        float f[E];
-        Vec<T>::unpack(w.row[at], f);
-        uint32_t n = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) n += f[e] >= from;
-        uint32_t i = atomicAdd(&w.candidates, n);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (f[e] >= from) put(i++, f[e], p.head + at * E + e);
+        const uint32_t i = atomicAdd(&w.hits, 1u);
+        if (i < kHits) w.hit[i] = at;
       }
+      const auto candidate = [&](float x, uint32_t id) {
+        const uint32_t i = atomicAdd(&w.candidates, 1u);
+        if (i < kCandidates) w.key[i] = list_key<T>(x, id), w.id[i] = id;
+      };
+      if (lane < p.loose && loose >= from) candidate(loose, loose_at(p, lane));
+      __syncwarp();
+      const uint32_t vectors = w.hits;
+      if (vectors <= kHits)
+        for (uint32_t i = lane; i < vectors * E; i += 32) {
+          const uint32_t j = w.hit[i / E] * E + i % E;
+          const float x = to_float(reinterpret_cast<const T *>(w.row)[j]);
+          if (x >= from) candidate(x, p.head + j);
+        }
       __syncwarp();
       uint32_t candidates = w.candidates;
-      if (candidates > kCandidates || candidates < a.top) {
+      if (vectors > kHits || candidates > kCandidates || candidates < a.top) {
         careful_warp_top(z, a.vocab, a.top, least, w.key, w.id);
         candidates = a.top;
       }
@@ -350,28 +354,27 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_backward_short_kernel(
   }
 }
 
-// Launches a kernel whose warps need `warp_bytes` of shared memory each.
-template <typename K> void launch_short(K kernel, const ScoreArgs &a, size_t warp_bytes, cudaStream_t s) {
-  const size_t smem = warp_bytes * kShortWarps;
-  if (smem > 48 * 1024)  // a failure shows in the launch's status
-    (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  launch_pdl(kernel, short_grid(a.rows, smem), kShortWarps * 32, smem, s, a);
+// Launches a kernel of CTAs of W warps that need `warp_bytes` of shared
+// memory each (40 KB at most).
+template <int W, typename K> void launch_short(K kernel, const ScoreArgs &a, size_t warp_bytes, cudaStream_t s) {
+  const size_t smem = warp_bytes * W;
+  launch_pdl(kernel, short_grid(a.rows, W, smem), W * 32, smem, s, a);
 }
 
 template <typename T, int NV> void launch(const ScoreArgs &a, cudaStream_t s) {
   constexpr size_t with = sizeof(WarpShared<NV, true>), without = sizeof(WarpShared<NV, false>);
   if (a.entropy) {
-    if (a.top) launch_short(score_short_kernel<T, NV, true, true>, a, with, s);
-    else launch_short(score_short_kernel<T, NV, true, false>, a, without, s);
+    if (a.top) launch_short<kScoreWarps>(score_short_kernel<T, NV, true, true>, a, with, s);
+    else launch_short<kScoreWarps>(score_short_kernel<T, NV, true, false>, a, without, s);
   } else {
-    if (a.top) launch_short(score_short_kernel<T, NV, false, true>, a, with, s);
-    else launch_short(score_short_kernel<T, NV, false, false>, a, without, s);
+    if (a.top) launch_short<kScoreWarps>(score_short_kernel<T, NV, false, true>, a, with, s);
+    else launch_short<kScoreWarps>(score_short_kernel<T, NV, false, false>, a, without, s);
   }
 }
 
 template <typename T, int NV> void launch_backward(const ScoreArgs &a, cudaStream_t s) {
-  if (a.d_entropy) launch_short(score_backward_short_kernel<T, NV, true>, a, NV * 512, s);
-  else launch_short(score_backward_short_kernel<T, NV, false>, a, NV * 512, s);
+  if (a.d_entropy) launch_short<kShortWarps>(score_backward_short_kernel<T, NV, true>, a, NV * 512, s);
+  else launch_short<kShortWarps>(score_backward_short_kernel<T, NV, false>, a, NV * 512, s);
 }
 
 }  // namespace

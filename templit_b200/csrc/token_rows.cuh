@@ -345,20 +345,24 @@ __device__ __forceinline__ void write_elements(const T *z, T *dz, const Part &p,
 
 // The same by vectors, BATCH of a thread's in flight, where logits and
 // gradient are aligned alike: two(pair) for the vectors' logits, one(z) for
-// the others.  dz may be z: a thread reads what it writes.
-template <int THREADS, int BATCH, typename T, typename F, typename G>
+// the others.  dz may be z: a thread reads what it writes.  AGAIN: the CTA
+// has just read the row, and L2 does not hold the rows of all CTAs; the
+// last batches come first, and neither they nor the gradient need to stay.
+template <int THREADS, int BATCH, bool AGAIN, typename T, typename F, typename G>
 __device__ __forceinline__ void write_vectors(const T *z, T *dz, const Part &p, F two, G one) {
-  constexpr uint32_t E = Vec<T>::kElems;
+  constexpr uint32_t E = Vec<T>::kElems, kStep = THREADS * BATCH;
   if ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u)
     return write_elements<THREADS>(z, dz, p, one);
   const uint4 *vec = reinterpret_cast<const uint4 *>(z + p.head);
   uint4 *out = reinterpret_cast<uint4 *>(dz + p.head);
-  for (uint32_t at = p.begin; at < p.end; at += THREADS * BATCH) {
+  const uint32_t batches = (p.end - p.begin + kStep - 1) / kStep;
+  for (uint32_t k = 0; k < batches; ++k) {
+    const uint32_t at = p.begin + (AGAIN ? batches - 1 - k : k) * kStep;
     uint4 r[BATCH];
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
       const uint32_t i = at + u * THREADS + threadIdx.x;
-      if (i < p.end) r[u] = vec[i];
+      if (i < p.end) r[u] = AGAIN ? __ldcs(vec + i) : vec[i];
     }
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
@@ -368,7 +372,8 @@ __device__ __forceinline__ void write_vectors(const T *z, T *dz, const Part &p, 
       Vec<T>::pairs(r[u], x);
 #pragma unroll
       for (uint32_t e = 0; e < E / 2; ++e) x[e] = two(x[e]);
-      out[i] = Vec<T>::pack_pairs(x);
+      if (AGAIN) __stcs(out + i, Vec<T>::pack_pairs(x));
+      else out[i] = Vec<T>::pack_pairs(x);
     }
   }
   if (threadIdx.x < p.loose) {
@@ -491,7 +496,8 @@ constexpr uint32_t kShortRows = 512;
 // warp finishes the last one; lane l works on vectors l + 32 i, i < NV.
 // Shared memory, not registers: 20 and more rows are in flight on an SM, and
 // single logits can be looked up and taken out.
-constexpr int kShortWarps = 4;  // warps (rows in flight) of a CTA
+constexpr int kShortWarps = 4;  // warps (rows in flight) of a CTA, 6 CTAs an SM
+constexpr int kScoreWarps = 3;  // for scoring: 7 CTAs an SM with the lists of alternatives, 9 without
 
 // Vectors of a lane for a row: 4, 16, or 0 where a row is too long.
 inline uint32_t short_vectors(uint32_t vocab, size_t type_bytes) {
@@ -499,10 +505,10 @@ inline uint32_t short_vectors(uint32_t vocab, size_t type_bytes) {
   return vecs <= 4 * 32 ? 4 : vecs <= 16 * 32 ? 16 : 0;
 }
 // CTAs that fill the SMs, given the shared memory of one.
-inline unsigned short_grid(uint32_t rows, size_t smem) {
-  const uint32_t ctas = (rows + kShortWarps - 1) / kShortWarps;
-  size_t per_sm = (227 * 1024) / (smem + 1024);
-  if (per_sm > 8) per_sm = 8;
+inline unsigned short_grid(uint32_t rows, uint32_t warps, size_t smem) {
+  const uint32_t ctas = (rows + warps - 1) / warps;
+  size_t per_sm = (228 * 1024) / (smem + 1024);
+  if (per_sm > 9) per_sm = 9;
   const uint32_t most = kNumSMs * static_cast<uint32_t>(per_sm);
   return ctas < most ? ctas : most;
 }
