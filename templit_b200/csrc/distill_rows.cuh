@@ -23,6 +23,7 @@ struct DistillArgs {
   uint32_t rows, vocab, top;
   float c, inv_t;   // log2(e) / temperature, 1 / temperature
   float u_scale;    // 1 / teacher_temperature
+  float inv_t_low;  // 1 / temperature is inv_t + inv_t_low
   float kd, ce;
   const uint32_t *teacher_ids;
   const float *teacher;
@@ -125,6 +126,22 @@ struct Outside {
   float m, s, s1;
 };
 
+// log x = e ln 2 + l, |l| < 0.41: only l is rounded (3e-8).
+struct Log {
+  float e, l;
+};
+__device__ __forceinline__ Log log_parts(float x) {
+  if (!(x > 1e-37f && x < 1e37f)) return {0.0f, logf(x)};  // 0, inf, NaN
+  const int32_t b = __float_as_int(x), up = (b & 0x7fffff) >= 0x400000;
+  return {static_cast<float>((b >> 23) - 127 + up),
+          logf(__int_as_float((b & 0x7fffff) | (up ? 0x3f000000 : 0x3f800000)))};
+}
+// x + (e ln 2 + l), of which x and e ln 2 nearly cancel: ln 2 in two parts,
+// the first of 12 bits, whose multiples are exact.
+__device__ __forceinline__ float add_log(float x, float e, float l) {
+  return fmaf(e, 0.693115234375f, x) + fmaf(e, 3.1946184945309e-5f, l);
+}
+
 template <bool TAIL>
 __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotLane &l,
                                                const Outside &o, bool target, float zt, float &loss,
@@ -159,7 +176,8 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
   // the teacher's p.  Their sum is taken in 64 bits: what is left of 1 may
   // be far smaller than the sum
   r.h = 0.0f, r.b = slots ? 1.0f : 0.0f;
-  float p[kPerLane], log_sum = 0.0f, rest = 0.0f;
+  float p[kPerLane], rest = 0.0f;
+  Log log_sum = {0.0f, 0.0f};
   if (!TAIL) r.h = slots ? warp_max(u_max) : 0.0f;
   double sum = 0.0;
 #pragma unroll
@@ -174,9 +192,16 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
     rest = slots ? fmaxf(0.0f, static_cast<float>(1.0 - sum)) : 0.0f;
   } else if (slots) {
     r.b = static_cast<float>(1.0 / sum);
-    log_sum = logf(static_cast<float>(sum));
+    log_sum = log_parts(static_cast<float>(sum));
   }
-  const float log_s = logf(r.s);
+  // The divergence is a small difference of logarithms of size 10, whose
+  // roundings alone would be 1e-6 of a divergence of 0.1: u - x, x = (z - m)
+  // / tau with its rounding, cancels against log s up to what is left.
+  const Log log_s = log_parts(r.s);
+  const auto scaled_less = [&](float u, float z) {  // u - (z - r.m) / tau
+    const float d = z - r.m, x = d * a.inv_t;
+    return (u - x) - fmaf(d, a.inv_t, -x) - d * a.inv_t_low;
+  };
   kl = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
@@ -185,9 +210,10 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
     if (p[i] != p[i]) {
       kl = p[i];
     } else if (l.slot[i] && p[i] > 0.0f) {
-      // a row of -inf has q = 0 everywhere
-      const float log_q = r.s == 0.0f ? -INFINITY : (l.z[i] - r.m) * a.inv_t - log_s;
-      kl += p[i] * ((l.u[i] - r.h) - log_sum - log_q);
+      // a row of -inf has q = 0 everywhere, as has a logit of -inf
+      const bool some = r.s != 0.0f && l.z[i] != -INFINITY;
+      kl += p[i] * (some ? add_log(scaled_less(l.u[i] - r.h, l.z[i]), log_s.e - log_sum.e, log_s.l - log_sum.l)
+                         : INFINITY);
     }
   }
   kl = warp_sum(kl);
@@ -195,9 +221,12 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
     r.g = o.m == -INFINITY ? 0.0f : o.m;
     r.a = 0.0f;
     if (o.m != -INFINITY) {
-      const float log_left = (o.m - r.m) * a.inv_t + logf(o.s) - log_s;  // log q_r
-      if (rest > 0.0f) kl += rest * (logf(rest) - log_left);
-      r.a = slots ? (expf(log_left) - rest) / o.s : 0.0f;
+      const Log log_o = log_parts(o.s), log_r = log_parts(rest);
+      // log rest - log q_r, q_r = o.s e^((o.m - m) / tau) / s
+      if (rest > 0.0f)
+        kl += rest * add_log(scaled_less(0.0f, o.m), log_r.e - log_o.e + log_s.e, log_r.l - log_o.l + log_s.l);
+      const float left = o.s * rescale(o.m, r.m, a.c) / r.s;
+      r.a = slots ? (left - rest) / o.s : 0.0f;
     }
   } else {
     r.g = r.m == -INFINITY ? 0.0f : r.m;

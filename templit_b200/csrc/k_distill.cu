@@ -286,6 +286,7 @@ int distill_args(const char *who, const tl_distill_desc *d, DistillArgs &a) {
   a.top = d->top;
   a.c = static_cast<float>(1.4426950408889634 / d->temperature);
   a.inv_t = static_cast<float>(1.0 / d->temperature);
+  a.inv_t_low = static_cast<float>(1.0 / d->temperature - a.inv_t);
   a.u_scale = static_cast<float>(1.0 / d->teacher_temperature);
   a.kd = d->kd_weight;
   a.ce = d->ce_weight;
