@@ -25,7 +25,7 @@ constexpr size_t kL2Again = 44 << 20, kL2Wide = 110 << 20;
 // before anything is written (dlogits may be logits); `target_here` has the
 // target's logit zt in the thread that writes it.  The slots and the target
 // are written a second time.
-template <int THREADS, bool AGAIN, bool DUAL, typename T>
+template <int THREADS, bool AGAIN, bool WHOLE, bool DUAL, typename T>
 __device__ __forceinline__ void gradient_part(const DistillArgs &a, size_t row, const T *z,
                                               const Part &part,
                                               const RowStats &r, uint32_t id, float p, float zk,
@@ -38,7 +38,7 @@ __device__ __forceinline__ void gradient_part(const DistillArgs &a, size_t row, 
   const auto careful = [&](float x) { return careful_distill_dz(g, r, a.c, x); };
   if (g.none) write_elements<THREADS>(z, dz, part, [](float) { return 0.0f; });
   else if (g.far) write_elements<THREADS>(z, dz, part, careful);
-  else write_vectors<THREADS, kBatch, AGAIN>(z, dz, part, fast2, fast);
+  else write_vectors<THREADS, kBatch, AGAIN, WHOLE>(z, dz, part, fast2, fast);
   __syncthreads();
   if (g.none) return;
   if (target_here && g.ce != 0.0f) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) - g.ce);
@@ -130,19 +130,24 @@ __global__ void __launch_bounds__(THREADS, THREADS > kThreads ? 2 : GRAD ? 4 : 5
     const uint4 *vec = reinterpret_cast<const uint4 *>(z + p.head);
     Pow2Sums v = {-kFar, 0.0f, 0.0f}, v1 = v;
     float largest = -INFINITY;
-    for (uint32_t at = p.begin; at < p.end; at += THREADS * kBatch) {
+    const auto add = [&](auto full, uint32_t at) {  // full: no vector of the batch is past the end
       uint4 q[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const uint32_t j = at + i * THREADS + tid;
-        q[i] = j < p.end ? vec[j] : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
+        q[i] = full || j < p.end ? vec[j] : make_uint4(Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone, Vec<T>::kNone);
       }
       if (TAIL) {
+        uint32_t m[kBatch], some = 0;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
           const uint32_t j = at + i * THREADS + tid;
-          const uint32_t m = j < p.end ? vector_marks<T>(marks, j) : 0;
-          if (m) Vec<T>::drop(q[i], m);
+          m[i] = full || j < p.end ? vector_marks<T>(marks, j) : 0;
+          some |= m[i];
+        }
+        if (some) {
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) Vec<T>::drop(q[i], m[i]);
         }
       }
       float most = Vec<T>::largest(q[0]);
@@ -153,7 +158,10 @@ __global__ void __launch_bounds__(THREADS, THREADS > kThreads ? 2 : GRAD ? 4 : 5
       if (DUAL) move_to<false>(v1, fmaxf(v1.n, shift_of(most, kLog2e)));
       add_terms<false, false, T>(v, q, a.c);
       if (DUAL) add_terms<false, false, T>(v1, q, kLog2e);
-    }
+    };
+    uint32_t at = p.begin;
+    for (; at + THREADS * kBatch <= p.end; at += THREADS * kBatch) add(std::true_type{}, at);
+    if (at < p.end) add(std::false_type{}, at);
     if (tid < p.loose) {
       const uint32_t j = loose_at(p, tid);
       float x = to_float(z[j]);
@@ -225,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > kThreads ? 2 : GRAD ? 4 : 5
       const RowStats r = sh.r;
       const float pk = id != TL_NO_TOKEN ? expf(u - r.h) * r.b : 0.0f;
       const bool here = id != TL_NO_TOKEN && holds<T>(p, id);
-      gradient_part<THREADS, AGAIN, DUAL>(a, row, z, p, r, here ? id : TL_NO_TOKEN, pk, zk, t,
+      gradient_part<THREADS, AGAIN, true, DUAL>(a, row, z, p, r, here ? id : TL_NO_TOKEN, pk, zk, t,
                              target && tid == 0 && holds<T>(p, t), zt);
     }
     everyone();  // shared memory is free for the next row
@@ -250,7 +258,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const Distil
     const bool here = t != TL_NO_TOKEN && threadIdx.x == 0 && holds<T>(p, t);
     const float zt = here ? to_float(z[t]) : 0.0f;
     __syncthreads();  // every slot's logit is read
-    gradient_part<kThreads, false, DUAL>(a, row, z, p, r, id, pk, zk, t, here, zt);
+    gradient_part<kThreads, false, false, DUAL>(a, row, z, p, r, id, pk, zk, t, here, zt);
     __syncthreads();
   }
 }
