@@ -188,6 +188,8 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_backward_short_kerne
 
 template <typename K> void launch_short(K kernel, const DistillArgs &a, int nv, cudaStream_t s) {
   const size_t smem = static_cast<size_t>(nv) * 512 * kShortWarps;
+  if (smem > 48 * 1024)  // a failure shows in the launch's status
+    (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   launch_pdl(kernel, short_grid(a.rows, kShortWarps, smem), kShortWarps * 32, smem, s, a);
 }
 
@@ -210,18 +212,20 @@ template <typename T, int NV> void launch_backward(const DistillArgs &a, cudaStr
 }  // namespace
 
 bool distill_short(const DistillArgs &a, int32_t type, bool tail, bool gradient, cudaStream_t s) {
-  const uint32_t nv = short_vectors(a.vocab, type_size(type));
-  if (!nv || a.rows < kShortRows) return false;
-#define L(T) nv == 4 ? launch_forward<T, 4>(a, tail, gradient, s) : launch_forward<T, 16>(a, tail, gradient, s)
+  const uint32_t nv = short_vectors(a.rows, a.vocab, type_size(type));
+  if (!nv) return false;
+#define L(T)                                            \
+  nv == 4 ? launch_forward<T, 4>(a, tail, gradient, s)  \
+          : nv == 16 ? launch_forward<T, 16>(a, tail, gradient, s) : launch_forward<T, 32>(a, tail, gradient, s)
   TL_BY_TYPE(type, L)
 #undef L
   return true;
 }
 
 bool distill_backward_short(const DistillArgs &a, int32_t type, cudaStream_t s) {
-  const uint32_t nv = short_vectors(a.vocab, type_size(type));
-  if (!nv || a.rows < kShortRows) return false;
-#define L(T) nv == 4 ? launch_backward<T, 4>(a, s) : launch_backward<T, 16>(a, s)
+  const uint32_t nv = short_vectors(a.rows, a.vocab, type_size(type));
+  if (!nv) return false;
+#define L(T) nv == 4 ? launch_backward<T, 4>(a, s) : nv == 16 ? launch_backward<T, 16>(a, s) : launch_backward<T, 32>(a, s)
   TL_BY_TYPE(type, L)
 #undef L
   return true;

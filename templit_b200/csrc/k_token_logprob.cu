@@ -47,7 +47,7 @@ int check_gradient(const char *who, const void *logits, uint64_t row_stride, voi
 
 dim3 gradient_grid(uint32_t rows, uint32_t vecs) {
   uint32_t parts = 1;
-  while (static_cast<uint64_t>(rows) * parts < 4 * kNumSMs && vecs / parts > 4 * 256) ++parts;
+  while (static_cast<uint64_t>(rows) * parts < 16 * kNumSMs && vecs / parts > 8 * 256) ++parts;
   return dim3(rows < kNumSMs * 64u ? rows : kNumSMs * 64u, parts);
 }
 

@@ -5,8 +5,8 @@ namespace tl {
 namespace token {
 namespace {
 
-constexpr uint32_t kCandidates = 192;  // a multiple of 32
-constexpr uint32_t kHits = 192;        // a multiple of 8
+constexpr uint32_t kCandidates = 224;  // a multiple of 32
+constexpr uint32_t kHits = 224;        // a multiple of 8
 
 // A warp's shared memory: the row, and what picks the alternatives.
 template <int NV, bool TOP> struct WarpShared {
@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32) score_short_kernel(const Sco
       else if (candidates <= 64) rank_candidates<T, 2>(a, r, s, w.key, w.id, candidates, lane);
       else if (candidates <= 96) rank_candidates<T, 3>(a, r, s, w.key, w.id, candidates, lane);
       else if (candidates <= 128) rank_candidates<T, 4>(a, r, s, w.key, w.id, candidates, lane);
+      else if (candidates <= 192) rank_candidates<T, 6>(a, r, s, w.key, w.id, candidates, lane);
       else rank_candidates<T, kCandidates / 32>(a, r, s, w.key, w.id, candidates, lane);
       __syncwarp();  // the list is free for the next row
     } else {
@@ -359,9 +360,11 @@ __global__ void __launch_bounds__(kShortWarps * 32) score_backward_short_kernel(
 }
 
 // Launches a kernel of CTAs of W warps that need `warp_bytes` of shared
-// memory each (40 KB at most).
+// memory each.
 template <int W, typename K> void launch_short(K kernel, const ScoreArgs &a, size_t warp_bytes, cudaStream_t s) {
   const size_t smem = warp_bytes * W;
+  if (smem > 48 * 1024)  // a failure shows in the launch's status
+    (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   launch_pdl(kernel, short_grid(a.rows, W, smem), W * 32, smem, s, a);
 }
 
@@ -384,18 +387,18 @@ template <typename T, int NV> void launch_backward(const ScoreArgs &a, cudaStrea
 }  // namespace
 
 bool score_short(const ScoreArgs &a, int32_t type, cudaStream_t s) {
-  const uint32_t nv = short_vectors(a.vocab, type_size(type));
-  if (!nv || a.rows < kShortRows) return false;
-#define L(T) nv == 4 ? launch<T, 4>(a, s) : launch<T, 16>(a, s)
+  const uint32_t nv = short_vectors(a.rows, a.vocab, type_size(type));
+  if (!nv) return false;
+#define L(T) nv == 4 ? launch<T, 4>(a, s) : nv == 16 ? launch<T, 16>(a, s) : launch<T, 32>(a, s)
   TL_BY_TYPE(type, L)
 #undef L
   return true;
 }
 
 bool score_backward_short(const ScoreArgs &a, int32_t type, cudaStream_t s) {
-  const uint32_t nv = short_vectors(a.vocab, type_size(type));
-  if (!nv || a.rows < kShortRows) return false;
-#define L(T) nv == 4 ? launch_backward<T, 4>(a, s) : launch_backward<T, 16>(a, s)
+  const uint32_t nv = short_vectors(a.rows, a.vocab, type_size(type));
+  if (!nv) return false;
+#define L(T) nv == 4 ? launch_backward<T, 4>(a, s) : nv == 16 ? launch_backward<T, 16>(a, s) : launch_backward<T, 32>(a, s)
   TL_BY_TYPE(type, L)
 #undef L
   return true;

@@ -483,7 +483,10 @@ __device__ __forceinline__ float sum_at(float s, float n, float m, float c) {
 // Vocabulary 2048, a warp and a CTA per row: scoring with 32 alternatives,
 // 300 rows 6.6 and 4.8 us, 450 rows 6.9 and 7.2, 900 rows 7.4 and 10.8;
 // distillation loss and gradient 5.7 and 6.3, 5.8 and 6.9, 6.7 and 11.7.
-constexpr uint32_t kShortRows = 3 * kNumSMs;
+// Rows above 8 KB leave room for half the warps and need twice the rows
+// (8000 bf16, loss and gradient: 500 rows 10.9 and 8.3 us, 6000 rows 59 and
+// 85; scoring with 20 alternatives 9.9 and 8.3, 42 and 61).
+constexpr uint32_t kShortRows = 3 * kNumSMs, kShortRowsWide = 6 * kNumSMs;
 
 // ---- short rows: a warp holds a row in shared memory -----------------------
 // A row's vectors go to shared memory by cp.async, the next row's while the
@@ -493,15 +496,18 @@ constexpr uint32_t kShortRows = 3 * kNumSMs;
 constexpr int kShortWarps = 4;  // warps (rows in flight) of a CTA, 6 CTAs an SM
 constexpr int kScoreWarps = 3;  // for scoring: 7 CTAs an SM with the lists of alternatives, 9 without
 
-// Vectors of a lane for a row: 4, 16, or 0 where a row is too long.
-inline uint32_t short_vectors(uint32_t vocab, size_t type_bytes) {
+// Vectors of a lane for a row: 4, 16, 32, or 0 where rows are too long or too
+// few for a warp each.
+inline uint32_t short_vectors(uint32_t rows, uint32_t vocab, size_t type_bytes) {
   const uint64_t vecs = static_cast<uint64_t>(vocab) * type_bytes / 16;
-  return vecs <= 4 * 32 ? 4 : vecs <= 16 * 32 ? 16 : 0;
+  if (rows < (vecs <= 16 * 32 ? kShortRows : kShortRowsWide)) return 0;
+  return vecs <= 4 * 32 ? 4 : vecs <= 16 * 32 ? 16 : vecs <= 32 * 32 ? 32 : 0;
 }
-// CTAs that fill the SMs, given the shared memory of one.
+// CTAs that fill the SMs, given the shared memory of one (each takes 1 KB
+// more): a second, short wave would double the time.
 inline unsigned short_grid(uint32_t rows, uint32_t warps, size_t smem) {
   const uint32_t ctas = (rows + warps - 1) / warps;
-  size_t per_sm = (228 * 1024) / (smem + 1024);
+  size_t per_sm = (227 * 1024) / (smem + 1024);
   if (per_sm > 9) per_sm = 9;
   const uint32_t most = kNumSMs * static_cast<uint32_t>(per_sm);
   return ctas < most ? ctas : most;

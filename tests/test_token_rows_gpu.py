@@ -160,12 +160,13 @@ SIZES = [(1, 1), (3, 2), (2, 7), (5, 31), (4, 33), (3, 200), (7, 511), (5, 1023)
          (3, 4096), (4, 4100), (3, 6001), (3, 8192), (4, 8193), (2, 16411), (3, 32768), (3, 50001), (2, 65536),
          (2, 131072), (1, 200003), (1, 2048), (160, 40000)]
 # many rows, some of them short enough for a warp each
+SIZES += [(900, 2500), (900, 4093), (900, 8000)]
 SIZES += [(700, v) for v in (1, 6, 30, 129, 511, 512, 1000, 1026, 2047, 2048, 2050, 4095, 4096, 4099)]
 
 
 def repeat(many, *arrays):
     """The rows many times over: enough of them to take a warp each."""
-    out = [a if a is None or not many else np.concatenate([a] * (-(-700 // len(a)))) for a in arrays]
+    out = [a if a is None or not many else np.concatenate([a] * (-(-900 // len(a)))) for a in arrays]
     return out if len(out) > 1 else out[0]
 
 
@@ -202,7 +203,7 @@ def test_scoring_alternatives(dev, top, vocab):
 
 @pytest.mark.parametrize("type", list(TYPES))
 @pytest.mark.parametrize("vocab,many", [(130, False), (2048, False), (5000, False), (70001, False),
-                                        (130, True), (512, True), (2047, True), (2048, True)])
+                                        (130, True), (512, True), (2047, True), (2048, True), (4001, True)])
 def test_scoring_ties_and_order(dev, type, vocab, many):
     """Equal rows, two values, ascending, descending, all in one place, zeros
     of both signs: the lowest ids first among equals, and more candidates
@@ -226,7 +227,7 @@ def test_scoring_ties_and_order(dev, type, vocab, many):
 
 @pytest.mark.parametrize("type", list(TYPES))
 @pytest.mark.parametrize("vocab,many", [(129, False), (2048, False), (20001, False), (100000, False),
-                                        (129, True), (1030, True), (2048, True)])
+                                        (129, True), (1030, True), (2048, True), (4001, True)])
 def test_scoring_masks(dev, type, vocab, many):
     """Masked tokens: -inf, the type's lowest value, rows with one token, and
     with none."""
