@@ -32,12 +32,13 @@ __device__ __forceinline__ uint32_t read_target(const DistillArgs &a, size_t row
 }
 
 // The gradient of the row in shared memory; slots and target, read before,
-// are written a second time.
-template <typename T, int NV, bool DUAL>
+// are written a second time, after `next`: the buffer is free then.
+template <typename T, int NV, bool DUAL, typename F>
 __device__ __forceinline__ void gradient_row(const DistillArgs &a, size_t row, const T *z, const Part &p,
                                              uint32_t lane, const uint4 *buffer, float loose,
                                              const RowStats &r, const uint32_t (&id)[kPerLane],
-                                             const SlotLane &l, uint32_t t, float zt, float scale) {
+                                             const SlotLane &l, uint32_t t, float zt, float scale,
+                                             F next) {
   T *dz = static_cast<T *>(a.dlogits) + row * a.d_row_stride;
   const DistillGradient g = distill_gradient<DUAL>(a, r, t, scale);
   const Pair c2 = pair(a.c, a.c);
@@ -51,6 +52,7 @@ __device__ __forceinline__ void gradient_row(const DistillArgs &a, size_t row, c
       dz[j] = from_float<T>(g.none ? 0.0f : careful(to_float(z[j])));
   }
   __syncwarp();
+  next();
   if (g.none) return;
   if (lane == 0 && g.ce != 0.0f) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) - g.ce);
   __syncwarp();  // a target in a slot: the slot's value stands
@@ -66,7 +68,7 @@ __device__ __forceinline__ void gradient_row(const DistillArgs &a, size_t row, c
 
 // As distill_kernel in k_distill.cu, with the row read once.  The slots'
 // logits are taken out of the row in shared memory (TAIL): no marks.  12288 x
-// 2048 fp32, 32 slots, tail and targets: 24.5 us for the loss, 42.5 with the
+// 2048 fp32, 32 slots, tail and targets: 25 us for the loss, 41.5 with the
 // gradient (4.7 TB/s; four exponentials a logit keep their unit 57 % busy, the
 // rest is 24 warps an SM waiting for their own steps); in registers, 67 us.
 template <typename T, int NV, bool TAIL, bool DUAL, bool GRAD>
@@ -76,11 +78,17 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_short_kernel(const D
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4 *buffer = shared + warp * NV * 32;
   const size_t stride = static_cast<size_t>(gridDim.x) * kShortWarps;
+  const auto stage = [&](size_t row) {
+    if (row >= a.rows) return;
+    const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
+    stage_row<T, NV>(z, part_of(z, a.vocab, 0, 1), lane, buffer);
+  };
   pdl_enter();
-  for (size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp; row < a.rows; row += stride) {
+  size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp;
+  stage(row);
+  for (; row < a.rows; row += stride) {
     const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
     const Part p = part_of(z, a.vocab, 0, 1);
-    stage_row<T, NV>(z, p, lane, buffer);
     float loose = lane < p.loose ? to_float(z[loose_at(p, lane)]) : -INFINITY;
     uint32_t id[kPerLane];
     SlotLane l;
@@ -151,8 +159,13 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_short_kernel(const D
       if (a.kl) a.kl[row] = kl;
       if (a.stats) write_stats(a.stats + row * TL_DISTILL_STATS, r);
     }
-    if (GRAD) gradient_row<T, NV, DUAL>(a, row, z, p, lane, buffer, loose, r, id, l, t, zt, scale);
-    __syncwarp();  // the buffer is free
+    if constexpr (GRAD) {
+      gradient_row<T, NV, DUAL>(a, row, z, p, lane, buffer, loose, r, id, l, t, zt, scale,
+                                [&] { stage(row + stride); });
+    } else {
+      __syncwarp();  // the buffer is free
+      stage(row + stride);
+    }
   }
 }
 
@@ -162,11 +175,17 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_backward_short_kerne
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4 *buffer = shared + warp * NV * 32;
   const size_t stride = static_cast<size_t>(gridDim.x) * kShortWarps;
+  const auto stage = [&](size_t row) {
+    if (row >= a.rows) return;
+    const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
+    stage_row<T, NV>(z, part_of(z, a.vocab, 0, 1), lane, buffer);
+  };
   pdl_enter();
-  for (size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp; row < a.rows; row += stride) {
+  size_t row = static_cast<size_t>(blockIdx.x) * kShortWarps + warp;
+  stage(row);
+  for (; row < a.rows; row += stride) {
     const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
     const Part p = part_of(z, a.vocab, 0, 1);
-    stage_row<T, NV>(z, p, lane, buffer);
     const float loose = lane < p.loose ? to_float(z[loose_at(p, lane)]) : 0.0f;
     const float *st = a.stats + row * TL_DISTILL_STATS;
     const RowStats r = {st[0], st[1], st[2], st[3], st[4], st[5], st[6]};
@@ -181,8 +200,8 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_backward_short_kerne
     for (int i = 0; i < kPerLane; ++i)
       if (l.slot[i]) l.z[i] = logit_at(z, p, buffer, id[i]);
     __syncwarp();  // loose logits among them are read: dz may be z
-    gradient_row<T, NV, DUAL>(a, row, z, p, lane, buffer, loose, r, id, l, t, zt, scale);
-    __syncwarp();  // the buffer is free
+    gradient_row<T, NV, DUAL>(a, row, z, p, lane, buffer, loose, r, id, l, t, zt, scale,
+                              [&] { stage(row + stride); });
   }
 }
 
