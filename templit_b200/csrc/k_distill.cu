@@ -20,6 +20,7 @@ constexpr int kBatch = 4;  // vectors of a thread in flight
 // us; 10000 x 40000 (47 MB) 346, 341, 453; 8192 x 65536 (78 MB) 495, 440,
 // 486; 4096 x 128000 (151 MB) 496, 461, 437.
 constexpr size_t kL2Again = 44 << 20, kL2Wide = 110 << 20;
+
 // The gradient of one row's part.  Thread k < top has slot k: id
 // (TL_NO_TOKEN if empty or in another part), its p and its logit, read
 // before anything is written (dlogits may be logits); `target_here` has the
@@ -27,9 +28,9 @@ constexpr size_t kL2Again = 44 << 20, kL2Wide = 110 << 20;
 // are written a second time.
 template <int THREADS, bool AGAIN, bool WHOLE, bool DUAL, typename T>
 __device__ __forceinline__ void gradient_part(const DistillArgs &a, size_t row, const T *z,
-                                              const Part &part,
-                                              const RowStats &r, uint32_t id, float p, float zk,
-                                              uint32_t t, bool target_here, float zt) {
+                                              const Part &part, const RowStats &r, uint32_t id,
+                                              float p, float zk, uint32_t t, bool target_here,
+                                              float zt) {
   T *dz = static_cast<T *>(a.dlogits) + row * a.d_row_stride;
   const DistillGradient g = distill_gradient<DUAL>(a, r, t, a.row_scale ? a.row_scale[row] : 1.0f);
   const auto fast = [&](float x) { return distill_dz<DUAL>(g, a.c, x); };
@@ -67,7 +68,6 @@ template <int THREADS> struct DistillShared {
   bool slot[TL_TOKEN_MAX_TOP];
   float u[TL_TOKEN_MAX_TOP], z[TL_TOKEN_MAX_TOP];
   float zt;
-  uint32_t t;
   RowStats r;
 };
 
@@ -228,7 +228,9 @@ __global__ void __launch_bounds__(THREADS, THREADS > kThreads ? 2 : GRAD ? 4 : 5
         }
       }
     }
-    if (far) __syncthreads();  // the marks were read once more
+    // the marks were read once more, and by every CTA all of the row, which
+    // the gradient may overwrite
+    if (far) everyone();
     if (TAIL && id != TL_NO_TOKEN) marks[(id + first) / 32] = 0;
     if (GRAD) {
       __syncthreads();
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > kThreads ? 2 : GRAD ? 4 : 5
       const float pk = id != TL_NO_TOKEN ? expf(u - r.h) * r.b : 0.0f;
       const bool here = id != TL_NO_TOKEN && holds<T>(p, id);
       gradient_part<THREADS, AGAIN, true, DUAL>(a, row, z, p, r, here ? id : TL_NO_TOKEN, pk, zk, t,
-                             target && tid == 0 && holds<T>(p, t), zt);
+                                                target && tid == 0 && holds<T>(p, t), zt);
     }
     everyone();  // shared memory is free for the next row
   }

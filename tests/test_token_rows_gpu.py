@@ -588,6 +588,33 @@ def test_distillation_slots_and_masks(dev, tail, vocab, many):
     assert np.isfinite(both["grad"]).all() and not both["grad"][6].any()
 
 
+@pytest.mark.parametrize("rows,vocab", [(2, 50001), (5, 131072), (200, 5000), (900, 2048)])
+def test_rows_at_the_lowest_value(dev, rows, vocab):
+    """Rows whose every logit (outside a few) is fp32's lowest value, beyond
+    what sums in powers of two hold: in a cluster, a CTA and a warp per row,
+    the gradient beside the logits and in their place."""
+    rng = np.random.default_rng(21)
+    zh = np.full((rows, vocab), -3.4028234663852886e38)
+    zh[1::2, vocab // 3] = 2.0
+    ids = np.stack([rng.permutation(vocab)[:8] for _ in range(rows)]).astype(np.uint32)
+    teacher = np.log(np.tile([.3, .2, .1, .1, .05, .05, .02, .01], (rows, 1)))
+    targets = rng.integers(0, vocab, rows)
+    # (log q of a wiped-out token is -3e38, its KL beyond fp32: gradients only)
+    for tail in (False, True):
+        args = dict(tail=tail, targets=targets, ce=0.5, kd=0.7)
+        z = Rows(dev, zh)
+        want = ops.distill_gradient(z.host, ids, np.asarray(teacher, np.float32), **args)
+        grads = []
+        for out in (z.like(), z):
+            grads.append(distill(dev, z, ids, teacher, "tl_distill_train_rows", out=out, **args)["grad"])
+        np.testing.assert_array_equal(grads[0], grads[1])
+        near(grads[0], want, 1e-5 * np.abs(want) + 1e-6)
+    z = Rows(dev, zh)
+    check_score(z, score(dev, z, targets, 20), targets, 20, 1.0)
+    one = np.ones(rows, np.float32)
+    check_score_gradient(z, score_gradient(dev, z, targets, one, one), targets, one, one, 1.0)
+
+
 def test_distillation_every_token_in_a_slot(dev):
     rng = np.random.default_rng(14)
     for rows in (5, 700):
