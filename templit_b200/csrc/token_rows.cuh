@@ -386,8 +386,12 @@ __device__ __forceinline__ float max_nan(float x, float lo) {
 // shift, which would scale one thread's terms against another's), and sums
 // with different shifts join by exact factors.  h = sum of e x with x = z c
 // - n.  n never leaves +-kFar; a row whose largest logit does (all logits
-// at the type's lowest value, say) is summed by add_logit instead.
-constexpr float kFar = 1e30f;
+// masked by a finite value, or a very small temperature) is summed by
+// add_logit instead.  n is the rounded product: at the largest logit x is what
+// the rounding left, up to half a unit of the product's last place.  Within
+// 2^27 that is 4, and e at most 16; from 2^32 on it would be 128 and more, e
+// infinite, and its product with a joining factor of 0 a NaN.
+constexpr float kFar = 1 << 27;
 
 struct Pow2Sums {
   float n, s, h;
