@@ -319,7 +319,10 @@ int tl_token_logprob_backward_rows(const tl_token_logprob_desc *desc, void *stre
  *     tl_token_logprob_rows gives at this temperature), and the tokens
  *     outside the slots share the rest, p_r = max(0, 1 - sum_k p_k) against
  *     q_r = sum of their q: KL gains p_r (log p_r - log q_r) (dropped in a
- *     row where the student has no token outside the slots)
+ *     row where the student has no token outside the slots).  The masses
+ *     need not add up to 1 (values at a teacher temperature above 1, rows
+ *     with p_r dropped): the gradient is the derivative of this loss, P q_j
+ *     - p_j in a slot, (P - p_r / q_r) q_j outside, P the masses counted
  *   loss[r] = kd_weight KL + ce_weight (-log softmax(z)_t), t = targets[r]
  * A row without slots has no KL term, a row whose target is TL_NO_TOKEN (or
  * a call without targets) no second term.  1 <= top <= min(vocab,
@@ -345,9 +348,10 @@ typedef struct tl_distill_desc {
   float *kl;                   /* [rows], optional: the KL term, unweighted */
   /* [rows, TL_DISTILL_STATS], optional in the forward, read by the
    * backward: { m = max z, sum e^((z - m) / temperature), sum e^(z - m) (0
-   * without a second term), g, a, h, b, 0 } with the slots' p_k = b e^(u_k
-   * - h) and, outside the slots, dKL/dz_j = a e^((z_j - g) / temperature) /
-   * temperature */
+   * without a second term), g, a, h, b, P - 1 } with the slots' p_k = b
+   * e^(u_k - h) and, outside the slots, dKL/dz_j = a e^((z_j - g) /
+   * temperature) / temperature; P - 1 is 0 unless the masses do not add up
+   * to 1 */
   float *stats;
   const float *row_scale; /* [rows], optional: the gradient of loss (1)   */
   void *dlogits;          /* row r at dlogits + r * d_row_stride          */

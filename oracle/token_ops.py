@@ -129,11 +129,14 @@ def distill_gradient(z, ids, teacher, temperature=1.0, teacher_temperature=1.0, 
     lq = log_softmax(z, temperature)
     empty = np.isneginf(lq).all(-1)
     q = np.exp(lq)
-    g = np.where(some[:, None], q - p, 0.0)
+    total = p.sum(-1, keepdims=True)  # the masses that the loss counts: 1, or what a row has
     if tail:
         out = np.where(inside, -np.inf, lq)
         m = out.max(-1, keepdims=True)
         has = ~np.isneginf(m)
+        total = total + np.where(has, rest[:, None], 0.0)
+    g = np.where(some[:, None], total * q - p, 0.0)
+    if tail:
         e = np.exp(np.where(has, out - np.where(has, m, 0.0), -np.inf))
         share = e / np.where(has, e.sum(-1, keepdims=True), 1.0)  # q_j / q_r
         g -= rest[:, None] * share

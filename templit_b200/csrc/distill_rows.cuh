@@ -3,11 +3,14 @@
 //
 // With the student's q = softmax(z / tau) and the teacher's p over the slots
 // (and p_r over the tokens outside, TL_DISTILL_TAIL), the gradient of
-// KL(p || q) is (q_j - p_j) / tau in a slot and, outside the slots, q_j (1 -
-// p_r / q_r) / tau.  The second is evaluated as e^((z_j - g) / tau) a / tau
-// with g the largest logit outside the slots, s_r the sum there and a =
-// (q_r - p_r) / s_r: neither q_r nor q_j / q_r can leave the range of fp32,
-// however small the student's mass outside the slots is.
+// KL(p || q) is (P q_j - p_j) / tau in a slot and, outside the slots, q_j (P -
+// p_r / q_r) / tau, P the masses that the divergence counts: sum p_k + p_r, or
+// sum p_k where the student has no token outside.  P is 1 unless p_r was held
+// at 0 (slots of more than 1 together) or dropped.  The second is evaluated as
+// e^((z_j - g) / tau) a / tau with g the largest logit outside the slots, s_r
+// the sum there and a = (P q_r - p_r) / s_r: neither q_r nor q_j / q_r can
+// leave the range of fp32, however small the student's mass outside the slots
+// is.
 #pragma once
 
 #include "token_rows.cuh"
@@ -40,6 +43,7 @@ struct RowStats {
   float m, s, s1;  // largest logit, sums at the temperature and at 1
   float g, a;      // outside the slots
   float h, b;      // the slots' p
+  float e;         // P - 1
 };
 
 // Slot k of a row: its id and value, empty ones as TL_NO_TOKEN.
@@ -106,10 +110,11 @@ __device__ __forceinline__ float careful_distill_dz(const DistillGradient &g, co
   return g.coef1 == 0.0f ? d : fmaf(g.coef1, ex2_approx((z - r.m) * kLog2e), d);
 }
 
-// In a slot with the teacher's p and the student's logit z.
+// In a slot with the teacher's p and the student's logit z: P q - p.
 __device__ __forceinline__ float slot_dz(const DistillGradient &g, const RowStats &r, float c, float p,
                                          float z, bool target) {
-  const float d = g.kd * (ex2_approx((z - r.m) * c) / r.s - p);
+  const float q = ex2_approx((z - r.m) * c) / r.s;
+  const float d = g.kd * (fmaf(r.e, q, q) - p);
   return g.ce == 0.0f ? d : d + fmaf(g.coef1, ex2_approx((z - r.m) * kLog2e), target ? -g.ce : 0.0f);
 }
 
@@ -175,7 +180,7 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
   if (!target) r.s1 = 0.0f;
   // the teacher's p.  Their sum is taken in 64 bits: what is left of 1 may
   // be far smaller than the sum
-  r.h = 0.0f, r.b = slots ? 1.0f : 0.0f;
+  r.h = 0.0f, r.b = slots ? 1.0f : 0.0f, r.e = 0.0f;
   float p[kPerLane], rest = 0.0f;
   Log log_sum = {0.0f, 0.0f};
   if (!TAIL) r.h = slots ? warp_max(u_max) : 0.0f;
@@ -189,7 +194,10 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   if (TAIL) {
-    rest = slots ? fmaxf(0.0f, static_cast<float>(1.0 - sum)) : 0.0f;
+    const float left = slots ? static_cast<float>(1.0 - sum) : 0.0f;
+    rest = fmaxf(0.0f, left);
+    // P - 1, not P: of a P near 1 no bits are lost
+    r.e = left >= 0.0f && o.m != -INFINITY ? 0.0f : -left;
   } else if (slots) {
     r.b = static_cast<float>(1.0 / sum);
     log_sum = log_parts(static_cast<float>(sum));
@@ -226,7 +234,7 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
       if (rest > 0.0f)
         kl += rest * add_log(scaled_less(0.0f, o.m), log_r.e - log_o.e + log_s.e, log_r.l - log_o.l + log_s.l);
       const float left = o.s * rescale(o.m, r.m, a.c) / r.s;
-      r.a = slots ? (left - rest) / o.s : 0.0f;
+      r.a = slots ? (fmaf(r.e, left, left) - rest) / o.s : 0.0f;
     }
   } else {
     r.g = r.m == -INFINITY ? 0.0f : r.m;
@@ -251,7 +259,7 @@ template <typename T> __device__ __forceinline__ uint32_t vector_marks(const uin
 
 __device__ __forceinline__ void write_stats(float *st, const RowStats &r) {
   st[0] = r.m, st[1] = r.s, st[2] = r.s1, st[3] = r.g;
-  st[4] = r.a, st[5] = r.h, st[6] = r.b, st[7] = 0.0f;
+  st[4] = r.a, st[5] = r.h, st[6] = r.b, st[7] = r.e;
 }
 
 // Whether the target's term needs exponentials of its own.

@@ -37,14 +37,17 @@ __device__ __forceinline__ void gradient_part(const DistillArgs &a, size_t row, 
   const Pair c2 = pair(a.c, a.c);
   const auto fast2 = [&](Pair x) { return distill_dz2<DUAL>(g, c2, x); };
   const auto careful = [&](float x) { return careful_distill_dz(g, r, a.c, x); };
+  // before the pass over the row: fewer registers to keep through it
+  const float at_slot = id != TL_NO_TOKEN ? slot_dz(g, r, a.c, p, zk, id == t) : 0.0f;
+  const float at_target = target_here && g.ce != 0.0f ? (g.far ? careful(zt) : fast(zt)) - g.ce : 0.0f;
   if (g.none) write_elements<THREADS>(z, dz, part, [](float) { return 0.0f; });
   else if (g.far) write_elements<THREADS>(z, dz, part, careful);
   else write_vectors<THREADS, kBatch, AGAIN, WHOLE>(z, dz, part, fast2, fast);
   __syncthreads();
   if (g.none) return;
-  if (target_here && g.ce != 0.0f) dz[t] = from_float<T>((g.far ? careful(zt) : fast(zt)) - g.ce);
+  if (target_here && g.ce != 0.0f) dz[t] = from_float<T>(at_target);
   __syncthreads();  // a target in a slot: the slot's value stands
-  if (id != TL_NO_TOKEN) dz[id] = from_float<T>(slot_dz(g, r, a.c, p, zk, id == t));
+  if (id != TL_NO_TOKEN) dz[id] = from_float<T>(at_slot);
 }
 
 // Slot k of a row in thread k.
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(const Distil
     const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
     const Part p = part_of(z, a.vocab, blockIdx.y, gridDim.y);
     const float *st = a.stats + row * TL_DISTILL_STATS;
-    const RowStats r = {st[0], st[1], st[2], st[3], st[4], st[5], st[6]};
+    const RowStats r = {st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7]};
     uint32_t id;
     float u;
     read_slot(a, row, id, u);

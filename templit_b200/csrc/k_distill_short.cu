@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) distill_backward_short_kerne
     const Part p = part_of(z, a.vocab, 0, 1);
     const float loose = lane < p.loose ? to_float(z[loose_at(p, lane)]) : 0.0f;
     const float *st = a.stats + row * TL_DISTILL_STATS;
-    const RowStats r = {st[0], st[1], st[2], st[3], st[4], st[5], st[6]};
+    const RowStats r = {st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7]};
     uint32_t id[kPerLane];
     SlotLane l;
     read_slots(a, row, lane, id, l);
