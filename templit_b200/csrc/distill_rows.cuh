@@ -226,7 +226,9 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
   }
   kl = warp_sum(kl);
   if (TAIL) {
-    r.g = o.m == -INFINITY ? 0.0f : o.m;
+    // nothing outside: the target's term still needs a shift that follows
+    // the row (from 0, e^(-m) is infinite below -88)
+    r.g = o.m != -INFINITY ? o.m : r.m == -INFINITY ? 0.0f : r.m;
     r.a = 0.0f;
     if (o.m != -INFINITY) {
       const Log log_o = log_parts(o.s), log_r = log_parts(rest);
