@@ -147,6 +147,11 @@ __device__ __forceinline__ float add_log(float x, float e, float l) {
   return fmaf(e, 0.693115234375f, x) + fmaf(e, 3.1946184945309e-5f, l);
 }
 
+// The divergence is summed in units of 2^16, which changes no bit of it: one
+// beyond fp32 (masks of the type's lowest value) may have a weight that brings
+// the loss back.
+constexpr float kUnit = 65536.0f;
+
 template <bool TAIL>
 __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotLane &l,
                                                const Outside &o, bool target, float zt, float &loss,
@@ -206,9 +211,12 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
   // roundings alone would be 1e-6 of a divergence of 0.1: u - x, x = (z - m)
   // / tau with its rounding, cancels against log s up to what is left.
   const Log log_s = log_parts(r.s);
-  const auto scaled_less = [&](float u, float z) {  // u - (z - r.m) / tau
+  const auto term = [&](float p, float u, float z, float e, float l) {  // p (u - (z - r.m) / tau + e ln 2 + l) / kUnit
     const float d = z - r.m, x = d * a.inv_t;
-    return (u - x) - fmaf(d, a.inv_t, -x) - d * a.inv_t_low;
+    // beyond fp32 (such masks at a temperature below 1) nothing else counts
+    // (but a NaN), and p may be small enough for p times it to be a number
+    if (isinf(x)) return fmaf(p, l, (r.m / kUnit - z / kUnit) * p * a.inv_t);
+    return p * (add_log((u - x) - fmaf(d, a.inv_t, -x) - d * a.inv_t_low, e, l) * (1.0f / kUnit));
   };
   kl = 0.0f;
 #pragma unroll
@@ -220,8 +228,7 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
     } else if (l.slot[i] && p[i] > 0.0f) {
       // a row of -inf has q = 0 everywhere, as has a logit of -inf
       const bool some = r.s != 0.0f && l.z[i] != -INFINITY;
-      kl += p[i] * (some ? add_log(scaled_less(l.u[i] - r.h, l.z[i]), log_s.e - log_sum.e, log_s.l - log_sum.l)
-                         : INFINITY);
+      kl += some ? term(p[i], l.u[i] - r.h, l.z[i], log_s.e - log_sum.e, log_s.l - log_sum.l) : INFINITY;
     }
   }
   kl = warp_sum(kl);
@@ -234,7 +241,7 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
       const Log log_o = log_parts(o.s), log_r = log_parts(rest);
       // log rest - log q_r, q_r = o.s e^((o.m - m) / tau) / s
       if (rest > 0.0f)
-        kl += rest * add_log(scaled_less(0.0f, o.m), log_r.e - log_o.e + log_s.e, log_r.l - log_o.l + log_s.l);
+        kl += term(rest, 0.0f, o.m, log_r.e - log_o.e + log_s.e, log_r.l - log_o.l + log_s.l);
       const float left = o.s * rescale(o.m, r.m, a.c) / r.s;
       r.a = slots ? (fmaf(r.e, left, left) - rest) / o.s : 0.0f;
     }
@@ -242,7 +249,8 @@ __device__ __forceinline__ RowStats join_slots(const DistillArgs &a, const SlotL
     r.g = r.m == -INFINITY ? 0.0f : r.m;
     r.a = slots && r.s != 0.0f ? 1.0f / r.s : 0.0f;
   }
-  loss = a.kd == 0.0f ? 0.0f : a.kd * kl;  // a KL of +inf without weight
+  loss = a.kd == 0.0f ? 0.0f : a.kd * kl * kUnit;  // a KL of +inf without weight
+  kl *= kUnit;
   if (target) {
     const float log_q1 = r.s1 == 0.0f ? -INFINITY : (zt - r.m) - logf(r.s1);
     loss -= a.ce * log_q1;

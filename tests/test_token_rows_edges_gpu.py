@@ -5,7 +5,7 @@ import pytest
 
 from oracle import token_ops as ops
 from tests.helpers import Dev
-from tests.test_token_rows_gpu import Rows, all_three, distill, teacher_of
+from tests.test_token_rows_gpu import U, Rows, all_three, distill, near, teacher_of
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,38 @@ def test_nothing_outside_the_slots_far_from_zero(dev, rows, vocab, shift, tau):
         masked[np.arange(rows), np.where(targets < vocab, targets, 0)] = False
         for got in (two, both):
             assert not got["grad"][masked].any()
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", SHAPES)
+@pytest.mark.parametrize("tau", [0.25, 0.5, 0.7, 1.0, 2.0])
+@pytest.mark.parametrize("tail", [False, True])
+def test_losses_of_masks_at_the_lowest_value(dev, type, rows, vocab, tau, tail):
+    """A slot of probability p at the type's lowest value L: p (-L) / tau is
+    the divergence to a part in 10^37, beyond fp32 (+inf) or not; so is the
+    rest's where every token outside the slots is at L.  A term's error is
+    that of p, 8 u (1 + |log p|), and 8 u more."""
+    rng = np.random.default_rng(52)
+    low = {"f32": -3.4028234663852886e38, "bf16": -3.3895313892515355e38}[type]
+    tau = float(np.float32(tau))
+    ids = np.stack([rng.choice(vocab, 9, replace=False) for _ in range(rows)]).astype(np.uint32)
+    teacher = np.log(np.tile([.3, .2, .1, .1, .05, .05, .02, .01, 1e-35], (rows, 1))).astype(np.float32)
+    z = rng.standard_normal((rows, vocab))
+    for i in range(rows):
+        if i % 4 == 0:
+            z[i, ids[i, 8]] = low      # p = 1e-35: a divergence of some 1000
+        elif i % 4 == 1:
+            z[i, ids[i, 0]] = low      # p = 0.3
+        elif i % 4 == 2:
+            z[i, np.setdiff1d(np.arange(vocab), ids[i])] = low
+        else:
+            z[i] = low
+    z = Rows(dev, z, type)
+    want_loss, want_kl = ops.distill(z.host, ids, teacher, temperature=tau, tail=tail, kd=0.5)
+    with np.errstate(over="ignore"):
+        want_loss, want_kl = (w.astype(np.float32).astype(np.float64) for w in (want_loss, want_kl))
+    for name, out in (("tl_distill_rows", None), ("tl_distill_train_rows", z.like())):
+        got = distill(dev, z, ids, teacher, name, tau=tau, tail=tail, kd=0.5, out=out)
+        for k, want in (("kl", want_kl), ("loss", want_loss)):
+            tol = 8 * U * (2 + 81) * (20 + np.where(np.isfinite(want), np.abs(want), 0))
+            near(got[k], want, tol)
