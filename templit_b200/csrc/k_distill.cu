@@ -328,12 +328,15 @@ int with_status(const char *who, DistillArgs &a) {
 template <typename T, int THREADS, bool TAIL, bool DUAL, bool GRAD, bool AGAIN, bool CLUSTER>
 int launch_team(const char *who, const DistillArgs &a, uint32_t parts, cudaStream_t s) {
   const uint32_t most = kNumSMs * 64u;
-  const size_t smem = TAIL ? (static_cast<size_t>(a.vocab) + 2 * Vec<T>::kElems + 31) / 32 * 4 : 0;
+  const auto marks_bytes = [](size_t vocab) { return (vocab + 2 * Vec<T>::kElems + 31) / 32 * 4; };
+  const size_t smem = TAIL ? marks_bytes(a.vocab) : 0;
   const unsigned grid = (a.rows < most ? a.rows : most) * parts;
   const auto kernel = distill_kernel<T, THREADS, TAIL, DUAL, GRAD, AGAIN, CLUSTER>;
   if (smem > 40 * 1024) {
+    // the limit is the kernel's, not the call's: the same for every call, so
+    // that none lowers it between another thread's two steps
     if (int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(smem)),
+                                                 static_cast<int>(marks_bytes(TL_DISTILL_MAX_VOCAB))),
                             who))
       return rc;
   }

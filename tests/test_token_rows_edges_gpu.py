@@ -1,11 +1,15 @@
 """Token scoring and distillation at single edges of what the entry points
 accept, against the float64 oracle (oracle/token_ops.py)."""
+import ctypes
+import threading
+
 import numpy as np
 import pytest
 
 from oracle import token_ops as ops
+from templit_b200 import capi
 from tests.helpers import Dev
-from tests.test_token_rows_gpu import U, Rows, all_three, distill, near, teacher_of
+from tests.test_token_rows_gpu import U, Rows, all_three, base_desc, distill, f32, near, teacher_of, u32
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +79,40 @@ def test_losses_of_masks_at_the_lowest_value(dev, type, rows, vocab, tau, tail):
         for k, want in (("kl", want_kl), ("loss", want_loss)):
             tol = 8 * U * (2 + 81) * (20 + np.where(np.isfinite(want), np.abs(want), 0))
             near(got[k], want, tol)
+
+
+def test_vocabularies_on_two_host_threads(dev):
+    """Calls of two vocabularies that need different amounts of shared memory,
+    from two host threads on a stream each: none may fail or change another's
+    result."""
+    torch, rng = dev.torch, np.random.default_rng(53)
+    plans = []
+    for vocab in (1 << 20, 500000):
+        z = Rows(dev, rng.standard_normal((1, vocab)))
+        ids = rng.choice(vocab, 16, replace=False)[None].astype(np.uint32)
+        teacher = np.log(np.full((1, 16), 0.05)).astype(np.float32)
+        want = distill(dev, z, ids, teacher, tail=True)["loss"]
+        held = [z, u32(dev, ids), f32(dev, teacher), dev.empty((1,)), torch.cuda.Stream()]
+        d = base_desc(capi.TlDistillDesc, dev, z, 1.0)
+        d.teacher_temperature, d.tail, d.top, d.kd_weight = 1.0, 1, 16, 1.0
+        d.teacher_ids, d.teacher, d.loss = held[1].data_ptr(), held[2].data_ptr(), held[3].data_ptr()
+        plans.append((d, held, want))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(d, stream):
+        ref, raw = ctypes.byref(d), ctypes.c_void_p(stream.cuda_stream)
+        for _ in range(3000):
+            if dev.lib.tl_distill_rows(ref, raw) != capi.TL_OK:
+                failed.append(dev.lib.tl_last_error())
+                return
+
+    threads = [threading.Thread(target=work, args=(d, held[-1])) for d, held, _ in plans]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for d, held, want in plans:
+        np.testing.assert_array_equal(dev.host(held[3]), want)
