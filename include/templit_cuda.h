@@ -282,7 +282,7 @@ typedef struct tl_token_logprob_desc {
   uint64_t row_stride;
   uint32_t rows, vocab, top;
   int32_t type;      /* tl_float_type                                     */
-  float temperature; /* > 0, finite                                       */
+  float temperature; /* > 0, finite; from 4.3e-39 on (its reciprocal)     */
   uint32_t reserved;
   const uint32_t *targets; /* [rows]                                      */
   float *logprob;          /* [rows]                                      */
@@ -337,7 +337,7 @@ typedef struct tl_distill_desc {
   uint64_t row_stride;
   uint32_t rows, vocab, top;
   int32_t type; /* tl_float_type                                          */
-  float temperature, teacher_temperature; /* > 0, finite                  */
+  float temperature, teacher_temperature; /* > 0, finite; from 4.3e-39 on */
   float kd_weight, ce_weight;             /* finite                       */
   int32_t tail;                           /* tl_distill_tail              */
   uint32_t reserved;

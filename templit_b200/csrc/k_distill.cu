@@ -285,6 +285,8 @@ int distill_args(const char *who, const tl_distill_desc *d, DistillArgs &a) {
     return rc;
   if (!positive(d->teacher_temperature))
     return bad(who, "teacher temperature must be positive and finite");
+  if (1.0 / d->teacher_temperature > FLT_MAX)
+    return fail(TL_ERR_RANGE, std::string(who) + ": teacher temperature's reciprocal is beyond fp32");
   if (!std::isfinite(d->kd_weight) || !std::isfinite(d->ce_weight))
     return bad(who, "weights must be finite");
   if (d->tail != TL_DISTILL_RENORM && d->tail != TL_DISTILL_TAIL)

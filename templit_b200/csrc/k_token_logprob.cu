@@ -20,6 +20,8 @@ int check_rows(const char *who, const void *logits, int32_t type, uint32_t rows,
   if (vocab > 1u << 31) return fail(TL_ERR_RANGE, std::string(who) + ": more than 2^31 tokens");
   if (!(temperature > 0.0f) || std::isinf(temperature))
     return bad(who, "temperature must be positive and finite");
+  if (1.4426950408889634 / temperature > FLT_MAX)  // or every product with it is NaN
+    return fail(TL_ERR_RANGE, std::string(who) + ": temperature's reciprocal is beyond fp32");
   if (rows == 0) return TL_OK;
   if (row_stride == 0) row_stride = vocab;
   if (row_stride < vocab && rows > 1) return bad(who, "row stride below the row's length");
