@@ -9,7 +9,8 @@ import pytest
 from oracle import token_ops as ops
 from templit_b200 import capi
 from tests.helpers import Dev
-from tests.test_token_rows_gpu import U, Rows, all_three, base_desc, distill, f32, near, teacher_of, u32
+from tests.test_token_rows_gpu import (U, Rows, all_three, base_desc, distill, f32, ids_of,
+                                       near, score, teacher_of, u32)
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +117,51 @@ def test_vocabularies_on_two_host_threads(dev):
     assert not failed, failed
     for d, held, want in plans:
         np.testing.assert_array_equal(dev.host(held[3]), want)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab,offset", [(1 << 20, 0), ((1 << 20) - 3, 3)])
+def test_the_longest_vocabularies_of_the_tail(dev, type, vocab, offset):
+    """A bit per token up to TL_DISTILL_MAX_VOCAB, slots at both ends."""
+    rng = np.random.default_rng(54)
+    z = Rows(dev, rng.standard_normal((2, vocab)), type, offset=offset)
+    ids = np.stack([np.concatenate([[0, 1, vocab - 1, vocab - 2], 2 + rng.choice(vocab - 4, 60, replace=False)])
+                    for _ in range(2)]).astype(np.uint32)
+    teacher = np.log(rng.dirichlet(np.ones(64), 2) * 0.9).astype(np.float32)
+    all_three(dev, z, ids, teacher, np.array([1, 2], np.float32), tail=True, targets=np.array([vocab - 1, 77]), ce=0.5,
+              tau=2.0)
+
+
+def test_calls_on_two_streams_at_once(dev):
+    """Long calls that overlap on two streams give what each gives alone."""
+    torch, rng = dev.torch, np.random.default_rng(55)
+    jobs = []
+    for seed in range(2):
+        zt, ids, teacher = teacher_of(rng, 300, 30000, 32)
+        jobs.append((Rows(dev, zt + rng.standard_normal(zt.shape), "bf16"), ids, teacher, torch.cuda.Stream()))
+    args = dict(tail=True, targets=None, tau=2.0)
+    alone = [distill(dev, z, ids, teacher, "tl_distill_train_rows", out=z.like(), **args) for z, ids, teacher, _ in jobs]
+    alone_score = [score(dev, z, None, 30) for z, *_ in jobs]
+    descs = []
+    for z, ids, teacher, stream in jobs:
+        out, loss = z.like(), dev.empty((300,))
+        tops = [dev.empty((300, 30)), dev.empty((300, 30), torch.int32)]
+        held = [u32(dev, ids), f32(dev, teacher), out, loss, tops]
+        d = base_desc(capi.TlDistillDesc, dev, z, 2.0)
+        d.teacher_temperature, d.tail, d.top, d.kd_weight = 1.0, 1, 32, 1.0
+        d.teacher_ids, d.teacher, d.loss = held[0].data_ptr(), held[1].data_ptr(), loss.data_ptr()
+        d.dlogits, d.d_row_stride = out.ptr(), out.stride
+        s = base_desc(capi.TlTokenLogprobDesc, dev, z, 1.0)
+        s.top, s.top_logprob, s.top_ids = 30, tops[0].data_ptr(), tops[1].data_ptr()
+        descs.append((d, s, held, ctypes.c_void_p(stream.cuda_stream)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for d, s, _, raw in descs:
+            capi.check(dev.lib.tl_distill_train_rows(ctypes.byref(d), raw), dev.lib, "tl_distill_train_rows")
+            capi.check(dev.lib.tl_token_logprob_rows(ctypes.byref(s), raw), dev.lib, "tl_token_logprob_rows")
+    torch.cuda.synchronize()
+    for (_, _, held, _), one, tops in zip(descs, alone, alone_score):
+        np.testing.assert_array_equal(held[2].get(), one["grad"])
+        np.testing.assert_array_equal(dev.host(held[3]), one["loss"])
+        np.testing.assert_array_equal(dev.host(held[4][0]), tops["top_logprob"])
+        np.testing.assert_array_equal(ids_of(dev, held[4][1]), tops["top_ids"])
