@@ -252,9 +252,13 @@ int tl_xent_backward_rows(const float *logits, const uint32_t *targets,
  * fp16 or bf16, row r at logits + r * row_stride (elements; 0 = vocab), of
  * any alignment of the type's own; all sums, statistics and per-row results
  * are fp32, and a gradient has the logits' type, rounded once.  A logit of
- * -inf is a token that cannot occur (probability 0, gradient 0); a row of
- * nothing else has log probabilities -inf, entropy 0 and a zero gradient.
- * A NaN or +inf logit makes its row's statistics NaN.  The calls allocate
+ * -inf is a token that cannot occur: probability 0, and gradient 0 unless it
+ * is the given token or in a teacher's slot, whose own terms remain
+ * (d_logprob / temperature; -kd_weight p / temperature and -ce_weight); a row
+ * of nothing else has log probabilities -inf, entropy 0 and a zero gradient.
+ * Masks may be finite too, down to the type's lowest value.  A NaN or +inf
+ * logit makes its row's sums NaN and what follows from them (its statistics
+ * keep the largest of the numbers, or +inf).  The calls allocate
  * nothing, need no workspace, keep no state between calls and are
  * deterministic; calls on different streams may overlap.  vocab <= 2^31. */
 enum tl_float_type { TL_FLOAT32 = 0, TL_FLOAT16 = 1, TL_BFLOAT16 = 2 };

@@ -97,8 +97,9 @@ __device__ __noinline__ Outside careful_outside(const T *z, uint32_t vocab, floa
 // the slots to the sums, and with GRAD a second pass, out of L2 as far as it
 // holds the row (AGAIN), writes the gradient.  DUAL: the target's term has
 // sums of its own, at temperature 1.  4096 x 128000 bf16, 64 slots, tail: the
-// loss 185 us (5.7 TB/s; 173 for a few calls at full clock), with the
-// gradient 444 us (4.7 TB/s of one read and one write; DRAM moves 8 % more).
+// loss 188 us (5.6 TB/s; 173 for a few calls at full clock), with the
+// gradient 451 us (4.7 TB/s of one read and one write, 431 at full clock; DRAM
+// moves 8 % more).
 template <typename T, int THREADS, bool TAIL, bool DUAL, bool GRAD, bool AGAIN, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, THREADS > kThreads ? 2 : GRAD ? 4 : 5) distill_kernel(const DistillArgs a) {
   extern __shared__ uint32_t marks[];

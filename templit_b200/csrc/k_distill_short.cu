@@ -68,9 +68,10 @@ __device__ __forceinline__ void gradient_row(const DistillArgs &a, size_t row, c
 
 // As distill_kernel in k_distill.cu, with the row read once.  The slots'
 // logits are taken out of the row in shared memory (TAIL): no marks.  12288 x
-// 2048 fp32, 32 slots, tail and targets: 25 us for the loss, 41.5 with the
-// gradient (4.9 TB/s; four exponentials a logit keep their unit 57 % busy, the
-// rest is 24 warps an SM waiting for their own steps); in registers, 67 us.
+// 2048 fp32, 32 slots, tail and targets: 25 us for the loss, 42 to 44 with the
+// gradient (4.7 to 4.9 TB/s; four exponentials a logit keep their unit 57 %
+// busy, the rest is 24 warps an SM waiting for their own steps); in registers,
+// 67 us.
 template <typename T, int NV, bool TAIL, bool DUAL, bool GRAD>
 __global__ void __launch_bounds__(kShortWarps * 32) distill_short_kernel(const DistillArgs a) {
   extern __shared__ uint4 shared[];

@@ -154,7 +154,7 @@ __device__ __noinline__ void careful_top(const T *z, uint32_t vocab, uint32_t to
 // whose maximum reaches it are looked at again; their ranks among one
 // another order the few candidates.  The registers hold four vectors of a
 // thread and five CTAs share an SM: while one joins and ranks, the others
-// read.  4096 x 128000 bf16: 205 us with 20 alternatives (5.1 TB/s; at full
+// read.  4096 x 128000 bf16: 208 us with 20 alternatives (5.0 TB/s; at full
 // clock, for a few calls, 188, and 174 without the alternatives), bound by
 // the instructions of a logit (issue slots 66 %, exponentials 70 %, memory
 // 69 % busy).  A copy through a ring in shared memory, running ahead over the

@@ -489,8 +489,11 @@ __device__ __forceinline__ float sum_at(float s, float n, float m, float c) {
 // 300 rows 6.6 and 4.8 us, 450 rows 6.9 and 7.2, 900 rows 7.4 and 10.8;
 // distillation loss and gradient 5.7 and 6.3, 5.8 and 6.9, 6.7 and 11.7.
 // Rows above 8 KB leave room for half the warps and need twice the rows
-// (8000 bf16, loss and gradient: 500 rows 10.9 and 8.3 us, 6000 rows 59 and
-// 85; scoring with 20 alternatives 9.9 and 8.3, 42 and 61).
+// (8000 bf16: loss and gradient, 600 rows 13.0 and 14.7 us, 800 rows 13.5 and
+// 16.0, 1000 rows 14.3 and 17.1, 6000 rows 59 and 85; scoring with 20
+// alternatives 11.2 and 10.0, 11.7 and 10.9, 13.6 and 14.1, 42 and 61; the
+// gradient of scoring 8.3 and 7.2, 9.0 and 8.1, 9.8 and 11.2; distillation
+// loss 8.1 and 6.1, 8.5 and 9.5, 8.9 and 10.2).
 constexpr uint32_t kShortRows = 3 * kNumSMs, kShortRowsWide = 6 * kNumSMs;
 
 // ---- short rows: a warp holds a row in shared memory -----------------------
@@ -598,7 +601,14 @@ int check_gradient(const char *who, const void *logits, uint64_t row_stride, voi
 constexpr uint32_t kMaxCluster = 8;
 uint32_t cluster_parts(uint32_t rows, uint32_t vecs);
 // Grid of a gradient without a reduction, CTAs of 256: rows x parts, more
-// than one part where the rows alone would leave SMs idle.
+// than one part where the rows alone are fewer than 16 CTAs an SM (two rounds)
+// and a part keeps more than eight vectors a thread.  Gradient of scoring,
+// bf16, vocabulary 50001, with parts and without: 64 rows 6.8 and 11.5 us, 148
+// rows 9.1 and 12.9, 300 rows 14.3 and 16.2, 1200 rows 44.5 and 45.6, 2300
+// rows 80.2 and 78.7; fp16, 130000: 300 rows 28.5 and 34.0, 1200 rows 105 and
+// 110, 2300 rows 196 and 202; of distillation, bf16, 50001: 148 rows 8.7 and
+// 12.1, 600 rows 26.3 and 23.8, 1800 rows 65.4 and 64.1.  Parts up to 4 CTAs an
+// SM only: 600 x 130000 59.4 against 54.1; up to 64: 4 % either way.
 dim3 gradient_grid(uint32_t rows, uint32_t vecs);
 
 }  // namespace token
