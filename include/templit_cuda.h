@@ -663,6 +663,189 @@ int tl_flash_attention_probs(const tl_flash_desc *d, float *p, void *stream);
  * above the diagonal, 0 elsewhere; include/nn/attention.h:10-22), else 0. */
 int tl_attention_mask_check(const float *mask, uint32_t T, uint32_t *flag, void *stream);
 
+/* ------------------------------------- heads: norm and rotation by position */
+/* Queries and keys per head, as the projections of nn::MultiHeadAttention
+ * (include/nn/multi_head.h) leave them, turned by their position in
+ * the sequence and optionally normed first.  No counterpart in the reference,
+ * whose positions are a learned embedding (include/nn/GPT.h) and whose
+ * RMSNorm is over whole rows (src/my_metal/runtime.cpp:1061-1072).
+ *
+ * Element (b, t, h, d) of a view is at p + b * batch_stride + t * row_stride
+ * + h * head_stride + d (strides in elements, any alignment of the type's
+ * own): [B, T, H, D], [B, H, T, D] and slices of a fused projection alike. */
+typedef struct tl_head_view {
+  const void *p;
+  uint64_t batch_stride, head_stride, row_stride;
+} tl_head_view;
+
+enum tl_rotary_layout {
+  TL_ROTARY_HALF = 0,       /* pair i is elements i and i + rotary_dim / 2 */
+  TL_ROTARY_INTERLEAVED = 1 /* pair i is elements 2 i and 2 i + 1          */
+};
+/* Angles per position f_i = base^(-2 i / dim), i < dim / 2, stretched for
+ * contexts longer than the trained one:
+ *   PLAIN   f_i
+ *   LINEAR  f_i / factor
+ *   NTK     base' = base * factor^(dim / (dim - 2)): the fastest pair stays,
+ *           the slowest is stretched by `factor`
+ *   PARTS   pairs with more than `high` turns over original_length stay, those
+ *           with fewer than `low` are stretched, with a linear ramp over the
+ *           pairs between (their indices rounded outwards); magnitude 0.1 ln
+ *           factor + 1 (YaRN, Peng et al. 2023)
+ *   SMOOTH  the same split, the ramp linear in the number of turns;
+ *           magnitude 1 */
+enum tl_rotary_scaling {
+  TL_ROTARY_PLAIN = 0,
+  TL_ROTARY_LINEAR = 1,
+  TL_ROTARY_NTK = 2,
+  TL_ROTARY_PARTS = 3,
+  TL_ROTARY_SMOOTH = 4
+};
+typedef struct tl_rotary_spec {
+  double base;            /* > 1, e.g. 10000                              */
+  double factor;          /* >= 1; not read by PLAIN                      */
+  double original_length; /* > 0; PARTS and SMOOTH                        */
+  double low, high;       /* 0 < low < high; PARTS and SMOOTH             */
+  uint32_t dim;           /* rotated elements of a head: even, 2..256     */
+  int32_t scaling;        /* tl_rotary_scaling                            */
+} tl_rotary_spec;
+/*
+ * frequencies[i], i < dim / 2 (host memory): f_i / (2 pi) * 2^64, the turns a
+ * position as a 64-bit fraction.  A kernel's angle is position * frequencies[i]
+ * mod 2^64, so that positions up to 2^32 - 1 lose no accuracy.  A program
+ * copies them to device memory once; it may fill them in itself.  *magnitude
+ * (optional) is what the rotated elements are multiplied by.  Host only.
+ */
+int tl_rotary_frequencies(const tl_rotary_spec *spec, uint64_t *frequencies, float *magnitude);
+
+#define TL_HEAD_MAX_DIM 256u
+typedef struct tl_rotary_part {
+  uint32_t heads; /* 0: this part is absent                               */
+  uint32_t reserved;
+  tl_head_view x;      /* input, `type`                                   */
+  tl_head_view out;    /* forward: output, `out_type`; may be x           */
+  tl_head_view d_out;  /* backward: gradient of out, `out_type`           */
+  tl_head_view dx;     /* backward: gradient of x, `type`; may be d_out   */
+  const float *weight; /* [D], optional: the norm's weights               */
+  float *dweight;      /* [D], optional, backward: their gradient (set)   */
+} tl_rotary_part;
+typedef struct tl_rotary_desc {
+  uint32_t B, T, D;    /* D <= TL_HEAD_MAX_DIM                            */
+  uint32_t rotary_dim; /* even, <= D; the elements behind it are not turned */
+  int32_t type, out_type; /* tl_float_type                                */
+  int32_t layout;      /* tl_rotary_layout                                */
+  int32_t norm;        /* 1: y = x / sqrt(mean(x^2) + eps) * weight first */
+  float eps;           /* >= 0, finite; 1e-6 in tl_rmsnorm_rows           */
+  float magnitude;     /* finite; 1 where no scaling asks for another     */
+  const uint64_t *frequencies; /* [rotary_dim / 2], device                */
+  const uint32_t *positions;   /* [B, T], device; NULL: first_position + t */
+  uint32_t first_position;
+  uint32_t reserved;
+  tl_rotary_part q, k;
+  void *workspace;     /* backward with dweight                           */
+  uint64_t workspace_bytes;
+} tl_rotary_desc;
+/*
+ * out = turn(norm(x)) of queries and keys in one pass: pair i of position p
+ * becomes magnitude * (a cos - b sin, a sin + b cos) at angle p f_i; sums and
+ * products are fp32, the result is rounded once.
+ */
+int tl_rotary_heads(const tl_rotary_desc *desc, void *stream);
+/*
+ * Its gradient: dx from d_out (and x and weight where normed, whose root mean
+ * squares are taken again), dweight = the sum over all tokens and heads, in a
+ * fixed order.  x is read only where normed.
+ */
+int tl_rotary_heads_backward(const tl_rotary_desc *desc, void *stream);
+size_t tl_rotary_heads_workspace_size(const tl_rotary_desc *desc);
+
+/* ---------------------------------------------------- paged key-value cache */
+/* Keys and values of many sequences in pages of page_size slots: key (page,
+ * slot, head, d) at k + page * page_stride + slot * slot_stride + head *
+ * head_stride + d, the value at the same place from v (k and v may be parts of
+ * one tensor).  The reference has no cache: its generation recomputes the
+ * whole window for each token (include/inference.h:45-97).
+ *
+ * A batch: sequence s has the keys 0 .. lengths[s] - 1, key j in page table[s *
+ * table_stride + j / page_size], slot j % page_size; its new tokens are the
+ * rows starts[s] .. starts[s + 1] - 1 of the call's tensors and the last
+ * positions, lengths[s] - (starts[s + 1] - starts[s]) and up.  Rows that no
+ * sequence has are left as they were.  The arrays are device memory and are
+ * read when the kernels run, so a captured call follows them.  What they hold
+ * cannot make a kernel read or write outside of the tensors: a page id >=
+ * pages, a length above table_stride * page_size, a sequence whose rows leave
+ * [0, tokens) or run backwards raise TL_FLAG_INDEX_RANGE; such keys are not
+ * there, such rows are not written. */
+typedef struct tl_paged_cache {
+  void *k, *v;
+  uint64_t page_stride, slot_stride, head_stride; /* elements             */
+  uint32_t pages, page_size, heads, D;
+  int32_t type;           /* tl_float_type of keys and values             */
+  uint32_t sequences;
+  uint32_t tokens;        /* rows of the call's tensors                   */
+  uint32_t table_stride;  /* pages a row of the table holds               */
+  const uint32_t *table;  /* [sequences, table_stride]                    */
+  const uint32_t *lengths; /* [sequences], the new tokens included        */
+  const uint32_t *starts; /* [sequences + 1], not descending              */
+} tl_paged_cache;
+
+typedef struct tl_cache_append_desc {
+  tl_paged_cache cache;
+  tl_head_view q, k, v; /* [tokens, heads, D] of `type` (batch_stride unused) */
+  tl_head_view q_out;   /* `q_out_type`; may be q                         */
+  uint32_t q_heads;     /* 0: no queries                                  */
+  int32_t type, q_out_type; /* tl_float_type                              */
+  uint32_t rotary_dim;  /* 0: no rotation                                 */
+  int32_t layout, norm; /* as in tl_rotary_desc; norm is of q and k       */
+  float eps, magnitude;
+  const uint64_t *frequencies;
+  const float *q_weight, *k_weight; /* [D], optional                      */
+} tl_cache_append_desc;
+/*
+ * The new tokens' keys, normed and turned by their positions as in
+ * tl_rotary_heads, and their values into the cache, rounded once to its type;
+ * their queries alike into q_out, in one launch.  A token whose position would
+ * be negative (more new tokens than keys) or behind the table, or whose page
+ * id is out of range, is not written and raises TL_FLAG_INDEX_RANGE.  Two
+ * tokens must not share a place in the cache.
+ */
+int tl_cache_append(const tl_cache_append_desc *desc, void *stream);
+
+typedef struct tl_paged_attention_desc {
+  tl_paged_cache cache;
+  tl_head_view q;       /* [tokens, q_heads, D] of the cache's type       */
+  tl_head_view out;     /* the same of out_type                           */
+  uint32_t q_heads;     /* a multiple of cache.heads: query head h reads
+                           key head h / (q_heads / heads)                 */
+  int32_t out_type;     /* the cache's type or TL_FLOAT32                 */
+  int32_t causal;       /* 1: a token sees no key behind its position     */
+  uint32_t window;      /* > 0: only the last `window` keys up to its position */
+  float scale;          /* finite; 1 / sqrt(D) as a rule                  */
+  uint32_t max_length;  /* no sequence has more keys; 0: what the table holds */
+  uint32_t max_new;     /* no sequence has more new tokens; 0: `tokens`.  Both
+                           only choose how the work is split: a longer chunk
+                           gives the same result, a longer sequence is cut
+                           and raises TL_FLAG_INDEX_RANGE                 */
+  uint32_t reserved;
+  float *lse;           /* [tokens, q_heads], optional: ln sum_j e^(s_j)  */
+  void *workspace;      /* tl_paged_attention_workspace_size() bytes      */
+  uint64_t workspace_bytes;
+} tl_paged_attention_desc;
+/*
+ * out = softmax(scale q k^T) v of the new tokens over their sequences' keys in
+ * the cache.  fp32 caches: fp32 products.  16-bit caches: products of 16-bit
+ * numbers summed in fp32, the softmax in fp32, its numerators rounded to the
+ * cache's type for the second product.  A row that sees no key (or only
+ * scores of -inf) is 0 with lse -inf.  What lies in slots behind a sequence's
+ * length, and keys and values that a row does not see, do not reach it, NaN
+ * and infinities included.
+ * D a multiple of 8, at most 128; rows 16-byte aligned (pointers and strides),
+ * else TL_ERR_UNSUPPORTED.  Deterministic; one call's workspace may be used by
+ * the next on the same stream, not by two calls that may overlap.
+ */
+int tl_paged_attention(const tl_paged_attention_desc *desc, void *stream);
+size_t tl_paged_attention_workspace_size(const tl_paged_attention_desc *desc);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,6 +38,9 @@ TL_TOKEN_MAX_TOP = 128
 TL_DISTILL_RENORM, TL_DISTILL_TAIL = range(2)
 TL_DISTILL_STATS = 8
 TL_DISTILL_MAX_VOCAB = 1 << 20
+TL_ROTARY_HALF, TL_ROTARY_INTERLEAVED = range(2)
+TL_ROTARY_PLAIN, TL_ROTARY_LINEAR, TL_ROTARY_NTK, TL_ROTARY_PARTS, TL_ROTARY_SMOOTH = range(5)
+TL_HEAD_MAX_DIM = 256
 
 
 class TlParamSlot(Structure):
@@ -106,6 +109,55 @@ class TlDistillDesc(Structure):
                 ("targets", c_void_p), ("loss", c_void_p), ("kl", c_void_p),
                 ("stats", c_void_p), ("row_scale", c_void_p), ("dlogits", c_void_p),
                 ("d_row_stride", c_uint64)]
+
+
+class TlHeadView(Structure):
+    _fields_ = [("p", c_void_p), ("batch_stride", c_uint64), ("head_stride", c_uint64),
+                ("row_stride", c_uint64)]
+
+
+class TlRotarySpec(Structure):
+    _fields_ = [("base", c_double), ("factor", c_double), ("original_length", c_double),
+                ("low", c_double), ("high", c_double), ("dim", c_uint32), ("scaling", c_int32)]
+
+
+class TlRotaryPart(Structure):
+    _fields_ = [("heads", c_uint32), ("reserved", c_uint32), ("x", TlHeadView),
+                ("out", TlHeadView), ("d_out", TlHeadView), ("dx", TlHeadView),
+                ("weight", c_void_p), ("dweight", c_void_p)]
+
+
+class TlRotaryDesc(Structure):
+    _fields_ = [("B", c_uint32), ("T", c_uint32), ("D", c_uint32), ("rotary_dim", c_uint32),
+                ("type", c_int32), ("out_type", c_int32), ("layout", c_int32), ("norm", c_int32),
+                ("eps", c_float), ("magnitude", c_float), ("frequencies", c_void_p),
+                ("positions", c_void_p), ("first_position", c_uint32), ("reserved", c_uint32),
+                ("q", TlRotaryPart), ("k", TlRotaryPart), ("workspace", c_void_p),
+                ("workspace_bytes", c_uint64)]
+
+
+class TlPagedCache(Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("page_stride", c_uint64),
+                ("slot_stride", c_uint64), ("head_stride", c_uint64), ("pages", c_uint32),
+                ("page_size", c_uint32), ("heads", c_uint32), ("D", c_uint32), ("type", c_int32),
+                ("sequences", c_uint32), ("tokens", c_uint32), ("table_stride", c_uint32),
+                ("table", c_void_p), ("lengths", c_void_p), ("starts", c_void_p)]
+
+
+class TlCacheAppendDesc(Structure):
+    _fields_ = [("cache", TlPagedCache), ("q", TlHeadView), ("k", TlHeadView), ("v", TlHeadView),
+                ("q_out", TlHeadView), ("q_heads", c_uint32), ("type", c_int32),
+                ("q_out_type", c_int32), ("rotary_dim", c_uint32), ("layout", c_int32),
+                ("norm", c_int32), ("eps", c_float), ("magnitude", c_float),
+                ("frequencies", c_void_p), ("q_weight", c_void_p), ("k_weight", c_void_p)]
+
+
+class TlPagedAttentionDesc(Structure):
+    _fields_ = [("cache", TlPagedCache), ("q", TlHeadView), ("out", TlHeadView),
+                ("q_heads", c_uint32), ("out_type", c_int32), ("causal", c_int32),
+                ("window", c_uint32), ("scale", c_float), ("max_length", c_uint32),
+                ("max_new", c_uint32), ("reserved", c_uint32), ("lse", c_void_p),
+                ("workspace", c_void_p), ("workspace_bytes", c_uint64)]
 
 
 class TlgConfig(Structure):
@@ -199,6 +251,13 @@ CUDA_ABI = {
     "tl_distill_rows": (c_int, [POINTER(TlDistillDesc), c_void_p]),
     "tl_distill_backward_rows": (c_int, [POINTER(TlDistillDesc), c_void_p]),
     "tl_distill_train_rows": (c_int, [POINTER(TlDistillDesc), c_void_p]),
+    "tl_rotary_frequencies": (c_int, [POINTER(TlRotarySpec), POINTER(c_uint64), POINTER(c_float)]),
+    "tl_rotary_heads": (c_int, [POINTER(TlRotaryDesc), c_void_p]),
+    "tl_rotary_heads_backward": (c_int, [POINTER(TlRotaryDesc), c_void_p]),
+    "tl_rotary_heads_workspace_size": (c_size_t, [POINTER(TlRotaryDesc)]),
+    "tl_cache_append": (c_int, [POINTER(TlCacheAppendDesc), c_void_p]),
+    "tl_paged_attention": (c_int, [POINTER(TlPagedAttentionDesc), c_void_p]),
+    "tl_paged_attention_workspace_size": (c_size_t, [POINTER(TlPagedAttentionDesc)]),
     "tl_embedding_gather": (c_int, [c_void_p, c_uint32, c_uint32, c_void_p, c_uint32,
                                     c_void_p, c_void_p]),
     "tl_embedding_scatter_add": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_void_p,

@@ -1,0 +1,255 @@
+// Queries and keys turned by their positions, optionally normed per head
+// (include/templit_cuda.h: tl_rotary_frequencies, tl_rotary_heads), and the
+// checks shared with the gradient and the cache.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w          (norm)
+//   (y_a, y_b) -> mag (y_a cos - y_b sin, y_a sin + y_b cos), angle = p f_i
+//
+// Bound by memory: every element is read once and written once.  A warp takes
+// one token (its angles are computed once, in registers) and a run of its
+// heads, 32 / lanes heads at a time, kBatch of those in flight.
+#include "rotary.cuh"
+
+#include <cmath>
+
+namespace tl {
+namespace heads {
+
+int check_turn(const char *who, uint32_t D, uint32_t rotary_dim, int32_t layout, int32_t norm, float eps,
+               float magnitude, const uint64_t *frequencies) {
+  const std::string w = std::string(who) + ": ";
+  if (D == 0 || D > TL_HEAD_MAX_DIM) return fail(TL_ERR_RANGE, w + "a head has 1 to 256 elements");
+  if (rotary_dim % 2 || rotary_dim > D) return fail(TL_ERR_INVALID, w + "rotary_dim is even and at most D");
+  if (layout != TL_ROTARY_HALF && layout != TL_ROTARY_INTERLEAVED) return fail(TL_ERR_INVALID, w + "unknown layout");
+  if (norm != 0 && norm != 1) return fail(TL_ERR_INVALID, w + "norm is 0 or 1");
+  if (norm && !(eps >= 0.0f && std::isfinite(eps))) return fail(TL_ERR_INVALID, w + "eps is finite and not negative");
+  if (rotary_dim && !std::isfinite(magnitude)) return fail(TL_ERR_INVALID, w + "magnitude is finite");
+  if (rotary_dim && !frequencies) return fail(TL_ERR_INVALID, w + "null frequencies");
+  if (reinterpret_cast<uintptr_t>(frequencies) % 8) return fail(TL_ERR_INVALID, w + "frequencies not aligned");
+  return TL_OK;
+}
+
+int check_view(const char *who, const char *name, const tl_head_view &v, int32_t type, uint64_t batches,
+               uint64_t rows, uint64_t heads, uint32_t D, bool written) {
+  const std::string w = std::string(who) + ": " + name;
+  if (!v.p) return fail(TL_ERR_INVALID, w + " is null");
+  if (reinterpret_cast<uintptr_t>(v.p) % type_size(type)) return fail(TL_ERR_INVALID, w + " is not aligned to its type");
+  // the farthest element's offset, kept clear of 64 bits
+  const uint64_t most = (1ull << 62) / type_size(type);
+  const auto far = [&](uint64_t n, uint64_t stride) { return n > 1 && stride > most / (n - 1) / 4; };
+  if (far(batches, v.batch_stride) || far(rows, v.row_stride) || far(heads, v.head_stride))
+    return fail(TL_ERR_RANGE, w + " leaves the address space");
+  if (written && ((batches > 1 && v.batch_stride < D) || (rows > 1 && v.row_stride < D) ||
+                  (heads > 1 && v.head_stride < D)))
+    return fail(TL_ERR_INVALID, w + " has a stride that is too small");
+  return TL_OK;
+}
+
+namespace {
+
+template <typename TI, typename TO, int V, int S, bool NORM, bool INTER>
+__global__ void __launch_bounds__(kThreads) rotate_kernel(const RotaryArgs a) {
+  constexpr int U = V == 1 ? 1 : kBatch;
+  pdl_enter();
+  const bool second = blockIdx.x >= a.part[0].ctas;
+  const RotaryPart &part = a.part[second];
+  const uint32_t cta = blockIdx.x - (second ? a.part[0].ctas : 0);
+  const bool inter = V == 1 ? a.interleaved : INTER;
+  const bool norm = V == 1 ? a.norm : NORM;
+  const uint32_t lane = threadIdx.x & 31, lanes = a.lanes, at = lane & (lanes - 1), sub = lane / lanes;
+  const uint32_t per = 32 / lanes;  // heads at a time
+
+  Slot slot[S];
+  float wa[S][V], wb[S][V];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    slot[s] = slot_of(at + s * lanes, V, a.D, a.rotary, inter);
+    load_weights<V>(norm ? part.weight : nullptr, slot[s], wa[s], wb[s]);
+  }
+  const uint64_t items = static_cast<uint64_t>(a.tokens) * part.chunks;
+  const uint64_t warps = static_cast<uint64_t>(part.ctas) * kWarps;
+  for (uint64_t item = static_cast<uint64_t>(cta) * kWarps + threadIdx.x / 32; item < items; item += warps) {
+    const uint32_t token = static_cast<uint32_t>(item / part.chunks), chunk = static_cast<uint32_t>(item % part.chunks);
+    const uint32_t b = token / a.T, t = token % a.T;
+    float cos[S][V], sin[S][V];
+    angles<V, S>(a.frequencies, a.positions ? a.positions[token] : a.first_position + t, a.magnitude, at, lanes,
+                 a.rotary, cos, sin);
+    const TI *x = static_cast<const TI *>(part.x.p) + b * part.x.batch_stride + t * part.x.row_stride;
+    TO *out = static_cast<TO *>(const_cast<void *>(part.out.p)) + b * part.out.batch_stride + t * part.out.row_stride;
+    const uint32_t heads = part.steps * per;
+    run_heads<TI, TO, V, S, U>(x, part.x.head_stride, out, part.out.head_stride, chunk * heads,
+                               min((chunk + 1) * heads, part.heads), lanes, sub, slot, wa, wb, cos, sin, norm, true,
+                               inter, a.inv_d, a.eps);
+  }
+}
+
+template <typename TI, typename TO> void launch_rotate(RotaryArgs &a, bool vectors, cudaStream_t s) {
+  constexpr int V = sizeof(TI) == 4 && sizeof(TO) == 4 ? 4 : 8;
+  if (!vectors) {
+    const unsigned grid = share_out(a, false);
+    launch_pdl(rotate_kernel<TI, TO, 1, 4, false, false>, grid, kThreads, 0, s, a);
+    return;
+  }
+  const unsigned grid = share_out(a, false);
+  if (a.norm) {
+    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, 1, true, true>, grid, kThreads, 0, s, a);
+    else launch_pdl(rotate_kernel<TI, TO, V, 1, true, false>, grid, kThreads, 0, s, a);
+  } else {
+    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, 1, false, true>, grid, kThreads, 0, s, a);
+    else launch_pdl(rotate_kernel<TI, TO, V, 1, false, false>, grid, kThreads, 0, s, a);
+  }
+}
+
+}  // namespace
+
+int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryArgs &a) {
+  const std::string w = std::string(who) + ": ";
+  if (!d) return fail(TL_ERR_INVALID, w + "null descriptor");
+  if (!known_type(d->type) || !known_type(d->out_type)) return fail(TL_ERR_INVALID, w + "unknown type");
+  if (mixed_halves(d->type, d->out_type)) return fail(TL_ERR_UNSUPPORTED, w + "fp16 and bf16 in one call");
+  if (int rc = check_turn(who, d->D, d->rotary_dim, d->layout, d->norm, d->eps, d->magnitude, d->frequencies))
+    return rc;
+  const uint64_t tokens = static_cast<uint64_t>(d->B) * d->T;
+  if (tokens >> 32) return fail(TL_ERR_RANGE, w + "more than 2^32 - 1 tokens");
+  if (!d->q.heads && !d->k.heads) return fail(TL_ERR_INVALID, w + "no heads");
+  a.D = d->D;
+  a.T = d->T;
+  a.tokens = static_cast<uint32_t>(tokens);
+  a.rotary = d->rotary_dim;
+  a.interleaved = d->layout == TL_ROTARY_INTERLEAVED;
+  a.norm = d->norm;
+  a.eps = d->eps;
+  a.inv_d = 1.0f / d->D;
+  a.magnitude = d->magnitude;
+  a.frequencies = d->frequencies;
+  a.positions = d->positions;
+  a.first_position = d->first_position;
+  bool aligned = true;
+  const tl_rotary_part *parts[2] = {&d->q, &d->k};
+  for (int i = 0; i < 2 && tokens; ++i) {
+    const tl_rotary_part &p = *parts[i];
+    RotaryPart &r = a.part[i];
+    r.heads = p.heads;
+    if (!p.heads) continue;
+    const auto view = [&](const char *name, const tl_head_view &v, int32_t type, bool written) {
+      aligned = aligned && aligned_view(v, type, d->B > 1);
+      return check_view(who, name, v, type, d->B, d->T, p.heads, d->D, written);
+    };
+    if (!backward || d->norm)
+      if (int rc = view("x", p.x, d->type, false)) return rc;
+    if (!backward) {
+      if (int rc = view("out", p.out, d->out_type, true)) return rc;
+    } else {
+      if (int rc = view("d_out", p.d_out, d->out_type, false)) return rc;
+      if (int rc = view("dx", p.dx, d->type, true)) return rc;
+      if (p.dweight && !d->norm) return fail(TL_ERR_INVALID, w + "dweight without a norm");
+    }
+    if (!backward && half_in_place(p.out, d->out_type, p.x, d->type, d->B > 1))
+      return fail(TL_ERR_INVALID, w + "out is x with another layout or type");
+    if (backward && (half_in_place(p.dx, d->type, p.d_out, d->out_type, d->B > 1) ||
+                     (d->norm && half_in_place(p.dx, d->type, p.x, d->type, d->B > 1))))
+      return fail(TL_ERR_INVALID, w + "dx in place with another layout or type");
+    r.x = p.x;
+    r.out = p.out;
+    r.d_out = p.d_out;
+    r.dx = p.dx;
+    r.weight = p.weight;
+    r.dweight = backward ? p.dweight : nullptr;
+  }
+  const uint32_t V = d->type == TL_FLOAT32 && d->out_type == TL_FLOAT32 ? 4 : 8;
+  const Shape shape = shape_for(d->D, d->rotary_dim, V, aligned);
+  a.lanes = shape.lanes;
+  a.vectors = shape.vectors;
+  return TL_OK;
+}
+
+unsigned share_out(RotaryArgs &a, bool persistent) {
+  // A warp's run of heads: all of them where the tokens alone make two warps a
+  // scheduler, shorter where they do not.
+  const uint32_t per = 32 / a.lanes, wanted = kNumSMs * 8;
+  unsigned grid = 0;
+  const uint64_t heads = a.part[0].heads + static_cast<uint64_t>(a.part[1].heads);
+  for (RotaryPart &p : a.part) {
+    p.ctas = 0;
+    if (!p.heads) continue;
+    p.all_steps = (p.heads + per - 1) / per;
+    p.steps = p.all_steps;
+    while (p.steps > 1 && static_cast<uint64_t>(a.tokens) * ((p.all_steps + p.steps - 1) / p.steps) < wanted)
+      p.steps = (p.steps + 1) / 2;
+    p.chunks = (p.all_steps + p.steps - 1) / p.steps;
+    const uint64_t items = static_cast<uint64_t>(a.tokens) * p.chunks;
+    uint64_t ctas = (items + kWarps - 1) / kWarps;
+    const uint64_t most = persistent ? (kMaxCtas * p.heads + heads - 1) / heads : kNumSMs * 256ull;
+    if (ctas > most) ctas = most;
+    p.ctas = static_cast<uint32_t>(ctas);
+    grid += p.ctas;
+  }
+  return grid;
+}
+
+}  // namespace heads
+}  // namespace tl
+
+using namespace tl;
+using namespace tl::heads;
+
+extern "C" {
+
+int tl_rotary_frequencies(const tl_rotary_spec *spec, uint64_t *frequencies, float *magnitude) {
+  const std::string w = "tl_rotary_frequencies: ";
+  if (!spec || !frequencies) return fail(TL_ERR_INVALID, w + "null argument");
+  const tl_rotary_spec &s = *spec;
+  if (s.dim < 2 || s.dim % 2 || s.dim > TL_HEAD_MAX_DIM) return fail(TL_ERR_RANGE, w + "dim is even, 2 to 256");
+  if (s.scaling < TL_ROTARY_PLAIN || s.scaling > TL_ROTARY_SMOOTH) return fail(TL_ERR_INVALID, w + "unknown scaling");
+  if (!(s.base > 1.0) || !std::isfinite(s.base)) return fail(TL_ERR_INVALID, w + "base is above 1");
+  if (s.scaling != TL_ROTARY_PLAIN && (!(s.factor >= 1.0) || !std::isfinite(s.factor)))
+    return fail(TL_ERR_INVALID, w + "factor is at least 1");
+  const bool split = s.scaling == TL_ROTARY_PARTS || s.scaling == TL_ROTARY_SMOOTH;
+  if (split && (!(s.original_length > 0.0) || !std::isfinite(s.original_length) || !(s.low > 0.0) ||
+                !(s.high > s.low) || !std::isfinite(s.high)))
+    return fail(TL_ERR_INVALID, w + "original_length and 0 < low < high are needed");
+  if (s.scaling == TL_ROTARY_NTK && s.dim == 2 && s.factor != 1.0)
+    return fail(TL_ERR_INVALID, w + "the base cannot stretch a single pair");
+
+  const double two_pi = 6.283185307179586;
+  const uint32_t n = s.dim / 2;
+  double base = s.base;
+  if (s.scaling == TL_ROTARY_NTK && s.dim > 2) base *= std::pow(s.factor, s.dim / (s.dim - 2.0));
+  double from = 0, to = 0;
+  if (s.scaling == TL_ROTARY_PARTS) {
+    // the pair that turns `r` times over original_length
+    const auto pair = [&](double r) {
+      return s.dim * std::log(s.original_length / (r * two_pi)) / (2 * std::log(base));
+    };
+    from = std::fmax(std::floor(pair(s.high)), 0.0);
+    to = std::fmin(std::ceil(pair(s.low)), s.dim - 1.0);
+    if (to - from < 0.001) to = from + 0.001;
+  }
+  for (uint32_t i = 0; i < n; ++i) {
+    double f = std::pow(base, -2.0 * i / s.dim), stretched = f / s.factor;
+    if (s.scaling == TL_ROTARY_LINEAR) f = stretched;
+    if (split) {
+      const double ramp = s.scaling == TL_ROTARY_PARTS
+                                   ? (i - from) / (to - from)
+                                   : 1 - (s.original_length * f / two_pi - s.low) / (s.high - s.low);
+      const double part = std::fmin(std::fmax(ramp, 0.0), 1.0);
+      f = f * (1 - part) + stretched * part;
+    }
+    frequencies[i] = static_cast<uint64_t>(std::round(f / two_pi * 18446744073709551616.0));
+  }
+  if (magnitude) *magnitude = s.scaling == TL_ROTARY_PARTS ? static_cast<float>(0.1 * std::log(s.factor) + 1.0) : 1.0f;
+  return TL_OK;
+}
+
+int tl_rotary_heads(const tl_rotary_desc *desc, void *stream) {
+  const char *who = "tl_rotary_heads";
+  RotaryArgs a{};
+  if (int rc = rotary_args(who, desc, false, a)) return rc;
+  if (a.tokens == 0) return TL_OK;
+#define L(TI, TO) launch_rotate<TI, TO>(a, a.vectors, as_stream(stream))
+  TL_BY_TYPES(desc->type, desc->out_type, L)
+#undef L
+  return launch_status(who);
+}
+
+}  // extern "C"
