@@ -1,6 +1,6 @@
 // Attention of new tokens over a paged cache (include/templit_cuda.h:
 // tl_paged_attention): softmax(scale q k^T) v over the keys that each token
-// sees.
+// sees.  Checks, and the choice between the kernels.
 #include "paged_attention.cuh"
 
 #include <cmath>
@@ -9,54 +9,10 @@ namespace tl {
 namespace paged {
 namespace {
 
-constexpr int kRowWarps = 4;
-
-template <typename T, typename TO>
-__global__ void __launch_bounds__(kRowWarps * 32) rows_kernel(const AttentionArgs a) {
-  pdl_enter();
-  const tl_paged_cache &c = a.cache;
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t items = static_cast<uint64_t>(c.tokens) * a.q_heads, warps = static_cast<uint64_t>(gridDim.x) * kRowWarps;
-  for (uint64_t item = static_cast<uint64_t>(blockIdx.x) * kRowWarps + threadIdx.x / 32; item < items; item += warps) {
-    const uint32_t token = static_cast<uint32_t>(item / a.q_heads), h = static_cast<uint32_t>(item % a.q_heads);
-    const uint32_t s = sequence_at(c, token, lane);
-    if (s == 0xffffffffu) continue;
-    const Sequence q = sequence_of(c, s, a.most);
-    if (q.bad && lane == 0) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
-    if (token < q.start || token - q.start >= q.count) continue;
-    const int64_t position = static_cast<int64_t>(q.length) - q.count + (token - q.start);
-    uint32_t from, to;
-    seen(a, q.length, position, from, to);
-    float m, l, acc[kMaxHead / 32];
-    const T *row = static_cast<const T *>(a.q.p) + token * a.q.row_stride + h * a.q.head_stride;
-    row_over_keys<T>(a, s, h / a.group, row, from, to, lane, m, l, acc);
-    TO *out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(kMaxHead) / 32; ++i)
-      if (lane + 32 * i < c.D) heads::set_element(out[lane + 32 * i], l == 0.0f ? 0.0f : acc[i] / l);
-    if (lane == 0 && a.lse) a.lse[static_cast<uint64_t>(token) * a.q_heads + h] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
-  }
-}
-
-}  // namespace
-}  // namespace paged
-}  // namespace tl
-
-using namespace tl;
-using namespace tl::paged;
-
-extern "C" {
-
-size_t tl_paged_attention_workspace_size(const tl_paged_attention_desc *d) {
-  (void)d;
-  return 0;
-}
-
-int tl_paged_attention(const tl_paged_attention_desc *d, void *stream) {
-  const char *who = "tl_paged_attention";
+// Checks a descriptor; *nothing where there is no work.
+int attention_args(const char *who, const tl_paged_attention_desc *d, AttentionArgs &a, bool *nothing) {
   const std::string w = std::string(who) + ": ";
   if (!d) return fail(TL_ERR_INVALID, w + "null descriptor");
-  AttentionArgs a{};
   a.cache = d->cache;
   bool aligned = false;
   if (int rc = check_cache(who, a.cache, &aligned)) return rc;
@@ -67,7 +23,9 @@ int tl_paged_attention(const tl_paged_attention_desc *d, void *stream) {
   if (d->causal != 0 && d->causal != 1) return fail(TL_ERR_INVALID, w + "causal is 0 or 1");
   if (d->window && !d->causal) return fail(TL_ERR_INVALID, w + "a window needs causal");
   if (!std::isfinite(d->scale)) return fail(TL_ERR_INVALID, w + "scale is finite");
-  if (!c.tokens || !c.sequences) return TL_OK;
+  if (static_cast<uint64_t>(c.tokens) * d->q_heads >> 32) return fail(TL_ERR_RANGE, w + "more than 2^32 - 1 query rows");
+  *nothing = !c.tokens || !c.sequences;
+  if (*nothing) return TL_OK;
   if (int rc = heads::check_view(who, "q", d->q, c.type, 1, c.tokens, d->q_heads, c.D, false)) return rc;
   if (int rc = heads::check_view(who, "out", d->out, d->out_type, 1, c.tokens, d->q_heads, c.D, true)) return rc;
   if (heads::half_in_place(d->out, d->out_type, d->q, c.type, false))
@@ -84,20 +42,48 @@ int tl_paged_attention(const tl_paged_attention_desc *d, void *stream) {
   if (d->max_length && d->max_length < a.most) a.most = d->max_length;
   a.scale = d->scale;
   a.lse = d->lse;
+  return TL_OK;
+}
+
+uint32_t most_new(const tl_paged_attention_desc *d) {
+  return d->max_new && d->max_new < d->cache.tokens ? d->max_new : d->cache.tokens;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace tl
+
+using namespace tl;
+using namespace tl::paged;
+
+extern "C" {
+
+size_t tl_paged_attention_workspace_size(const tl_paged_attention_desc *d) {
+  AttentionArgs a{};
+  bool nothing = false;
+  if (attention_args("tl_paged_attention_workspace_size", d, a, &nothing) || nothing) return 0;
+  return plan_bytes(step_plan(a, most_new(d)));
+}
+
+int tl_paged_attention(const tl_paged_attention_desc *d, void *stream) {
+  const char *who = "tl_paged_attention";
+  const std::string w = std::string(who) + ": ";
+  AttentionArgs a{};
+  bool nothing = false;
+  if (int rc = attention_args(who, d, a, &nothing)) return rc;
+  if (nothing) return TL_OK;
+  const Plan p = step_plan(a, most_new(d));
+  const uint64_t bytes = plan_bytes(p);
+  if (bytes) {
+    if (!d->workspace || d->workspace_bytes < bytes) return fail(TL_ERR_INVALID, w + "workspace too small");
+    if (!aligned16(d->workspace)) return fail(TL_ERR_INVALID, w + "workspace is not 16-byte aligned");
+  }
+  a.whole = p.whole;
+  a.joins = static_cast<Join *>(d->workspace);
+  a.parts = reinterpret_cast<float *>(a.joins + p.ctas);
   a.status = device_status_ptr();
   if (!a.status) return fail(TL_ERR_CUDA, w + "no status word");
-  const uint64_t ctas = (static_cast<uint64_t>(c.tokens) * a.q_heads + kRowWarps - 1) / kRowWarps;
-  const unsigned grid = static_cast<unsigned>(ctas < kNumSMs * 64ull ? ctas : kNumSMs * 64ull);
-  cudaStream_t s = as_stream(stream);
-  const bool wide = d->out_type == TL_FLOAT32;
-  if (c.type == TL_FLOAT32) launch_pdl(rows_kernel<float, float>, grid, kRowWarps * 32, 0, s, a);
-  else if (c.type == TL_FLOAT16) {
-    if (wide) launch_pdl(rows_kernel<__half, float>, grid, kRowWarps * 32, 0, s, a);
-    else launch_pdl(rows_kernel<__half, __half>, grid, kRowWarps * 32, 0, s, a);
-  } else {
-    if (wide) launch_pdl(rows_kernel<__nv_bfloat16, float>, grid, kRowWarps * 32, 0, s, a);
-    else launch_pdl(rows_kernel<__nv_bfloat16, __nv_bfloat16>, grid, kRowWarps * 32, 0, s, a);
-  }
+  launch_step(a, p, d->out_type != a.cache.type, as_stream(stream));
   return launch_status(who);
 }
 
