@@ -4,7 +4,7 @@
 //
 // Bound by memory: every key and value is read once for up to 16 query rows
 // (a token's heads that share a key head lie side by side), so the rows' own
-// arithmetic is small and mma.sync is enough.  A warp works alone: it brings 16
+// arithmetic is small and mma.sync (fp32: the CUDA cores) is enough.  A warp works alone: it brings 16
 // keys and values (8 of 32 bits) at a time into its own ring in shared memory
 // by cp.async, several steps ahead, multiplies and keeps its rows' maxima,
 // sums and outputs in registers; no barrier but the warp's own until its
@@ -18,31 +18,18 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr uint32_t kRows = 16;
+constexpr uint32_t kLeast = 4;  // blocks of a share, where there is that much
 
-template <typename T> struct Step;
-// 16-bit types: m16n8k16, 16 keys a step.  Numerators are at most 2^kShift, so
-// that fp16's small ones keep their bits (normal down to 2^-28 of the largest).
-template <> struct Step<__nv_bfloat16> {
-  static constexpr uint32_t kKeys = 16;
-  static constexpr float kShift = 0.0f;
-};
-template <> struct Step<__half> {
-  static constexpr uint32_t kKeys = 16;
-  static constexpr float kShift = 14.0f;
-};
-// fp32: m16n8k8 of operands split into two tf32 parts, 8 keys a step.
-template <> struct Step<float> {
-  static constexpr uint32_t kKeys = 8;
-  static constexpr float kShift = 0.0f;
-};
+// Keys of a warp's step.
+template <typename T> constexpr uint32_t step_keys() { return sizeof(T) == 2 ? 16 : 8; }
 
 constexpr int kStages = 3;
-template <typename T, int DP> constexpr uint32_t stage_bytes() { return 2 * Step<T>::kKeys * DP * sizeof(T); }
+template <typename T, int DP> constexpr uint32_t stage_bytes() { return 2 * step_keys<T>() * DP * sizeof(T); }
+// fp32: the queries and the warps' probabilities too
 template <typename T, int DP> constexpr size_t smem_bytes() {
-  return static_cast<size_t>(kWarps) * kStages * stage_bytes<T, DP>() + (sizeof(T) == 4 ? DP / 8 * 32 * 2 * sizeof(uint4) : 0);
+  return static_cast<size_t>(kWarps) * kStages * stage_bytes<T, DP>() +
+         (sizeof(T) == 4 ? (kRows * DP + kWarps * kRows * 8) * sizeof(float) : 0);
 }
-// floats of a partial result: outputs, maxima, sums
-template <int DP> constexpr uint32_t part_floats() { return kRows * DP + 2 * kRows; }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
@@ -62,9 +49,9 @@ __device__ __forceinline__ void load_transposed(uint32_t at, uint32_t (&r)[4]) {
                : "r"(at)
                : "memory");
 }
-__device__ __forceinline__ float load_word(uint32_t at) {
-  float x;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+__device__ __forceinline__ float4 load_vector(uint32_t at) {
+  float4 x;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
   return x;
 }
 
@@ -79,132 +66,308 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// x = big + small to 2^-22 of x, both of tf32's 11 bits (rounded to nearest)
-__device__ __forceinline__ void split(float x, uint32_t &big, uint32_t &small) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(big) : "f"(x));
-  const float rest = x - __uint_as_float(big);
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(small) : "f"(rest));
-}
+// What a row of the tile sees.
+struct Bounds {
+  uint32_t from[kRows], to[kRows];
+};
 
-// Rows of a job that a lane holds (its two of 16): keys [from, to) of each.
-struct Rows {
-  uint32_t from[2], to[2];
+// A warp's rows of 16-bit types, m16n8k16: lane i holds rows i / 4 and i / 4 + 8.
+template <typename T, int DP> struct Lane {
+  static constexpr int KS = DP / 16;
+  static constexpr uint32_t N = 16, kHalf = N * DP * 2;
+  // Numerators are at most 2^kShift, so that fp16's small ones keep their bits
+  // (normal down to 2^-28 of the largest).
+  static constexpr float kShift = std::is_same<T, __half>::value ? 14.0f : 0.0f;
+  uint32_t q[KS][4];  // the first product's left operand
+  float m[2], l[2], o[DP / 8][4];
+
+  static __device__ __forceinline__ uint32_t spot(uint32_t row, uint32_t ch) { return row * (DP * 2) + ((ch ^ (row & 7)) << 4); }
+
+  __device__ __forceinline__ void begin(const AttentionArgs &a, const Piece &w, float *) {
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t row = lane / 4 + 8 * i;
+      const uint64_t place = w.row0 + row;
+      const T *p = static_cast<const T *>(a.q.p) + (w.start + place / a.group) * a.q.row_stride +
+                   (w.head * a.group + place % a.group) * a.q.head_stride;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t d = k * 16 + j * 8 + (lane & 3) * 2;
+          q[k][i + 2 * j] = row <= w.last && d < a.cache.D ? *reinterpret_cast<const uint32_t *>(p + d) : 0u;
+        }
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  }
+
+  __device__ __forceinline__ void step(const AttentionArgs &a, uint32_t from, uint32_t key, unsigned good, bool full,
+                                       uint32_t, const Bounds &bounds, float *) {
+    const uint32_t lane = threadIdx.x & 31;
+    const float scale = a.scale * kLog2e;
+    float x[2][4] = {};
+    {
+      const uint32_t row = (lane >> 4) * 8 + (lane & 7), ch = (lane >> 3) & 1;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t b[4];
+        load_matrices(from + spot(row, k * 2 + ch), b);
+        mma16<T>(x[0], q[k], b[0], b[1]);
+        mma16<T>(x[1], q[k], b[2], b[3]);
+      }
+    }
+    // element e of x[n]: row lane / 4 + 8 (e / 2), key 8 n + 2 (lane & 3) + (e & 1)
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[n][e] *= scale;
+        if (!full) {
+          const uint32_t i = n * 8 + (lane & 3) * 2 + (e & 1), j = key + i, row = lane / 4 + 8 * (e >> 1);
+          if (!(good >> i & 1) || j < bounds.from[row] || j >= bounds.to[row]) x[n][e] = -INFINITY;
+        }
+        top[e >> 1] = fmaxf(top[e >> 1], x[n][e]);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2)) - kShift;
+    }
+    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float now = fmaxf(m[i], top[i]);
+        const float f = now == m[i] ? 1.0f : ex2_approx(m[i] - now);
+        m[i] = now;
+        l[i] *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) {
+          o[d][2 * i] *= f;
+          o[d][2 * i + 1] *= f;
+        }
+      }
+    }
+    const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[n][e] = ex2_approx(x[n][e] - base[e >> 1]);
+        l[e >> 1] += x[n][e];
+      }
+    // the numerators' rounding to the type, which the matrix instructions ask for;
+    // their sum stays in fp32
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float lo = x[i >> 1][(i & 1) * 2], hi = x[i >> 1][(i & 1) * 2 + 1];
+      if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2 &>(p[i]) = __floats2half2_rn(lo, hi);
+      else reinterpret_cast<__nv_bfloat162 &>(p[i]) = __floats2bfloat162_rn(lo, hi);
+    }
+    const uint32_t row = lane & 15, ch = lane >> 4;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      uint32_t b[4];
+      load_transposed(from + kHalf + spot(row, d * 2 + ch), b);
+      mma16<T>(o[2 * d], p, b[0], b[1]);
+      mma16<T>(o[2 * d + 1], p, b[2], b[3]);
+    }
+  }
+
+  // outs: [row][DP]
+  __device__ __forceinline__ void leave(uint32_t, float *outs, float *ms, float *ls) {
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t row = lane / 4 + 8 * i;
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d)
+        *reinterpret_cast<float2 *>(outs + row * DP + d * 8 + (lane & 3) * 2) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+      if ((lane & 3) == 0) {
+        ms[row] = m[i];
+        ls[row] = l[i];
+      }
+    }
+  }
+};
+
+// fp32 on the CUDA cores (split into tf32 parts on the tensor cores the
+// output was 1.0e-6 from the exact one where this is at 2e-7): four lanes a
+// key for the scores, every lane a few elements of all rows for the output.
+template <int DP> struct Lane<float, DP> {
+  static constexpr uint32_t N = 8, kHalf = N * DP * 4;
+  static constexpr int V = DP / 16;  // vectors of a lane's part of a key
+  static constexpr int E = DP / 32;  // elements of the output that a lane has
+  float m[kRows], l[kRows], o[kRows][E];
+
+  // lanes 0..7 read two keys at once
+  static __device__ __forceinline__ uint32_t spot(uint32_t row, uint32_t ch) { return row * (DP * 4) + ((ch ^ ((row & 1) << 2)) << 4); }
+
+  // shared: the queries, negated where the scale is negative, then each warp's probabilities
+  __device__ __forceinline__ void begin(const AttentionArgs &a, const Piece &w, float *shared) {
+    const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
+    for (uint32_t i = threadIdx.x; i < kRows * DP; i += kThreads) {
+      const uint32_t row = i / DP, d = i % DP;
+      const uint64_t place = w.row0 + row;
+      float x = 0.0f;
+      if (row <= w.last && d < a.cache.D)
+        x = sign * (static_cast<const float *>(a.q.p) + (w.start + place / a.group) * a.q.row_stride +
+                    (w.head * a.group + place % a.group) * a.q.head_stride)[d];
+      shared[i] = x;
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < kRows; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[r][e] = 0.0f;
+    }
+  }
+
+  __device__ __forceinline__ void step(const AttentionArgs &a, uint32_t from, uint32_t key, unsigned good, bool full,
+                                       uint32_t last, const Bounds &bounds, float *shared) {
+    const uint32_t lane = threadIdx.x & 31, k = lane >> 2, part = lane & 3;
+    const float c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
+    const uint32_t queries = static_cast<uint32_t>(__cvta_generic_to_shared(shared));
+    float *const p = shared + kRows * DP + threadIdx.x / 32 * kRows * 8;
+    float4 x[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = load_vector(from + spot(k, i * 4 + part));
+#pragma unroll
+    for (uint32_t r = 0; r < kRows; ++r) {
+      if (r > last) break;
+      float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float4 q = load_vector(queries + (r * DP + (i * 4 + part) * 4) * 4);
+        s0 = fmaf(x[i].x, q.x, s0);
+        s1 = fmaf(x[i].y, q.y, s1);
+        s2 = fmaf(x[i].z, q.z, s2);
+        s3 = fmaf(x[i].w, q.w, s3);
+      }
+      float s = (s0 + s1) + (s2 + s3);
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (!full && (!(good >> k & 1) || key + k < bounds.from[r] || key + k >= bounds.to[r])) s = -INFINITY;
+      float top = s;
+#pragma unroll
+      for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+      top *= c;
+      if (top > m[r]) {
+        const float f = ex2_approx(m[r] - top);
+        m[r] = top;
+        l[r] *= f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[r][e] *= f;
+      }
+      const float e = ex2_approx(fmaf(s, c, m[r] == -INFINITY ? 0.0f : -m[r]));
+      l[r] += e;
+      if (part == 0) p[r * 8 + k] = e;
+    }
+    __syncwarp();
+    float v[N][E];
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+      const uint32_t at = from + kHalf + spot(i, lane * E / 4) + lane * E % 4 * 4;
+      if constexpr (E == 4) {
+        const float4 y = load_vector(at);
+        v[i][0] = y.x, v[i][1] = y.y, v[i][2] = y.z, v[i][3] = y.w;
+      } else {
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[i][0]), "=f"(v[i][1]) : "r"(at) : "memory");
+      }
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < kRows; ++r) {
+      if (r > last) break;
+      const float4 p0 = reinterpret_cast<const float4 *>(p + r * 8)[0], p1 = reinterpret_cast<const float4 *>(p + r * 8)[1];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float y = fmaf(p0.x, v[0][e], o[r][e]);
+        y = fmaf(p0.y, v[1][e], y);
+        y = fmaf(p0.z, v[2][e], y);
+        y = fmaf(p0.w, v[3][e], y);
+        y = fmaf(p1.x, v[4][e], y);
+        y = fmaf(p1.y, v[5][e], y);
+        y = fmaf(p1.z, v[6][e], y);
+        o[r][e] = fmaf(p1.w, v[7][e], y);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void leave(uint32_t last, float *outs, float *ms, float *ls) {
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (uint32_t r = 0; r < kRows; ++r) {
+      if (r > last) break;
+#pragma unroll
+      for (int i = 4; i < 32; i <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], i);
+#pragma unroll
+      for (int e = 0; e < E; ++e) outs[r * DP + lane * E + e] = o[r][e];
+      if (lane == 0) {
+        ms[r] = m[r];
+        ls[r] = l[r];
+      }
+    }
+  }
 };
 
 template <typename T, typename TO, int DP>
 __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a) {
-  constexpr uint32_t N = Step<T>::kKeys;       // keys of a warp's step
+  using L = Lane<T, DP>;
+  constexpr uint32_t N = L::N;                 // keys of a warp's step
   constexpr uint32_t KEYS = N * kWarps;        // of a block
   constexpr uint32_t E = 16 / sizeof(T);       // elements of a vector
   constexpr uint32_t CH = DP / E;              // vectors of a row
-  constexpr int KS = DP / (sizeof(T) == 2 ? 16 : 8);  // steps of the first product
-  constexpr uint32_t kHalf = N * DP * sizeof(T);
+  constexpr uint32_t kHalf = L::kHalf;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
+  __shared__ Bounds bounds;
+  float *const shared = reinterpret_cast<float *>(smem + kWarps * kStages * 2 * kHalf);
   pdl_enter();
   const tl_paged_cache &c = a.cache;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-  const Share share = share_of<kRows, KEYS, kThreads>(a, blockIdx.x, gridDim.x, a.whole ? 1 : 4);
+  const Share share = share_of<kRows, KEYS, kThreads>(a, blockIdx.x, gridDim.x, a.whole ? 1 : kLeast * KEYS);
   Join join{0xffffffffu, 0, 0, 0};
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * kStages * 2 * kHalf;
-  const float scale = a.scale * kLog2e;
 
-  uint32_t s = share.sequence;
-  uint64_t offset = share.offset, left = share.any ? share.size : 0, at = share.begin;
-  Work<kRows, KEYS> w;
-  if (left) w.set(a, s);
-  while (left) {
-    const uint64_t line = w.cost(a);
-    if (offset >= line) {  // the next sequence with any rows
-      offset -= line;
-      ++s;
-      w.set(a, s);
-      continue;
-    }
-    // this job, and the part of its blocks that is ours
-    const uint32_t span = a.whole ? 1 : w.blocks;
-    const uint32_t job = static_cast<uint32_t>(offset / span), block0 = static_cast<uint32_t>(offset % span);
-    const uint32_t tile = job / c.heads, head = job % c.heads;
-    const uint32_t take = static_cast<uint32_t>(min(left, static_cast<uint64_t>(span - block0)));
-    const bool opens = block0 == 0, ends = block0 + take == span;
-    const uint32_t b_lo = w.first + (a.whole ? 0 : block0), b_hi = w.first + (a.whole ? w.blocks : block0 + take);
-
+  Walk<kRows, KEYS> walk;
+  Piece w;
+  walk.start(a, share);
+  while (walk.next(a, share, w)) {
     // rows
-    const uint64_t row0 = static_cast<uint64_t>(tile) * kRows, rows = static_cast<uint64_t>(w.q.count) * a.group;
-    const int64_t position0 = static_cast<int64_t>(w.q.length) - w.q.count;
-    const uint32_t last = static_cast<uint32_t>(min(row0 + kRows, rows) - 1 - row0);
-    uint32_t all_from, all_to, f, t;
-    seen(a, w.q.length, position0 + static_cast<int64_t>(row0 / a.group), all_from, t);
-    uint32_t least_to = t;
-    seen(a, w.q.length, position0 + static_cast<int64_t>((row0 + last) / a.group), f, all_to);
-    const uint32_t most_from = f;
+    const uint32_t head = w.head, last = w.last;
+    const uint64_t row0 = w.row0;
+    uint32_t all_from = w.from, all_to = w.to, most_from, least_to, f, t;
+    seen(a, w.length, w.position(a, 0), f, least_to);
+    seen(a, w.length, w.position(a, last), most_from, t);
     const bool uneven = all_from != most_from || all_to != least_to;
-    Rows r;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t row = lane / 4 + 8 * i;
-      r.from[i] = r.to[i] = 0;
-      if (row <= last) seen(a, w.q.length, position0 + static_cast<int64_t>((row0 + row) / a.group), r.from[i], r.to[i]);
+    if (threadIdx.x < kRows) {
+      uint32_t from = 0, to = 0;
+      if (threadIdx.x <= last) seen(a, w.length, w.position(a, threadIdx.x), from, to);
+      bounds.from[threadIdx.x] = from;
+      bounds.to[threadIdx.x] = to;
     }
-    const uint32_t key_lo = max(b_lo * KEYS, all_from / N * N);
-    const uint32_t key_hi = static_cast<uint32_t>(min(static_cast<uint64_t>(b_hi) * KEYS, static_cast<uint64_t>(all_to)));
+    const uint32_t key_hi = static_cast<uint32_t>(min(static_cast<uint64_t>(w.block_hi) * KEYS, static_cast<uint64_t>(all_to)));
     // this warp's steps: keys first_key + i KEYS
-    const uint32_t skip = key_lo > b_lo * KEYS ? (key_lo - b_lo * KEYS) / KEYS : 0;
-    const uint32_t first_key = b_lo * KEYS + skip * KEYS + warp * N;
+    const uint32_t first_key = w.block_lo * KEYS + warp * N;
     const uint32_t steps = first_key < key_hi ? (key_hi - first_key + KEYS - 1) / KEYS : 0;
 
-    // queries as the first product's left operand
-    // (fp32: split, in shared memory, as 128 registers a lane would not be left)
-    uint32_t qa[sizeof(T) == 2 ? KS : 1][4];
-    uint4 *const halves = reinterpret_cast<uint4 *>(smem + kWarps * kStages * 2 * kHalf) + lane;
-    if constexpr (sizeof(T) == 4) {
-      for (uint32_t k = warp; k < KS; k += kWarps) {
-        uint32_t big[4], small[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t row = lane / 4 + 8 * i;
-          const uint64_t place = row0 + row;
-          const T *p = static_cast<const T *>(a.q.p) + (w.q.start + place / a.group) * a.q.row_stride +
-                       (head * a.group + place % a.group) * a.q.head_stride;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t d = k * 8 + j * 4 + (lane & 3);
-            split(row <= last && d < c.D ? heads::element_of(p[d]) : 0.0f, big[i + 2 * j], small[i + 2 * j]);
-          }
-        }
-        halves[k * 64] = make_uint4(big[0], big[1], big[2], big[3]);
-        halves[k * 64 + 32] = make_uint4(small[0], small[1], small[2], small[3]);
-      }
-      __syncthreads();
-    } else {
-      const T *q = static_cast<const T *>(a.q.p);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t row = lane / 4 + 8 * i;
-        const uint64_t place = row0 + row;
-        const T *p = q + (w.q.start + place / a.group) * a.q.row_stride + (head * a.group + place % a.group) * a.q.head_stride;
-        const bool there = row <= last;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t d = k * 16 + j * 8 + (lane & 3) * 2;
-            qa[k][i + 2 * j] = there && d < c.D ? *reinterpret_cast<const uint32_t *>(p + d) : 0u;
-          }
-      }
-    }
-
+    L rows;
+    rows.begin(a, w, shared);
+    __syncthreads();
     const T *kp = static_cast<const T *>(c.k) + head * c.head_stride;
     const T *vp = static_cast<const T *>(c.v) + head * c.head_stride;
     // where lane i's key of a step lies, -1 where there is none
     const auto offset_of = [&](uint32_t step) -> int64_t {
       const uint32_t j = first_key + step * KEYS + lane;
-      return step < steps && lane < N && j >= all_from && j < key_hi ? key_offset(a, s, j) : -1;
+      return step < steps && lane < N && j >= all_from && j < key_hi ? key_offset(a, w.sequence, j) : -1;
     };
     const auto bring = [&](uint32_t step, int64_t from) {
       const uint32_t to = ring + (step % kStages) * 2 * kHalf;
@@ -214,14 +377,11 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
         const int64_t place = __shfl_sync(0xffffffffu, from, row);
         const bool there = place >= 0 && ch * E < c.D;
         const uint64_t e = there ? place + ch * E : 0;
-        const uint32_t spot = to + row * (DP * sizeof(T)) + ((ch ^ (row & 7)) << 4);
+        const uint32_t spot = to + L::spot(row, ch);
         copy16(spot, kp + e, there);
         copy16(spot + kHalf, vp + e, there);
       }
     };
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[DP / 8][4];
-#pragma unroll
-    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     unsigned good[kStages];  // a bit for every key that is there
     int64_t next = offset_of(0);
 #pragma unroll
@@ -244,135 +404,17 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
         __syncwarp();
         const uint32_t from = ring + u * 2 * kHalf, key = first_key + step * KEYS;
         const bool full = good[u] == (1u << N) - 1 && key >= most_from && key + N <= least_to;
-        float x[N / 8][4];
-#pragma unroll
-        for (uint32_t n = 0; n < N / 8; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
-        if constexpr (sizeof(T) == 2) {
-          const uint32_t row = (lane >> 4) * 8 + (lane & 7), ch = (lane >> 3) & 1;
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            uint32_t b[4];
-            load_matrices(from + row * (DP * 2) + (((k * 2 + ch) ^ (row & 7)) << 4), b);
-            mma16<T>(x[0], qa[k], b[0], b[1]);
-            mma16<T>(x[1], qa[k], b[2], b[3]);
-          }
-        } else {
-          const uint32_t row = lane >> 2;
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            uint32_t b0, b1, s0, s1;
-            split(load_word(from + row * (DP * 4) + (((k * 2) ^ row) << 4) + (lane & 3) * 4), b0, s0);
-            split(load_word(from + row * (DP * 4) + (((k * 2 + 1) ^ row) << 4) + (lane & 3) * 4), b1, s1);
-            const uint4 qb = halves[k * 64], qs = halves[k * 64 + 32];
-            const uint32_t big[4] = {qb.x, qb.y, qb.z, qb.w}, small[4] = {qs.x, qs.y, qs.z, qs.w};
-            mma8(x[0], small, b0, b1);
-            mma8(x[0], big, s0, s1);
-            mma8(x[0], big, b0, b1);
-          }
-        }
-        // element e of x[n]: row lane / 4 + 8 (e / 2), key 8 n + 2 (lane & 3) + (e & 1)
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (uint32_t n = 0; n < N / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[n][e] *= scale;
-            if (!full) {
-              const uint32_t i = n * 8 + (lane & 3) * 2 + (e & 1), j = key + i;
-              if (!(good[u] >> i & 1) || j < r.from[e >> 1] || j >= r.to[e >> 1]) x[n][e] = -INFINITY;
-            }
-            top[e >> 1] = fmaxf(top[e >> 1], x[n][e]);
-          }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-          top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2)) - Step<T>::kShift;
-        }
-        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float now = fmaxf(m[i], top[i]);
-            const float f = now == m[i] ? 1.0f : ex2_approx(m[i] - now);
-            m[i] = now;
-            l[i] *= f;
-#pragma unroll
-            for (int d = 0; d < DP / 8; ++d) {
-              o[d][2 * i] *= f;
-              o[d][2 * i + 1] *= f;
-            }
-          }
-        }
-        const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-#pragma unroll
-        for (uint32_t n = 0; n < N / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[n][e] = ex2_approx(x[n][e] - base[e >> 1]);
-            l[e >> 1] += x[n][e];
-          }
-        const uint32_t values = from + kHalf;
-        if constexpr (sizeof(T) == 2) {
-          uint32_t p[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float lo = x[i >> 1][(i & 1) * 2], hi = x[i >> 1][(i & 1) * 2 + 1];
-            if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2 &>(p[i]) = __floats2half2_rn(lo, hi);
-            else reinterpret_cast<__nv_bfloat162 &>(p[i]) = __floats2bfloat162_rn(lo, hi);
-          }
-          const uint32_t row = lane & 15, ch = lane >> 4;
-#pragma unroll
-          for (int d = 0; d < DP / 16; ++d) {
-            uint32_t b[4];
-            load_transposed(values + row * (DP * 2) + (((d * 2 + ch) ^ (row & 7)) << 4), b);
-            mma16<T>(o[2 * d], p, b[0], b[1]);
-            mma16<T>(o[2 * d + 1], p, b[2], b[3]);
-          }
-        } else {
-          // The left operand's column j (and j + 4) of a lane is key 2 j (2 j + 1), as the
-          // scores lie, so the values' rows are taken in the same order.
-          uint32_t p[4], ps[4];
-          split(x[0][0], p[0], ps[0]);
-          split(x[0][2], p[1], ps[1]);
-          split(x[0][1], p[2], ps[2]);
-          split(x[0][3], p[3], ps[3]);
-          const uint32_t k0 = (lane & 3) * 2, n = lane >> 2;
-#pragma unroll
-          for (int d = 0; d < DP / 8; ++d) {
-            uint32_t b0, b1, s0, s1;
-            const uint32_t ch = d * 2 + (n >> 2);
-            split(load_word(values + k0 * (DP * 4) + ((ch ^ k0) << 4) + (n & 3) * 4), b0, s0);
-            split(load_word(values + (k0 + 1) * (DP * 4) + ((ch ^ (k0 + 1)) << 4) + (n & 3) * 4), b1, s1);
-            mma8(o[d], ps, b0, b1);
-            mma8(o[d], p, s0, s1);
-            mma8(o[d], p, b0, b1);
-          }
-        }
+        rows.step(a, from, key, good[u], full, last, bounds, shared);
         __syncwarp();
       }
     }
     await<0>();
     // the CTA's warps into one: outputs through the ring, a row's four warps by one warp
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    }
     __syncthreads();
     float *const outs = reinterpret_cast<float *>(smem);  // [warp][row][DP]
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t row = lane / 4 + 8 * i;
-#pragma unroll
-      for (int d = 0; d < DP / 8; ++d)
-        *reinterpret_cast<float2 *>(outs + (warp * kRows + row) * DP + d * 8 + (lane & 3) * 2) =
-            make_float2(o[d][2 * i], o[d][2 * i + 1]);
-      if ((lane & 3) == 0) {
-        sm_m[warp][row] = m[i];
-        sm_l[warp][row] = l[i];
-      }
-    }
+    rows.leave(last, outs + warp * kRows * DP, sm_m[warp], sm_l[warp]);
     __syncthreads();
-    float *const part = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (opens ? 1 : 0)) * part_floats<DP>();
+    float *const part = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (w.opens ? 1 : 0)) * part_floats<kRows, DP>();
     for (uint32_t row = warp; row <= last; row += kWarps) {
       float mm = sm_m[0][row], ll = 0.0f, acc[DP / 32];
 #pragma unroll
@@ -389,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
         for (int e = 0; e < DP / 32; ++e) acc[e] = fmaf(f, outs[(i * kRows + row) * DP + lane + 32 * e], acc[e]);
       }
       const uint64_t place = row0 + row;
-      const uint64_t token = w.q.start + place / a.group;
+      const uint64_t token = w.start + place / a.group;
       const uint32_t h = head * a.group + static_cast<uint32_t>(place % a.group);
       bool nan = false;
 #pragma unroll
@@ -398,18 +440,18 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
         // A value that other rows of the tile see, and this one does not, is not
         // finite (0 times it is NaN): the row's own keys one by one.
         float again[kMaxHead / 32];
-        seen(a, w.q.length, position0 + static_cast<int64_t>(place / a.group), f, t);
+        seen(a, w.length, w.position(a, row), f, t);
         const T *q = static_cast<const T *>(a.q.p) + token * a.q.row_stride + h * a.q.head_stride;
-        row_over_keys<T>(a, s, head, q, max(f, b_lo * KEYS), min(t, key_hi), lane, mm, ll, again);
+        row_over_keys<T>(a, w.sequence, head, q, max(f, w.block_lo * KEYS), min(t, key_hi), lane, mm, ll, again);
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) acc[e] = again[e];
       }
-      if (opens && ends) {
+      if (w.opens && w.ends) {
         TO *out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e)
           if (lane + 32 * e < c.D) heads::set_element(out[lane + 32 * e], ll == 0.0f ? 0.0f : acc[e] / ll);
-        if (lane == 0 && a.lse) a.lse[token * a.q_heads + h] = ll == 0.0f ? -INFINITY : mm * kLn2 + logf(ll);
+        if (lane == 0) put_lse<TO>(a, token, h, mm, ll);
       } else {
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) part[row * DP + lane + 32 * e] = acc[e];
@@ -419,64 +461,23 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
         }
       }
     }
-    if (!opens && ends) join = Join{static_cast<uint32_t>((at - block0) / share.full), s, head, tile};
+    if (!w.opens && w.ends) join = Join{w.first_cta, w.sequence, head, w.tile};
     __syncthreads();  // the ring is free again
-    offset += take;
-    at += take;
-    left -= take;
   }
   if (!a.whole && threadIdx.x == 0) a.joins[blockIdx.x] = join;
-}
-
-// The jobs that were cut: a warp per row adds the partial results up in the
-// order of the keys.
-template <typename TO, int DP>
-__global__ void __launch_bounds__(kThreads) join_kernel(const AttentionArgs a) {
-  pdl_enter();
-  const Join j = a.joins[blockIdx.x];
-  if (j.first == 0xffffffffu) return;
-  const uint32_t lane = threadIdx.x & 31, row = blockIdx.y * kWarps + threadIdx.x / 32, end = blockIdx.x;
-  const Sequence q = sequence_of(a.cache, j.sequence, a.most);
-  const uint64_t place = static_cast<uint64_t>(j.tile) * kRows + row;
-  if (place >= static_cast<uint64_t>(q.count) * a.group) return;
-  const auto part = [&](uint32_t cta) { return a.parts + (static_cast<size_t>(cta) * 2 + (cta == j.first ? 1 : 0)) * part_floats<DP>(); };
-  float mm = -INFINITY;
-  for (uint32_t i = j.first + lane; i <= end; i += 32) mm = fmaxf(mm, part(i)[kRows * DP + row]);
-  mm = warp_max(mm);
-  float ll = 0.0f, acc[DP / 32];
-#pragma unroll
-  for (int e = 0; e < DP / 32; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-  for (uint32_t i = j.first; i <= end; ++i) {
-    const float *p = part(i);
-    const float wm = p[kRows * DP + row], f = wm == -INFINITY ? 0.0f : ex2_approx(wm - mm);
-    ll = fmaf(f, p[kRows * DP + kRows + row], ll);
-#pragma unroll
-    for (int e = 0; e < DP / 32; ++e) {
-      const float x = p[row * DP + lane + 32 * e];
-      if (f != 0.0f) acc[e] = fmaf(f, x, acc[e]);
-    }
-  }
-  const uint64_t token = q.start + place / a.group;
-  const uint32_t h = j.head * a.group + static_cast<uint32_t>(place % a.group);
-  TO *out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;
-#pragma unroll
-  for (int e = 0; e < DP / 32; ++e)
-    if (lane + 32 * e < a.cache.D) heads::set_element(out[lane + 32 * e], ll == 0.0f ? 0.0f : acc[e] / ll);
-  if (lane == 0 && a.lse) a.lse[token * a.q_heads + h] = ll == 0.0f ? -INFINITY : mm * kLn2 + logf(ll);
 }
 
 template <typename T, typename TO, int DP> void launch(const AttentionArgs &a, const Plan &p, cudaStream_t s) {
   constexpr size_t smem = smem_bytes<T, DP>();
   (void)cudaFuncSetAttribute(step_kernel<T, TO, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   launch_pdl(step_kernel<T, TO, DP>, p.ctas, kThreads, smem, s, a);
-  if (!p.whole) launch_pdl(join_kernel<TO, DP>, dim3(p.ctas, kRows / kWarps), kThreads, 0, s, a);
+  if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, kRows / 4), 128, 0, s, a);
 }
 
 }  // namespace
 
 Plan step_plan(const AttentionArgs &a, uint32_t max_new) {
-  const uint32_t keys = kWarps * (a.cache.type == TL_FLOAT32 ? Step<float>::kKeys : Step<__half>::kKeys);
+  const uint32_t keys = kWarps * (a.cache.type == TL_FLOAT32 ? step_keys<float>() : step_keys<__half>());
   const uint32_t dp = a.cache.D > 64 ? 128 : 64;
   Plan p{};
   p.whole = most_blocks(a, max_new, keys) <= 8;

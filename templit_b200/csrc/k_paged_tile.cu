@@ -1,0 +1,563 @@
+// Attention over a paged cache for many query rows a key head (chunks of a
+// prompt) in 16-bit types (include/templit_cuda.h: tl_paged_attention).
+//
+// Bound by the tensor cores and the softmax's exponentials: 128 x 128 scores
+// of 128 elements are 512 cycles of each product and 1024 of the 16
+// exponentials a cycle of an SM.  So a CTA, one an SM, holds two tiles of 128
+// query rows (tokens, a token's heads of one key head side by side), and
+// while one is in the softmax the other is multiplied:
+//   warps 0-3, 4-7  softmax of tile 0 and 1, a row a thread: scores out of
+//                   TMEM, numerators rounded to the type back into the same
+//                   TMEM columns, where the second product takes them from;
+//                   running maximum and sum in registers.  The output stays
+//                   in TMEM and is rescaled only when a row's maximum grew
+//                   by more than 2^8 (numerators then are at most 2^8, which
+//                   fp32 sums and 16-bit types hold)
+//   warps 8-11      keys and values, 128 at a time, by cp.async into a ring
+//                   (pages end anywhere, so rows come one by one, 16 bytes a
+//                   lane, a page's address looked up once a row), and the queries
+//   warp 12         one thread issues S = Q K^T and O += P V (tcgen05.mma
+//                   kind::f16, fp32 in TMEM)
+// TMEM: 2 x 128 columns of scores (numerators over their second half), 2 x
+// 128 of outputs.  Every wait is bounded (2 s); where one gives up, the CTA
+// raises TL_FLAG_TIMEOUT, waits for what it issued and returns.  Shares of
+// the keys and their joining: paged_attention.cuh.
+#include "paged_attention.cuh"
+#include "tc_ptx.cuh"
+
+namespace tl {
+namespace paged {
+namespace {
+
+constexpr uint32_t kTile = 128, kRows = 2 * kTile, kKeys = 128;
+constexpr int kThreads = 13 * 32, kLoaders = 128;
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
+constexpr float kSlack = 8.0f;  // log2 of how far numerators may pass 1
+constexpr int kLag = 2;         // ring places between a copy's issue and its hand-over
+constexpr int kMasks = 8;       // blocks whose missing keys are remembered: more than the ring is ahead
+
+template <int DP> constexpr uint32_t tile_bytes() { return kTile * DP * 2; }
+template <int DP> constexpr int stages() { return DP == 128 ? 5 : 8; }
+
+struct Barriers {
+  uint64_t full[8], empty[8];
+  uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free[2], drained;
+};
+struct Shared {
+  Barriers b;
+  uint32_t tmem, gave_up;
+  uint32_t mask[kMasks][4];  // a bit for every key of a block that is there
+};
+template <int DP> constexpr size_t smem_bytes() {
+  return 1024 + 2 * tile_bytes<DP>() + stages<DP>() * static_cast<size_t>(tile_bytes<DP>()) + sizeof(Shared);
+}
+
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Waits for a phase; false where it gave up, here or elsewhere in the CTA.
+__device__ __forceinline__ bool wait(Shared &sh, uint64_t *bar, uint32_t parity, uint32_t *status) {
+  if (ptx::mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = ptx::global_timer_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 0) {
+      if (*reinterpret_cast<volatile uint32_t *>(&sh.gave_up)) return false;
+      if (ptx::global_timer_ns() - t0 > kWaitLimitNs) {
+        *reinterpret_cast<volatile uint32_t *>(&sh.gave_up) = 1;
+        raise_flag(status, TL_FLAG_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+
+// Vector `ch` (16 bytes) of row `r` of a tile: 128-byte rows of 64 elements
+// with the 128-byte swizzle, one block of 128 rows after another.
+__device__ __forceinline__ uint32_t spot(uint32_t r, uint32_t ch) {
+  return (ch >> 3) * (kTile * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+}
+// Queries and keys, K-major: elements [16 k, 16 k + 16).
+__device__ __forceinline__ uint64_t row_desc(uint32_t base, uint32_t k) {
+  return ptx::smem_desc(base + (k >> 2) * (kTile * 128) + (k & 3) * 32, 16, 1024, ptx::kSwizzle128B);
+}
+// Values, MN-major (a row is a key): keys [16 k, 16 k + 16), 64 elements a block.
+__device__ __forceinline__ uint64_t value_desc(uint32_t base, uint32_t k) {
+  return ptx::smem_desc(base + k * 2048, kTile * 128, 1024, ptx::kSwizzle128B);
+}
+// kind::f16 with fp32 sums: type 0 = fp16, 1 = bf16.
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t type, uint32_t M, uint32_t N, bool b_mn) {
+  return (1u << 4) | (type << 7) | (type << 10) | ((b_mn ? 1u : 0u) << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 16 and 32 columns of this warp's 32 lanes into TMEM
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2 &>(r) = __floats2half2_rn(lo, hi);
+  else reinterpret_cast<__nv_bfloat162 &>(r) = __floats2bfloat162_rn(lo, hi);
+  return r;
+}
+// log2 of what the largest numerator is at least: with kSlack, fp16's stay
+// below 2^15 and keep their bits down to 2^-21 of the largest
+template <typename T> constexpr float shift() { return std::is_same<T, __half>::value ? 7.0f : 0.0f; }
+
+// Blocks of a piece that tile t takes, from the piece's first on; both tiles
+// start there.
+__device__ __forceinline__ uint32_t tile_blocks(const AttentionArgs &a, const Piece &p, uint32_t t) {
+  if (t * kTile > p.last) return 0;
+  uint32_t from, to;
+  seen(a, p.length, p.position(a, min((t + 1) * kTile - 1, p.last)), from, to);
+  const uint32_t end = min((to + (kKeys - 1)) / kKeys, p.block_hi);
+  return end > p.block_lo ? end - p.block_lo : 0;
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void load(const AttentionArgs &a, const Share &share, Shared &sh, uint32_t queries, uint32_t ring) {
+  constexpr int S = stages<DP>();
+  constexpr uint32_t CH = DP / 8, kBytes = tile_bytes<DP>();
+  const uint32_t lane = threadIdx.x & 31, warp = (threadIdx.x - 256) / 32;
+  const tl_paged_cache &c = a.cache;
+  uint32_t item = 0, handed = 0, block_count = 0, q_phase = 0;
+  // copies up to `upto` have arrived and are the tensor cores' to read
+  const auto hand_over = [&](uint32_t upto) {
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    for (; handed < upto; ++handed)
+      if (lane == 0) ptx::mbar_arrive(&sh.b.full[handed % S]);
+  };
+  Walk<kRows, kKeys> walk;
+  Piece p;
+  walk.start(a, share);
+  while (walk.next(a, share, p)) {
+    const uint32_t n0 = tile_blocks(a, p, 0), n1 = tile_blocks(a, p, 1), n = max(n0, n1);
+    if (!n) continue;
+    // the queries: the rows of this warp, 32 of each tile
+    await<0>();
+    hand_over(item);
+    if (!wait(sh, &sh.b.q_empty, (q_phase & 1) ^ 1, a.status)) return;
+    ++q_phase;
+#pragma unroll
+    for (uint32_t t = 0; t < 2; ++t) {
+      const uint32_t mine = t * kTile + warp * 32 + lane;
+      const uint64_t place = p.row0 + mine;
+      int64_t at = -1;
+      if (mine <= p.last)
+        at = static_cast<int64_t>((p.start + place / a.group) * a.q.row_stride + (p.head * a.group + place % a.group) * a.q.head_stride);
+#pragma unroll 4
+      for (uint32_t i = 0; i < CH; ++i) {
+        const uint32_t row = (lane + 32 * i) / CH, ch = (lane + 32 * i) % CH;
+        const int64_t from = __shfl_sync(0xffffffffu, at, row);
+        const bool there = from >= 0 && ch * 8 < c.D;
+        copy16(queries + t * kBytes + spot(warp * 32 + row, ch), static_cast<const T *>(a.q.p) + (there ? from + ch * 8 : 0), there);
+      }
+    }
+    commit();
+    await<0>();
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&sh.b.q_full);
+
+    const T *kp = static_cast<const T *>(c.k) + p.head * c.head_stride;
+    const T *vp = static_cast<const T *>(c.v) + p.head * c.head_stride;
+    const auto offset_of = [&](uint32_t block) -> int64_t {
+      const uint32_t j = (p.block_lo + block) * kKeys + warp * 32 + lane;
+      return block < n && j >= p.from && j < p.to ? key_offset(a, p.sequence, j) : -1;
+    };
+    int64_t at = offset_of(0);
+    for (uint32_t j = 0; j < n; ++j) {
+      const int64_t next = offset_of(j + 1);
+      const uint32_t good = __ballot_sync(0xffffffffu, at >= 0);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // a slot is free again when what was multiplied from it is done
+        if (!wait(sh, &sh.b.empty[item % S], ((item / S) & 1) ^ 1, a.status)) return;
+        if (half == 0 && lane == 0) sh.mask[block_count % kMasks][warp] = good;
+        const T *base = half ? vp : kp;
+        const uint32_t to = ring + (item % S) * kBytes;
+#pragma unroll 8
+        for (uint32_t i = 0; i < CH; ++i) {
+          const uint32_t row = (lane + 32 * i) / CH, ch = (lane + 32 * i) % CH;
+          const int64_t from = __shfl_sync(0xffffffffu, at, row);
+          const bool there = from >= 0 && ch * 8 < c.D;
+          copy16(to + spot(warp * 32 + row, ch), base + (there ? from + ch * 8 : 0), there);
+        }
+        commit();
+        ++item;
+        await<kLag>();
+        if (item > kLag) hand_over(max(handed, item - kLag));
+      }
+      ++block_count;
+      at = next;
+    }
+  }
+  await<0>();
+  hand_over(item);
+  // the last reads of the ring are over
+  for (uint32_t i = item > static_cast<uint32_t>(S) ? item - S : 0; i < item; ++i)
+    if (!wait(sh, &sh.b.empty[i % S], (i / S) & 1, a.status)) return;
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void multiply(const AttentionArgs &a, const Share &share, Shared &sh, uint32_t queries, uint32_t ring) {
+  constexpr int S = stages<DP>();
+  constexpr uint32_t kBytes = tile_bytes<DP>();
+  constexpr uint32_t type = std::is_same<T, __half>::value ? 0 : 1;
+  const uint32_t ksteps = (a.cache.D + 15) / 16;
+  const uint32_t score = idesc_f16(type, kTile, kKeys, false), output = idesc_f16(type, kTile, ksteps * 16, true);
+  const uint32_t tmem = sh.tmem;
+  uint32_t item = 0, piece = 0, s_count[2] = {0, 0}, opened[2] = {0, 0};
+  Walk<kRows, kKeys> walk;
+  Piece p;
+  walk.start(a, share);
+  const auto scores = [&](uint32_t t, uint32_t slot) {
+    ptx::tc_fence_after();
+    for (uint32_t k = 0; k < ksteps; ++k)
+      mma_smem(tmem + t * 128, row_desc(queries + t * kBytes, k), row_desc(ring + slot * kBytes, k), score, k > 0);
+    ptx::mma_commit(&sh.b.s_full[t]);
+  };
+  while (walk.next(a, share, p)) {
+    const uint32_t n[2] = {tile_blocks(a, p, 0), tile_blocks(a, p, 1)}, most = max(n[0], n[1]);
+    if (!most) continue;
+    if (!wait(sh, &sh.b.q_full, piece & 1, a.status)) return;
+    ++piece;
+    const uint32_t first = item;  // block j: keys in place first + 2 j, values behind them
+    if (!wait(sh, &sh.b.full[first % S], (first / S) & 1, a.status)) return;
+#pragma unroll
+    for (uint32_t t = 0; t < 2; ++t)
+      if (n[t]) scores(t, first % S);
+    ptx::mma_commit(&sh.b.empty[first % S]);
+    for (uint32_t j = 0; j < most; ++j) {
+      const uint32_t v = first + 2 * j + 1, k = v + 1;
+      bool have_v = false, have_k = false;
+#pragma unroll
+      for (uint32_t t = 0; t < 2; ++t) {
+        if (j < n[t]) {
+          if (!wait(sh, &sh.b.p_full[t], s_count[t] & 1, a.status)) return;
+          ++s_count[t];
+          if (!have_v && !wait(sh, &sh.b.full[v % S], (v / S) & 1, a.status)) return;
+          have_v = true;
+          if (j == 0) {  // the tile's last output has been read
+            if (!wait(sh, &sh.b.o_free[t], (opened[t] & 1) ^ 1, a.status)) return;
+            ++opened[t];
+          }
+          ptx::tc_fence_after();
+          for (uint32_t i = 0; i < kKeys / 16; ++i)
+            mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + 64 + i * 8, value_desc(ring + (v % S) * kBytes, i), output, (j | i) > 0);
+          ptx::mma_commit(&sh.b.pv_done[t]);
+        }
+        if (j + 1 < n[t]) {
+          if (!have_k && !wait(sh, &sh.b.full[k % S], (k / S) & 1, a.status)) return;
+          have_k = true;
+          scores(t, k % S);
+        }
+      }
+      ptx::mma_commit(&sh.b.empty[v % S]);
+      if (j + 1 < most) ptx::mma_commit(&sh.b.empty[k % S]);
+    }
+    ptx::mma_commit(&sh.b.q_empty);
+    item += 2 * most;
+  }
+}
+
+template <typename T, typename TO, int DP>
+__device__ __forceinline__ void soften(const AttentionArgs &a, const Share &share, Shared &sh) {
+  const uint32_t lane = threadIdx.x & 31, t = threadIdx.x / 128, row = threadIdx.x & 127;
+  const uint32_t lanes = (threadIdx.x / 32 & 3) << 21;  // this warp's 32 lanes of TMEM
+  const uint32_t s_at = sh.tmem + t * 128 + lanes, p_at = s_at + 64, o_at = sh.tmem + 256 + t * 128 + lanes;
+  const float c = a.scale * kLog2e;
+  const tl_paged_cache &cache = a.cache;
+  uint32_t done = 0, block_count = 0;  // of this tile: blocks whose scores were taken
+  Walk<kRows, kKeys> walk;
+  Piece p;
+  walk.start(a, share);
+  while (walk.next(a, share, p)) {
+    const uint32_t n0 = tile_blocks(a, p, 0), n1 = tile_blocks(a, p, 1), n = t ? n1 : n0, most = max(n0, n1);
+    const uint32_t in_job = t * kTile + row;
+    const bool there = in_job <= p.last;
+    // rows behind the last one see everything: their scores are 0 and go nowhere
+    uint32_t from = 0, to = 0xffffffffu;
+    if (there) seen(a, p.length, p.position(a, in_job), from, to);
+    float m = -INFINITY, l = 0.0f;
+    for (uint32_t j = 0; j < n; ++j) {
+      if (!wait(sh, &sh.b.s_full[t], done & 1, a.status)) return;
+      ptx::tc_fence_after();
+      const uint32_t key = (p.block_lo + j) * kKeys;
+      const uint32_t *good = sh.mask[(block_count + j) % kMasks];
+      const uint32_t all = good[0] & good[1] & good[2] & good[3];
+      const bool whole = __all_sync(0xffffffffu, key >= from && key + kKeys <= to && all == 0xffffffffu);
+      // bit i of a word: the row sees key 32 w + i
+      uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+      if (!whole) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int64_t lo = static_cast<int64_t>(from) - key - 32 * w, hi = static_cast<int64_t>(to) - key - 32 * w;
+          uint32_t bits = hi <= 0 || lo >= 32 ? 0u : 0xffffffffu;
+          if (bits && hi < 32) bits &= (1u << hi) - 1;
+          if (bits && lo > 0) bits &= ~((1u << lo) - 1);
+          see[w] = there ? bits & good[w] : 0xffffffffu;
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t x[32];
+        ptx::tmem_load_32x32b_x32(s_at + 32 * w, x);
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (see[w] >> i & 1) top = fmaxf(top, __uint_as_float(x[i]));
+        }
+      }
+      top = top * c - shift<T>();
+      const bool grow = top > m + kSlack || (m == -INFINITY && top > m);
+      if (__any_sync(0xffffffffu, grow)) {
+        float f = 1.0f;
+        if (grow) {
+          f = ex2_approx(m - top);
+          m = top;
+          l *= f;
+        }
+        if (j > 0) {  // the output so far
+          if (!wait(sh, &sh.b.pv_done[t], (done - 1) & 1, a.status)) return;
+          ptx::tc_fence_after();
+#pragma unroll 1
+          for (uint32_t d = 0; d < cache.D; d += 32) {
+            uint32_t x[32];
+            ptx::tmem_load_32x32b_x32(o_at + d, x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+            tmem_store32(o_at + d, x);
+          }
+          tmem_store_wait();
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int w = 3; w >= 0; --w) {  // numerators lie over the scores' second half
+        uint32_t x[32], y[16];
+        ptx::tmem_load_32x32b_x32(s_at + 32 * w, x);
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(see[w] >> i & 1)) x[i] = __float_as_uint(-INFINITY);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e0 = ex2_approx(fmaf(__uint_as_float(x[2 * i]), c, -base));
+          const float e1 = ex2_approx(fmaf(__uint_as_float(x[2 * i + 1]), c, -base));
+          l += e0 + e1;
+          // the numerators' rounding to the type, which the second product asks for;
+          // their sum stays in fp32
+          y[i] = pack<T>(e0, e1);
+        }
+        tmem_store16(p_at + 16 * w, y);
+      }
+      tmem_store_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&sh.b.p_full[t]);
+      ++done;
+    }
+    block_count += most;
+    if (n) {
+      if (!wait(sh, &sh.b.pv_done[t], (done - 1) & 1, a.status)) return;
+      ptx::tc_fence_after();
+    }
+    const uint64_t place = p.row0 + in_job, token = p.start + place / a.group;
+    const uint32_t h = p.head * a.group + static_cast<uint32_t>(place % a.group);
+    const bool complete = p.opens && p.ends;
+    float *const part = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (p.opens ? 1 : 0)) * part_floats<kRows, DP>();
+    TO *const out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    bool nan = false;
+#pragma unroll 1
+    for (uint32_t d = 0; d < cache.D; d += 32) {
+      uint32_t x[32];
+      if (n) ptx::tmem_load_32x32b_x32(o_at + d, x);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        if (!there || d + 8 * v >= cache.D) continue;
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[i] = n ? __uint_as_float(x[8 * v + i]) : 0.0f;
+          nan = nan || y[i] != y[i];
+          if (complete) y[i] = l == 0.0f ? 0.0f : y[i] * inv;
+        }
+        if (complete) {
+          heads::Raw<TO, 8> raw;
+          raw.set(y);
+          raw.store(out + d + 8 * v);
+        } else {
+          float4 *q = reinterpret_cast<float4 *>(part + in_job * DP + d + 8 * v);
+          q[0] = make_float4(y[0], y[1], y[2], y[3]);
+          q[1] = make_float4(y[4], y[5], y[6], y[7]);
+        }
+      }
+    }
+    if (n) {
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&sh.b.o_free[t]);
+    }
+    // A value that other rows of the tile see, and this one does not, is not finite (0
+    // times it is NaN): the row's own keys one by one.
+    const uint32_t lo = max(from, p.block_lo * kKeys);
+    const uint32_t hi = static_cast<uint32_t>(min(static_cast<uint64_t>(to), static_cast<uint64_t>(p.block_hi) * kKeys));
+    const bool again = there && nan && l == l && (from > p.from || to < p.to);
+    if (there && !again) {
+      if (complete) put_lse<TO>(a, token, h, m, l);
+      else {
+        part[kRows * DP + in_job] = m;
+        part[kRows * DP + kRows + in_job] = l;
+      }
+    }
+    unsigned rows = __ballot_sync(0xffffffffu, again);
+    while (rows) {
+      const int r = __ffs(rows) - 1;
+      rows &= rows - 1;
+      const uint32_t r_job = __shfl_sync(0xffffffffu, in_job, r);
+      const uint64_t r_place = p.row0 + r_job, r_token = p.start + r_place / a.group;
+      const uint32_t r_h = p.head * a.group + static_cast<uint32_t>(r_place % a.group);
+      float acc[kMaxHead / 32], rm, rl;
+      const T *q = static_cast<const T *>(a.q.p) + r_token * a.q.row_stride + r_h * a.q.head_stride;
+      row_over_keys<T>(a, p.sequence, p.head, q, __shfl_sync(0xffffffffu, lo, r), __shfl_sync(0xffffffffu, hi, r), lane, rm, rl, acc);
+      TO *const r_out = static_cast<TO *>(const_cast<void *>(a.out.p)) + r_token * a.out.row_stride + r_h * a.out.head_stride;
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < static_cast<int>(kMaxHead) / 32; ++e) {
+        if (lane + 32 * e >= cache.D) continue;
+        if (complete) heads::set_element(r_out[lane + 32 * e], rl == 0.0f ? 0.0f : acc[e] / rl);
+        else part[r_job * DP + lane + 32 * e] = acc[e];
+      }
+      if (lane == 0) {
+        if (complete) put_lse<TO>(a, r_token, r_h, rm, rl);
+        else {
+          part[kRows * DP + r_job] = rm;
+          part[kRows * DP + kRows + r_job] = rl;
+        }
+      }
+    }
+    if (threadIdx.x == 0 && !p.opens && p.ends) a.joins[blockIdx.x] = Join{p.first_cta, p.sequence, p.head, p.tile};
+  }
+}
+
+template <typename T, typename TO, int DP>
+__global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a) {
+  constexpr int S = stages<DP>();
+  extern __shared__ uint8_t raw[];
+  uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t queries = ptx::smem_addr(smem), ring = queries + 2 * tile_bytes<DP>();
+  Shared &sh = *reinterpret_cast<Shared *>(smem + (2 + S) * tile_bytes<DP>());
+  const uint32_t warp = threadIdx.x / 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      ptx::mbar_init(&sh.b.full[i], kLoaders / 32);
+      ptx::mbar_init(&sh.b.empty[i], 1);
+    }
+    ptx::mbar_init(&sh.b.q_full, kLoaders / 32);
+    ptx::mbar_init(&sh.b.q_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      ptx::mbar_init(&sh.b.s_full[t], 1);
+      ptx::mbar_init(&sh.b.p_full[t], 4);
+      ptx::mbar_init(&sh.b.pv_done[t], 1);
+      ptx::mbar_init(&sh.b.o_free[t], 4);
+    }
+    ptx::mbar_init(&sh.b.drained, 1);
+    sh.gave_up = 0;
+    ptx::fence_barrier_init();
+  }
+  if (warp == 12) {
+    ptx::tmem_alloc(&sh.tmem, 512);
+    ptx::tmem_relinquish();
+  }
+  pdl_enter();
+  if (!a.whole && threadIdx.x == 0) a.joins[blockIdx.x] = Join{0xffffffffu, 0, 0, 0};
+  ptx::tc_fence_before();
+  const Share share = share_of<kRows, kKeys, kThreads>(a, blockIdx.x, gridDim.x, a.whole ? 1 : 2 * kKeys);
+  ptx::tc_fence_after();
+  if (warp < 8) soften<T, TO, DP>(a, share, sh);
+  else if (warp < 12) {
+    load<T, DP>(a, share, sh, queries, ring);
+    await<0>();
+  } else if ((threadIdx.x & 31) == 0) {
+    multiply<T, DP>(a, share, sh, queries, ring);
+    // everything issued is done before TMEM and the barriers go
+    ptx::mma_commit(&sh.b.drained);
+    wait(sh, &sh.b.drained, 0, a.status);
+  }
+  __syncthreads();
+  if (warp == 12) ptx::tmem_dealloc(sh.tmem, 512);
+}
+
+template <typename T, typename TO, int DP> void launch(const AttentionArgs &a, const Plan &p, cudaStream_t s) {
+  constexpr size_t smem = smem_bytes<DP>();
+  (void)cudaFuncSetAttribute(tile_kernel<T, TO, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  launch_pdl(tile_kernel<T, TO, DP>, p.ctas, kThreads, smem, s, a);
+  if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, 8), 128, 0, s, a);
+}
+
+}  // namespace
+
+Plan tile_plan(const AttentionArgs &a, uint32_t max_new) {
+  Plan p{};
+  (void)max_new;
+  p.whole = 0;
+  p.ctas = kNumSMs;
+  p.part_floats = kRows * (a.cache.D > 64 ? 128 : 64) + 2 * kRows;
+  return p;
+}
+
+void launch_tile(const AttentionArgs &a, const Plan &p, bool wide, cudaStream_t s) {
+  const bool narrow = a.cache.D <= 64;
+#define L(T, TO) narrow ? launch<T, TO, 64>(a, p, s) : launch<T, TO, 128>(a, p, s)
+  if (a.cache.type == TL_FLOAT16) { if (wide) L(__half, float); else L(__half, __half); }
+  else if (wide) L(__nv_bfloat16, float);
+  else L(__nv_bfloat16, __nv_bfloat16);
+#undef L
+}
+
+}  // namespace paged
+}  // namespace tl

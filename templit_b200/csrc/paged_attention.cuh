@@ -103,34 +103,47 @@ __device__ __forceinline__ void row_over_keys(const AttentionArgs &a, uint32_t s
 }
 
 // How the work is shared out.  A job is one key head's query rows of one
-// sequence, `ROWS` rows at most (token by token, the group's heads of a token
-// side by side), over the sequence's keys in blocks of `KEYS`.  All blocks of
-// all jobs lie in one line, which is cut into equal shares; a share that starts
-// or ends inside a job leaves a partial result (numerators' sum, maximum and
-// sum of the softmax), and join_kernel adds those up in the order of the keys.
+// sequence, `ROWS` rows at most (a tile; token by token, the group's heads of
+// a token side by side), over the keys that they see, in blocks of `KEYS`.
+// The jobs lie in one line, sequence by sequence, tile by tile, head by head, each
+// as long as its keys (for causal tiles an even slope, at least what they see)
+// and kJob blocks more, about what starting and ending a job costs: with
+// shares of keys alone, 64 sequences of 16 to 8191 keys took 139 us where some
+// CTAs met many short ones.  The line is cut into equal shares; a share that starts or ends
+// inside a job leaves a partial result (numerators' sum, maximum and sum of
+// the softmax), and join_kernel adds those up in the order of the keys.
 // Every CTA works its share out by itself from the lengths on the device, so
 // that a captured call follows them.
 template <uint32_t ROWS, uint32_t KEYS> struct Work {
+  static constexpr uint64_t kJob = 3 * KEYS;
   Sequence q;
-  uint32_t first, blocks;  // the sequence's blocks, from the first that any of its rows sees
   uint64_t tiles;
+  uint64_t base, slope;  // line of tile t: base + slope t, for each head
 
   __device__ __forceinline__ void set(const AttentionArgs &a, uint32_t s) {
     q = sequence_of(a.cache, s, a.most);
-    const int64_t lo = a.window ? static_cast<int64_t>(q.length) - q.count + 1 - static_cast<int64_t>(a.window) : 0;
-    first = lo > 0 ? static_cast<uint32_t>(lo / KEYS) : 0;
-    const uint32_t end = static_cast<uint32_t>((static_cast<uint64_t>(q.length) + KEYS - 1) / KEYS);
-    blocks = end > first ? end - first : 1;
     tiles = (static_cast<uint64_t>(q.count) * a.group + ROWS - 1) / ROWS;
+    const uint32_t step = (ROWS + a.group - 1) / a.group;  // tokens of a tile
+    slope = 0;
+    if (a.whole) {
+      base = 1;
+      return;
+    }
+    base = q.length;
+    if (a.window) base = min(base, static_cast<uint64_t>(a.window) + step + KEYS);
+    else if (a.causal) {
+      slope = step;
+      base = (q.length > q.count ? q.length - q.count : 0) + step;
+    }
+    base += kJob;
   }
-  // places in the line
-  __device__ __forceinline__ uint64_t cost(const AttentionArgs &a) const {
-    return tiles * a.cache.heads * (a.whole ? 1 : blocks);
+  // the line before tile t
+  __device__ __forceinline__ uint64_t before(const AttentionArgs &a, uint64_t t) const {
+    return a.cache.heads * (t * base + (t ? t * (t - 1) / 2 : 0) * slope);
   }
 };
 
-// The sequence in which this CTA's share starts, the share's offset in it and
-// its size; the line's length is cut into `ctas` shares of at least `least`.
+// This CTA's share: its place in the line and the sequence it starts in.
 struct Share {
   uint64_t begin, size;  // in the line
   uint64_t full;         // what every share but the last is
@@ -139,18 +152,18 @@ struct Share {
   bool any;
 };
 template <uint32_t ROWS, uint32_t KEYS, int THREADS>
-__device__ __forceinline__ Share share_of(const AttentionArgs &a, uint32_t cta, uint32_t ctas, uint32_t least) {
+__device__ __forceinline__ Share share_of(const AttentionArgs &a, uint32_t cta, uint32_t ctas, uint64_t least) {
   constexpr int kWarps = THREADS / 32;
-  __shared__ uint64_t warp_sum[kWarps + 1];
+  __shared__ uint64_t warp_sum[kWarps];
   __shared__ Share found;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32, n = a.cache.sequences;
-  const uint32_t per = (n + THREADS - 1) / THREADS, s0 = tid * per, s1 = min(s0 + per, n);
+  const uint32_t per = (n + THREADS - 1) / THREADS, s0 = min(tid * per, n), s1 = min(s0 + per, n);
   Work<ROWS, KEYS> w;
   uint64_t mine = 0;
   for (uint32_t s = s0; s < s1; ++s) {
     w.set(a, s);
     if (w.q.bad && cta == 0) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
-    mine += w.cost(a);
+    mine += w.before(a, w.tiles);
   }
   uint64_t up = mine;  // inclusive sums over the warp, then over the CTA
 #pragma unroll
@@ -174,7 +187,7 @@ __device__ __forceinline__ Share share_of(const AttentionArgs &a, uint32_t cta, 
     uint32_t s = s0;
     for (; s < s1; ++s) {
       w.set(a, s);
-      const uint64_t c = w.cost(a);
+      const uint64_t c = w.before(a, w.tiles);
       if (begin < before + c) break;
       before += c;
     }
@@ -184,6 +197,136 @@ __device__ __forceinline__ Share share_of(const AttentionArgs &a, uint32_t cta, 
   return found;
 }
 
+// A part of a job: what a CTA does of it.
+struct Piece {
+  uint32_t sequence, head, tile;
+  uint32_t start;              // first row of its sequence's tokens
+  uint32_t block_lo, block_hi; // blocks of the keys [block * KEYS, ..)
+  bool opens, ends;            // the job's first block, its last one
+  uint32_t first_cta;          // that has its first block
+  uint64_t row0;               // of the tile, among the sequence's rows
+  uint32_t last;               // its last row
+  uint32_t length;             // the sequence's keys
+  int64_t position0;           // of the sequence's first new token
+  uint32_t from, to;           // keys that any of its rows sees
+  __device__ __forceinline__ int64_t position(const AttentionArgs &a, uint32_t row) const {
+    return position0 + static_cast<int64_t>((row0 + row) / a.group);
+  }
+};
+
+// The pieces of a share, in order.
+template <uint32_t ROWS, uint32_t KEYS> struct Walk {
+  Work<ROWS, KEYS> w;
+  uint64_t offset, left, at;
+  uint32_t s;
+
+  __device__ __forceinline__ void start(const AttentionArgs &a, const Share &share) {
+    s = share.sequence;
+    offset = share.offset;
+    at = share.begin;
+    left = share.any ? share.size : 0;
+    if (left) w.set(a, s);
+  }
+  __device__ __forceinline__ bool next(const AttentionArgs &a, const Share &share, Piece &p) {
+    while (left) {
+      const uint64_t line = w.before(a, w.tiles);
+      if (offset >= line) {  // the next sequence with any rows
+        offset -= line;
+        w.set(a, ++s);
+        continue;
+      }
+      uint64_t lo = 0, hi = w.tiles;  // the last tile that starts at or before offset
+      while (hi - lo > 1) {
+        const uint64_t mid = (lo + hi) / 2;
+        if (w.before(a, mid) <= offset) lo = mid;
+        else hi = mid;
+      }
+      const uint64_t job = w.base + w.slope * lo, in_tile = offset - w.before(a, lo);
+      const uint64_t x0 = in_tile % job, take = min(left, job - x0), x1 = x0 + take;
+      p.sequence = s;
+      p.head = static_cast<uint32_t>(in_tile / job);
+      p.tile = static_cast<uint32_t>(lo);
+      p.start = w.q.start;
+      p.row0 = lo * ROWS;
+      p.last = static_cast<uint32_t>(min(p.row0 + ROWS, static_cast<uint64_t>(w.q.count) * a.group) - 1 - p.row0);
+      p.length = w.q.length;
+      p.position0 = static_cast<int64_t>(w.q.length) - w.q.count;
+      uint32_t unused;
+      seen(a, w.q.length, p.position(a, 0), p.from, unused);
+      seen(a, w.q.length, p.position(a, p.last), unused, p.to);
+      const uint32_t first = p.from / KEYS;
+      const uint32_t end = static_cast<uint32_t>((static_cast<uint64_t>(p.to) + KEYS - 1) / KEYS);
+      const uint32_t blocks = end > first ? end - first : 1;  // rows without keys are written too
+      const auto block = [&](uint64_t x) {
+        if (a.whole || x == job) return x ? blocks : 0u;
+        return static_cast<uint32_t>(min(x > w.kJob ? (x - w.kJob) / KEYS : 0, static_cast<uint64_t>(blocks)));
+      };
+      const uint32_t b0 = block(x0), b1 = block(x1);
+      const uint64_t job_at = at - x0;
+      offset += take;
+      at += take;
+      left -= take;
+      if (b0 == b1) continue;  // nothing but a job's overhead, or behind its keys
+      p.block_lo = first + b0;
+      p.block_hi = first + b1;
+      p.opens = b0 == 0;
+      p.ends = b1 == blocks;
+      p.first_cta = static_cast<uint32_t>((job_at + w.kJob + KEYS - 1) / share.full);
+      return true;
+    }
+    return false;
+  }
+};
+
+// One row's result: the whole of it, or a part in the workspace.
+template <typename TO>
+__device__ __forceinline__ void put_lse(const AttentionArgs &a, uint64_t token, uint32_t h, float m, float l) {
+  if (a.lse) a.lse[token * a.q_heads + h] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+}
+
+// floats of a partial result of a tile: outputs, maxima, sums
+template <uint32_t ROWS, int DP> constexpr uint32_t part_floats() { return ROWS * DP + 2 * ROWS; }
+
+// The jobs that were cut, each where it ends: a warp per row adds the partial
+// results up in the order of the keys.
+template <typename TO, uint32_t ROWS, int DP>
+__global__ void __launch_bounds__(128) join_kernel(const AttentionArgs a) {
+  pdl_enter();
+  const Join j = a.joins[blockIdx.x];
+  if (j.first == 0xffffffffu) return;
+  const uint32_t lane = threadIdx.x & 31, end = blockIdx.x;
+  const Sequence q = sequence_of(a.cache, j.sequence, a.most);
+  const uint64_t rows = static_cast<uint64_t>(q.count) * a.group, row0 = static_cast<uint64_t>(j.tile) * ROWS;
+  const auto part = [&](uint32_t cta) {
+    return a.parts + (static_cast<size_t>(cta) * 2 + (cta == j.first ? 1 : 0)) * part_floats<ROWS, DP>();
+  };
+  for (uint32_t row = blockIdx.y * 4 + threadIdx.x / 32; row < ROWS && row0 + row < rows; row += gridDim.y * 4) {
+    float mm = -INFINITY;
+    for (uint32_t i = j.first + lane; i <= end; i += 32) mm = fmaxf(mm, part(i)[ROWS * DP + row]);
+    mm = warp_max(mm);
+    float ll = 0.0f, acc[DP / 32];
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+    for (uint32_t i = j.first; i <= end; ++i) {
+      const float *p = part(i);
+      const float wm = p[ROWS * DP + row], f = wm == -INFINITY ? 0.0f : ex2_approx(wm - mm);
+      ll = fmaf(f, p[ROWS * DP + ROWS + row], ll);
+#pragma unroll
+      for (int e = 0; e < DP / 32; ++e) {
+        const float x = p[row * DP + lane + 32 * e];
+        if (f != 0.0f) acc[e] = fmaf(f, x, acc[e]);
+      }
+    }
+    const uint64_t token = q.start + (row0 + row) / a.group;
+    const uint32_t h = j.head * a.group + static_cast<uint32_t>((row0 + row) % a.group);
+    TO *out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e)
+      if (lane + 32 * e < a.cache.D) heads::set_element(out[lane + 32 * e], ll == 0.0f ? 0.0f : acc[e] / ll);
+    if (lane == 0) put_lse<TO>(a, token, h, mm, ll);
+  }
+}
 
 // What a call asks of a kernel family: its grid and the workspace's floats
 // behind the joins.
@@ -206,6 +349,8 @@ inline uint64_t most_jobs(const AttentionArgs &a, uint32_t rows) {
 
 Plan step_plan(const AttentionArgs &a, uint32_t max_new);
 void launch_step(const AttentionArgs &a, const Plan &p, bool wide, cudaStream_t s);
+Plan tile_plan(const AttentionArgs &a, uint32_t max_new);
+void launch_tile(const AttentionArgs &a, const Plan &p, bool wide, cudaStream_t s);
 
 }  // namespace paged
 }  // namespace tl
