@@ -773,7 +773,7 @@ size_t tl_rotary_heads_workspace_size(const tl_rotary_desc *desc);
  * sequence has are left as they were.  The arrays are device memory and are
  * read when the kernels run, so a captured call follows them.  What they hold
  * cannot make a kernel read or write outside of the tensors: a page id >=
- * pages, a length above table_stride * page_size, a sequence whose rows leave
+ * pages, a length above table_stride * page_size (or 2^31), a sequence whose rows leave
  * [0, tokens) or run backwards raise TL_FLAG_INDEX_RANGE; such keys are not
  * there, such rows are not written. */
 typedef struct tl_paged_cache {

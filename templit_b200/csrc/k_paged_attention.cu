@@ -45,6 +45,12 @@ int attention_args(const char *who, const tl_paged_attention_desc *d, AttentionA
   return TL_OK;
 }
 
+// Many rows a key head go to the tensor cores' tiles (16-bit types; a scale
+// that is not positive would turn the order of the scores round there).
+bool tiled(const tl_paged_attention_desc *d, const AttentionArgs &a, uint32_t max_new) {
+  return a.cache.type != TL_FLOAT32 && d->scale > 0.0f && static_cast<uint64_t>(max_new) * a.group > 16;
+}
+
 uint32_t most_new(const tl_paged_attention_desc *d) {
   return d->max_new && d->max_new < d->cache.tokens ? d->max_new : d->cache.tokens;
 }
@@ -62,7 +68,8 @@ size_t tl_paged_attention_workspace_size(const tl_paged_attention_desc *d) {
   AttentionArgs a{};
   bool nothing = false;
   if (attention_args("tl_paged_attention_workspace_size", d, a, &nothing) || nothing) return 0;
-  return plan_bytes(step_plan(a, most_new(d)));
+  const uint32_t n = most_new(d);
+  return plan_bytes(tiled(d, a, n) ? tile_plan(a, n) : step_plan(a, n));
 }
 
 int tl_paged_attention(const tl_paged_attention_desc *d, void *stream) {
@@ -72,7 +79,9 @@ int tl_paged_attention(const tl_paged_attention_desc *d, void *stream) {
   bool nothing = false;
   if (int rc = attention_args(who, d, a, &nothing)) return rc;
   if (nothing) return TL_OK;
-  const Plan p = step_plan(a, most_new(d));
+  const uint32_t n = most_new(d);
+  const bool tiles = tiled(d, a, n);
+  const Plan p = tiles ? tile_plan(a, n) : step_plan(a, n);
   const uint64_t bytes = plan_bytes(p);
   if (bytes) {
     if (!d->workspace || d->workspace_bytes < bytes) return fail(TL_ERR_INVALID, w + "workspace too small");
@@ -83,7 +92,7 @@ int tl_paged_attention(const tl_paged_attention_desc *d, void *stream) {
   a.parts = reinterpret_cast<float *>(a.joins + p.ctas);
   a.status = device_status_ptr();
   if (!a.status) return fail(TL_ERR_CUDA, w + "no status word");
-  launch_step(a, p, d->out_type != a.cache.type, as_stream(stream));
+  (tiles ? launch_tile : launch_step)(a, p, d->out_type != a.cache.type, as_stream(stream));
   return launch_status(who);
 }
 

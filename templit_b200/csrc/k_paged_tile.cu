@@ -75,6 +75,11 @@ __device__ __forceinline__ bool wait(Shared &sh, uint64_t *bar, uint32_t parity,
   }
 }
 
+// The same for a whole warp, with one answer.
+__device__ __forceinline__ bool wait_warp(Shared &sh, uint64_t *bar, uint32_t parity, uint32_t *status) {
+  return __all_sync(0xffffffffu, wait(sh, bar, parity, status));
+}
+
 // Vector `ch` (16 bytes) of row `r` of a tile: 128-byte rows of 64 elements
 // with the 128-byte swizzle, one block of 128 rows after another.
 __device__ __forceinline__ uint32_t spot(uint32_t r, uint32_t ch) {
@@ -146,7 +151,7 @@ __device__ __forceinline__ uint32_t tile_blocks(const AttentionArgs &a, const Pi
   if (t * kTile > p.last) return 0;
   uint32_t from, to;
   seen(a, p.length, p.position(a, min((t + 1) * kTile - 1, p.last)), from, to);
-  const uint32_t end = min((to + (kKeys - 1)) / kKeys, p.block_hi);
+  const uint32_t end = min(to / kKeys + (to % kKeys != 0), p.block_hi);
   return end > p.block_lo ? end - p.block_lo : 0;
 }
 
@@ -173,7 +178,7 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Share &share,
     // the queries: the rows of this warp, 32 of each tile
     await<0>();
     hand_over(item);
-    if (!wait(sh, &sh.b.q_empty, (q_phase & 1) ^ 1, a.status)) return;
+    if (!wait_warp(sh, &sh.b.q_empty, (q_phase & 1) ^ 1, a.status)) return;
     ++q_phase;
 #pragma unroll
     for (uint32_t t = 0; t < 2; ++t) {
@@ -209,7 +214,7 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Share &share,
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         // a slot is free again when what was multiplied from it is done
-        if (!wait(sh, &sh.b.empty[item % S], ((item / S) & 1) ^ 1, a.status)) return;
+        if (!wait_warp(sh, &sh.b.empty[item % S], ((item / S) & 1) ^ 1, a.status)) return;
         if (half == 0 && lane == 0) sh.mask[block_count % kMasks][warp] = good;
         const T *base = half ? vp : kp;
         const uint32_t to = ring + (item % S) * kBytes;
@@ -233,7 +238,7 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Share &share,
   hand_over(item);
   // the last reads of the ring are over
   for (uint32_t i = item > static_cast<uint32_t>(S) ? item - S : 0; i < item; ++i)
-    if (!wait(sh, &sh.b.empty[i % S], (i / S) & 1, a.status)) return;
+    if (!wait_warp(sh, &sh.b.empty[i % S], (i / S) & 1, a.status)) return;
 }
 
 template <typename T, int DP>
@@ -318,12 +323,12 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, const Share &shar
     if (there) seen(a, p.length, p.position(a, in_job), from, to);
     float m = -INFINITY, l = 0.0f;
     for (uint32_t j = 0; j < n; ++j) {
-      if (!wait(sh, &sh.b.s_full[t], done & 1, a.status)) return;
+      if (!wait_warp(sh, &sh.b.s_full[t], done & 1, a.status)) return;
       ptx::tc_fence_after();
       const uint32_t key = (p.block_lo + j) * kKeys;
       const uint32_t *good = sh.mask[(block_count + j) % kMasks];
       const uint32_t all = good[0] & good[1] & good[2] & good[3];
-      const bool whole = __all_sync(0xffffffffu, key >= from && key + kKeys <= to && all == 0xffffffffu);
+      const bool whole = __all_sync(0xffffffffu, key >= from && to >= kKeys && key <= to - kKeys && all == 0xffffffffu);
       // bit i of a word: the row sees key 32 w + i
       uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
       if (!whole) {
@@ -360,7 +365,7 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, const Share &shar
           l *= f;
         }
         if (j > 0) {  // the output so far
-          if (!wait(sh, &sh.b.pv_done[t], (done - 1) & 1, a.status)) return;
+          if (!wait_warp(sh, &sh.b.pv_done[t], (done - 1) & 1, a.status)) return;
           ptx::tc_fence_after();
 #pragma unroll 1
           for (uint32_t d = 0; d < cache.D; d += 32) {
@@ -402,7 +407,7 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, const Share &shar
     }
     block_count += most;
     if (n) {
-      if (!wait(sh, &sh.b.pv_done[t], (done - 1) & 1, a.status)) return;
+      if (!wait_warp(sh, &sh.b.pv_done[t], (done - 1) & 1, a.status)) return;
       ptx::tc_fence_after();
     }
     const uint64_t place = p.row0 + in_job, token = p.start + place / a.group;
@@ -526,9 +531,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
     multiply<T, DP>(a, share, sh, queries, ring);
     // everything issued is done before TMEM and the barriers go
     ptx::mma_commit(&sh.b.drained);
-    wait(sh, &sh.b.drained, 0, a.status);
+    if (!ptx::mbar_wait_bounded(&sh.b.drained, 0, kWaitLimitNs)) raise_flag(a.status, TL_FLAG_TIMEOUT);
   }
+  __syncwarp();
+  ptx::tc_fence_before();
   __syncthreads();
+  ptx::tc_fence_after();
   if (warp == 12) ptx::tmem_dealloc(sh.tmem, 512);
 }
 

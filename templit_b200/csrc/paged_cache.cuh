@@ -32,10 +32,10 @@ __device__ __forceinline__ Sequence sequence_of(const tl_paged_cache &c, uint32_
   }
   return q;
 }
-// keys that a row of the table can hold
+// keys that a row of the table can hold, 2^31 at most
 __host__ __device__ __forceinline__ uint64_t table_keys(const tl_paged_cache &c) {
   const uint64_t n = static_cast<uint64_t>(c.table_stride) * c.page_size;
-  return n < 0xffffffffull ? n : 0xffffffffull;
+  return n < 1ull << 31 ? n : 1ull << 31;
 }
 
 // The last sequence that starts at or before row `token`, by a warp: 32
