@@ -16,6 +16,7 @@
 //   warps 8-11      keys and values, 128 at a time, by cp.async into a ring
 //                   (pages end anywhere, so rows come one by one, 16 bytes a
 //                   lane, a page's address looked up once a row), and the queries
+//   warp 13         one thread works out the CTA's pieces of jobs, ahead of the others
 //   warp 12         one thread issues S = Q K^T and O += P V (tcgen05.mma
 //                   kind::f16, fp32 in TMEM)
 // TMEM: 2 x 128 columns of scores (numerators over their second half), 2 x
@@ -30,10 +31,11 @@ namespace paged {
 namespace {
 
 constexpr uint32_t kTile = 128, kRows = 2 * kTile, kKeys = 128;
-constexpr int kThreads = 13 * 32, kLoaders = 128;
+constexpr int kThreads = 16 * 32, kLoaders = 128;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr float kSlack = 8.0f;  // log2 of how far numerators may pass 1
 constexpr int kLag = 2;         // ring places between a copy's issue and its hand-over
+constexpr int kJobs = 4;        // pieces worked out ahead
 constexpr int kMasks = 8;       // blocks whose missing keys are remembered: more than the ring is ahead
 
 template <int DP> constexpr uint32_t tile_bytes() { return kTile * DP * 2; }
@@ -41,10 +43,19 @@ template <int DP> constexpr int stages() { return DP == 128 ? 5 : 8; }
 
 struct Barriers {
   uint64_t full[8], empty[8];
+  uint64_t job_full[kJobs], job_free[kJobs];
   uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free[2], drained;
+};
+// A piece and the blocks that its two tiles take, from the piece's first on;
+// more == false: there are no more.
+struct Job {
+  Piece p;
+  uint32_t n[2], most;
+  bool more;
 };
 struct Shared {
   Barriers b;
+  Job jobs[kJobs];
   uint32_t tmem, gave_up;
   uint32_t mask[kMasks][4];  // a bit for every key of a block that is there
 };
@@ -113,15 +124,38 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uin
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 16 and 32 columns of this warp's 32 lanes into TMEM
-__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+// 64 columns of this warp's 32 lanes, with their wait (see tmem_load_32x32b_x16)
+template <int O> __device__ __forceinline__ void tmem_load64(uint32_t taddr, uint32_t (&r)[128]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[O + 0]), "=r"(r[O + 1]), "=r"(r[O + 2]), "=r"(r[O + 3]), "=r"(r[O + 4]), "=r"(r[O + 5]), "=r"(r[O + 6]), "=r"(r[O + 7]), "=r"(r[O + 8]), "=r"(r[O + 9]), "=r"(r[O + 10]), "=r"(r[O + 11]), "=r"(r[O + 12]), "=r"(r[O + 13]), "=r"(r[O + 14]), "=r"(r[O + 15]), "=r"(r[O + 16]), "=r"(r[O + 17]), "=r"(r[O + 18]), "=r"(r[O + 19]), "=r"(r[O + 20]), "=r"(r[O + 21]), "=r"(r[O + 22]), "=r"(r[O + 23]), "=r"(r[O + 24]), "=r"(r[O + 25]), "=r"(r[O + 26]), "=r"(r[O + 27]), "=r"(r[O + 28]), "=r"(r[O + 29]), "=r"(r[O + 30]), "=r"(r[O + 31]), "=r"(r[O + 32]), "=r"(r[O + 33]), "=r"(r[O + 34]), "=r"(r[O + 35]), "=r"(r[O + 36]), "=r"(r[O + 37]), "=r"(r[O + 38]), "=r"(r[O + 39]), "=r"(r[O + 40]), "=r"(r[O + 41]), "=r"(r[O + 42]), "=r"(r[O + 43]), "=r"(r[O + 44]), "=r"(r[O + 45]), "=r"(r[O + 46]), "=r"(r[O + 47]), "=r"(r[O + 48]), "=r"(r[O + 49]), "=r"(r[O + 50]), "=r"(r[O + 51]), "=r"(r[O + 52]), "=r"(r[O + 53]), "=r"(r[O + 54]), "=r"(r[O + 55]), "=r"(r[O + 56]), "=r"(r[O + 57]), "=r"(r[O + 58]), "=r"(r[O + 59]), "=r"(r[O + 60]), "=r"(r[O + 61]), "=r"(r[O + 62]), "=r"(r[O + 63])
+      : "r"(taddr)
       : "memory");
 }
+// Two fp32 in a register pair: one issued instruction for both.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(uint32_t lo, uint32_t hi) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(lo), "r"(hi));
+  return p;
+}
+__device__ __forceinline__ float2 halves(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 32 columns of this warp's 32 lanes into TMEM
 __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -155,8 +189,37 @@ __device__ __forceinline__ uint32_t tile_blocks(const AttentionArgs &a, const Pi
   return end > p.block_lo ? end - p.block_lo : 0;
 }
 
+// The next piece, when it has been worked out; its readers are done with it
+// after release_job().
+__device__ __forceinline__ const Job *next_job(Shared &sh, uint32_t i, uint32_t *status, bool *ok) {
+  *ok = wait(sh, &sh.b.job_full[i % kJobs], (i / kJobs) & 1, status);
+  return &sh.jobs[i % kJobs];
+}
+__device__ __forceinline__ void release_job(Shared &sh, uint32_t i) { ptx::mbar_arrive(&sh.b.job_free[i % kJobs]); }
+
+__device__ __forceinline__ void plan_jobs(const AttentionArgs &a, const Share &share, Shared &sh) {
+  Walk<kRows, kKeys> walk;
+  Piece p;
+  walk.start(a, share);
+  bool more = true;
+  for (uint32_t i = 0; more; ++i) {
+    more = walk.next(a, share, p);
+    if (!wait(sh, &sh.b.job_free[i % kJobs], ((i / kJobs) & 1) ^ 1, a.status)) return;
+    Job &job = sh.jobs[i % kJobs];
+    job.more = more;
+    if (more) {
+      job.p = p;
+      job.n[0] = tile_blocks(a, p, 0);
+      job.n[1] = tile_blocks(a, p, 1);
+      job.most = max(job.n[0], job.n[1]);
+      if (!p.opens && p.ends) a.joins[blockIdx.x] = Join{p.first_cta, p.sequence, p.head, p.tile};
+    }
+    ptx::mbar_arrive(&sh.b.job_full[i % kJobs]);
+  }
+}
+
 template <typename T, int DP>
-__device__ __forceinline__ void load(const AttentionArgs &a, const Share &share, Shared &sh, uint32_t queries, uint32_t ring) {
+__device__ __forceinline__ void load(const AttentionArgs &a, Shared &sh, uint32_t queries, uint32_t ring) {
   constexpr int S = stages<DP>();
   constexpr uint32_t CH = DP / 8, kBytes = tile_bytes<DP>();
   const uint32_t lane = threadIdx.x & 31, warp = (threadIdx.x - 256) / 32;
@@ -169,12 +232,18 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Share &share,
     for (; handed < upto; ++handed)
       if (lane == 0) ptx::mbar_arrive(&sh.b.full[handed % S]);
   };
-  Walk<kRows, kKeys> walk;
-  Piece p;
-  walk.start(a, share);
-  while (walk.next(a, share, p)) {
-    const uint32_t n0 = tile_blocks(a, p, 0), n1 = tile_blocks(a, p, 1), n = max(n0, n1);
-    if (!n) continue;
+  for (uint32_t i_job = 0;; ++i_job) {
+    bool ok;
+    const Job *const job = next_job(sh, i_job, a.status, &ok);
+    if (!__all_sync(0xffffffffu, ok)) return;
+    if (!job->more) break;
+    const Piece &p = job->p;
+    const uint32_t n = job->most;
+    if (!n) {
+      __syncwarp();
+      if (lane == 0) release_job(sh, i_job);
+      continue;
+    }
     // the queries: the rows of this warp, 32 of each tile
     await<0>();
     hand_over(item);
@@ -233,6 +302,8 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Share &share,
       ++block_count;
       at = next;
     }
+    __syncwarp();
+    if (lane == 0) release_job(sh, i_job);
   }
   await<0>();
   hand_over(item);
@@ -242,7 +313,7 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Share &share,
 }
 
 template <typename T, int DP>
-__device__ __forceinline__ void multiply(const AttentionArgs &a, const Share &share, Shared &sh, uint32_t queries, uint32_t ring) {
+__device__ __forceinline__ void multiply(const AttentionArgs &a, Shared &sh, uint32_t queries, uint32_t ring) {
   constexpr int S = stages<DP>();
   constexpr uint32_t kBytes = tile_bytes<DP>();
   constexpr uint32_t type = std::is_same<T, __half>::value ? 0 : 1;
@@ -250,17 +321,18 @@ __device__ __forceinline__ void multiply(const AttentionArgs &a, const Share &sh
   const uint32_t score = idesc_f16(type, kTile, kKeys, false), output = idesc_f16(type, kTile, ksteps * 16, true);
   const uint32_t tmem = sh.tmem;
   uint32_t item = 0, piece = 0, s_count[2] = {0, 0}, opened[2] = {0, 0};
-  Walk<kRows, kKeys> walk;
-  Piece p;
-  walk.start(a, share);
   const auto scores = [&](uint32_t t, uint32_t slot) {
     ptx::tc_fence_after();
     for (uint32_t k = 0; k < ksteps; ++k)
       mma_smem(tmem + t * 128, row_desc(queries + t * kBytes, k), row_desc(ring + slot * kBytes, k), score, k > 0);
     ptx::mma_commit(&sh.b.s_full[t]);
   };
-  while (walk.next(a, share, p)) {
-    const uint32_t n[2] = {tile_blocks(a, p, 0), tile_blocks(a, p, 1)}, most = max(n[0], n[1]);
+  for (uint32_t i_job = 0;; ++i_job) {
+    bool ok;
+    const Job *const job = next_job(sh, i_job, a.status, &ok);
+    if (!ok || !job->more) return;
+    const uint32_t n[2] = {job->n[0], job->n[1]}, most = job->most;
+    release_job(sh, i_job);
     if (!most) continue;
     if (!wait(sh, &sh.b.q_full, piece & 1, a.status)) return;
     ++piece;
@@ -304,18 +376,19 @@ __device__ __forceinline__ void multiply(const AttentionArgs &a, const Share &sh
 }
 
 template <typename T, typename TO, int DP>
-__device__ __forceinline__ void soften(const AttentionArgs &a, const Share &share, Shared &sh) {
+__device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh) {
   const uint32_t lane = threadIdx.x & 31, t = threadIdx.x / 128, row = threadIdx.x & 127;
   const uint32_t lanes = (threadIdx.x / 32 & 3) << 21;  // this warp's 32 lanes of TMEM
   const uint32_t s_at = sh.tmem + t * 128 + lanes, p_at = s_at + 64, o_at = sh.tmem + 256 + t * 128 + lanes;
   const float c = a.scale * kLog2e;
   const tl_paged_cache &cache = a.cache;
   uint32_t done = 0, block_count = 0;  // of this tile: blocks whose scores were taken
-  Walk<kRows, kKeys> walk;
-  Piece p;
-  walk.start(a, share);
-  while (walk.next(a, share, p)) {
-    const uint32_t n0 = tile_blocks(a, p, 0), n1 = tile_blocks(a, p, 1), n = t ? n1 : n0, most = max(n0, n1);
+  for (uint32_t i_job = 0;; ++i_job) {
+    bool ok;
+    const Job *const job = next_job(sh, i_job, a.status, &ok);
+    if (!__all_sync(0xffffffffu, ok) || !job->more) return;
+    const Piece &p = job->p;
+    const uint32_t n = job->n[t];
     const uint32_t in_job = t * kTile + row;
     const bool there = in_job <= p.last;
     // rows behind the last one see everything: their scores are 0 and go nowhere
@@ -329,32 +402,35 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, const Share &shar
       const uint32_t *good = sh.mask[(block_count + j) % kMasks];
       const uint32_t all = good[0] & good[1] & good[2] & good[3];
       const bool whole = __all_sync(0xffffffffu, key >= from && to >= kKeys && key <= to - kKeys && all == 0xffffffffu);
-      // bit i of a word: the row sees key 32 w + i
-      uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-      if (!whole) {
+      // bit i: the row sees key 32 w + i
+      const auto see = [&](int w) {
+        const int64_t lo = static_cast<int64_t>(from) - key - 32 * w, hi = static_cast<int64_t>(to) - key - 32 * w;
+        uint32_t bits = hi <= 0 || lo >= 32 ? 0u : 0xffffffffu;
+        if (bits && hi < 32) bits &= (1u << hi) - 1;
+        if (bits && lo > 0) bits &= ~((1u << lo) - 1);
+        return there ? bits & good[w] : 0xffffffffu;
+      };
+      uint32_t x[128];
+      tmem_load64<0>(s_at, x);
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      const auto peak = [&](int o) {
+        if (!whole) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int64_t lo = static_cast<int64_t>(from) - key - 32 * w, hi = static_cast<int64_t>(to) - key - 32 * w;
-          uint32_t bits = hi <= 0 || lo >= 32 ? 0u : 0xffffffffu;
-          if (bits && hi < 32) bits &= (1u << hi) - 1;
-          if (bits && lo > 0) bits &= ~((1u << lo) - 1);
-          see[w] = there ? bits & good[w] : 0xffffffffu;
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t bits = see(o / 32 + w);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(bits >> i & 1)) x[o + 32 * w + i] = 0xff800000u;
+          }
         }
-      }
-      float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t x[32];
-        ptx::tmem_load_32x32b_x32(s_at + 32 * w, x);
-        if (whole) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (see[w] >> i & 1) top = fmaxf(top, __uint_as_float(x[i]));
-        }
-      }
+        for (int i = 0; i < 64; i += 2)
+          tops[i / 2 & 3] = fmaxf(fmaxf(tops[i / 2 & 3], __uint_as_float(x[o + i])), __uint_as_float(x[o + i + 1]));
+      };
+      peak(0);
+      tmem_load64<64>(s_at + 64, x);
+      peak(64);
+      float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       top = top * c - shift<T>();
       const bool grow = top > m + kSlack || (m == -INFINITY && top > m);
       if (__any_sync(0xffffffffu, grow)) {
@@ -378,34 +454,32 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, const Share &shar
           tmem_store_wait();
         }
       }
-      const float base = m == -INFINITY ? 0.0f : m;
+      const uint32_t base = __float_as_uint(m == -INFINITY ? 0.0f : -m);
+      const Pair c2 = pair(__float_as_uint(c), __float_as_uint(c)), base2 = pair(base, base);
+      Pair sums[2] = {0, 0};
 #pragma unroll
-      for (int w = 3; w >= 0; --w) {  // numerators lie over the scores' second half
-        uint32_t x[32], y[16];
-        ptx::tmem_load_32x32b_x32(s_at + 32 * w, x);
-        if (!whole) {
+      for (int w = 0; w < 2; ++w) {
+        uint32_t y[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!(see[w] >> i & 1)) x[i] = __float_as_uint(-INFINITY);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e0 = ex2_approx(fmaf(__uint_as_float(x[2 * i]), c, -base));
-          const float e1 = ex2_approx(fmaf(__uint_as_float(x[2 * i + 1]), c, -base));
-          l += e0 + e1;
+        for (int i = 0; i < 32; ++i) {
+          const float2 z = halves(fma2(pair(x[64 * w + 2 * i], x[64 * w + 2 * i + 1]), c2, base2));
+          const float e0 = ex2_approx(z.x), e1 = ex2_approx(z.y);
+          sums[i & 1] = add2(sums[i & 1], pair(__float_as_uint(e0), __float_as_uint(e1)));
           // the numerators' rounding to the type, which the second product asks for;
           // their sum stays in fp32
           y[i] = pack<T>(e0, e1);
         }
-        tmem_store16(p_at + 16 * w, y);
+        tmem_store32(p_at + 32 * w, y);
       }
+      const float2 sum = halves(add2(sums[0], sums[1]));
+      l += sum.x + sum.y;
       tmem_store_wait();
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&sh.b.p_full[t]);
       ++done;
     }
-    block_count += most;
+    block_count += job->most;
     if (n) {
       if (!wait_warp(sh, &sh.b.pv_done[t], (done - 1) & 1, a.status)) return;
       ptx::tc_fence_after();
@@ -485,7 +559,8 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, const Share &shar
         }
       }
     }
-    if (threadIdx.x == 0 && !p.opens && p.ends) a.joins[blockIdx.x] = Join{p.first_cta, p.sequence, p.head, p.tile};
+    __syncwarp();
+    if (lane == 0) release_job(sh, i_job);
   }
 }
 
@@ -510,6 +585,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
       ptx::mbar_init(&sh.b.pv_done[t], 1);
       ptx::mbar_init(&sh.b.o_free[t], 4);
     }
+    for (int i = 0; i < kJobs; ++i) {
+      ptx::mbar_init(&sh.b.job_full[i], 1);
+      ptx::mbar_init(&sh.b.job_free[i], 8 + kLoaders / 32 + 1);  // softmax, loading, multiplying
+    }
     ptx::mbar_init(&sh.b.drained, 1);
     sh.gave_up = 0;
     ptx::fence_barrier_init();
@@ -519,19 +598,28 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
     ptx::tmem_relinquish();
   }
   pdl_enter();
-  if (!a.whole && threadIdx.x == 0) a.joins[blockIdx.x] = Join{0xffffffffu, 0, 0, 0};
+  if (!a.whole && threadIdx.x == 13 * 32) a.joins[blockIdx.x] = Join{0xffffffffu, 0, 0, 0};
   ptx::tc_fence_before();
   const Share share = share_of<kRows, kKeys, kThreads>(a, blockIdx.x, gridDim.x, a.whole ? 1 : 2 * kKeys);
   ptx::tc_fence_after();
-  if (warp < 8) soften<T, TO, DP>(a, share, sh);
-  else if (warp < 12) {
-    load<T, DP>(a, share, sh, queries, ring);
-    await<0>();
-  } else if ((threadIdx.x & 31) == 0) {
-    multiply<T, DP>(a, share, sh, queries, ring);
-    // everything issued is done before TMEM and the barriers go
-    ptx::mma_commit(&sh.b.drained);
-    if (!ptx::mbar_wait_bounded(&sh.b.drained, 0, kWaitLimitNs)) raise_flag(a.status, TL_FLAG_TIMEOUT);
+  // A row's 128 scores stay in registers: of the 512 x 128 that the CTA was launched
+  // with, 256 x 200 go to the softmax and 256 x 56 to the others.
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    soften<T, TO, DP>(a, sh);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp < 12) {
+      load<T, DP>(a, sh, queries, ring);
+      await<0>();
+    } else if (threadIdx.x == 12 * 32) {
+      multiply<T, DP>(a, sh, queries, ring);
+      // everything issued is done before TMEM and the barriers go
+      ptx::mma_commit(&sh.b.drained);
+      if (!ptx::mbar_wait_bounded(&sh.b.drained, 0, kWaitLimitNs)) raise_flag(a.status, TL_FLAG_TIMEOUT);
+    } else if (threadIdx.x == 13 * 32) {
+      plan_jobs(a, share, sh);
+    }
   }
   __syncwarp();
   ptx::tc_fence_before();
