@@ -35,6 +35,9 @@ constexpr int kThreads = 16 * 32, kLoaders = 128;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr float kSlack = 8.0f;  // log2 of how far numerators may pass 1
 constexpr int kLag = 2;         // ring places between a copy's issue and its hand-over
+// Values of block j and keys of block j + 1 (places 2 j + 1 and 2 j + 2 of the ring's
+// sequence) are given back together: one arrival in place of two, 200 cycles each.
+constexpr int kPairs = 8;
 constexpr int kJobs = 4;        // pieces worked out ahead
 constexpr int kMasks = 8;       // blocks whose missing keys are remembered: more than the ring is ahead
 
@@ -42,9 +45,9 @@ template <int DP> constexpr uint32_t tile_bytes() { return kTile * DP * 2; }
 template <int DP> constexpr int stages() { return DP == 128 ? 5 : 8; }
 
 struct Barriers {
-  uint64_t full[8], empty[8];
+  uint64_t full[8], empty[kPairs];
   uint64_t job_full[kJobs], job_free[kJobs];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], pv_done[2], o_free[2], drained;
+  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], o_free[2], drained;
 };
 // A piece and the blocks that its two tiles take, from the piece's first on;
 // more == false: there are no more.
@@ -96,13 +99,18 @@ __device__ __forceinline__ bool wait_warp(Shared &sh, uint64_t *bar, uint32_t pa
 __device__ __forceinline__ uint32_t spot(uint32_t r, uint32_t ch) {
   return (ch >> 3) * (kTile * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
 }
-// Queries and keys, K-major: elements [16 k, 16 k + 16).
-__device__ __forceinline__ uint64_t row_desc(uint32_t base, uint32_t k) {
-  return ptx::smem_desc(base + (k >> 2) * (kTile * 128) + (k & 3) * 32, 16, 1024, ptx::kSwizzle128B);
+// Queries and keys, K-major, from element 0 on; 16 elements further are 2, 64
+// are a block of 128 rows more.
+__device__ __forceinline__ uint64_t row_desc(uint32_t base) { return ptx::smem_desc(base, 16, 1024, ptx::kSwizzle128B); }
+__host__ __device__ constexpr uint32_t row_step(uint32_t k) { return (k >> 2) * (kTile * 128 / 16) + (k & 3) * 2; }
+// Values, MN-major (a row is a key), 64 elements a block; 16 keys further are 128 more.
+__device__ __forceinline__ uint64_t value_desc(uint32_t base) {
+  return ptx::smem_desc(base, kTile * 128, 1024, ptx::kSwizzle128B);
 }
-// Values, MN-major (a row is a key): keys [16 k, 16 k + 16), 64 elements a block.
-__device__ __forceinline__ uint64_t value_desc(uint32_t base, uint32_t k) {
-  return ptx::smem_desc(base + k * 2048, kTile * 128, 1024, ptx::kSwizzle128B);
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 // kind::f16 with fp32 sums: type 0 = fp16, 1 = bf16.
 __host__ __device__ constexpr uint32_t idesc_f16(uint32_t type, uint32_t M, uint32_t N, bool b_mn) {
@@ -283,7 +291,10 @@ __device__ __forceinline__ void load(const AttentionArgs &a, Shared &sh, uint32_
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         // a slot is free again when what was multiplied from it is done
-        if (!wait_warp(sh, &sh.b.empty[item % S], ((item / S) & 1) ^ 1, a.status)) return;
+        if (item >= static_cast<uint32_t>(S)) {
+          const uint32_t pair = (item - S + 1) / 2;
+          if (!wait_warp(sh, &sh.b.empty[pair % kPairs], (pair / kPairs) & 1, a.status)) return;
+        }
         if (half == 0 && lane == 0) sh.mask[block_count % kMasks][warp] = good;
         const T *base = half ? vp : kp;
         const uint32_t to = ring + (item % S) * kBytes;
@@ -308,71 +319,91 @@ __device__ __forceinline__ void load(const AttentionArgs &a, Shared &sh, uint32_
   await<0>();
   hand_over(item);
   // the last reads of the ring are over
-  for (uint32_t i = item > static_cast<uint32_t>(S) ? item - S : 0; i < item; ++i)
-    if (!wait_warp(sh, &sh.b.empty[i % S], (i / S) & 1, a.status)) return;
+  if (item && !wait_warp(sh, &sh.b.empty[item / 2 % kPairs], (item / 2 / kPairs) & 1, a.status)) return;
 }
 
+// By one warp, so that operands are in uniform registers; one thread issues.
+// A product's instructions are unrolled with descriptors that differ by
+// constants: worked out one by one they took 100 cycles each, as long as the
+// product itself.
 template <typename T, int DP>
 __device__ __forceinline__ void multiply(const AttentionArgs &a, Shared &sh, uint32_t queries, uint32_t ring) {
   constexpr int S = stages<DP>();
   constexpr uint32_t kBytes = tile_bytes<DP>();
   constexpr uint32_t type = std::is_same<T, __half>::value ? 0 : 1;
+  const bool leader = elect();
   const uint32_t ksteps = (a.cache.D + 15) / 16;
   const uint32_t score = idesc_f16(type, kTile, kKeys, false), output = idesc_f16(type, kTile, ksteps * 16, true);
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+  const uint64_t q_desc = row_desc(queries), k_desc = row_desc(ring), v_desc = value_desc(ring);
   uint32_t item = 0, piece = 0, s_count[2] = {0, 0}, opened[2] = {0, 0};
   const auto scores = [&](uint32_t t, uint32_t slot) {
     ptx::tc_fence_after();
-    for (uint32_t k = 0; k < ksteps; ++k)
-      mma_smem(tmem + t * 128, row_desc(queries + t * kBytes, k), row_desc(ring + slot * kBytes, k), score, k > 0);
-    ptx::mma_commit(&sh.b.s_full[t]);
+    const uint64_t q = q_desc + t * (kBytes / 16), k = k_desc + slot * (kBytes / 16);
+    if (leader) {
+#pragma unroll
+      for (uint32_t i = 0; i < DP / 16; ++i)
+        if (i < ksteps) mma_smem(tmem + t * 128, q + row_step(i), k + row_step(i), score, i > 0);
+      ptx::mma_commit(&sh.b.s_full[t]);
+    }
+  };
+  const auto give_back = [&](uint32_t pair) {
+    if (leader) ptx::mma_commit(&sh.b.empty[pair % kPairs]);
   };
   for (uint32_t i_job = 0;; ++i_job) {
     bool ok;
     const Job *const job = next_job(sh, i_job, a.status, &ok);
-    if (!ok || !job->more) return;
-    const uint32_t n[2] = {job->n[0], job->n[1]}, most = job->most;
-    release_job(sh, i_job);
+    if (!__all_sync(0xffffffffu, ok)) return;
+    const bool more = job->more;
+    const uint32_t n[2] = {__shfl_sync(0xffffffffu, job->n[0], 0), __shfl_sync(0xffffffffu, job->n[1], 0)}, most = max(n[0], n[1]);
+    __syncwarp();
+    if (!more) break;
+    if (leader) release_job(sh, i_job);
     if (!most) continue;
-    if (!wait(sh, &sh.b.q_full, piece & 1, a.status)) return;
+    if (!wait_warp(sh, &sh.b.q_full, piece & 1, a.status)) return;
     ++piece;
     const uint32_t first = item;  // block j: keys in place first + 2 j, values behind them
-    if (!wait(sh, &sh.b.full[first % S], (first / S) & 1, a.status)) return;
+    if (!wait_warp(sh, &sh.b.full[first % S], (first / S) & 1, a.status)) return;
 #pragma unroll
     for (uint32_t t = 0; t < 2; ++t)
       if (n[t]) scores(t, first % S);
-    ptx::mma_commit(&sh.b.empty[first % S]);
+    give_back(first / 2);
     for (uint32_t j = 0; j < most; ++j) {
-      const uint32_t v = first + 2 * j + 1, k = v + 1;
+      const uint32_t v = first + 2 * j + 1, k = v + 1, v_slot = v % S, k_slot = k % S;
       bool have_v = false, have_k = false;
 #pragma unroll
       for (uint32_t t = 0; t < 2; ++t) {
         if (j < n[t]) {
-          if (!wait(sh, &sh.b.p_full[t], s_count[t] & 1, a.status)) return;
-          ++s_count[t];
-          if (!have_v && !wait(sh, &sh.b.full[v % S], (v / S) & 1, a.status)) return;
+          if (!have_v && !wait_warp(sh, &sh.b.full[v_slot], (v / S) & 1, a.status)) return;
           have_v = true;
           if (j == 0) {  // the tile's last output has been read
-            if (!wait(sh, &sh.b.o_free[t], (opened[t] & 1) ^ 1, a.status)) return;
+            if (!wait_warp(sh, &sh.b.o_free[t], (opened[t] & 1) ^ 1, a.status)) return;
             ++opened[t];
           }
+          if (!wait_warp(sh, &sh.b.p_full[t], s_count[t] & 1, a.status)) return;
+          ++s_count[t];
           ptx::tc_fence_after();
-          for (uint32_t i = 0; i < kKeys / 16; ++i)
-            mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + 64 + i * 8, value_desc(ring + (v % S) * kBytes, i), output, (j | i) > 0);
-          ptx::mma_commit(&sh.b.pv_done[t]);
+          const uint64_t values = v_desc + v_slot * (kBytes / 16);
+          if (leader) {
+#pragma unroll
+            for (uint32_t i = 0; i < kKeys / 16; ++i)
+              mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + 64 + i * 8, values + i * 128, output, (j | i) > 0);
+            if (j + 1 == n[t]) ptx::mma_commit(&sh.b.o_full[t]);
+          }
         }
         if (j + 1 < n[t]) {
-          if (!have_k && !wait(sh, &sh.b.full[k % S], (k / S) & 1, a.status)) return;
+          if (!have_k && !wait_warp(sh, &sh.b.full[k_slot], (k / S) & 1, a.status)) return;
           have_k = true;
-          scores(t, k % S);
+          scores(t, k_slot);
         }
       }
-      ptx::mma_commit(&sh.b.empty[v % S]);
-      if (j + 1 < most) ptx::mma_commit(&sh.b.empty[k % S]);
+      // the last block's values go back with the next piece's first keys
+      if (j + 1 < most) give_back(k / 2);
     }
-    ptx::mma_commit(&sh.b.q_empty);
+    if (leader) ptx::mma_commit(&sh.b.q_empty);
     item += 2 * most;
   }
+  if (item) give_back(item / 2);
 }
 
 template <typename T, typename TO, int DP>
@@ -382,7 +413,7 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh) {
   const uint32_t s_at = sh.tmem + t * 128 + lanes, p_at = s_at + 64, o_at = sh.tmem + 256 + t * 128 + lanes;
   const float c = a.scale * kLog2e;
   const tl_paged_cache &cache = a.cache;
-  uint32_t done = 0, block_count = 0;  // of this tile: blocks whose scores were taken
+  uint32_t done = 0, outputs = 0, block_count = 0;  // of this tile: blocks whose scores were taken, pieces
   for (uint32_t i_job = 0;; ++i_job) {
     bool ok;
     const Job *const job = next_job(sh, i_job, a.status, &ok);
@@ -440,9 +471,7 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh) {
           m = top;
           l *= f;
         }
-        if (j > 0) {  // the output so far
-          if (!wait_warp(sh, &sh.b.pv_done[t], (done - 1) & 1, a.status)) return;
-          ptx::tc_fence_after();
+        if (j > 0) {  // the output so far, complete where these scores are
 #pragma unroll 1
           for (uint32_t d = 0; d < cache.D; d += 32) {
             uint32_t x[32];
@@ -481,7 +510,8 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh) {
     }
     block_count += job->most;
     if (n) {
-      if (!wait_warp(sh, &sh.b.pv_done[t], (done - 1) & 1, a.status)) return;
+      if (!wait_warp(sh, &sh.b.o_full[t], outputs & 1, a.status)) return;
+      ++outputs;
       ptx::tc_fence_after();
     }
     const uint64_t place = p.row0 + in_job, token = p.start + place / a.group;
@@ -575,14 +605,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       ptx::mbar_init(&sh.b.full[i], kLoaders / 32);
-      ptx::mbar_init(&sh.b.empty[i], 1);
     }
+    for (int i = 0; i < kPairs; ++i) ptx::mbar_init(&sh.b.empty[i], 1);
     ptx::mbar_init(&sh.b.q_full, kLoaders / 32);
     ptx::mbar_init(&sh.b.q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(&sh.b.s_full[t], 1);
       ptx::mbar_init(&sh.b.p_full[t], 4);
-      ptx::mbar_init(&sh.b.pv_done[t], 1);
+      ptx::mbar_init(&sh.b.o_full[t], 1);
       ptx::mbar_init(&sh.b.o_free[t], 4);
     }
     for (int i = 0; i < kJobs; ++i) {
@@ -612,10 +642,11 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
     if (warp < 12) {
       load<T, DP>(a, sh, queries, ring);
       await<0>();
-    } else if (threadIdx.x == 12 * 32) {
+    } else if (warp == 12) {
       multiply<T, DP>(a, sh, queries, ring);
+      __syncwarp();
       // everything issued is done before TMEM and the barriers go
-      ptx::mma_commit(&sh.b.drained);
+      if (elect()) ptx::mma_commit(&sh.b.drained);
       if (!ptx::mbar_wait_bounded(&sh.b.drained, 0, kWaitLimitNs)) raise_flag(a.status, TL_FLAG_TIMEOUT);
     } else if (threadIdx.x == 13 * 32) {
       plan_jobs(a, share, sh);
