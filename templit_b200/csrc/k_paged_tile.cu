@@ -13,9 +13,12 @@
 //                   in TMEM and is rescaled only when a row's maximum grew
 //                   by more than 2^8 (numerators then are at most 2^8, which
 //                   fp32 sums and 16-bit types hold)
-//   warps 8-11      keys and values, 128 at a time, by cp.async into a ring
-//                   (pages end anywhere, so rows come one by one, 16 bytes a
-//                   lane, a page's address looked up once a row), and the queries
+//   warps 8-11      keys and values, 128 at a time (32 a warp), into a ring, and
+//                   the queries.  By TMA where a page holds whole runs of 8, 16 or
+//                   32 keys and all 32 are there; else row by row with cp.async,
+//                   16 bytes a lane, which writes zeros for the keys that are
+//                   not there (3600 cycles of a warp for a block, more than its
+//                   products take; TMA's boxes are a few instructions)
 //   warp 13         one thread works out the CTA's pieces of jobs, ahead of the others
 //   warp 12         one thread issues S = Q K^T and O += P V (tcgen05.mma
 //                   kind::f16, fp32 in TMEM)
@@ -92,6 +95,29 @@ __device__ __forceinline__ bool wait(Shared &sh, uint64_t *bar, uint32_t parity,
 // The same for a whole warp, with one answer.
 __device__ __forceinline__ bool wait_warp(Shared &sh, uint64_t *bar, uint32_t parity, uint32_t *status) {
   return __all_sync(0xffffffffu, wait(sh, bar, parity, status));
+}
+
+// How keys, values and queries lie, for TMA: boxes of `rows` keys (0: none), of
+// a tile's queries where `queries` (a power of two of query heads a key head).
+struct Maps {
+  CUtensorMap k, v, q;  // (D, slot, head, page); (D, head, token)
+  uint32_t rows, queries;
+};
+__device__ __forceinline__ void tma_box4(uint32_t to, const CUtensorMap *map, uint64_t *bar, uint32_t x, uint32_t slot,
+                                         uint32_t head, uint32_t page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(ptx::smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_box3(uint32_t to, const CUtensorMap *map, uint64_t *bar, uint32_t x, uint32_t head,
+                                         uint32_t token) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(ptx::smem_addr(bar))
+      : "memory");
 }
 
 // Vector `ch` (16 bytes) of row `r` of a tile: 128-byte rows of 64 elements
@@ -227,18 +253,24 @@ __device__ __forceinline__ void plan_jobs(const AttentionArgs &a, const Share &s
 }
 
 template <typename T, int DP>
-__device__ __forceinline__ void load(const AttentionArgs &a, Shared &sh, uint32_t queries, uint32_t ring) {
+__device__ __forceinline__ void load(const AttentionArgs &a, const Maps &maps, Shared &sh, uint32_t queries, uint32_t ring) {
   constexpr int S = stages<DP>();
-  constexpr uint32_t CH = DP / 8, kBytes = tile_bytes<DP>();
+  constexpr uint32_t CH = DP / 8, kBytes = tile_bytes<DP>(), kBlocks = DP / 64;
   const uint32_t lane = threadIdx.x & 31, warp = (threadIdx.x - 256) / 32;
   const tl_paged_cache &c = a.cache;
-  uint32_t item = 0, handed = 0, block_count = 0, q_phase = 0;
-  // copies up to `upto` have arrived and are the tensor cores' to read
+  uint32_t item = 0, handed = 0, by_rows = 0, block_count = 0, q_phase = 0;
+  // cp.async's copies up to `upto` (a bit of by_rows each) have arrived and are
+  // the tensor cores' to read
   const auto hand_over = [&](uint32_t upto) {
-    ptx::fence_proxy_async_smem();
-    __syncwarp();
-    for (; handed < upto; ++handed)
-      if (lane == 0) ptx::mbar_arrive(&sh.b.full[handed % S]);
+    if (by_rows) {
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+    }
+    for (; handed < upto; ++handed) {
+      const uint32_t bit = 1u << (handed & 31);
+      if (by_rows & bit && lane == 0) ptx::mbar_arrive(&sh.b.full[handed % S]);
+      by_rows &= ~bit;
+    }
   };
   for (uint32_t i_job = 0;; ++i_job) {
     bool ok;
@@ -246,48 +278,23 @@ __device__ __forceinline__ void load(const AttentionArgs &a, Shared &sh, uint32_
     if (!__all_sync(0xffffffffu, ok)) return;
     if (!job->more) break;
     const Piece &p = job->p;
-    const uint32_t n = job->most;
-    if (!n) {
-      __syncwarp();
-      if (lane == 0) release_job(sh, i_job);
-      continue;
-    }
-    // the queries: the rows of this warp, 32 of each tile
-    await<0>();
-    hand_over(item);
-    if (!wait_warp(sh, &sh.b.q_empty, (q_phase & 1) ^ 1, a.status)) return;
-    ++q_phase;
-#pragma unroll
-    for (uint32_t t = 0; t < 2; ++t) {
-      const uint32_t mine = t * kTile + warp * 32 + lane;
-      const uint64_t place = p.row0 + mine;
-      int64_t at = -1;
-      if (mine <= p.last)
-        at = static_cast<int64_t>((p.start + place / a.group) * a.q.row_stride + (p.head * a.group + place % a.group) * a.q.head_stride);
-#pragma unroll 4
-      for (uint32_t i = 0; i < CH; ++i) {
-        const uint32_t row = (lane + 32 * i) / CH, ch = (lane + 32 * i) % CH;
-        const int64_t from = __shfl_sync(0xffffffffu, at, row);
-        const bool there = from >= 0 && ch * 8 < c.D;
-        copy16(queries + t * kBytes + spot(warp * 32 + row, ch), static_cast<const T *>(a.q.p) + (there ? from + ch * 8 : 0), there);
-      }
-    }
-    commit();
-    await<0>();
-    ptx::fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) ptx::mbar_arrive(&sh.b.q_full);
-
-    const T *kp = static_cast<const T *>(c.k) + p.head * c.head_stride;
-    const T *vp = static_cast<const T *>(c.v) + p.head * c.head_stride;
-    const auto offset_of = [&](uint32_t block) -> int64_t {
-      const uint32_t j = (p.block_lo + block) * kKeys + warp * 32 + lane;
-      return block < n && j >= p.from && j < p.to ? key_offset(a, p.sequence, j) : -1;
+    const uint32_t n = job->most, head = p.head;
+    // this lane's key of a block: its page (no page: UINT32_MAX) and slot
+    const uint32_t *const table = c.table + static_cast<uint64_t>(p.sequence) * c.table_stride;
+    const auto look_up = [&](uint32_t block, uint32_t &page, uint32_t &slot) {
+      const uint32_t j = (p.block_lo + block) * kKeys + warp * 32 + lane, i = j / c.page_size;
+      slot = j - i * c.page_size;
+      page = block < n && j >= p.from && j < p.to ? table[i] : 0xffffffffu;
     };
-    int64_t at = offset_of(0);
+    uint32_t page, slot, next_page, next_slot;
+    look_up(0, page, slot);
     for (uint32_t j = 0; j < n; ++j) {
-      const int64_t next = offset_of(j + 1);
-      const uint32_t good = __ballot_sync(0xffffffffu, at >= 0);
+      look_up(j + 1, next_page, next_slot);
+      const uint32_t key = (p.block_lo + j) * kKeys + warp * 32 + lane;
+      const bool there = page < c.pages;
+      if (!there && key >= p.from && key < p.to) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
+      const uint32_t good = __ballot_sync(0xffffffffu, there);
+      const bool boxes = maps.rows && good == 0xffffffffu;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         // a slot is free again when what was multiplied from it is done
@@ -296,22 +303,79 @@ __device__ __forceinline__ void load(const AttentionArgs &a, Shared &sh, uint32_
           if (!wait_warp(sh, &sh.b.empty[pair % kPairs], (pair / kPairs) & 1, a.status)) return;
         }
         if (half == 0 && lane == 0) sh.mask[block_count % kMasks][warp] = good;
-        const T *base = half ? vp : kp;
-        const uint32_t to = ring + (item % S) * kBytes;
-#pragma unroll 8
-        for (uint32_t i = 0; i < CH; ++i) {
-          const uint32_t row = (lane + 32 * i) / CH, ch = (lane + 32 * i) % CH;
-          const int64_t from = __shfl_sync(0xffffffffu, at, row);
-          const bool there = from >= 0 && ch * 8 < c.D;
-          copy16(to + spot(warp * 32 + row, ch), base + (there ? from + ch * 8 : 0), there);
+        const uint32_t to = ring + (item % S) * kBytes + warp * 32 * 128;
+        uint64_t *const full = &sh.b.full[item % S];
+        if (boxes) {
+          const uint32_t from = lane * maps.rows & 31;
+          const uint32_t b_page = __shfl_sync(0xffffffffu, page, from), b_slot = __shfl_sync(0xffffffffu, slot, from);
+          if (lane == 0) ptx::mbar_arrive_expect_tx(full, 32 * 128 * kBlocks);
+          __syncwarp();
+          if (lane * maps.rows < 32)
+#pragma unroll
+            for (uint32_t b = 0; b < kBlocks; ++b)
+              tma_box4(to + b * (kTile * 128) + from * 128, half ? &maps.v : &maps.k, full, b * 64, b_slot, head, b_page);
+        } else {
+          const T *base = static_cast<const T *>(half ? c.v : c.k) + head * c.head_stride;
+          const int64_t at = there ? static_cast<int64_t>(page * c.page_stride + slot * c.slot_stride) : -1;
+#pragma unroll 4
+          for (uint32_t i = 0; i < CH; ++i) {
+            const uint32_t row = (lane + 32 * i) / CH, ch = (lane + 32 * i) % CH;
+            const int64_t from = __shfl_sync(0xffffffffu, at, row);
+            const bool put = from >= 0 && ch * 8 < c.D;
+            copy16(to + spot(row, ch), base + (put ? from + ch * 8 : 0), put);
+          }
+          by_rows |= 1u << (item & 31);
         }
         commit();
         ++item;
-        await<kLag>();
-        if (item > kLag) hand_over(max(handed, item - kLag));
+        if (j == 0 && half == 0) {
+          // the queries: the rows of this warp, 32 of each tile
+          await<0>();
+          hand_over(item);
+          if (!wait_warp(sh, &sh.b.q_empty, (q_phase & 1) ^ 1, a.status)) return;
+          ++q_phase;
+          if (maps.queries) {
+            if (warp == 0 && lane == 0) {
+              const bool both = p.last >= kTile;
+              ptx::mbar_arrive_expect_tx(&sh.b.q_full, (both ? 2 : 1) * kBytes);
+              const uint32_t token = p.start + static_cast<uint32_t>(p.row0 / a.group);
+              for (uint32_t t = 0; t < (both ? 2u : 1u); ++t)
+                for (uint32_t b = 0; b < kBlocks; ++b)
+                  tma_box3(queries + t * kBytes + b * (kTile * 128), &maps.q, &sh.b.q_full, b * 64, head * a.group,
+                           token + t * (kTile / a.group));
+            } else if (lane == 0) {
+              ptx::mbar_arrive(&sh.b.q_full);
+            }
+          } else {
+            for (uint32_t t = 0; t < 2; ++t) {
+              const uint32_t mine = t * kTile + warp * 32 + lane;
+              const uint64_t place = p.row0 + mine;
+              int64_t at = -1;
+              if (mine <= p.last)
+                at = static_cast<int64_t>((p.start + place / a.group) * a.q.row_stride +
+                                          (head * a.group + place % a.group) * a.q.head_stride);
+#pragma unroll 4
+              for (uint32_t i = 0; i < CH; ++i) {
+                const uint32_t row = (lane + 32 * i) / CH, ch = (lane + 32 * i) % CH;
+                const int64_t from = __shfl_sync(0xffffffffu, at, row);
+                const bool put = from >= 0 && ch * 8 < c.D;
+                copy16(queries + t * kBytes + warp * 32 * 128 + spot(row, ch), static_cast<const T *>(a.q.p) + (put ? from + ch * 8 : 0), put);
+              }
+            }
+            commit();
+            await<0>();
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&sh.b.q_full);
+          }
+        } else {
+          await<kLag>();
+          if (item > kLag) hand_over(max(handed, item - kLag));
+        }
       }
       ++block_count;
-      at = next;
+      page = next_page;
+      slot = next_slot;
     }
     __syncwarp();
     if (lane == 0) release_job(sh, i_job);
@@ -595,7 +659,7 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh) {
 }
 
 template <typename T, typename TO, int DP>
-__global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a, const __grid_constant__ Maps maps) {
   constexpr int S = stages<DP>();
   extern __shared__ uint8_t raw[];
   uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -640,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp < 12) {
-      load<T, DP>(a, sh, queries, ring);
+      load<T, DP>(a, maps, sh, queries, ring);
       await<0>();
     } else if (warp == 12) {
       multiply<T, DP>(a, sh, queries, ring);
@@ -659,10 +723,44 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
   if (warp == 12) ptx::tmem_dealloc(sh.tmem, 512);
 }
 
+bool encode(CUtensorMap *map, int32_t type, const void *base, uint32_t rank, const cuuint64_t *dims, const uint64_t *strides,
+            const cuuint32_t *box) {
+  EncodeTiledFn enc = tensor_map_encoder();
+  if (!enc) return false;
+  cuuint64_t bytes[3];
+  for (uint32_t i = 0; i + 1 < rank; ++i) bytes[i] = strides[i] * 2;
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return enc(map, type == TL_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+             const_cast<void *>(base), dims, bytes, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Boxes where the layout allows them; without, rows are copied one by one.
+// x is 0 or 64 elements, so that every box starts on a 16-byte boundary.
+Maps make_maps(const AttentionArgs &a) {
+  const tl_paged_cache &c = a.cache;
+  Maps m{};
+  uint32_t rows = 32;
+  while (rows >= 8 && c.page_size % rows) rows /= 2;
+  if (rows >= 8 && c.pages) {
+    const cuuint64_t dims[4] = {c.D, c.page_size, c.heads, c.pages};
+    const uint64_t strides[3] = {c.slot_stride, c.heads > 1 ? c.head_stride : c.slot_stride, c.pages > 1 ? c.page_stride : c.slot_stride};
+    const cuuint32_t box[4] = {64, rows, 1, 1};
+    if (encode(&m.k, c.type, c.k, 4, dims, strides, box) && encode(&m.v, c.type, c.v, 4, dims, strides, box)) m.rows = rows;
+  }
+  if (a.group <= kTile && (a.group & (a.group - 1)) == 0) {
+    const cuuint64_t dims[3] = {c.D, a.q_heads, c.tokens};
+    const uint64_t strides[2] = {a.q_heads > 1 ? a.q.head_stride : c.D * 2u, c.tokens > 1 ? a.q.row_stride : c.D * 2u};
+    const cuuint32_t box[3] = {64, a.group, kTile / a.group};
+    m.queries = encode(&m.q, c.type, a.q.p, 3, dims, strides, box);
+  }
+  return m;
+}
+
 template <typename T, typename TO, int DP> void launch(const AttentionArgs &a, const Plan &p, cudaStream_t s) {
   constexpr size_t smem = smem_bytes<DP>();
   (void)cudaFuncSetAttribute(tile_kernel<T, TO, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  launch_pdl(tile_kernel<T, TO, DP>, p.ctas, kThreads, smem, s, a);
+  launch_pdl(tile_kernel<T, TO, DP>, p.ctas, kThreads, smem, s, a, make_maps(a));
   if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, 8), 128, 0, s, a);
 }
 
