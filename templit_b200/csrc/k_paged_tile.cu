@@ -37,6 +37,8 @@ constexpr uint32_t kTile = 128, kRows = 2 * kTile, kKeys = 128;
 constexpr int kThreads = 16 * 32, kLoaders = 128;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr float kSlack = 8.0f;  // log2 of how far numerators may pass 1
+// Pairs of exponentials in 8 that the FMA pipe takes: 0 ... measured below.
+constexpr int kPolynomial = 0;
 constexpr int kLag = 2;         // ring places between a copy's issue and its hand-over
 // Values of block j and keys of block j + 1 (places 2 j + 1 and 2 j + 2 of the ring's
 // sequence) are given back together: one arrival in place of two, 200 cycles each.
@@ -45,12 +47,13 @@ constexpr int kJobs = 4;        // pieces worked out ahead
 constexpr int kMasks = 8;       // blocks whose missing keys are remembered: more than the ring is ahead
 
 template <int DP> constexpr uint32_t tile_bytes() { return kTile * DP * 2; }
-template <int DP> constexpr int stages() { return DP == 128 ? 5 : 8; }
+template <int DP> constexpr int stages() { return DP == 128 ? 4 : 8; }
+constexpr uint32_t kStaging = 8 * 4096;  // 32 rows of 128 bytes for each softmax warp
 
 struct Barriers {
   uint64_t full[8], empty[kPairs];
   uint64_t job_full[kJobs], job_free[kJobs];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], o_free[2], drained;
+  uint64_t q_full, q_empty, s_full[2], p_full[2][2], o_half[2], o_full[2], o_free[2], drained;
 };
 // A piece and the blocks that its two tiles take, from the piece's first on;
 // more == false: there are no more.
@@ -66,7 +69,7 @@ struct Shared {
   uint32_t mask[kMasks][4];  // a bit for every key of a block that is there
 };
 template <int DP> constexpr size_t smem_bytes() {
-  return 1024 + 2 * tile_bytes<DP>() + stages<DP>() * static_cast<size_t>(tile_bytes<DP>()) + sizeof(Shared);
+  return 1024 + 2 * tile_bytes<DP>() + stages<DP>() * static_cast<size_t>(tile_bytes<DP>()) + kStaging + sizeof(Shared);
 }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
@@ -158,15 +161,6 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uin
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 64 columns of this warp's 32 lanes, with their wait (see tmem_load_32x32b_x16)
-template <int O> __device__ __forceinline__ void tmem_load64(uint32_t taddr, uint32_t (&r)[128]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[O + 0]), "=r"(r[O + 1]), "=r"(r[O + 2]), "=r"(r[O + 3]), "=r"(r[O + 4]), "=r"(r[O + 5]), "=r"(r[O + 6]), "=r"(r[O + 7]), "=r"(r[O + 8]), "=r"(r[O + 9]), "=r"(r[O + 10]), "=r"(r[O + 11]), "=r"(r[O + 12]), "=r"(r[O + 13]), "=r"(r[O + 14]), "=r"(r[O + 15]), "=r"(r[O + 16]), "=r"(r[O + 17]), "=r"(r[O + 18]), "=r"(r[O + 19]), "=r"(r[O + 20]), "=r"(r[O + 21]), "=r"(r[O + 22]), "=r"(r[O + 23]), "=r"(r[O + 24]), "=r"(r[O + 25]), "=r"(r[O + 26]), "=r"(r[O + 27]), "=r"(r[O + 28]), "=r"(r[O + 29]), "=r"(r[O + 30]), "=r"(r[O + 31]), "=r"(r[O + 32]), "=r"(r[O + 33]), "=r"(r[O + 34]), "=r"(r[O + 35]), "=r"(r[O + 36]), "=r"(r[O + 37]), "=r"(r[O + 38]), "=r"(r[O + 39]), "=r"(r[O + 40]), "=r"(r[O + 41]), "=r"(r[O + 42]), "=r"(r[O + 43]), "=r"(r[O + 44]), "=r"(r[O + 45]), "=r"(r[O + 46]), "=r"(r[O + 47]), "=r"(r[O + 48]), "=r"(r[O + 49]), "=r"(r[O + 50]), "=r"(r[O + 51]), "=r"(r[O + 52]), "=r"(r[O + 53]), "=r"(r[O + 54]), "=r"(r[O + 55]), "=r"(r[O + 56]), "=r"(r[O + 57]), "=r"(r[O + 58]), "=r"(r[O + 59]), "=r"(r[O + 60]), "=r"(r[O + 61]), "=r"(r[O + 62]), "=r"(r[O + 63])
-      : "r"(taddr)
-      : "memory");
-}
 // Two fp32 in a register pair: one issued instruction for both.
 typedef unsigned long long Pair;
 __device__ __forceinline__ Pair pair(uint32_t lo, uint32_t hi) {
@@ -189,7 +183,41 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// 32 columns of this warp's 32 lanes into TMEM
+// The larger of three; NaN where one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of two finite numbers on the FMA pipe, which the softmax leaves idle while
+// it waits for 16 exponentials a cycle of the other: x = n + f, |f| <= 1/2, 2^f by
+// a polynomial fitted to it (1.7e-7 relative in fp32, 1 at 0), n into the
+// exponent.  x is 15 at most; below -126 it is taken as -126, which no sum of
+// 2^-21 and more notices.
+__device__ __forceinline__ void exp2_pair(Pair x, float &lo, float &hi) {
+  const float2 v = halves(x);
+  const Pair z = pair(__float_as_uint(fmaxf(v.x, -126.0f)), __float_as_uint(fmaxf(v.y, -126.0f)));
+  const auto both = [](float c) { return pair(__float_as_uint(c), __float_as_uint(c)); };
+  const Pair t = add2(z, both(12582912.0f));  // 1.5 * 2^23: whole numbers in the low bits
+  const Pair f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), z);
+  Pair p = fma2(both(0.001326472731307149f), f, both(0.009671512991189957f));
+  p = fma2(p, f, both(0.05550733581185341f));
+  p = fma2(p, f, both(0.24022242426872253f));
+  p = fma2(p, f, both(0.6931470036506653f));
+  p = fma2(p, f, both(1.0f));
+  const float2 q = halves(p), n = halves(t);
+  lo = __uint_as_float(__float_as_uint(q.x) + (__float_as_uint(n.x) << 23));
+  hi = __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(n.y) << 23));
+}
+// 16 and 32 columns of this warp's 32 lanes into TMEM
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -444,16 +472,20 @@ __device__ __forceinline__ void multiply(const AttentionArgs &a, Shared &sh, uin
             if (!wait_warp(sh, &sh.b.o_free[t], (opened[t] & 1) ^ 1, a.status)) return;
             ++opened[t];
           }
-          if (!wait_warp(sh, &sh.b.p_full[t], s_count[t] & 1, a.status)) return;
-          ++s_count[t];
-          ptx::tc_fence_after();
           const uint64_t values = v_desc + v_slot * (kBytes / 16);
-          if (leader) {
 #pragma unroll
-            for (uint32_t i = 0; i < kKeys / 16; ++i)
-              mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + 64 + i * 8, values + i * 128, output, (j | i) > 0);
-            if (j + 1 == n[t]) ptx::mma_commit(&sh.b.o_full[t]);
+          for (uint32_t h = 0; h < 2; ++h) {
+            if (!wait_warp(sh, &sh.b.p_full[t][h], s_count[t] & 1, a.status)) return;
+            ptx::tc_fence_after();
+            if (leader) {
+#pragma unroll
+              for (uint32_t i = 0; i < kKeys / 32; ++i)
+                mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + h * 64 + i * 8, values + (h * 4 + i) * 128, output, (j | h | i) > 0);
+              if (h == 0) ptx::mma_commit(&sh.b.o_half[t]);
+              else if (j + 1 == n[t]) ptx::mma_commit(&sh.b.o_full[t]);
+            }
           }
+          ++s_count[t];
         }
         if (j + 1 < n[t]) {
           if (!have_k && !wait_warp(sh, &sh.b.full[k_slot], (k / S) & 1, a.status)) return;
@@ -470,14 +502,78 @@ __device__ __forceinline__ void multiply(const AttentionArgs &a, Shared &sh, uin
   if (item) give_back(item / 2);
 }
 
+// Whether a value of the keys [from, to) is not finite, by a warp.
+template <typename T>
+__device__ __forceinline__ bool any_infinite(const AttentionArgs &a, uint32_t s, uint32_t head, uint32_t from, uint32_t to, uint32_t lane) {
+  const T *v = static_cast<const T *>(a.cache.v) + head * a.cache.head_stride;
+  bool found = false;
+  for (uint32_t j = from; j < to && !found; ++j) {
+    const int64_t at = key_offset(a, s, j);
+    for (uint32_t d = lane; at >= 0 && d < a.cache.D; d += 32) {
+      const float x = heads::element_of(v[at + d]);
+      found = found || x - x != 0.0f;
+    }
+    found = __any_sync(0xffffffffu, found);
+  }
+  return found;
+}
+
+// A warp's 32 rows of the output, 128 bytes of each at a time through its 4 KB
+// of shared memory: stored row by row, a lane 16 bytes of its own, each
+// instruction touched 32 lines and a piece took 9000 cycles to end.  `row` is where the
+// lane's row begins, null where it goes nowhere.
+template <typename U>
+__device__ __forceinline__ bool put_rows(uint32_t o_at, bool any, uint32_t D, float factor, U *row, uint4 *staging) {
+  constexpr uint32_t E = 128 / sizeof(U);  // elements of a row at a time
+  const uint32_t lane = threadIdx.x & 31;
+  bool nan = false;
+#pragma unroll 1
+  for (uint32_t d0 = 0; d0 < D; d0 += E) {
+#pragma unroll
+    for (uint32_t b = 0; b < E / 32; ++b) {
+      uint32_t x[32];
+      if (any) ptx::tmem_load_32x32b_x32(o_at + d0 + 32 * b, x);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (!any) x[i] = 0;
+        const float y = __uint_as_float(x[i]);
+        nan = nan || (y != y && d0 + 32 * b + i < D);
+        x[i] = __float_as_uint(y * factor);
+      }
+#pragma unroll
+      for (uint32_t v = 0; v < 32 * sizeof(U) / 16; ++v) {
+        constexpr int N = 16 / sizeof(U);
+        float y[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[i] = __uint_as_float(x[v * N + i]);
+        heads::Raw<U, N> raw;
+        raw.set(y);
+        const uint32_t ch = b * (32 * sizeof(U) / 16) + v;
+        staging[lane * 8 + (ch ^ (lane & 7))] = raw.r[0];
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t r = i * 4 + lane / 8, ch = lane & 7, d = d0 + ch * (16 / sizeof(U));
+      U *const to = reinterpret_cast<U *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r));
+      if (to && d < D) *reinterpret_cast<uint4 *>(to + d) = staging[r * 8 + (ch ^ (r & 7))];
+    }
+    __syncwarp();
+  }
+  return nan;
+}
+
 template <typename T, typename TO, int DP>
-__device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh) {
+__device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8_t *all_staging) {
   const uint32_t lane = threadIdx.x & 31, t = threadIdx.x / 128, row = threadIdx.x & 127;
   const uint32_t lanes = (threadIdx.x / 32 & 3) << 21;  // this warp's 32 lanes of TMEM
-  const uint32_t s_at = sh.tmem + t * 128 + lanes, p_at = s_at + 64, o_at = sh.tmem + 256 + t * 128 + lanes;
+  const uint32_t s_at = sh.tmem + t * 128 + lanes, o_at = sh.tmem + 256 + t * 128 + lanes;
+  uint4 *const staging = reinterpret_cast<uint4 *>(all_staging + threadIdx.x / 32 * 4096);
   const float c = a.scale * kLog2e;
+  const Pair c2 = pair(__float_as_uint(c), __float_as_uint(c));
   const tl_paged_cache &cache = a.cache;
-  uint32_t done = 0, outputs = 0, block_count = 0;  // of this tile: blocks whose scores were taken, pieces
+  uint32_t done = 0, outputs = 0, block_count = 0;  // of this tile: blocks whose scores were taken, pieces; all blocks
   for (uint32_t i_job = 0;; ++i_job) {
     bool ok;
     const Job *const job = next_job(sh, i_job, a.status, &ok);
@@ -486,90 +582,124 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh) {
     const uint32_t n = job->n[t];
     const uint32_t in_job = t * kTile + row;
     const bool there = in_job <= p.last;
-    // rows behind the last one see everything: their scores are 0 and go nowhere
+    // rows behind the last one see everything: their scores go nowhere
     uint32_t from = 0, to = 0xffffffffu;
     if (there) seen(a, p.length, p.position(a, in_job), from, to);
     float m = -INFINITY, l = 0.0f;
     for (uint32_t j = 0; j < n; ++j) {
       if (!wait_warp(sh, &sh.b.s_full[t], done & 1, a.status)) return;
       ptx::tc_fence_after();
-      const uint32_t key = (p.block_lo + j) * kKeys;
-      const uint32_t *good = sh.mask[(block_count + j) % kMasks];
-      const uint32_t all = good[0] & good[1] & good[2] & good[3];
-      const bool whole = __all_sync(0xffffffffu, key >= from && to >= kKeys && key <= to - kKeys && all == 0xffffffffu);
-      // bit i: the row sees key 32 w + i
-      const auto see = [&](int w) {
-        const int64_t lo = static_cast<int64_t>(from) - key - 32 * w, hi = static_cast<int64_t>(to) - key - 32 * w;
-        uint32_t bits = hi <= 0 || lo >= 32 ? 0u : 0xffffffffu;
-        if (bits && hi < 32) bits &= (1u << hi) - 1;
-        if (bits && lo > 0) bits &= ~((1u << lo) - 1);
-        return there ? bits & good[w] : 0xffffffffu;
-      };
-      uint32_t x[128];
-      tmem_load64<0>(s_at, x);
-      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      const auto peak = [&](int o) {
-        if (!whole) {
+      // By halves of 64 keys, so that the second product starts on the first; one copy
+      // of the code, which the warps' instruction caches hold.
+#pragma unroll 1
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t key = (p.block_lo + j) * kKeys + h * 64, at = s_at + h * 64;
+        const uint32_t *good = &sh.mask[(block_count + j) % kMasks][2 * h];
+        const bool whole = key >= from && to >= 64 && key <= to - 64 && (good[0] & good[1]) == 0xffffffffu;
+        // Numerators by the maximum of the keys before, in one pass: the scores' own
+        // maximum is looked at behind it, and seldom passes that one by 2^8.
+        bool settled = __all_sync(0xffffffffu, whole && m != -INFINITY);
+        if (settled) {
+          const uint32_t base = __float_as_uint(-m);
+          const Pair base2 = pair(base, base);
+          float top[2] = {-INFINITY, -INFINITY};
+          Pair sums[2] = {0, 0};
+          uint32_t y[32];
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            const uint32_t bits = see(o / 32 + w);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(bits >> i & 1)) x[o + 32 * w + i] = 0xff800000u;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 64; i += 2)
-          tops[i / 2 & 3] = fmaxf(fmaxf(tops[i / 2 & 3], __uint_as_float(x[o + i])), __uint_as_float(x[o + i + 1]));
-      };
-      peak(0);
-      tmem_load64<64>(s_at + 64, x);
-      peak(64);
-      float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      top = top * c - shift<T>();
-      const bool grow = top > m + kSlack || (m == -INFINITY && top > m);
-      if (__any_sync(0xffffffffu, grow)) {
-        float f = 1.0f;
-        if (grow) {
-          f = ex2_approx(m - top);
-          m = top;
-          l *= f;
-        }
-        if (j > 0) {  // the output so far, complete where these scores are
-#pragma unroll 1
-          for (uint32_t d = 0; d < cache.D; d += 32) {
             uint32_t x[32];
-            ptx::tmem_load_32x32b_x32(o_at + d, x);
+            ptx::tmem_load_32x32b_x32(at + 32 * w, x);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
-            tmem_store32(o_at + d, x);
+            for (int i = 0; i < 16; ++i) {
+              top[i & 1] = max3_nan(top[i & 1], __uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+              const Pair z = fma2(pair(x[2 * i], x[2 * i + 1]), c2, base2);
+              float e0, e1;
+              if (i % 8 < kPolynomial) {
+                exp2_pair(z, e0, e1);
+              } else {
+                const float2 v = halves(z);
+                e0 = ex2_approx(v.x);
+                e1 = ex2_approx(v.y);
+              }
+              sums[i & 1] = add2(sums[i & 1], pair(__float_as_uint(e0), __float_as_uint(e1)));
+              // the numerators' rounding to the type, which the second product asks for;
+              // their sum stays in fp32
+              y[16 * w + i] = pack<T>(e0, e1);
+            }
           }
-          tmem_store_wait();
+          // (not so for NaN)
+          settled = __all_sync(0xffffffffu, max3_nan(top[0], top[0], top[1]) * c - shift<T>() <= m + kSlack);
+          if (settled) {
+            tmem_store32(at, y);
+            const float2 sum = halves(add2(sums[0], sums[1]));
+            l += sum.x + sum.y;
+          }
         }
-      }
-      const uint32_t base = __float_as_uint(m == -INFINITY ? 0.0f : -m);
-      const Pair c2 = pair(__float_as_uint(c), __float_as_uint(c)), base2 = pair(base, base);
-      Pair sums[2] = {0, 0};
+        if (!settled) {
+          // bit i: the row sees key 32 w + i
+          const auto see = [&](uint32_t w) {
+            const int64_t lo = static_cast<int64_t>(from) - key - 32 * w, hi = static_cast<int64_t>(to) - key - 32 * w;
+            uint32_t bits = hi <= 0 || lo >= 32 ? 0u : 0xffffffffu;
+            if (bits && hi < 32) bits &= (1u << hi) - 1;
+            if (bits && lo > 0) bits &= ~((1u << lo) - 1);
+            return there ? bits & good[w] : 0xffffffffu;
+          };
+          float top = -INFINITY;
+#pragma unroll 1
+          for (uint32_t w = 0; w < 2; ++w) {
+            uint32_t x[32];
+            ptx::tmem_load_32x32b_x32(at + 32 * w, x);
+            const uint32_t bits = see(w);
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        uint32_t y[32];
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, bits >> i & 1 ? __uint_as_float(x[i]) : -INFINITY);
+          }
+          top = top * c - shift<T>();
+          const bool grow = top > m + kSlack || (m == -INFINITY && top > m);
+          if (__any_sync(0xffffffffu, grow)) {
+            float f = 1.0f;
+            if (grow) {
+              f = ex2_approx(m - top);
+              m = top;
+              l *= f;
+            }
+            if (j + h > 0) {
+              // the output so far: complete where a block's scores are, and behind its
+              // first half by an arrival of its own
+              if (h) {
+                if (!wait_warp(sh, &sh.b.o_half[t], done & 1, a.status)) return;
+                ptx::tc_fence_after();
+              }
+#pragma unroll 1
+              for (uint32_t d = 0; d < cache.D; d += 32) {
+                uint32_t x[32];
+                ptx::tmem_load_32x32b_x32(o_at + d, x);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float2 z = halves(fma2(pair(x[64 * w + 2 * i], x[64 * w + 2 * i + 1]), c2, base2));
-          const float e0 = ex2_approx(z.x), e1 = ex2_approx(z.y);
-          sums[i & 1] = add2(sums[i & 1], pair(__float_as_uint(e0), __float_as_uint(e1)));
-          // the numerators' rounding to the type, which the second product asks for;
-          // their sum stays in fp32
-          y[i] = pack<T>(e0, e1);
+                for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+                tmem_store32(o_at + d, x);
+              }
+            }
+          }
+          const float base = m == -INFINITY ? 0.0f : -m;
+#pragma unroll 1
+          for (uint32_t w = 0; w < 2; ++w) {
+            uint32_t x[32], y[16];
+            ptx::tmem_load_32x32b_x32(at + 32 * w, x);
+            const uint32_t bits = see(w);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float e0 = bits >> 2 * i & 1 ? ex2_approx(fmaf(__uint_as_float(x[2 * i]), c, base)) : 0.0f;
+              const float e1 = bits >> (2 * i + 1) & 1 ? ex2_approx(fmaf(__uint_as_float(x[2 * i + 1]), c, base)) : 0.0f;
+              l += e0 + e1;
+              y[i] = pack<T>(e0, e1);
+            }
+            tmem_store16(at + 16 * w, y);
+          }
         }
-        tmem_store32(p_at + 32 * w, y);
+        tmem_store_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&sh.b.p_full[t][h]);
       }
-      const float2 sum = halves(add2(sums[0], sums[1]));
-      l += sum.x + sum.y;
-      tmem_store_wait();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sh.b.p_full[t]);
       ++done;
     }
     block_count += job->most;
@@ -582,61 +712,42 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh) {
     const uint32_t h = p.head * a.group + static_cast<uint32_t>(place % a.group);
     const bool complete = p.opens && p.ends;
     float *const part = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (p.opens ? 1 : 0)) * part_floats<kRows, DP>();
-    TO *const out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    bool nan = false;
-#pragma unroll 1
-    for (uint32_t d = 0; d < cache.D; d += 32) {
-      uint32_t x[32];
-      if (n) ptx::tmem_load_32x32b_x32(o_at + d, x);
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        if (!there || d + 8 * v >= cache.D) continue;
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          y[i] = n ? __uint_as_float(x[8 * v + i]) : 0.0f;
-          nan = nan || y[i] != y[i];
-          if (complete) y[i] = l == 0.0f ? 0.0f : y[i] * inv;
-        }
-        if (complete) {
-          heads::Raw<TO, 8> raw;
-          raw.set(y);
-          raw.store(out + d + 8 * v);
-        } else {
-          float4 *q = reinterpret_cast<float4 *>(part + in_job * DP + d + 8 * v);
-          q[0] = make_float4(y[0], y[1], y[2], y[3]);
-          q[1] = make_float4(y[4], y[5], y[6], y[7]);
-        }
-      }
+    bool nan;
+    if (complete) {
+      TO *const out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;
+      nan = put_rows<TO>(o_at, n > 0, cache.D, l == 0.0f ? 0.0f : 1.0f / l, there ? out : nullptr, staging);
+    } else {
+      nan = put_rows<float>(o_at, n > 0, cache.D, 1.0f, there ? part + in_job * DP : nullptr, staging);
     }
     if (n) {
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&sh.b.o_free[t]);
     }
-    // A value that other rows of the tile see, and this one does not, is not finite (0
-    // times it is NaN): the row's own keys one by one.
-    const uint32_t lo = max(from, p.block_lo * kKeys);
-    const uint32_t hi = static_cast<uint32_t>(min(static_cast<uint64_t>(to), static_cast<uint64_t>(p.block_hi) * kKeys));
-    const bool again = there && nan && l == l && (from > p.from || to < p.to);
-    if (there && !again) {
+    if (there) {
       if (complete) put_lse<TO>(a, token, h, m, l);
       else {
         part[kRows * DP + in_job] = m;
         part[kRows * DP + kRows + in_job] = l;
       }
     }
-    unsigned rows = __ballot_sync(0xffffffffu, again);
+    // NaN from finite sums: where a value that other rows of the tile see, and this one
+    // does not, is not finite (0 times it is NaN), the row's own keys one by one.
+    unsigned rows = __ballot_sync(0xffffffffu, there && nan && l == l);
+    const uint32_t lo = p.block_lo * kKeys, hi = (p.block_lo + n) * kKeys;
     while (rows) {
       const int r = __ffs(rows) - 1;
       rows &= rows - 1;
+      const uint32_t r_from = __shfl_sync(0xffffffffu, from, r), r_to = __shfl_sync(0xffffffffu, to, r);
+      if (!any_infinite<T>(a, p.sequence, p.head, max(lo, p.from), min(r_from, min(hi, p.to)), lane) &&
+          !any_infinite<T>(a, p.sequence, p.head, max(r_to, max(lo, p.from)), min(hi, p.to), lane))
+        continue;
       const uint32_t r_job = __shfl_sync(0xffffffffu, in_job, r);
       const uint64_t r_place = p.row0 + r_job, r_token = p.start + r_place / a.group;
       const uint32_t r_h = p.head * a.group + static_cast<uint32_t>(r_place % a.group);
       float acc[kMaxHead / 32], rm, rl;
       const T *q = static_cast<const T *>(a.q.p) + r_token * a.q.row_stride + r_h * a.q.head_stride;
-      row_over_keys<T>(a, p.sequence, p.head, q, __shfl_sync(0xffffffffu, lo, r), __shfl_sync(0xffffffffu, hi, r), lane, rm, rl, acc);
+      row_over_keys<T>(a, p.sequence, p.head, q, max(r_from, lo), min(r_to, min(hi, p.to)), lane, rm, rl, acc);
       TO *const r_out = static_cast<TO *>(const_cast<void *>(a.out.p)) + r_token * a.out.row_stride + r_h * a.out.head_stride;
       __syncwarp();
 #pragma unroll
@@ -664,7 +775,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
   extern __shared__ uint8_t raw[];
   uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t queries = ptx::smem_addr(smem), ring = queries + 2 * tile_bytes<DP>();
-  Shared &sh = *reinterpret_cast<Shared *>(smem + (2 + S) * tile_bytes<DP>());
+  uint8_t *const staging = smem + (2 + S) * tile_bytes<DP>();
+  Shared &sh = *reinterpret_cast<Shared *>(staging + kStaging);
   const uint32_t warp = threadIdx.x / 32;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -675,7 +787,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
     ptx::mbar_init(&sh.b.q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(&sh.b.s_full[t], 1);
-      ptx::mbar_init(&sh.b.p_full[t], 4);
+      ptx::mbar_init(&sh.b.p_full[t][0], 4);
+      ptx::mbar_init(&sh.b.p_full[t][1], 4);
+      ptx::mbar_init(&sh.b.o_half[t], 1);
       ptx::mbar_init(&sh.b.o_full[t], 1);
       ptx::mbar_init(&sh.b.o_free[t], 4);
     }
@@ -696,25 +810,19 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
   ptx::tc_fence_before();
   const Share share = share_of<kRows, kKeys, kThreads>(a, blockIdx.x, gridDim.x, a.whole ? 1 : 2 * kKeys);
   ptx::tc_fence_after();
-  // A row's 128 scores stay in registers: of the 512 x 128 that the CTA was launched
-  // with, 256 x 200 go to the softmax and 256 x 56 to the others.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    soften<T, TO, DP>(a, sh);
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp < 12) {
-      load<T, DP>(a, maps, sh, queries, ring);
-      await<0>();
-    } else if (warp == 12) {
-      multiply<T, DP>(a, sh, queries, ring);
-      __syncwarp();
-      // everything issued is done before TMEM and the barriers go
-      if (elect()) ptx::mma_commit(&sh.b.drained);
-      if (!ptx::mbar_wait_bounded(&sh.b.drained, 0, kWaitLimitNs)) raise_flag(a.status, TL_FLAG_TIMEOUT);
-    } else if (threadIdx.x == 13 * 32) {
-      plan_jobs(a, share, sh);
-    }
+    soften<T, TO, DP>(a, sh, staging);
+  } else if (warp < 12) {
+    load<T, DP>(a, maps, sh, queries, ring);
+    await<0>();
+  } else if (warp == 12) {
+    multiply<T, DP>(a, sh, queries, ring);
+    __syncwarp();
+    // everything issued is done before TMEM and the barriers go
+    if (elect()) ptx::mma_commit(&sh.b.drained);
+    if (!ptx::mbar_wait_bounded(&sh.b.drained, 0, kWaitLimitNs)) raise_flag(a.status, TL_FLAG_TIMEOUT);
+  } else if (threadIdx.x == 13 * 32) {
+    plan_jobs(a, share, sh);
   }
   __syncwarp();
   ptx::tc_fence_before();
@@ -761,7 +869,7 @@ template <typename T, typename TO, int DP> void launch(const AttentionArgs &a, c
   constexpr size_t smem = smem_bytes<DP>();
   (void)cudaFuncSetAttribute(tile_kernel<T, TO, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   launch_pdl(tile_kernel<T, TO, DP>, p.ctas, kThreads, smem, s, a, make_maps(a));
-  if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, 8), 128, 0, s, a);
+  if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, kRows / 8), 128, 0, s, a);
 }
 
 }  // namespace
