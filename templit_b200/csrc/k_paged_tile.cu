@@ -53,7 +53,7 @@ constexpr uint32_t kStaging = 8 * 4096;  // 32 rows of 128 bytes for each softma
 struct Barriers {
   uint64_t full[8], empty[kPairs];
   uint64_t job_full[kJobs], job_free[kJobs];
-  uint64_t q_full, q_empty, s_full[2], p_full[2][2], o_half[2], o_full[2], o_free[2], drained;
+  uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], o_tail[2], o_full[2], o_free[2], drained;
 };
 // A piece and the blocks that its two tiles take, from the piece's first on;
 // more == false: there are no more.
@@ -78,9 +78,9 @@ __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Waits for a phase; false where it gave up, here or elsewhere in the CTA.
-__device__ __forceinline__ bool wait(Shared &sh, uint64_t *bar, uint32_t parity, uint32_t *status) {
-  if (ptx::mbar_try_wait(bar, parity)) return true;
+// Waits for a phase; false where it gave up, here or elsewhere in the CTA.  The
+// first look is inline, a few instructions; the rest is not.
+__device__ __noinline__ bool wait_longer(Shared &sh, uint64_t *bar, uint32_t parity, uint32_t *status) {
   const uint64_t t0 = ptx::global_timer_ns();
   for (uint32_t i = 1;; ++i) {
     if (ptx::mbar_try_wait(bar, parity)) return true;
@@ -93,6 +93,9 @@ __device__ __forceinline__ bool wait(Shared &sh, uint64_t *bar, uint32_t parity,
       }
     }
   }
+}
+__device__ __forceinline__ bool wait(Shared &sh, uint64_t *bar, uint32_t parity, uint32_t *status) {
+  return ptx::mbar_try_wait(bar, parity) || wait_longer(sh, bar, parity, status);
 }
 
 // The same for a whole warp, with one answer.
@@ -414,92 +417,78 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Maps &maps, S
   if (item && !wait_warp(sh, &sh.b.empty[item / 2 % kPairs], (item / 2 / kPairs) & 1, a.status)) return;
 }
 
-// By one warp, so that operands are in uniform registers; one thread issues.
-// A product's instructions are unrolled with descriptors that differ by
-// constants: worked out one by one they took 100 cycles each, as long as the
-// product itself.
+// By one thread.  A product's instructions are unrolled with descriptors that
+// differ by constants (worked out one by one they took 100 cycles each, as long
+// as the product itself), the four steps of a block are one copy of the code,
+// and a wait that is over costs a few instructions: what this thread does
+// between products the tensor cores wait for.
 template <typename T, int DP>
 __device__ __forceinline__ void multiply(const AttentionArgs &a, Shared &sh, uint32_t queries, uint32_t ring) {
-  constexpr int S = stages<DP>();
+  constexpr uint32_t S = stages<DP>();
   constexpr uint32_t kBytes = tile_bytes<DP>();
   constexpr uint32_t type = std::is_same<T, __half>::value ? 0 : 1;
-  const bool leader = elect();
   const uint32_t ksteps = (a.cache.D + 15) / 16;
-  const uint32_t score = idesc_f16(type, kTile, kKeys, false), output = idesc_f16(type, kTile, ksteps * 16, true);
-  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+  const uint32_t score = idesc_f16(type, kTile, kKeys / 2, false), output = idesc_f16(type, kTile, ksteps * 16, true);
+  const uint32_t tmem = sh.tmem;
   const uint64_t q_desc = row_desc(queries), k_desc = row_desc(ring), v_desc = value_desc(ring);
   uint32_t item = 0, piece = 0, s_count[2] = {0, 0}, opened[2] = {0, 0};
-  const auto scores = [&](uint32_t t, uint32_t slot) {
-    ptx::tc_fence_after();
-    const uint64_t q = q_desc + t * (kBytes / 16), k = k_desc + slot * (kBytes / 16);
-    if (leader) {
+  // scores of the 64 keys of half h
+  const auto scores = [&](uint32_t t, uint32_t slot, uint32_t h) {
+    const uint64_t q = q_desc + t * (kBytes / 16), k = k_desc + slot * (kBytes / 16) + h * (64 * 128 / 16);
 #pragma unroll
-      for (uint32_t i = 0; i < DP / 16; ++i)
-        if (i < ksteps) mma_smem(tmem + t * 128, q + row_step(i), k + row_step(i), score, i > 0);
-      ptx::mma_commit(&sh.b.s_full[t]);
-    }
-  };
-  const auto give_back = [&](uint32_t pair) {
-    if (leader) ptx::mma_commit(&sh.b.empty[pair % kPairs]);
+    for (uint32_t i = 0; i < DP / 16; ++i)
+      if (i < ksteps) mma_smem(tmem + t * 128 + h * 64, q + row_step(i), k + row_step(i), score, i > 0);
+    ptx::mma_commit(&sh.b.s_full[t][h]);
   };
   for (uint32_t i_job = 0;; ++i_job) {
     bool ok;
     const Job *const job = next_job(sh, i_job, a.status, &ok);
-    if (!__all_sync(0xffffffffu, ok)) return;
-    const bool more = job->more;
-    const uint32_t n[2] = {__shfl_sync(0xffffffffu, job->n[0], 0), __shfl_sync(0xffffffffu, job->n[1], 0)}, most = max(n[0], n[1]);
-    __syncwarp();
-    if (!more) break;
-    if (leader) release_job(sh, i_job);
+    if (!ok) return;
+    if (!job->more) break;
+    const uint32_t n0 = job->n[0], n1 = job->n[1], most = job->most;
+    release_job(sh, i_job);
     if (!most) continue;
-    if (!wait_warp(sh, &sh.b.q_full, piece & 1, a.status)) return;
+    if (!wait(sh, &sh.b.q_full, piece & 1, a.status)) return;
     ++piece;
     const uint32_t first = item;  // block j: keys in place first + 2 j, values behind them
-    if (!wait_warp(sh, &sh.b.full[first % S], (first / S) & 1, a.status)) return;
-#pragma unroll
-    for (uint32_t t = 0; t < 2; ++t)
-      if (n[t]) scores(t, first % S);
-    give_back(first / 2);
+    if (!wait(sh, &sh.b.full[first % S], (first / S) & 1, a.status)) return;
+    ptx::tc_fence_after();
+#pragma unroll 1
+    for (uint32_t e = 0; e < 4; ++e)
+      if (e & 1 ? n1 : n0) scores(e & 1, first % S, e >> 1);
+    ptx::mma_commit(&sh.b.empty[first / 2 % kPairs]);
+#pragma unroll 1
     for (uint32_t j = 0; j < most; ++j) {
-      const uint32_t v = first + 2 * j + 1, k = v + 1, v_slot = v % S, k_slot = k % S;
-      bool have_v = false, have_k = false;
-#pragma unroll
-      for (uint32_t t = 0; t < 2; ++t) {
-        if (j < n[t]) {
-          if (!have_v && !wait_warp(sh, &sh.b.full[v_slot], (v / S) & 1, a.status)) return;
-          have_v = true;
-          if (j == 0) {  // the tile's last output has been read
-            if (!wait_warp(sh, &sh.b.o_free[t], (opened[t] & 1) ^ 1, a.status)) return;
-            ++opened[t];
-          }
-          const uint64_t values = v_desc + v_slot * (kBytes / 16);
-#pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) {
-            if (!wait_warp(sh, &sh.b.p_full[t][h], s_count[t] & 1, a.status)) return;
-            ptx::tc_fence_after();
-            if (leader) {
-#pragma unroll
-              for (uint32_t i = 0; i < kKeys / 32; ++i)
-                mma_tmem(tmem + 256 + t * 128, tmem + t * 128 + h * 64 + i * 8, values + (h * 4 + i) * 128, output, (j | h | i) > 0);
-              if (h == 0) ptx::mma_commit(&sh.b.o_half[t]);
-              else if (j + 1 == n[t]) ptx::mma_commit(&sh.b.o_full[t]);
-            }
-          }
-          ++s_count[t];
+      const uint32_t v = first + 2 * j + 1, k = v + 1;
+      if (!wait(sh, &sh.b.full[v % S], (v / S) & 1, a.status)) return;
+      if (j + 1 < most && !wait(sh, &sh.b.full[k % S], (k / S) & 1, a.status)) return;
+      const uint64_t values = v_desc + v % S * (kBytes / 16);
+#pragma unroll 1
+      for (uint32_t e = 0; e < 4; ++e) {
+        const uint32_t t = e & 1, h = e >> 1, n = t ? n1 : n0;
+        if (j >= n) continue;
+        if (j + h == 0) {  // the tile's last output has been read
+          if (!wait(sh, &sh.b.o_free[t], (opened[t] & 1) ^ 1, a.status)) return;
+          ++opened[t];
         }
-        if (j + 1 < n[t]) {
-          if (!have_k && !wait_warp(sh, &sh.b.full[k_slot], (k / S) & 1, a.status)) return;
-          have_k = true;
-          scores(t, k_slot);
-        }
+        if (!wait(sh, &sh.b.p_full[t][h], s_count[t] & 1, a.status)) return;
+        s_count[t] += h;
+        ptx::tc_fence_after();
+        const uint32_t o_at = tmem + 256 + t * 128, p_at = tmem + t * 128 + h * 64;
+        const uint64_t rows = values + h * 512;
+#pragma unroll
+        for (uint32_t i = 0; i < kKeys / 32; ++i) mma_tmem(o_at, p_at + i * 8, rows + i * 128, output, (j | h | i) > 0);
+        if (j + 1 == n) ptx::mma_commit(h ? &sh.b.o_full[t] : &sh.b.o_tail[t]);
+        // the buffer is free again behind that product: the tensor cores keep the order
+        else scores(t, k % S, h);
       }
       // the last block's values go back with the next piece's first keys
-      if (j + 1 < most) give_back(k / 2);
+      if (j + 1 < most) ptx::mma_commit(&sh.b.empty[k / 2 % kPairs]);
     }
-    if (leader) ptx::mma_commit(&sh.b.q_empty);
+    ptx::mma_commit(&sh.b.q_empty);
     item += 2 * most;
   }
-  if (item) give_back(item / 2);
+  if (item) ptx::mma_commit(&sh.b.empty[item / 2 % kPairs]);
 }
 
 // Whether a value of the keys [from, to) is not finite, by a warp.
@@ -587,12 +576,12 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
     if (there) seen(a, p.length, p.position(a, in_job), from, to);
     float m = -INFINITY, l = 0.0f;
     for (uint32_t j = 0; j < n; ++j) {
-      if (!wait_warp(sh, &sh.b.s_full[t], done & 1, a.status)) return;
-      ptx::tc_fence_after();
-      // By halves of 64 keys, so that the second product starts on the first; one copy
-      // of the code, which the warps' instruction caches hold.
+      // By halves of 64 keys, each with its scores' buffer; one copy of the code, which
+      // the warps' instruction caches hold.
 #pragma unroll 1
       for (uint32_t h = 0; h < 2; ++h) {
+        if (!wait_warp(sh, &sh.b.s_full[t][h], done & 1, a.status)) return;
+        ptx::tc_fence_after();
         const uint32_t key = (p.block_lo + j) * kKeys + h * 64, at = s_at + h * 64;
         const uint32_t *good = &sh.mask[(block_count + j) % kMasks][2 * h];
         const bool whole = key >= from && to >= 64 && key <= to - 64 && (good[0] & good[1]) == 0xffffffffu;
@@ -663,12 +652,16 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
               l *= f;
             }
             if (j + h > 0) {
-              // the output so far: complete where a block's scores are, and behind its
-              // first half by an arrival of its own
-              if (h) {
-                if (!wait_warp(sh, &sh.b.o_half[t], done & 1, a.status)) return;
-                ptx::tc_fence_after();
+              // The output so far: complete where the next half's scores are, which were
+              // multiplied behind it, or by an arrival of its own before the last half.
+              if (h == 0) {
+                if (!wait_warp(sh, &sh.b.s_full[t][1], done & 1, a.status)) return;
+              } else if (j + 1 < n) {
+                if (!wait_warp(sh, &sh.b.s_full[t][0], (done + 1) & 1, a.status)) return;
+              } else if (!wait_warp(sh, &sh.b.o_tail[t], outputs & 1, a.status)) {
+                return;
               }
+              ptx::tc_fence_after();
 #pragma unroll 1
               for (uint32_t d = 0; d < cache.D; d += 32) {
                 uint32_t x[32];
@@ -786,10 +779,11 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
     ptx::mbar_init(&sh.b.q_full, kLoaders / 32);
     ptx::mbar_init(&sh.b.q_empty, 1);
     for (int t = 0; t < 2; ++t) {
-      ptx::mbar_init(&sh.b.s_full[t], 1);
-      ptx::mbar_init(&sh.b.p_full[t][0], 4);
-      ptx::mbar_init(&sh.b.p_full[t][1], 4);
-      ptx::mbar_init(&sh.b.o_half[t], 1);
+      for (int h = 0; h < 2; ++h) {
+        ptx::mbar_init(&sh.b.s_full[t][h], 1);
+        ptx::mbar_init(&sh.b.p_full[t][h], 4);
+      }
+      ptx::mbar_init(&sh.b.o_tail[t], 1);
       ptx::mbar_init(&sh.b.o_full[t], 1);
       ptx::mbar_init(&sh.b.o_free[t], 4);
     }
@@ -816,11 +810,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
     load<T, DP>(a, maps, sh, queries, ring);
     await<0>();
   } else if (warp == 12) {
-    multiply<T, DP>(a, sh, queries, ring);
-    __syncwarp();
-    // everything issued is done before TMEM and the barriers go
-    if (elect()) ptx::mma_commit(&sh.b.drained);
-    if (!ptx::mbar_wait_bounded(&sh.b.drained, 0, kWaitLimitNs)) raise_flag(a.status, TL_FLAG_TIMEOUT);
+    if (elect()) {
+      multiply<T, DP>(a, sh, queries, ring);
+      // everything issued is done before TMEM and the barriers go
+      ptx::mma_commit(&sh.b.drained);
+      if (!ptx::mbar_wait_bounded(&sh.b.drained, 0, kWaitLimitNs)) raise_flag(a.status, TL_FLAG_TIMEOUT);
+    }
   } else if (threadIdx.x == 13 * 32) {
     plan_jobs(a, share, sh);
   }
