@@ -88,8 +88,8 @@ template <typename T, int DP> struct Lane {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t row = lane / 4 + 8 * i;
-      const uint64_t place = w.row0 + row;
-      const T *p = static_cast<const T *>(a.q.p) + (w.start + place / a.group) * a.q.row_stride +
+      const uint32_t place = w.row0 + row;
+      const T *p = static_cast<const T *>(a.q.p) + (w.start + static_cast<uint64_t>(place / a.group)) * a.q.row_stride +
                    (w.head * a.group + place % a.group) * a.q.head_stride;
 #pragma unroll
       for (int k = 0; k < KS; ++k)
@@ -215,10 +215,10 @@ template <int DP> struct Lane<float, DP> {
     const float sign = a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : 0.0f;
     for (uint32_t i = threadIdx.x; i < kRows * DP; i += kThreads) {
       const uint32_t row = i / DP, d = i % DP;
-      const uint64_t place = w.row0 + row;
+      const uint32_t place = w.row0 + row;
       float x = 0.0f;
       if (row <= w.last && d < a.cache.D)
-        x = sign * (static_cast<const float *>(a.q.p) + (w.start + place / a.group) * a.q.row_stride +
+        x = sign * (static_cast<const float *>(a.q.p) + (w.start + static_cast<uint64_t>(place / a.group)) * a.q.row_stride +
                     (w.head * a.group + place % a.group) * a.q.head_stride)[d];
       shared[i] = x;
     }
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
   while (walk.next(a, share, w)) {
     // rows
     const uint32_t head = w.head, last = w.last;
-    const uint64_t row0 = w.row0;
+    const uint32_t row0 = w.row0;
     uint32_t all_from = w.from, all_to = w.to, most_from, least_to, f, t;
     seen(a, w.length, w.position(a, 0), f, least_to);
     seen(a, w.length, w.position(a, last), most_from, t);
@@ -430,9 +430,8 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) acc[e] = fmaf(f, outs[(i * kRows + row) * DP + lane + 32 * e], acc[e]);
       }
-      const uint64_t place = row0 + row;
-      const uint64_t token = w.start + place / a.group;
-      const uint32_t h = head * a.group + static_cast<uint32_t>(place % a.group);
+      const uint32_t place = row0 + row, h = head * a.group + place % a.group;
+      const uint64_t token = w.start + static_cast<uint64_t>(place / a.group);
       bool nan = false;
 #pragma unroll
       for (int e = 0; e < DP / 32; ++e) nan = nan || (lane + 32 * e < c.D && acc[e] != acc[e]);

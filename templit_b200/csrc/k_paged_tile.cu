@@ -37,8 +37,6 @@ constexpr uint32_t kTile = 128, kRows = 2 * kTile, kKeys = 128;
 constexpr int kThreads = 16 * 32, kLoaders = 128;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr float kSlack = 8.0f;  // log2 of how far numerators may pass 1
-// Pairs of exponentials in 8 that the FMA pipe takes: 0 ... measured below.
-constexpr int kPolynomial = 0;
 constexpr int kLag = 2;         // ring places between a copy's issue and its hand-over
 // Values of block j and keys of block j + 1 (places 2 j + 1 and 2 j + 2 of the ring's
 // sequence) are given back together: one arrival in place of two, 200 cycles each.
@@ -191,26 +189,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-// 2^x of two finite numbers on the FMA pipe, which the softmax leaves idle while
-// it waits for 16 exponentials a cycle of the other: x = n + f, |f| <= 1/2, 2^f by
-// a polynomial fitted to it (1.7e-7 relative in fp32, 1 at 0), n into the
-// exponent.  x is 15 at most; below -126 it is taken as -126, which no sum of
-// 2^-21 and more notices.
-__device__ __forceinline__ void exp2_pair(Pair x, float &lo, float &hi) {
-  const float2 v = halves(x);
-  const Pair z = pair(__float_as_uint(fmaxf(v.x, -126.0f)), __float_as_uint(fmaxf(v.y, -126.0f)));
-  const auto both = [](float c) { return pair(__float_as_uint(c), __float_as_uint(c)); };
-  const Pair t = add2(z, both(12582912.0f));  // 1.5 * 2^23: whole numbers in the low bits
-  const Pair f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), z);
-  Pair p = fma2(both(0.001326472731307149f), f, both(0.009671512991189957f));
-  p = fma2(p, f, both(0.05550733581185341f));
-  p = fma2(p, f, both(0.24022242426872253f));
-  p = fma2(p, f, both(0.6931470036506653f));
-  p = fma2(p, f, both(1.0f));
-  const float2 q = halves(p), n = halves(t);
-  lo = __uint_as_float(__float_as_uint(q.x) + (__float_as_uint(n.x) << 23));
-  hi = __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(n.y) << 23));
 }
 // 16 and 32 columns of this warp's 32 lanes into TMEM
 __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -369,7 +347,7 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Maps &maps, S
             if (warp == 0 && lane == 0) {
               const bool both = p.last >= kTile;
               ptx::mbar_arrive_expect_tx(&sh.b.q_full, (both ? 2 : 1) * kBytes);
-              const uint32_t token = p.start + static_cast<uint32_t>(p.row0 / a.group);
+              const uint32_t token = p.start + p.row0 / a.group;
               for (uint32_t t = 0; t < (both ? 2u : 1u); ++t)
                 for (uint32_t b = 0; b < kBlocks; ++b)
                   tma_box3(queries + t * kBytes + b * (kTile * 128), &maps.q, &sh.b.q_full, b * 64, head * a.group,
@@ -380,10 +358,10 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Maps &maps, S
           } else {
             for (uint32_t t = 0; t < 2; ++t) {
               const uint32_t mine = t * kTile + warp * 32 + lane;
-              const uint64_t place = p.row0 + mine;
+              const uint32_t place = p.row0 + mine;
               int64_t at = -1;
               if (mine <= p.last)
-                at = static_cast<int64_t>((p.start + place / a.group) * a.q.row_stride +
+                at = static_cast<int64_t>((p.start + static_cast<uint64_t>(place / a.group)) * a.q.row_stride +
                                           (head * a.group + place % a.group) * a.q.head_stride);
 #pragma unroll 4
               for (uint32_t i = 0; i < CH; ++i) {
@@ -431,7 +409,7 @@ __device__ __forceinline__ void multiply(const AttentionArgs &a, Shared &sh, uin
   const uint32_t score = idesc_f16(type, kTile, kKeys / 2, false), output = idesc_f16(type, kTile, ksteps * 16, true);
   const uint32_t tmem = sh.tmem;
   const uint64_t q_desc = row_desc(queries), k_desc = row_desc(ring), v_desc = value_desc(ring);
-  uint32_t item = 0, piece = 0, s_count[2] = {0, 0}, opened[2] = {0, 0};
+  uint32_t item = 0, piece = 0, p_phase = 0, o_phase = 3;  // a bit for each tile
   // scores of the 64 keys of half h
   const auto scores = [&](uint32_t t, uint32_t slot, uint32_t h) {
     const uint64_t q = q_desc + t * (kBytes / 16), k = k_desc + slot * (kBytes / 16) + h * (64 * 128 / 16);
@@ -468,11 +446,11 @@ __device__ __forceinline__ void multiply(const AttentionArgs &a, Shared &sh, uin
         const uint32_t t = e & 1, h = e >> 1, n = t ? n1 : n0;
         if (j >= n) continue;
         if (j + h == 0) {  // the tile's last output has been read
-          if (!wait(sh, &sh.b.o_free[t], (opened[t] & 1) ^ 1, a.status)) return;
-          ++opened[t];
+          if (!wait(sh, &sh.b.o_free[t], o_phase >> t & 1, a.status)) return;
+          o_phase ^= 1u << t;
         }
-        if (!wait(sh, &sh.b.p_full[t][h], s_count[t] & 1, a.status)) return;
-        s_count[t] += h;
+        if (!wait(sh, &sh.b.p_full[t][h], p_phase >> t & 1, a.status)) return;
+        p_phase ^= h << t;
         ptx::tc_fence_after();
         const uint32_t o_at = tmem + 256 + t * 128, p_at = tmem + t * 128 + h * 64;
         const uint64_t rows = values + h * 512;
@@ -602,14 +580,8 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
             for (int i = 0; i < 16; ++i) {
               top[i & 1] = max3_nan(top[i & 1], __uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
               const Pair z = fma2(pair(x[2 * i], x[2 * i + 1]), c2, base2);
-              float e0, e1;
-              if (i % 8 < kPolynomial) {
-                exp2_pair(z, e0, e1);
-              } else {
-                const float2 v = halves(z);
-                e0 = ex2_approx(v.x);
-                e1 = ex2_approx(v.y);
-              }
+              const float2 v = halves(z);
+              const float e0 = ex2_approx(v.x), e1 = ex2_approx(v.y);
               sums[i & 1] = add2(sums[i & 1], pair(__float_as_uint(e0), __float_as_uint(e1)));
               // the numerators' rounding to the type, which the second product asks for;
               // their sum stays in fp32
@@ -701,8 +673,9 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
       ++outputs;
       ptx::tc_fence_after();
     }
-    const uint64_t place = p.row0 + in_job, token = p.start + place / a.group;
-    const uint32_t h = p.head * a.group + static_cast<uint32_t>(place % a.group);
+    const uint32_t place = p.row0 + in_job, in_sequence = place / a.group;
+    const uint64_t token = p.start + in_sequence;
+    const uint32_t h = p.head * a.group + (place - in_sequence * a.group);
     const bool complete = p.opens && p.ends;
     float *const part = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (p.opens ? 1 : 0)) * part_floats<kRows, DP>();
     bool nan;
@@ -736,8 +709,8 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
           !any_infinite<T>(a, p.sequence, p.head, max(r_to, max(lo, p.from)), min(hi, p.to), lane))
         continue;
       const uint32_t r_job = __shfl_sync(0xffffffffu, in_job, r);
-      const uint64_t r_place = p.row0 + r_job, r_token = p.start + r_place / a.group;
-      const uint32_t r_h = p.head * a.group + static_cast<uint32_t>(r_place % a.group);
+      const uint32_t r_place = p.row0 + r_job, r_h = p.head * a.group + r_place % a.group;
+      const uint64_t r_token = p.start + r_place / a.group;
       float acc[kMaxHead / 32], rm, rl;
       const T *q = static_cast<const T *>(a.q.p) + r_token * a.q.row_stride + r_h * a.q.head_stride;
       row_over_keys<T>(a, p.sequence, p.head, q, max(r_from, lo), min(r_to, min(hi, p.to)), lane, rm, rl, acc);

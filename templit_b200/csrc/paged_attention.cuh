@@ -204,7 +204,7 @@ struct Piece {
   uint32_t block_lo, block_hi; // blocks of the keys [block * KEYS, ..)
   bool opens, ends;            // the job's first block, its last one
   uint32_t first_cta;          // that has its first block
-  uint64_t row0;               // of the tile, among the sequence's rows
+  uint32_t row0;               // of the tile, among the sequence's rows (fewer than 2^32)
   uint32_t last;               // its last row
   uint32_t length;             // the sequence's keys
   int64_t position0;           // of the sequence's first new token
@@ -247,8 +247,8 @@ template <uint32_t ROWS, uint32_t KEYS> struct Walk {
       p.head = static_cast<uint32_t>(in_tile / job);
       p.tile = static_cast<uint32_t>(lo);
       p.start = w.q.start;
-      p.row0 = lo * ROWS;
-      p.last = static_cast<uint32_t>(min(p.row0 + ROWS, static_cast<uint64_t>(w.q.count) * a.group) - 1 - p.row0);
+      p.row0 = static_cast<uint32_t>(lo) * ROWS;
+      p.last = min(ROWS, w.q.count * a.group - p.row0) - 1;
       p.length = w.q.length;
       p.position0 = static_cast<int64_t>(w.q.length) - w.q.count;
       uint32_t unused;
