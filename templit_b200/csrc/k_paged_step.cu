@@ -470,7 +470,7 @@ template <typename T, typename TO, int DP> void launch(const AttentionArgs &a, c
   constexpr size_t smem = smem_bytes<T, DP>();
   (void)cudaFuncSetAttribute(step_kernel<T, TO, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   launch_pdl(step_kernel<T, TO, DP>, p.ctas, kThreads, smem, s, a);
-  if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, kRows / 4), 128, 0, s, a);
+  if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, kRows), 128, 0, s, a);
 }
 
 }  // namespace

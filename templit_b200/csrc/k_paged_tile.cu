@@ -837,7 +837,7 @@ template <typename T, typename TO, int DP> void launch(const AttentionArgs &a, c
   constexpr size_t smem = smem_bytes<DP>();
   (void)cudaFuncSetAttribute(tile_kernel<T, TO, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   launch_pdl(tile_kernel<T, TO, DP>, p.ctas, kThreads, smem, s, a, make_maps(a));
-  if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, kRows / 8), 128, 0, s, a);
+  if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, kRows / 16), 128, 0, s, a);
 }
 
 }  // namespace

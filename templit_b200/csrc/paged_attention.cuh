@@ -287,44 +287,88 @@ __device__ __forceinline__ void put_lse(const AttentionArgs &a, uint64_t token, 
 // floats of a partial result of a tile: outputs, maxima, sums
 template <uint32_t ROWS, int DP> constexpr uint32_t part_floats() { return ROWS * DP + 2 * ROWS; }
 
-// The jobs that were cut, each where it ends: a warp per row adds the partial
-// results up in the order of the keys.
+// The jobs that were cut, each where it ends: the partial results of a row are
+// added up in the order of the keys, a lane DP / 32 neighbouring elements.  Large
+// tiles are cut in two or three: a warp takes four rows, all their loads under
+// way at once (one row after another took 22 us for 147 joins of 256 rows).
+// Small ones may be cut in many: four warps share a row's parts (37 parts of 8 jobs
+// of 4 rows: 40 us by one warp).
 template <typename TO, uint32_t ROWS, int DP>
 __global__ void __launch_bounds__(128) join_kernel(const AttentionArgs a) {
+  constexpr bool kShare = ROWS <= 16;
+  constexpr int R = kShare ? 1 : 4, E = DP / 32;
+  __shared__ float sums[kShare ? 4 : 1][DP + 1];
   pdl_enter();
   const Join j = a.joins[blockIdx.x];
   if (j.first == 0xffffffffu) return;
   const uint32_t lane = threadIdx.x & 31, end = blockIdx.x;
   const Sequence q = sequence_of(a.cache, j.sequence, a.most);
-  const uint64_t rows = static_cast<uint64_t>(q.count) * a.group, row0 = static_cast<uint64_t>(j.tile) * ROWS;
+  const uint32_t row0 = j.tile * ROWS, rows = min(ROWS, q.count * a.group - row0);
+  const uint32_t warp = threadIdx.x / 32, r0 = kShare ? blockIdx.y : (blockIdx.y * 4 + warp) * R;
+  if (r0 >= rows) return;
   const auto part = [&](uint32_t cta) {
     return a.parts + (static_cast<size_t>(cta) * 2 + (cta == j.first ? 1 : 0)) * part_floats<ROWS, DP>();
   };
-  for (uint32_t row = blockIdx.y * 4 + threadIdx.x / 32; row < ROWS && row0 + row < rows; row += gridDim.y * 4) {
-    float mm = -INFINITY;
-    for (uint32_t i = j.first + lane; i <= end; i += 32) mm = fmaxf(mm, part(i)[ROWS * DP + row]);
-    mm = warp_max(mm);
-    float ll = 0.0f, acc[DP / 32];
+  float mm[R], ll[R], acc[R][E];
 #pragma unroll
-    for (int e = 0; e < DP / 32; ++e) acc[e] = 0.0f;
+  for (int r = 0; r < R; ++r) {
+    mm[r] = -INFINITY;
+    ll[r] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[r][e] = 0.0f;
+  }
+  for (uint32_t i = j.first + lane; i <= end; i += 32)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (r0 + r < rows) mm[r] = fmaxf(mm[r], part(i)[ROWS * DP + r0 + r]);
+#pragma unroll
+  for (int r = 0; r < R; ++r) mm[r] = warp_max(mm[r]);
 #pragma unroll 4
-    for (uint32_t i = j.first; i <= end; ++i) {
-      const float *p = part(i);
-      const float wm = p[ROWS * DP + row], f = wm == -INFINITY ? 0.0f : ex2_approx(wm - mm);
-      ll = fmaf(f, p[ROWS * DP + ROWS + row], ll);
+  for (uint32_t i = j.first + (kShare ? warp : 0); i <= end; i += kShare ? 4 : 1) {
+    const float *const p = part(i);
 #pragma unroll
-      for (int e = 0; e < DP / 32; ++e) {
-        const float x = p[row * DP + lane + 32 * e];
-        if (f != 0.0f) acc[e] = fmaf(f, x, acc[e]);
+    for (int r = 0; r < R; ++r) {
+      if (r0 + r >= rows) continue;
+      const uint32_t row = r0 + r;
+      const float wm = p[ROWS * DP + row], f = wm == -INFINITY ? 0.0f : ex2_approx(wm - mm[r]);
+      ll[r] = fmaf(f, p[ROWS * DP + ROWS + row], ll[r]);
+      float x[E];
+      if constexpr (E == 4) {
+        const float4 y = *reinterpret_cast<const float4 *>(p + row * DP + lane * E);
+        x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2 *>(p + row * DP + lane * E);
+        x[0] = y.x, x[1] = y.y;
       }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (f != 0.0f) acc[r][e] = fmaf(f, x[e], acc[r][e]);
     }
-    const uint64_t token = q.start + (row0 + row) / a.group;
-    const uint32_t h = j.head * a.group + static_cast<uint32_t>((row0 + row) % a.group);
+  }
+  if constexpr (kShare) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[0][e];
+    if (lane == 0) sums[warp][DP] = ll[0];
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      ll[0] += sums[w][DP];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[0][e] += sums[w][lane * E + e];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (r0 + r >= rows) continue;
+    const uint32_t place = row0 + r0 + r, in_sequence = place / a.group;
+    const uint64_t token = q.start + static_cast<uint64_t>(in_sequence);
+    const uint32_t h = j.head * a.group + (place - in_sequence * a.group);
     TO *out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;
 #pragma unroll
-    for (int e = 0; e < DP / 32; ++e)
-      if (lane + 32 * e < a.cache.D) heads::set_element(out[lane + 32 * e], ll == 0.0f ? 0.0f : acc[e] / ll);
-    if (lane == 0) put_lse<TO>(a, token, h, mm, ll);
+    for (int e = 0; e < E; ++e)
+      if (lane * E + e < a.cache.D) heads::set_element(out[lane * E + e], ll[r] == 0.0f ? 0.0f : acc[r][e] / ll[r]);
+    if (lane == 0) put_lse<TO>(a, token, h, mm[r], ll[r]);
   }
 }
 
