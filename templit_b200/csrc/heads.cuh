@@ -20,19 +20,32 @@ namespace tl {
 namespace heads {
 
 inline size_t type_size(int32_t type) { return type == TL_FLOAT32 ? 4 : 2; }
+// Elements of a vector: 16 bytes of each, and of the smaller where the types
+// differ 8 (12288 x 12 heads of 64 fp32 with 8 elements a vector 37 us, with 4 25).
+constexpr int vector_of(size_t in, size_t out) { return in == 2 && out == 2 ? 8 : 4; }
+inline int vector_for(int32_t in, int32_t out) { return vector_of(type_size(in), type_size(out)); }
 inline bool known_type(int32_t type) { return type >= TL_FLOAT32 && type <= TL_BFLOAT16; }
 
-// V elements of T as they lie in memory (V = 1: one element).
+// V elements of T as they lie in memory, in words of 8 or 16 bytes (V = 1: one
+// element).
 template <typename T, int V> struct Raw {
-  static constexpr int kVecs = V * sizeof(T) / 16;
-  uint4 r[kVecs];
+  using Word = typename std::conditional<V * sizeof(T) % 16 == 0, uint4, uint2>::type;
+  static constexpr int kWords = V * sizeof(T) / sizeof(Word);
+  Word r[kWords];
   __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) r[i] = reinterpret_cast<const uint4 *>(p)[i];
+    for (int i = 0; i < kWords; ++i) r[i] = reinterpret_cast<const Word *>(p)[i];
   }
   __device__ __forceinline__ void store(T *p) const {
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4 *>(p)[i] = r[i];
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<Word *>(p)[i] = r[i];
+  }
+  __device__ __forceinline__ float squares() const {
+    float x[V], sum = 0.0f;
+    get(x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum = fmaf(x[i], x[i], sum);
+    return sum;
   }
   __device__ __forceinline__ void get(float (&x)[V]) const {
     const uint32_t *w = reinterpret_cast<const uint32_t *>(r);
@@ -78,6 +91,7 @@ template <typename T> struct Raw<T, 1> {
   __device__ __forceinline__ void load(const T *p) { r = *p; }
   __device__ __forceinline__ void store(T *p) const { *p = r; }
   __device__ __forceinline__ void get(float (&x)[1]) const { x[0] = element_of(r); }
+  __device__ __forceinline__ float squares() const { return element_of(r) * element_of(r); }
   __device__ __forceinline__ void set(const float (&x)[1]) { set_element(r, x[0]); }
 };
 
@@ -144,25 +158,37 @@ template <int V> __device__ __forceinline__ void turn(float (&a)[V], float (&b)[
 }
 
 // Angles of a lane's slots at one position, `magnitude` included; cosine 1
-// and sine 0 behind the turned elements.
+// and sine 0 behind the turned elements.  The lanes at one place of the heads
+// that lie side by side in a warp share the work.
 template <int V, int S>
 __device__ __forceinline__ void angles(const uint64_t *frequencies, uint32_t position, float magnitude,
                                        uint32_t p0, uint32_t lanes, uint32_t rotary, float (&cos)[S][V],
                                        float (&sin)[S][V]) {
+  const uint32_t per = 32 / lanes, sub = (threadIdx.x & 31) / lanes;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const uint32_t p = p0 + s * lanes;
     const bool turned = 2 * p * V < rotary;
+    float cs[V], sn[V];  // pairs sub, sub + per, ..
+#pragma unroll
+    for (int r = 0; r < V; ++r) {
+      cs[r] = 1.0f;
+      sn[r] = 0.0f;
+      const uint32_t i = r * per + sub;
+      if (r * per < V && i < V && turned) {
+        sine_cosine(position * frequencies[p * V + i], sn[r], cs[r]);
+        cs[r] *= magnitude;
+        sn[r] *= magnitude;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      cos[s][i] = 1.0f;
-      sin[s][i] = 0.0f;
-      if (turned) {
-        float sn, cs;
-        sine_cosine(position * frequencies[p * V + i], sn, cs);
-        cos[s][i] = cs * magnitude;
-        sin[s][i] = sn * magnitude;
-      }
+      const uint32_t from = p0 + lanes * (i & (per - 1));
+      // pair i is the (i / per)-th of that lane
+      const float c = per == 1 ? cs[i] : per == 2 ? cs[i / 2] : per == 4 ? cs[i / 4] : cs[0];
+      const float n = per == 1 ? sn[i] : per == 2 ? sn[i / 2] : per == 4 ? sn[i / 4] : sn[0];
+      cos[s][i] = __shfl_sync(0xffffffffu, c, from);
+      sin[s][i] = __shfl_sync(0xffffffffu, n, from);
     }
   }
 }
@@ -177,73 +203,95 @@ __device__ __forceinline__ void load_weights(const float *w, const Slot &s, floa
   }
 }
 
-// Sum over the `lanes` lanes of a head (a power of two), in each of them.
-__device__ __forceinline__ float head_sum(float x, uint32_t lanes) {
-  for (uint32_t o = lanes >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
+// Sums over the `lanes` lanes of a head (a power of two), in each of them; all
+// of them step by step together, so that one's shuffles cover the others'.
+template <int N> __device__ __forceinline__ void head_sums(float (&x)[N], uint32_t lanes) {
+#pragma unroll
+  for (uint32_t o = 1; o < 32; o <<= 1) {
+    if (o >= lanes) break;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
+  }
 }
 
 // Heads [first, end) of one token from x to out: the norm of each where
-// `norm`, the turn of its first `rotary` elements where `turned`. U head rows
-// a lane are loaded before the first is used.
-template <typename TI, typename TO, int V, int S, int U>
+// `norm`, the turn of its first `rotary` elements where `turned`.  U head rows
+// a lane are loaded before the first is used, the first ones before `angles`
+// works out cos and sin.
+template <typename TI, typename TO, int V, int S, int U, typename Angles>
 __device__ __forceinline__ void run_heads(const TI *x, uint64_t x_stride, TO *out, uint64_t out_stride,
                                           uint32_t first, uint32_t end, uint32_t lanes, uint32_t sub,
                                           const Slot (&slot)[S], const float (&wa)[S][V], const float (&wb)[S][V],
-                                          const float (&cos)[S][V], const float (&sin)[S][V], bool norm,
-                                          bool turned, bool inter, float inv_d, float eps) {
+                                          Angles angles, bool norm, bool turned, bool inter, float inv_d, float eps) {
   const uint32_t per = 32 / lanes;
-  for (uint32_t h0 = first; h0 < end; h0 += U * per) {
-    Raw<TI, V> ra[U][S], rb[U][S];
+  const uint64_t x_step = per * x_stride, out_step = per * out_stride;
+  x += (first + sub) * x_stride;
+  out += (first + sub) * out_stride;
+  Raw<TI, V> ra[U][S], rb[U][S];
+  const auto load = [&](uint32_t h0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t h = h0 + u * per + sub;
-      const TI *row = x + h * x_stride;
+      const bool there = h0 + u * per + sub < end;
+      const TI *row = x + u * x_step;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         ra[u][s] = rb[u][s] = Raw<TI, V>{};
-        if (h < end && slot[s].has_a) ra[u][s].load(row + slot[s].a);
-        if (h < end && slot[s].has_b) rb[u][s].load(row + slot[s].b);
+        if (there && slot[s].has_a) ra[u][s].load(row + slot[s].a);
+        if (there && slot[s].has_b) rb[u][s].load(row + slot[s].b);
       }
+    }
+    x += U * x_step;
+  };
+  load(first);
+  float cos[S][V], sin[S][V];
+  angles(cos, sin);
+  for (uint32_t h0 = first; h0 < end; h0 += U * per) {
+    if (h0 != first) load(h0);
+    float r[U];
+    if (norm) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        r[u] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; ++s) r[u] += ra[u][s].squares() + rb[u][s].squares();
+      }
+      head_sums<U>(r, lanes);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t h = h0 + u * per + sub;
-      float va[S][V], vb[S][V], squares = 0.0f;
+      const bool there = h0 + u * per + sub < end;
+      float va[S][V], vb[S][V];
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         ra[u][s].get(va[s]);
         rb[u][s].get(vb[s]);
-        if (norm) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) squares = fmaf(va[s][i], va[s][i], fmaf(vb[s][i], vb[s][i], squares));
-        }
       }
       if (norm) {
-        const float r = __frsqrt_rn(head_sum(squares, lanes) * inv_d + eps);
+        const float f = rsqrtf(fmaf(r[u], inv_d, eps));
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            va[s][i] = va[s][i] * r * wa[s][i];
-            vb[s][i] = vb[s][i] * r * wb[s][i];
+            va[s][i] *= f * wa[s][i];
+            vb[s][i] *= f * wb[s][i];
           }
       }
-      TO *row = out + h * out_stride;
+      TO *row = out + u * out_step;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         if (turned && slot[s].turned) turn<V>(va[s], vb[s], cos[s], sin[s], inter);
         Raw<TO, V> y;
-        if (h < end && slot[s].has_a) {
+        if (there && slot[s].has_a) {
           y.set(va[s]);
           y.store(row + slot[s].a);
         }
-        if (h < end && slot[s].has_b) {
+        if (there && slot[s].has_b) {
           y.set(vb[s]);
           y.store(row + slot[s].b);
         }
       }
     }
+    out += U * out_step;
   }
 }
 
@@ -252,7 +300,7 @@ struct Shape {
   uint32_t lanes;
   bool vectors;
 };
-// `V` elements a vector; rotated pairs and the rest have to come in whole ones.
+// Vectors of V elements; rotated pairs and the rest have to come in whole ones.
 inline Shape shape_for(uint32_t D, uint32_t rotary, uint32_t V, bool aligned) {
   Shape s{32, aligned && D % V == 0 && (rotary / 2) % V == 0 && (D - rotary) % V == 0};
   if (s.vectors) {
@@ -261,10 +309,11 @@ inline Shape shape_for(uint32_t D, uint32_t rotary, uint32_t V, bool aligned) {
   }
   return s;
 }
-// Whether every row of a view starts on a 16-byte boundary.
-inline bool aligned_view(const tl_head_view &v, int32_t type, bool batches) {
-  const uint64_t e = 16 / type_size(type);
-  return aligned16(v.p) && (!batches || v.batch_stride % e == 0) && v.head_stride % e == 0 &&
+// Whether every row of a view starts on the boundary that its words of up to 16
+// bytes ask for, of vectors of V elements.
+inline bool aligned_view(const tl_head_view &v, int32_t type, bool batches, uint32_t V) {
+  const uint64_t bytes = V * type_size(type) < 16 ? V * type_size(type) : 16, e = bytes / type_size(type);
+  return reinterpret_cast<uintptr_t>(v.p) % bytes == 0 && (!batches || v.batch_stride % e == 0) && v.head_stride % e == 0 &&
          v.row_stride % e == 0;
 }
 

@@ -108,29 +108,30 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
       if (lane == 0) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
       continue;
     }
-    float cos[S][V], sin[S][V];
-    if (part.turned)
-      heads::angles<V, S>(a.frequencies, static_cast<uint32_t>(position), a.magnitude, at, lanes, a.rotary, cos, sin);
     const TI *x = static_cast<const TI *>(part.x.p) + token * part.x.row_stride;
     TO *out = static_cast<TO *>(part.out);
     out += part.cache ? page * c.page_stride + static_cast<uint32_t>(position) % c.page_size * c.slot_stride
                       : token * part.out_row;
     heads::run_heads<TI, TO, V, S, U>(x, part.x.head_stride, out, part.out_head, chunk * part.run,
-                                      min((chunk + 1) * part.run, part.heads), lanes, sub, slot, wa, wb, cos, sin,
+                                      min((chunk + 1) * part.run, part.heads), lanes, sub, slot, wa, wb,
+                                      [&](float (&cos)[S][V], float (&sin)[S][V]) {
+                                        if (part.turned)
+                                          heads::angles<V, S>(a.frequencies, static_cast<uint32_t>(position), a.magnitude,
+                                                              at, lanes, a.rotary, cos, sin);
+                                      },
                                       norm, part.turned, a.interleaved, a.inv_d, a.eps);
   }
 }
 
 template <typename TI, typename TO> void launch_append(const AppendArgs &a, bool vectors, unsigned grid, cudaStream_t s) {
-  constexpr int V = sizeof(TI) == 4 && sizeof(TO) == 4 ? 4 : 8;
+  constexpr int V = heads::vector_of(sizeof(TI), sizeof(TO));
   if (vectors) launch_pdl(append_kernel<TI, TO, V, 1>, grid, kThreads, 0, s, a);
   else launch_pdl(append_kernel<TI, TO, 1, 4>, grid, kThreads, 0, s, a);
 }
 
 // One launch for parts [0, a.parts) of one output type.
 int append(const char *who, AppendArgs a, int32_t type, int32_t out_type, bool aligned, cudaStream_t s) {
-  const uint32_t V = type == TL_FLOAT32 && out_type == TL_FLOAT32 ? 4 : 8;
-  const heads::Shape shape = heads::shape_for(a.cache.D, a.rotary, V, aligned);
+  const heads::Shape shape = heads::shape_for(a.cache.D, a.rotary, heads::vector_for(type, out_type), aligned);
   a.lanes = shape.lanes;
   // Short runs of heads while the tokens are few: each warp's chain of loads
   // is what a small call costs.
@@ -185,7 +186,8 @@ extern "C" int tl_cache_append(const tl_cache_append_desc *d, void *stream) {
     if (int rc = heads::check_view(who, "q_out", d->q_out, d->q_out_type, 1, c.tokens, d->q_heads, c.D, true)) return rc;
     if (heads::half_in_place(d->q_out, d->q_out_type, d->q, d->type, false))
       return fail(TL_ERR_INVALID, w + "q_out is q with another layout or type");
-    q_aligned = heads::aligned_view(d->q, d->type, false) && heads::aligned_view(d->q_out, d->q_out_type, false);
+    q_aligned = heads::aligned_view(d->q, d->type, false, heads::vector_for(d->type, d->q_out_type)) &&
+                heads::aligned_view(d->q_out, d->q_out_type, false, heads::vector_for(d->type, d->q_out_type));
   }
   a.rotary = d->rotary_dim;
   a.interleaved = d->layout == TL_ROTARY_INTERLEAVED;
@@ -200,8 +202,8 @@ extern "C" int tl_cache_append(const tl_cache_append_desc *d, void *stream) {
                      d->q_heads, 0, 0, 0, false, true};
   const AppendPart k{d->k, c.k, 0, c.head_stride, d->k_weight, c.heads, 0, 0, 0, true, true};
   const AppendPart v{d->v, c.v, 0, c.head_stride, nullptr, c.heads, 0, 0, 0, true, false};
-  const bool aligned = cache_aligned && heads::aligned_view(d->k, d->type, false) &&
-                       heads::aligned_view(d->v, d->type, false);
+  const bool aligned = cache_aligned && heads::aligned_view(d->k, d->type, false, heads::vector_for(d->type, c.type)) &&
+                       heads::aligned_view(d->v, d->type, false, heads::vector_for(d->type, c.type));
   cudaStream_t s = as_stream(stream);
   if (d->q_heads && d->q_out_type != c.type) {
     // queries of another type than the cache's: a launch of their own

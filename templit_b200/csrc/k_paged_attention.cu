@@ -30,7 +30,7 @@ int attention_args(const char *who, const tl_paged_attention_desc *d, AttentionA
   if (int rc = heads::check_view(who, "out", d->out, d->out_type, 1, c.tokens, d->q_heads, c.D, true)) return rc;
   if (heads::half_in_place(d->out, d->out_type, d->q, c.type, false))
     return fail(TL_ERR_INVALID, w + "out is q with another layout or type");
-  if (!aligned || !heads::aligned_view(d->q, c.type, false) || !heads::aligned_view(d->out, d->out_type, false))
+  if (!aligned || !heads::aligned_view(d->q, c.type, false, 8) || !heads::aligned_view(d->out, d->out_type, false, 8))
     return fail(TL_ERR_UNSUPPORTED, w + "rows are not 16-byte aligned");
   a.q = d->q;
   a.out = d->out;

@@ -6,8 +6,8 @@
 //   (y_a, y_b) -> mag (y_a cos - y_b sin, y_a sin + y_b cos), angle = p f_i
 //
 // Bound by memory: every element is read once and written once.  A warp takes
-// one token (its angles are computed once, in registers) and a run of its
-// heads, 32 / lanes heads at a time, kBatch of those in flight.
+// one token (its angles are worked out once, shared by the lanes) and a run of
+// its heads, some side by side.
 #include "rotary.cuh"
 
 #include <cmath>
@@ -47,56 +47,106 @@ int check_view(const char *who, const char *name, const tl_head_view &v, int32_t
 
 namespace {
 
-template <typename TI, typename TO, int V, int S, bool NORM, bool INTER>
-__global__ void __launch_bounds__(kThreads) rotate_kernel(const RotaryArgs a) {
-  constexpr int U = V == 1 ? 1 : kBatch;
+template <typename TI, typename TO, int V, int S, int U, bool NORM, bool INTER>
+__global__ void __launch_bounds__(kThreads, 4) rotate_kernel(const RotaryArgs a) {
   pdl_enter();
-  const bool second = blockIdx.x >= a.part[0].ctas;
-  const RotaryPart &part = a.part[second];
-  const uint32_t cta = blockIdx.x - (second ? a.part[0].ctas : 0);
   const bool inter = V == 1 ? a.interleaved : INTER;
   const bool norm = V == 1 ? a.norm : NORM;
-  const uint32_t lane = threadIdx.x & 31, lanes = a.lanes, at = lane & (lanes - 1), sub = lane / lanes;
-  const uint32_t per = 32 / lanes;  // heads at a time
-
+  const uint32_t lane = threadIdx.x & 31, lanes = a.lanes, at = lane & (lanes - 1), sub = lane / lanes, per = 32 / lanes;
+  const uint64_t first_groups = static_cast<uint64_t>(a.tokens) * a.part[0].chunks;
+  const uint64_t groups = first_groups + static_cast<uint64_t>(a.tokens) * a.part[1].chunks;
+  const uint64_t warps = static_cast<uint64_t>(gridDim.x) * kWarps;
   Slot slot[S];
-  float wa[S][V], wb[S][V];
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    slot[s] = slot_of(at + s * lanes, V, a.D, a.rotary, inter);
-    load_weights<V>(norm ? part.weight : nullptr, slot[s], wa[s], wb[s]);
-  }
-  const uint64_t items = static_cast<uint64_t>(a.tokens) * part.chunks;
-  const uint64_t warps = static_cast<uint64_t>(part.ctas) * kWarps;
-  for (uint64_t item = static_cast<uint64_t>(cta) * kWarps + threadIdx.x / 32; item < items; item += warps) {
-    const uint32_t token = static_cast<uint32_t>(item / part.chunks), chunk = static_cast<uint32_t>(item % part.chunks);
-    const uint32_t b = token / a.T, t = token % a.T;
-    float cos[S][V], sin[S][V];
-    angles<V, S>(a.frequencies, a.positions ? a.positions[token] : a.first_position + t, a.magnitude, at, lanes,
-                 a.rotary, cos, sin);
-    const TI *x = static_cast<const TI *>(part.x.p) + b * part.x.batch_stride + t * part.x.row_stride;
-    TO *out = static_cast<TO *>(const_cast<void *>(part.out.p)) + b * part.out.batch_stride + t * part.out.row_stride;
-    const uint32_t heads = part.steps * per;
-    run_heads<TI, TO, V, S, U>(x, part.x.head_stride, out, part.out.head_stride, chunk * heads,
-                               min((chunk + 1) * heads, part.heads), lanes, sub, slot, wa, wb, cos, sin, norm, true,
-                               inter, a.inv_d, a.eps);
+  for (int s = 0; s < S; ++s) slot[s] = slot_of(at + s * lanes, V, a.D, a.rotary, inter);
+
+  const auto load = [&](HeadRows<TI, V, S, U> &r, const Batch &s) {
+    const tl_head_view &v = a.part[s.part].x;
+    const uint32_t left = s.end > s.head + sub ? s.end - s.head - sub : 0;
+    r.load(static_cast<const TI *>(v.p) + place(v, s, sub), per * v.head_stride, slot, left, per);
+  };
+  Batch s;
+  s.group = static_cast<uint64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
+  set_batch(a, s, first_groups, groups);
+  if (!s.any) return;
+  HeadRows<TI, V, S, U> rows, next_rows;
+  load(rows, s);
+  uint64_t turned = ~0ull;  // the group whose angles are in cos and sin
+  uint32_t part = 2;        // whose weights are in wa and wb
+  float cos[S][V], sin[S][V], wa[S][V], wb[S][V];
+  while (true) {
+    Batch n = s;
+    next_batch(a, n, U * per, warps, first_groups, groups);
+    if (n.any) load(next_rows, n);
+    if (s.part != part) {
+      part = s.part;
+#pragma unroll
+      for (int i = 0; i < S; ++i) load_weights<V>(norm ? a.part[part].weight : nullptr, slot[i], wa[i], wb[i]);
+    }
+    if (s.group != turned) {
+      turned = s.group;
+      angles<V, S>(a.frequencies, s.position, a.magnitude, at, lanes, a.rotary, cos, sin);
+    }
+    float r[U];
+    if (norm) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        r[u] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S; ++i) r[u] += rows.a[u][i].squares() + rows.b[u][i].squares();
+      }
+      head_sums<U>(r, lanes);
+    }
+    const tl_head_view &v = a.part[s.part].out;
+    TO *out = static_cast<TO *>(const_cast<void *>(v.p)) + place(v, s, sub);
+    const uint32_t left = s.end > s.head + sub ? s.end - s.head - sub : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        float va[V], vb[V];
+        rows.a[u][i].get(va);
+        rows.b[u][i].get(vb);
+        if (norm) {
+          const float f = rsqrtf(fmaf(r[u], a.inv_d, a.eps));
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            va[e] *= f * wa[i][e];
+            vb[e] *= f * wb[i][e];
+          }
+        }
+        if (slot[i].turned) turn<V>(va, vb, cos[i], sin[i], inter);
+        Raw<TO, V> y;
+        if (u * per < left && slot[i].has_a) {
+          y.set(va);
+          y.store(out + u * (per * v.head_stride) + slot[i].a);
+        }
+        if (u * per < left && slot[i].has_b) {
+          y.set(vb);
+          y.store(out + u * (per * v.head_stride) + slot[i].b);
+        }
+      }
+    }
+    if (!n.any) return;
+    s = n;
+    rows = next_rows;
   }
 }
 
-template <typename TI, typename TO> void launch_rotate(RotaryArgs &a, bool vectors, cudaStream_t s) {
-  constexpr int V = sizeof(TI) == 4 && sizeof(TO) == 4 ? 4 : 8;
-  if (!vectors) {
-    const unsigned grid = share_out(a, false);
-    launch_pdl(rotate_kernel<TI, TO, 1, 4, false, false>, grid, kThreads, 0, s, a);
+template <typename TI, typename TO> void launch_rotate(RotaryArgs &a, cudaStream_t s) {
+  constexpr int V = vector_of(sizeof(TI), sizeof(TO)), U = V == 8 ? 2 : 3;
+  if (!a.vectors) {
+    const unsigned grid = share_out(a, 1, false);
+    launch_pdl(rotate_kernel<TI, TO, 1, 4, 1, false, false>, grid, kThreads, 0, s, a);
     return;
   }
-  const unsigned grid = share_out(a, false);
+  const unsigned grid = share_out(a, U, false);
   if (a.norm) {
-    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, 1, true, true>, grid, kThreads, 0, s, a);
-    else launch_pdl(rotate_kernel<TI, TO, V, 1, true, false>, grid, kThreads, 0, s, a);
+    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, 1, U, true, true>, grid, kThreads, 0, s, a);
+    else launch_pdl(rotate_kernel<TI, TO, V, 1, U, true, false>, grid, kThreads, 0, s, a);
   } else {
-    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, 1, false, true>, grid, kThreads, 0, s, a);
-    else launch_pdl(rotate_kernel<TI, TO, V, 1, false, false>, grid, kThreads, 0, s, a);
+    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, 1, U, false, true>, grid, kThreads, 0, s, a);
+    else launch_pdl(rotate_kernel<TI, TO, V, 1, U, false, false>, grid, kThreads, 0, s, a);
   }
 }
 
@@ -124,6 +174,7 @@ int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryA
   a.frequencies = d->frequencies;
   a.positions = d->positions;
   a.first_position = d->first_position;
+  const uint32_t V = vector_for(d->type, d->out_type);
   bool aligned = true;
   const tl_rotary_part *parts[2] = {&d->q, &d->k};
   for (int i = 0; i < 2 && tokens; ++i) {
@@ -132,7 +183,7 @@ int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryA
     r.heads = p.heads;
     if (!p.heads) continue;
     const auto view = [&](const char *name, const tl_head_view &v, int32_t type, bool written) {
-      aligned = aligned && aligned_view(v, type, d->B > 1);
+      aligned = aligned && aligned_view(v, type, d->B > 1, V);
       return check_view(who, name, v, type, d->B, d->T, p.heads, d->D, written);
     };
     if (!backward || d->norm)
@@ -156,35 +207,40 @@ int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryA
     r.weight = p.weight;
     r.dweight = backward ? p.dweight : nullptr;
   }
-  const uint32_t V = d->type == TL_FLOAT32 && d->out_type == TL_FLOAT32 ? 4 : 8;
   const Shape shape = shape_for(d->D, d->rotary_dim, V, aligned);
   a.lanes = shape.lanes;
   a.vectors = shape.vectors;
   return TL_OK;
 }
 
-unsigned share_out(RotaryArgs &a, bool persistent) {
-  // A warp's run of heads: all of them where the tokens alone make two warps a
-  // scheduler, shorter where they do not.
-  const uint32_t per = 32 / a.lanes, wanted = kNumSMs * 8;
-  unsigned grid = 0;
-  const uint64_t heads = a.part[0].heads + static_cast<uint64_t>(a.part[1].heads);
+unsigned share_out(RotaryArgs &a, uint32_t rows, bool apart) {
+  // A warp's run of a token's heads: all of them where the tokens alone keep two warps a
+  // scheduler busy, shorter where they do not.
+  const uint32_t per = 32 / a.lanes * rows, wanted = kNumSMs * 8;
+  uint64_t groups = 0;
   for (RotaryPart &p : a.part) {
-    p.ctas = 0;
+    p.chunks = p.ctas = 0;
     if (!p.heads) continue;
-    p.all_steps = (p.heads + per - 1) / per;
-    p.steps = p.all_steps;
-    while (p.steps > 1 && static_cast<uint64_t>(a.tokens) * ((p.all_steps + p.steps - 1) / p.steps) < wanted)
-      p.steps = (p.steps + 1) / 2;
-    p.chunks = (p.all_steps + p.steps - 1) / p.steps;
-    const uint64_t items = static_cast<uint64_t>(a.tokens) * p.chunks;
-    uint64_t ctas = (items + kWarps - 1) / kWarps;
-    const uint64_t most = persistent ? (kMaxCtas * p.heads + heads - 1) / heads : kNumSMs * 256ull;
-    if (ctas > most) ctas = most;
-    p.ctas = static_cast<uint32_t>(ctas);
-    grid += p.ctas;
+    const uint32_t batches = (p.heads + per - 1) / per;
+    uint32_t run = batches;
+    while (run > 1 && static_cast<uint64_t>(a.tokens) * ((batches + run - 1) / run) < wanted) run = (run + 1) / 2;
+    p.run = run * per;
+    p.chunks = (batches + run - 1) / run;
+    groups += static_cast<uint64_t>(a.tokens) * p.chunks;
   }
-  return grid;
+  const auto fewest = [](uint64_t x, uint64_t y) { return static_cast<uint32_t>(x < y ? x : y); };
+  if (!apart) return fewest((groups + kWarps - 1) / kWarps, kMaxCtas);
+  const uint64_t heads = a.part[0].heads + static_cast<uint64_t>(a.part[1].heads);
+  uint32_t left = kMaxCtas;
+  for (RotaryPart &p : a.part) {
+    if (!p.heads) continue;
+    const bool last = &p == &a.part[1] || !a.part[1].heads;
+    uint64_t share = last ? left : kMaxCtas * static_cast<uint64_t>(p.heads) / heads;
+    share = share < 1 ? 1 : share > kMaxCtas - 1 ? kMaxCtas - 1 : share;
+    p.ctas = fewest((static_cast<uint64_t>(a.tokens) * p.chunks + kWarps - 1) / kWarps, share);
+    left -= p.ctas;
+  }
+  return a.part[0].ctas + a.part[1].ctas;
 }
 
 }  // namespace heads
@@ -246,7 +302,7 @@ int tl_rotary_heads(const tl_rotary_desc *desc, void *stream) {
   RotaryArgs a{};
   if (int rc = rotary_args(who, desc, false, a)) return rc;
   if (a.tokens == 0) return TL_OK;
-#define L(TI, TO) launch_rotate<TI, TO>(a, a.vectors, as_stream(stream))
+#define L(TI, TO) launch_rotate<TI, TO>(a, as_stream(stream))
   TL_BY_TYPES(desc->type, desc->out_type, L)
 #undef L
   return launch_status(who);

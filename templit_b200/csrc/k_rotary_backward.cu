@@ -13,9 +13,10 @@ namespace tl {
 namespace heads {
 namespace {
 
-template <typename TI, typename TO, int V, int S, bool NORM, bool INTER>
-__global__ void __launch_bounds__(kThreads) rotate_backward_kernel(const RotaryArgs a) {
-  constexpr int U = V == 1 ? 1 : kBatch / 2;
+constexpr int kGradientRows = 2;  // head rows a lane
+
+template <typename TI, typename TO, int V, int S, int U, bool NORM, bool INTER>
+__global__ void __launch_bounds__(kThreads, NORM || V == 1 ? 3 : 4) rotate_backward_kernel(const RotaryArgs a) {
   __shared__ float sums[kWarps][TL_HEAD_MAX_DIM];
   pdl_enter();
   const bool second = blockIdx.x >= a.part[0].ctas;
@@ -25,6 +26,10 @@ __global__ void __launch_bounds__(kThreads) rotate_backward_kernel(const RotaryA
   const bool norm = V == 1 ? a.norm : NORM;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const uint32_t lanes = a.lanes, at = lane & (lanes - 1), sub = lane / lanes, per = 32 / lanes;
+  // this part's groups only
+  const uint64_t first_groups = static_cast<uint64_t>(a.tokens) * a.part[0].chunks;
+  const uint64_t groups = second ? first_groups + static_cast<uint64_t>(a.tokens) * a.part[1].chunks : first_groups;
+  const uint64_t warps = static_cast<uint64_t>(part.ctas) * kWarps;
 
   Slot slot[S];
   float wa[S][V], wb[S][V], dwa[S][V], dwb[S][V];
@@ -35,101 +40,84 @@ __global__ void __launch_bounds__(kThreads) rotate_backward_kernel(const RotaryA
 #pragma unroll
     for (int i = 0; i < V; ++i) dwa[s][i] = dwb[s][i] = 0.0f;
   }
-  const uint64_t items = static_cast<uint64_t>(a.tokens) * part.chunks;
-  const uint64_t warps = static_cast<uint64_t>(part.ctas) * kWarps;
-  for (uint64_t item = static_cast<uint64_t>(cta) * kWarps + warp; item < items; item += warps) {
-    const uint32_t token = static_cast<uint32_t>(item / part.chunks), chunk = static_cast<uint32_t>(item % part.chunks);
-    const uint32_t b = token / a.T, t = token % a.T;
-    float cos[S][V], sin[S][V];
-    angles<V, S>(a.frequencies, a.positions ? a.positions[token] : a.first_position + t, a.magnitude, at, lanes,
-                 a.rotary, cos, sin);
+  struct Rows {
+    HeadRows<TO, V, S, U> g;
+    HeadRows<TI, V, S, U> x;
+  };
+  const auto load = [&](Rows &r, const Batch &s) {
+    const uint32_t left = s.end > s.head + sub ? s.end - s.head - sub : 0;
+    r.g.load(static_cast<const TO *>(part.d_out.p) + place(part.d_out, s, sub), per * part.d_out.head_stride, slot, left, per);
+    if (norm) r.x.load(static_cast<const TI *>(part.x.p) + place(part.x, s, sub), per * part.x.head_stride, slot, left, per);
+  };
+  Batch s;
+  s.group = (second ? first_groups : 0) + static_cast<uint64_t>(cta) * kWarps + warp;
+  set_batch(a, s, first_groups, groups);
+  Rows rows, next_rows;
+  if (s.any) load(rows, s);
+  uint64_t turned = ~0ull;
+  float cos[S][V], sin[S][V];
+  while (s.any) {
+    Batch n = s;
+    next_batch(a, n, U * per, warps, first_groups, groups);
+    if (n.any) load(next_rows, n);
+    if (s.group != turned) {
+      turned = s.group;
+      angles<V, S>(a.frequencies, s.position, a.magnitude, at, lanes, a.rotary, cos, sin);
 #pragma unroll
-    for (int s = 0; s < S; ++s)
+      for (int i = 0; i < S; ++i)
 #pragma unroll
-      for (int i = 0; i < V; ++i) sin[s][i] = -sin[s][i];
-    const TI *x = static_cast<const TI *>(part.x.p) + b * part.x.batch_stride + t * part.x.row_stride;
-    const TO *g = static_cast<const TO *>(part.d_out.p) + b * part.d_out.batch_stride + t * part.d_out.row_stride;
-    TI *dx = static_cast<TI *>(const_cast<void *>(part.dx.p)) + b * part.dx.batch_stride + t * part.dx.row_stride;
-    const uint32_t end = min((chunk + 1) * part.steps, part.all_steps);
-    for (uint32_t step = chunk * part.steps; step < end; step += U) {
-      Raw<TO, V> ra[U][S], rb[U][S];
-      Raw<TI, V> xa[U][S], xb[U][S];
+        for (int e = 0; e < V; ++e) sin[i][e] = -sin[i][e];
+    }
+    TI *const dx = static_cast<TI *>(const_cast<void *>(part.dx.p)) + place(part.dx, s, sub);
+    const uint32_t left = s.end > s.head + sub ? s.end - s.head - sub : 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t h = (step + u) * per + sub;
-        const bool there = step + u < end && h < part.heads;
+    for (int u = 0; u < U; ++u) {
+      float ga[S][V], gb[S][V], va[S][V], vb[S][V], both[2] = {0.0f, 0.0f};  // sum x^2, sum g w x
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          ra[u][s] = rb[u][s] = Raw<TO, V>{};
-          xa[u][s] = xb[u][s] = Raw<TI, V>{};
-          if (there && slot[s].has_a) {
-            ra[u][s].load(g + h * part.d_out.head_stride + slot[s].a);
-            if (norm) xa[u][s].load(x + h * part.x.head_stride + slot[s].a);
-          }
-          if (there && slot[s].has_b) {
-            rb[u][s].load(g + h * part.d_out.head_stride + slot[s].b);
-            if (norm) xb[u][s].load(x + h * part.x.head_stride + slot[s].b);
+      for (int i = 0; i < S; ++i) {
+        rows.g.a[u][i].get(ga[i]);
+        rows.g.b[u][i].get(gb[i]);
+        if (slot[i].turned) turn<V>(ga[i], gb[i], cos[i], sin[i], inter);
+        if (norm) {
+          rows.x.a[u][i].get(va[i]);
+          rows.x.b[u][i].get(vb[i]);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            both[0] = fmaf(va[i][e], va[i][e], fmaf(vb[i][e], vb[i][e], both[0]));
+            both[1] = fmaf(ga[i][e] * wa[i][e], va[i][e], fmaf(gb[i][e] * wb[i][e], vb[i][e], both[1]));
           }
         }
       }
+      if (norm) {
+        head_sums<2>(both, lanes);
+        const float r = rsqrtf(fmaf(both[0], a.inv_d, a.eps)), dot = both[1] * r * a.inv_d;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t h = (step + u) * per + sub;
-        float ga[S][V], gb[S][V];
+        for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          ra[u][s].get(ga[s]);
-          rb[u][s].get(gb[s]);
-          if (slot[s].turned) turn<V>(ga[s], gb[s], cos[s], sin[s], inter);
+          for (int e = 0; e < V; ++e) {
+            va[i][e] *= r;
+            vb[i][e] *= r;
+            dwa[i][e] = fmaf(ga[i][e], va[i][e], dwa[i][e]);
+            dwb[i][e] = fmaf(gb[i][e], vb[i][e], dwb[i][e]);
+            ga[i][e] = fmaf(-va[i][e], dot, ga[i][e] * wa[i][e]) * r;
+            gb[i][e] = fmaf(-vb[i][e], dot, gb[i][e] * wb[i][e]) * r;
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        Raw<TI, V> y;
+        if (u * per < left && slot[i].has_a) {
+          y.set(ga[i]);
+          y.store(dx + u * (per * part.dx.head_stride) + slot[i].a);
         }
-        if (norm) {
-          float va[S][V], vb[S][V], squares = 0.0f;
-#pragma unroll
-          for (int s = 0; s < S; ++s) {
-            xa[u][s].get(va[s]);
-            xb[u][s].get(vb[s]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) squares = fmaf(va[s][i], va[s][i], fmaf(vb[s][i], vb[s][i], squares));
-          }
-          const float r = __frsqrt_rn(head_sum(squares, lanes) * a.inv_d + a.eps);
-          float dot = 0.0f;
-#pragma unroll
-          for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              va[s][i] *= r;
-              vb[s][i] *= r;
-              dwa[s][i] = fmaf(ga[s][i], va[s][i], dwa[s][i]);
-              dwb[s][i] = fmaf(gb[s][i], vb[s][i], dwb[s][i]);
-              ga[s][i] *= wa[s][i];
-              gb[s][i] *= wb[s][i];
-              dot = fmaf(ga[s][i], va[s][i], fmaf(gb[s][i], vb[s][i], dot));
-            }
-          dot = head_sum(dot, lanes) * a.inv_d;
-#pragma unroll
-          for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              ga[s][i] = fmaf(-va[s][i], dot, ga[s][i]) * r;
-              gb[s][i] = fmaf(-vb[s][i], dot, gb[s][i]) * r;
-            }
-        }
-        const bool there = step + u < end && h < part.heads;
-        TI *row = dx + h * part.dx.head_stride;
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-          Raw<TI, V> y;
-          if (there && slot[s].has_a) {
-            y.set(ga[s]);
-            y.store(row + slot[s].a);
-          }
-          if (there && slot[s].has_b) {
-            y.set(gb[s]);
-            y.store(row + slot[s].b);
-          }
+        if (u * per < left && slot[i].has_b) {
+          y.set(gb[i]);
+          y.store(dx + u * (per * part.dx.head_stride) + slot[i].b);
         }
       }
     }
+    s = n;
+    rows = next_rows;
   }
   if constexpr (V > 1 && !NORM) return;
   if (!part.dweight) return;
@@ -177,15 +165,15 @@ __global__ void __launch_bounds__(1024) weight_gradient_kernel(const RotaryArgs 
   }
 }
 
-template <typename TI, typename TO> void launch_backward(RotaryArgs &a, unsigned grid, cudaStream_t s) {
-  constexpr int V = sizeof(TI) == 4 && sizeof(TO) == 4 ? 4 : 8;
-  if (!a.vectors) launch_pdl(rotate_backward_kernel<TI, TO, 1, 4, false, false>, grid, kThreads, 0, s, a);
+template <typename TI, typename TO> void launch_backward(const RotaryArgs &a, unsigned grid, cudaStream_t s) {
+  constexpr int V = vector_of(sizeof(TI), sizeof(TO)), U = kGradientRows;
+  if (!a.vectors) launch_pdl(rotate_backward_kernel<TI, TO, 1, 4, 1, false, false>, grid, kThreads, 0, s, a);
   else if (a.norm) {
-    if (a.interleaved) launch_pdl(rotate_backward_kernel<TI, TO, V, 1, true, true>, grid, kThreads, 0, s, a);
-    else launch_pdl(rotate_backward_kernel<TI, TO, V, 1, true, false>, grid, kThreads, 0, s, a);
+    if (a.interleaved) launch_pdl(rotate_backward_kernel<TI, TO, V, 1, U, true, true>, grid, kThreads, 0, s, a);
+    else launch_pdl(rotate_backward_kernel<TI, TO, V, 1, U, true, false>, grid, kThreads, 0, s, a);
   } else {
-    if (a.interleaved) launch_pdl(rotate_backward_kernel<TI, TO, V, 1, false, true>, grid, kThreads, 0, s, a);
-    else launch_pdl(rotate_backward_kernel<TI, TO, V, 1, false, false>, grid, kThreads, 0, s, a);
+    if (a.interleaved) launch_pdl(rotate_backward_kernel<TI, TO, V, 1, U, false, true>, grid, kThreads, 0, s, a);
+    else launch_pdl(rotate_backward_kernel<TI, TO, V, 1, U, false, false>, grid, kThreads, 0, s, a);
   }
 }
 
@@ -220,7 +208,7 @@ int tl_rotary_heads_backward(const tl_rotary_desc *desc, void *stream) {
         if (int rc = check_cuda(cudaMemsetAsync(p->dweight, 0, desc->D * sizeof(float), s), who)) return rc;
     return TL_OK;
   }
-  const unsigned grid = share_out(a, true);
+  const unsigned grid = share_out(a, a.vectors ? kGradientRows : 1, true);
   a.part[0].partial = static_cast<float *>(desc->workspace);
   a.part[1].partial = a.part[0].partial + static_cast<size_t>(a.part[0].ctas) * a.D;
 #define L(TI, TO) launch_backward<TI, TO>(a, grid, s)

@@ -9,15 +9,14 @@ namespace heads {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kBatch = 4;                   // head rows in flight a lane
-constexpr uint32_t kMaxCtas = kNumSMs * 4;  // of the gradient: a row of partial weight gradients each
+constexpr uint32_t kMaxCtas = kNumSMs * 4;  // one round of the SMs
 
 struct RotaryPart {
   tl_head_view x, out, d_out, dx;
   const float *weight;
   float *dweight, *partial;  // partial: [ctas, D]
   uint32_t heads, ctas;
-  uint32_t chunks, steps, all_steps;  // a token's heads in runs of `steps` head rows
+  uint32_t chunks, run;  // a token's heads in runs of `run`, a warp each
 };
 struct RotaryArgs {
   RotaryPart part[2];
@@ -29,10 +28,63 @@ struct RotaryArgs {
   uint32_t first_position;
 };
 
+// Where a warp is: a batch of heads of one token.  Warps stay on the SMs and
+// load the next batch before they work on the one that they hold, so that
+// loads are always under way (a warp a token, without: 12288 x 12 heads of 64
+// fp32 20 us, norm and rotation of 16384 x 40 heads of 128 bf16 86 us).
+struct Batch {
+  uint64_t group;  // run of a token's heads, over the parts
+  uint32_t part, token, b, t, position;
+  uint32_t head, end;
+  bool any;
+};
+__device__ __forceinline__ void set_batch(const RotaryArgs &a, Batch &s, uint64_t first_groups, uint64_t groups) {
+  s.any = s.group < groups;
+  if (!s.any) return;
+  s.part = s.group >= first_groups;
+  const RotaryPart &p = a.part[s.part];
+  const uint64_t g = s.part ? s.group - first_groups : s.group;
+  // groups fit in 32 bits where chunks > 1 (few tokens)
+  s.token = p.chunks == 1 ? static_cast<uint32_t>(g) : static_cast<uint32_t>(g) / p.chunks;
+  const uint32_t chunk = p.chunks == 1 ? 0 : static_cast<uint32_t>(g) - s.token * p.chunks;
+  s.b = s.token / a.T;
+  s.t = s.token - s.b * a.T;
+  s.position = a.positions ? a.positions[s.token] : a.first_position + s.t;
+  s.head = chunk * p.run;
+  s.end = min(s.head + p.run, p.heads);
+}
+// the batch behind it, `step` heads on
+__device__ __forceinline__ void next_batch(const RotaryArgs &a, Batch &s, uint32_t step, uint64_t stride, uint64_t first_groups,
+                                           uint64_t groups) {
+  s.head += step;
+  if (s.head < s.end) return;
+  s.group += stride;
+  set_batch(a, s, first_groups, groups);
+}
+__device__ __forceinline__ uint64_t place(const tl_head_view &v, const Batch &s, uint32_t sub) {
+  return s.b * v.batch_stride + s.t * v.row_stride + (s.head + sub) * v.head_stride;
+}
+
+// U head rows a lane.
+template <typename T, int V, int S, int U> struct HeadRows {
+  Raw<T, V> a[U][S], b[U][S];
+  __device__ __forceinline__ void load(const T *x, uint64_t step, const Slot (&slot)[S], uint32_t left, uint32_t per) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        a[u][s] = b[u][s] = Raw<T, V>{};
+        if (u * per < left && slot[s].has_a) a[u][s].load(x + u * step + slot[s].a);
+        if (u * per < left && slot[s].has_b) b[u][s].load(x + u * step + slot[s].b);
+      }
+  }
+};
+
 // Checks a descriptor and fills in everything but the shares.
 int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryArgs &a);
-// Shares the work out; the grid.
-unsigned share_out(RotaryArgs &a, bool persistent);
+// Shares the work out, `rows` head rows a batch; the grid.  `apart`: each CTA takes heads of
+// one part only.
+unsigned share_out(RotaryArgs &a, uint32_t rows, bool apart);
 
 }  // namespace heads
 }  // namespace tl
