@@ -3,10 +3,11 @@
 // head (k_rotary*.cu, k_cache_append.cu).
 //
 // A head of D elements belongs to `lanes` neighbouring lanes of a warp (a
-// power of two), each with S slots of two vectors of V elements: slot p holds
+// power of two), each with a slot of two vectors of V elements: slot p holds
 // the V pairs p V .. p V + V - 1 while those are turned, or 2 V elements
 // behind the turned ones.  So a rotation needs no exchange between lanes in
-// either layout, and the norm one sum over the head's lanes.
+// either layout, and the norm one sum over the head's lanes.  Heads that vectors do
+// not fit go by single elements (scalar_head).
 #pragma once
 
 #include "tl_common.cuh"
@@ -26,8 +27,7 @@ constexpr int vector_of(size_t in, size_t out) { return in == 2 && out == 2 ? 8 
 inline int vector_for(int32_t in, int32_t out) { return vector_of(type_size(in), type_size(out)); }
 inline bool known_type(int32_t type) { return type >= TL_FLOAT32 && type <= TL_BFLOAT16; }
 
-// V elements of T as they lie in memory, in words of 8 or 16 bytes (V = 1: one
-// element).
+// V elements of T as they lie in memory, in words of 8 or 16 bytes.
 template <typename T, int V> struct Raw {
   using Word = typename std::conditional<V * sizeof(T) % 16 == 0, uint4, uint2>::type;
   static constexpr int kWords = V * sizeof(T) / sizeof(Word);
@@ -39,13 +39,6 @@ template <typename T, int V> struct Raw {
   __device__ __forceinline__ void store(T *p) const {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) reinterpret_cast<Word *>(p)[i] = r[i];
-  }
-  __device__ __forceinline__ float squares() const {
-    float x[V], sum = 0.0f;
-    get(x);
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum = fmaf(x[i], x[i], sum);
-    return sum;
   }
   __device__ __forceinline__ void get(float (&x)[V]) const {
     const uint32_t *w = reinterpret_cast<const uint32_t *>(r);
@@ -80,21 +73,54 @@ template <typename T, int V> struct Raw {
     }
   }
 };
+// Two fp32 in a register pair: one issued instruction for both.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ float2 halves(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ float sum2(Pair p) {
+  const float2 f = halves(p);
+  return f.x + f.y;
+}
+template <typename T, int V> __device__ __forceinline__ void get_pairs(const Raw<T, V> &r, Pair (&x)[V / 2]) {
+  float f[V];
+  r.get(f);
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) x[i] = pair(f[2 * i], f[2 * i + 1]);
+}
+template <typename T, int V> __device__ __forceinline__ void set_pairs(Raw<T, V> &r, const Pair (&x)[V / 2]) {
+  float f[V];
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) {
+    const float2 h = halves(x[i]);
+    f[2 * i] = h.x;
+    f[2 * i + 1] = h.y;
+  }
+  r.set(f);
+}
 __device__ __forceinline__ float element_of(float x) { return x; }
 __device__ __forceinline__ float element_of(__half x) { return __half2float(x); }
 __device__ __forceinline__ float element_of(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void set_element(float &y, float x) { y = x; }
 __device__ __forceinline__ void set_element(__half &y, float x) { y = __float2half_rn(x); }
 __device__ __forceinline__ void set_element(__nv_bfloat16 &y, float x) { y = __float2bfloat16_rn(x); }
-template <typename T> struct Raw<T, 1> {
-  T r;
-  __device__ __forceinline__ void load(const T *p) { r = *p; }
-  __device__ __forceinline__ void store(T *p) const { *p = r; }
-  __device__ __forceinline__ void get(float (&x)[1]) const { x[0] = element_of(r); }
-  __device__ __forceinline__ float squares() const { return element_of(r) * element_of(r); }
-  __device__ __forceinline__ void set(const float (&x)[1]) { set_element(r, x[0]); }
-};
-
 // Sine and cosine of `turns` / 2^64 of a full turn.  The quarter turn is split
 // off exactly in whole numbers; what is left, |x| <= pi / 4, goes through the
 // Taylor series, whose first terms left out are x^11 / 11! < 1.8e-9 and
@@ -134,68 +160,95 @@ __device__ __forceinline__ Slot slot_of(uint32_t p, uint32_t V, uint32_t D, uint
   return s;
 }
 
-// Pair i of a slot's two vectors.
-template <int V> __device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], const float (&cos)[V],
-                                                      const float (&sin)[V], bool interleaved) {
-  if (V == 1 || !interleaved) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float u = a[i], w = b[i];
-      a[i] = fmaf(u, cos[i], -(w * sin[i]));
-      b[i] = fmaf(u, sin[i], w * cos[i]);
-    }
-  } else {
+// A lane's slot turned, in register pairs (the gradient, which has more to do
+// for an element than memory gives it time).  HALF: elements i of a and of b are a
+// pair; INTERLEAVED: neighbours are.
+template <int V> struct Turn {
+  Pair a1[V / 2], a2[V / 2], b1[V / 2], b2[V / 2];
+  __device__ __forceinline__ void set(const float (&cos)[V], const float (&sin)[V], bool interleaved) {
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) {
-      const float u = a[2 * i], w = a[2 * i + 1];
-      a[2 * i] = fmaf(u, cos[i], -(w * sin[i]));
-      a[2 * i + 1] = fmaf(u, sin[i], w * cos[i]);
-      const float u2 = b[2 * i], w2 = b[2 * i + 1];
-      b[2 * i] = fmaf(u2, cos[V / 2 + i], -(w2 * sin[V / 2 + i]));
-      b[2 * i + 1] = fmaf(u2, sin[V / 2 + i], w2 * cos[V / 2 + i]);
-    }
-  }
-}
-
-// Angles of a lane's slots at one position, `magnitude` included; cosine 1
-// and sine 0 behind the turned elements.  The lanes at one place of the heads
-// that lie side by side in a warp share the work.
-template <int V, int S>
-__device__ __forceinline__ void angles(const uint64_t *frequencies, uint32_t position, float magnitude,
-                                       uint32_t p0, uint32_t lanes, uint32_t rotary, float (&cos)[S][V],
-                                       float (&sin)[S][V]) {
-  const uint32_t per = 32 / lanes, sub = (threadIdx.x & 31) / lanes;
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    const uint32_t p = p0 + s * lanes;
-    const bool turned = 2 * p * V < rotary;
-    float cs[V], sn[V];  // pairs sub, sub + per, ..
-#pragma unroll
-    for (int r = 0; r < V; ++r) {
-      cs[r] = 1.0f;
-      sn[r] = 0.0f;
-      const uint32_t i = r * per + sub;
-      if (r * per < V && i < V && turned) {
-        sine_cosine(position * frequencies[p * V + i], sn[r], cs[r]);
-        cs[r] *= magnitude;
-        sn[r] *= magnitude;
+      if (!interleaved) {  // a' = a a1 + b a2, b' = a b1 + b b2
+        a1[i] = b2[i] = pair(cos[2 * i], cos[2 * i + 1]);
+        a2[i] = pair(-sin[2 * i], -sin[2 * i + 1]);
+        b1[i] = pair(sin[2 * i], sin[2 * i + 1]);
+      } else {  // (a0, a1)' = (a0, a1) a1 + (a1, a0) a2, likewise b
+        const int j = V / 2 + i;
+        a1[i] = pair(cos[i], cos[i]);
+        a2[i] = pair(-sin[i], sin[i]);
+        b1[i] = pair(cos[j], cos[j]);
+        b2[i] = pair(-sin[j], sin[j]);
       }
     }
+  }
+  // (elements behind the turned ones stay apart: 0 times a neighbour's NaN is NaN)
+  __device__ __forceinline__ void apply(Pair (&a)[V / 2], Pair (&b)[V / 2], bool turned, bool interleaved) const {
+    if (!turned) return;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const uint32_t from = p0 + lanes * (i & (per - 1));
-      // pair i is the (i / per)-th of that lane
-      const float c = per == 1 ? cs[i] : per == 2 ? cs[i / 2] : per == 4 ? cs[i / 4] : cs[0];
-      const float n = per == 1 ? sn[i] : per == 2 ? sn[i / 2] : per == 4 ? sn[i / 4] : sn[0];
-      cos[s][i] = __shfl_sync(0xffffffffu, c, from);
-      sin[s][i] = __shfl_sync(0xffffffffu, n, from);
+    for (int i = 0; i < V / 2; ++i) {
+      if (!interleaved) {
+        const Pair x = a[i], y = b[i];
+        a[i] = fma2(x, a1[i], mul2(y, a2[i]));
+        b[i] = fma2(x, b1[i], mul2(y, b2[i]));
+      } else {
+        const float2 x = halves(a[i]), y = halves(b[i]);
+        a[i] = fma2(a[i], a1[i], mul2(pair(x.y, x.x), a2[i]));
+        b[i] = fma2(b[i], b1[i], mul2(pair(y.y, y.x), b2[i]));
+      }
     }
   }
+};
+
+// Angles of a lane's slot p0 at one position, `magnitude` included; cosine 1
+// and sine 0 behind the turned elements.  The `PER` lanes at one place of the heads
+// that lie side by side in a warp share the work.
+template <int V, int PER>
+__device__ __forceinline__ void shared_angles(const uint64_t *frequencies, uint32_t position, float magnitude, uint32_t p0,
+                                              uint32_t lanes, uint32_t rotary, float (&cos)[V], float (&sin)[V]) {
+  constexpr int N = V > PER ? V / PER : 1;  // a lane's: pairs sub, sub + PER, ..
+  const uint32_t sub = (threadIdx.x & 31) / lanes;
+  const bool turned = 2 * p0 * V < rotary;
+  float cs[N], sn[N];
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    cs[r] = 1.0f;
+    sn[r] = 0.0f;
+    const uint32_t i = r * PER + sub;
+    if (i < V && turned) {
+      sine_cosine(position * frequencies[p0 * V + i], sn[r], cs[r]);
+      cs[r] *= magnitude;
+      sn[r] *= magnitude;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    cos[i] = PER == 1 ? cs[i % N] : __shfl_sync(0xffffffffu, cs[i / PER], p0 + lanes * (i % PER));
+    sin[i] = PER == 1 ? sn[i % N] : __shfl_sync(0xffffffffu, sn[i / PER], p0 + lanes * (i % PER));
+  }
+}
+template <int V>
+__device__ __forceinline__ void angles(const uint64_t *frequencies, uint32_t position, float magnitude, uint32_t p0,
+                                       uint32_t lanes, uint32_t rotary, float (&cos)[V], float (&sin)[V]) {
+  if (lanes == 8) shared_angles<V, 4>(frequencies, position, magnitude, p0, lanes, rotary, cos, sin);
+  else if (lanes <= 4) shared_angles<V, 8>(frequencies, position, magnitude, p0, lanes, rotary, cos, sin);
+  else if (lanes == 16) shared_angles<V, 2>(frequencies, position, magnitude, p0, lanes, rotary, cos, sin);
+  else shared_angles<V, 1>(frequencies, position, magnitude, p0, lanes, rotary, cos, sin);
 }
 
 // The norm's weights of a lane's slot: 1 without any.
 template <int V>
 __device__ __forceinline__ void load_weights(const float *w, const Slot &s, float (&a)[V], float (&b)[V]) {
+  if (w && aligned16(w)) {  // slots begin at whole vectors
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 one = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+      const float4 x = s.has_a ? *reinterpret_cast<const float4 *>(w + s.a + i) : one;
+      const float4 y = s.has_b ? *reinterpret_cast<const float4 *>(w + s.b + i) : one;
+      a[i] = x.x, a[i + 1] = x.y, a[i + 2] = x.z, a[i + 3] = x.w;
+      b[i] = y.x, b[i + 1] = y.y, b[i + 2] = y.z, b[i + 3] = y.w;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     a[i] = w && s.has_a ? w[s.a + i] : 1.0f;
@@ -214,84 +267,88 @@ template <int N> __device__ __forceinline__ void head_sums(float (&x)[N], uint32
   }
 }
 
-// Heads [first, end) of one token from x to out: the norm of each where
-// `norm`, the turn of its first `rotary` elements where `turned`.  U head rows
-// a lane are loaded before the first is used, the first ones before `angles`
-// works out cos and sin.
-template <typename TI, typename TO, int V, int S, int U, typename Angles>
-__device__ __forceinline__ void run_heads(const TI *x, uint64_t x_stride, TO *out, uint64_t out_stride,
-                                          uint32_t first, uint32_t end, uint32_t lanes, uint32_t sub,
-                                          const Slot (&slot)[S], const float (&wa)[S][V], const float (&wb)[S][V],
-                                          Angles angles, bool norm, bool turned, bool inter, float inv_d, float eps) {
-  const uint32_t per = 32 / lanes;
-  const uint64_t x_step = per * x_stride, out_step = per * out_stride;
-  x += (first + sub) * x_stride;
-  out += (first + sub) * out_stride;
-  Raw<TI, V> ra[U][S], rb[U][S];
-  const auto load = [&](uint32_t h0) {
+// A lane's part of a head: normed (f the norm's factor), turned, rounded.
+template <typename TI, typename TO, int V>
+__device__ __forceinline__ void finish_head(const Raw<TI, V> &ra, const Raw<TI, V> &rb, const Slot &slot, const float (&cos)[V],
+                                            const float (&sin)[V], const float (&wa)[V], const float (&wb)[V], float f, bool norm,
+                                            bool inter, bool there, TO *row) {
+  float a[V], b[V];
+  ra.get(a);
+  rb.get(b);
+  if (norm) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool there = h0 + u * per + sub < end;
-      const TI *row = x + u * x_step;
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        ra[u][s] = rb[u][s] = Raw<TI, V>{};
-        if (there && slot[s].has_a) ra[u][s].load(row + slot[s].a);
-        if (there && slot[s].has_b) rb[u][s].load(row + slot[s].b);
-      }
+    for (int i = 0; i < V; ++i) {
+      a[i] *= f * wa[i];
+      b[i] *= f * wb[i];
     }
-    x += U * x_step;
-  };
-  load(first);
-  float cos[S][V], sin[S][V];
-  angles(cos, sin);
-  for (uint32_t h0 = first; h0 < end; h0 += U * per) {
-    if (h0 != first) load(h0);
-    float r[U];
+  }
+  if (slot.turned) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      // pair i: elements i of both vectors, or neighbours in one
+      float &u = !inter ? a[i] : i < V / 2 ? a[2 * i] : b[2 * i - V], &w = !inter ? b[i] : i < V / 2 ? a[2 * i + 1] : b[2 * i + 1 - V];
+      const float u0 = u, w0 = w;
+      u = fmaf(u0, cos[i], -(w0 * sin[i]));
+      w = fmaf(u0, sin[i], w0 * cos[i]);
+    }
+  }
+  Raw<TO, V> y;
+  if (there && slot.has_a) {
+    y.set(a);
+    y.store(row + slot.a);
+  }
+  if (there && slot.has_b) {
+    y.set(b);
+    y.store(row + slot.b);
+  }
+}
+template <typename T, int V> __device__ __forceinline__ float squares(const Raw<T, V> &ra, const Raw<T, V> &rb) {
+  float a[V], b[V], sum = 0.0f;
+  ra.get(a);
+  rb.get(b);
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
+  return sum;
+}
+
+// One head by single elements, a warp, lane + 32 s the slots of two elements:
+// any size, alignment and type.
+template <typename TI, typename TO>
+__device__ __forceinline__ void scalar_head(const TI *x, TO *out, uint32_t D, uint32_t rotary, const uint64_t *frequencies,
+                                            uint32_t position, float magnitude, const float *weight, bool norm, bool inter,
+                                            float inv_d, float eps) {
+  constexpr int S = TL_HEAD_MAX_DIM / 64;
+  const uint32_t lane = threadIdx.x & 31;
+  float a[S], b[S], sum[1] = {0.0f};
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const Slot slot = slot_of(lane + 32 * s, 1, D, rotary, inter);
+    a[s] = slot.has_a ? element_of(x[slot.a]) : 0.0f;
+    b[s] = slot.has_b ? element_of(x[slot.b]) : 0.0f;
+    sum[0] = fmaf(a[s], a[s], fmaf(b[s], b[s], sum[0]));
+  }
+  float f = 1.0f;
+  if (norm) {
+    head_sums<1>(sum, 32);
+    f = rsqrtf(fmaf(sum[0], inv_d, eps));
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const Slot slot = slot_of(lane + 32 * s, 1, D, rotary, inter);
+    float u = a[s], w = b[s];
     if (norm) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        r[u] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < S; ++s) r[u] += ra[u][s].squares() + rb[u][s].squares();
-      }
-      head_sums<U>(r, lanes);
+      u *= f * (weight && slot.has_a ? weight[slot.a] : 1.0f);
+      w *= f * (weight && slot.has_b ? weight[slot.b] : 1.0f);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool there = h0 + u * per + sub < end;
-      float va[S][V], vb[S][V];
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        ra[u][s].get(va[s]);
-        rb[u][s].get(vb[s]);
-      }
-      if (norm) {
-        const float f = rsqrtf(fmaf(r[u], inv_d, eps));
-#pragma unroll
-        for (int s = 0; s < S; ++s)
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            va[s][i] *= f * wa[s][i];
-            vb[s][i] *= f * wb[s][i];
-          }
-      }
-      TO *row = out + u * out_step;
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        if (turned && slot[s].turned) turn<V>(va[s], vb[s], cos[s], sin[s], inter);
-        Raw<TO, V> y;
-        if (there && slot[s].has_a) {
-          y.set(va[s]);
-          y.store(row + slot[s].a);
-        }
-        if (there && slot[s].has_b) {
-          y.set(vb[s]);
-          y.store(row + slot[s].b);
-        }
-      }
+    if (slot.turned) {
+      float sn, cs;
+      sine_cosine(position * frequencies[lane + 32 * s], sn, cs);
+      const float c = cs * magnitude, n = sn * magnitude, u0 = u;
+      u = fmaf(u, c, -(w * n));
+      w = fmaf(u0, n, w * c);
     }
-    out += U * out_step;
+    if (slot.has_a) set_element(out[slot.a], u);
+    if (slot.has_b) set_element(out[slot.b], w);
   }
 }
 

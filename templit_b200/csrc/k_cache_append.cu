@@ -68,37 +68,45 @@ struct AppendArgs {
   uint32_t *status;
 };
 
-template <typename TI, typename TO, int V, int S>
+// By vectors (V > 1) or by single elements (V = 1, a head at a time).
+template <typename TI, typename TO, int V>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
-  constexpr int U = V == 1 ? 1 : kBatch;
   pdl_enter();
   uint32_t cta = blockIdx.x, which = 0;
   while (which + 1 < a.parts && cta >= a.part[which].ctas) cta -= a.part[which++].ctas;
   const AppendPart &part = a.part[which];
   const tl_paged_cache &c = a.cache;
-  const uint32_t lane = threadIdx.x & 31, lanes = a.lanes, at = lane & (lanes - 1), sub = lane / lanes;
+  const uint32_t lane = threadIdx.x & 31, lanes = a.lanes, at = lane & (lanes - 1), sub = lane / lanes, per = 32 / lanes;
   const uint64_t most = table_keys(c);
   const bool norm = a.norm && part.turned;
-
-  Slot slot[S];
-  float wa[S][V], wb[S][V];
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    slot[s] = heads::slot_of(at + s * lanes, V, c.D, a.rotary, a.interleaved);
-    heads::load_weights<V>(norm ? part.weight : nullptr, slot[s], wa[s], wb[s]);
-  }
   const uint64_t items = static_cast<uint64_t>(c.tokens) * part.chunks;
   const uint64_t warps = static_cast<uint64_t>(part.ctas) * kWarps;
   for (uint64_t item = static_cast<uint64_t>(cta) * kWarps + threadIdx.x / 32; item < items; item += warps) {
     const uint32_t token = static_cast<uint32_t>(item / part.chunks), chunk = static_cast<uint32_t>(item % part.chunks);
+    const uint32_t first = chunk * part.run, end = min(first + part.run, part.heads);
+    const TI *x = static_cast<const TI *>(part.x.p) + token * part.x.row_stride;
+    // the first heads are on their way while the token's place is looked up
+    const uint32_t rotary = part.turned ? a.rotary : 0;
+    const Slot slot = heads::slot_of(at, V, c.D, rotary, a.interleaved);
+    constexpr int W = V > 1 ? V : 4;  // (arrays of the single elements' form are not used)
+    heads::Raw<TI, W> ra[kBatch], rb[kBatch];
+    const auto load = [&](uint32_t h0) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const uint32_t h = h0 + u * per + sub;
+        const TI *row = x + h * part.x.head_stride;
+        ra[u] = rb[u] = heads::Raw<TI, W>{};
+        if (h < end && slot.has_a) ra[u].load(row + slot.a);
+        if (h < end && slot.has_b) rb[u].load(row + slot.b);
+      }
+    };
+    if constexpr (V > 1) load(first);
     const uint32_t s = sequence_at(c, token, lane);
     if (s == 0xffffffffu) continue;
-    const uint32_t start = c.starts[s], end = c.starts[s + 1];
-    if (end <= token) continue;  // behind the last sequence
-    const int64_t position = static_cast<int64_t>(c.lengths[s]) - (end - token);
-    bool ok = end <= c.tokens && start <= token && position >= static_cast<int64_t>(0) &&
-              static_cast<uint64_t>(position) < most &&
-              c.lengths[s] >= end - start;
+    const uint32_t start = c.starts[s], stop = c.starts[s + 1], length = c.lengths[s];
+    if (stop <= token) continue;  // behind the last sequence
+    const int64_t position = static_cast<int64_t>(length) - (stop - token);
+    bool ok = stop <= c.tokens && start <= token && length >= stop - start && static_cast<uint64_t>(position) < most;
     uint32_t page = 0;
     if (ok) {
       page = c.table[static_cast<uint64_t>(s) * c.table_stride + static_cast<uint32_t>(position) / c.page_size];
@@ -108,25 +116,40 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
       if (lane == 0) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
       continue;
     }
-    const TI *x = static_cast<const TI *>(part.x.p) + token * part.x.row_stride;
     TO *out = static_cast<TO *>(part.out);
     out += part.cache ? page * c.page_stride + static_cast<uint32_t>(position) % c.page_size * c.slot_stride
                       : token * part.out_row;
-    heads::run_heads<TI, TO, V, S, U>(x, part.x.head_stride, out, part.out_head, chunk * part.run,
-                                      min((chunk + 1) * part.run, part.heads), lanes, sub, slot, wa, wb,
-                                      [&](float (&cos)[S][V], float (&sin)[S][V]) {
-                                        if (part.turned)
-                                          heads::angles<V, S>(a.frequencies, static_cast<uint32_t>(position), a.magnitude,
-                                                              at, lanes, a.rotary, cos, sin);
-                                      },
-                                      norm, part.turned, a.interleaved, a.inv_d, a.eps);
+    if constexpr (V > 1) {
+      float cos[V], sin[V], wa[V], wb[V];
+      heads::angles<V>(a.frequencies, static_cast<uint32_t>(position), a.magnitude, at, lanes, rotary, cos, sin);
+      if (norm) heads::load_weights<V>(part.weight, slot, wa, wb);
+      for (uint32_t h0 = first; h0 < end; h0 += kBatch * per) {
+        if (h0 != first) load(h0);
+        float r[kBatch];
+        if (norm) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) r[u] = heads::squares(ra[u], rb[u]);
+          heads::head_sums<kBatch>(r, lanes);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const uint32_t h = h0 + u * per + sub;
+          heads::finish_head<TI, TO, V>(ra[u], rb[u], slot, cos, sin, wa, wb, norm ? rsqrtf(fmaf(r[u], a.inv_d, a.eps)) : 1.0f, norm,
+                                        a.interleaved, h < end, out + h * part.out_head);
+        }
+      }
+    } else {
+      for (uint32_t h = first; h < end; ++h)
+        heads::scalar_head<TI, TO>(x + h * part.x.head_stride, out + h * part.out_head, c.D, rotary, a.frequencies,
+                                   static_cast<uint32_t>(position), a.magnitude, part.weight, norm, a.interleaved, a.inv_d, a.eps);
+    }
   }
 }
 
 template <typename TI, typename TO> void launch_append(const AppendArgs &a, bool vectors, unsigned grid, cudaStream_t s) {
   constexpr int V = heads::vector_of(sizeof(TI), sizeof(TO));
-  if (vectors) launch_pdl(append_kernel<TI, TO, V, 1>, grid, kThreads, 0, s, a);
-  else launch_pdl(append_kernel<TI, TO, 1, 4>, grid, kThreads, 0, s, a);
+  if (vectors) launch_pdl(append_kernel<TI, TO, V>, grid, kThreads, 0, s, a);
+  else launch_pdl(append_kernel<TI, TO, 1>, grid, kThreads, 0, s, a);
 }
 
 // One launch for parts [0, a.parts) of one output type.

@@ -47,106 +47,104 @@ int check_view(const char *who, const char *name, const tl_head_view &v, int32_t
 
 namespace {
 
-template <typename TI, typename TO, int V, int S, int U, bool NORM, bool INTER>
+constexpr int kRotateRows = 2;  // head rows of a lane's batch
+
+template <typename TI, typename TO, int V, int U, bool NORM, bool INTER>
 __global__ void __launch_bounds__(kThreads, 4) rotate_kernel(const RotaryArgs a) {
   pdl_enter();
-  const bool inter = V == 1 ? a.interleaved : INTER;
-  const bool norm = V == 1 ? a.norm : NORM;
   const uint32_t lane = threadIdx.x & 31, lanes = a.lanes, at = lane & (lanes - 1), sub = lane / lanes, per = 32 / lanes;
   const uint64_t first_groups = static_cast<uint64_t>(a.tokens) * a.part[0].chunks;
-  const uint64_t groups = first_groups + static_cast<uint64_t>(a.tokens) * a.part[1].chunks;
+  const uint64_t groups = a.whole ? a.tokens : first_groups + static_cast<uint64_t>(a.tokens) * a.part[1].chunks;
   const uint64_t warps = static_cast<uint64_t>(gridDim.x) * kWarps;
-  Slot slot[S];
-#pragma unroll
-  for (int s = 0; s < S; ++s) slot[s] = slot_of(at + s * lanes, V, a.D, a.rotary, inter);
+  const Slot slot = slot_of(at, V, a.D, a.rotary, INTER);
 
-  const auto load = [&](HeadRows<TI, V, S, U> &r, const Batch &s) {
-    const tl_head_view &v = a.part[s.part].x;
-    const uint32_t left = s.end > s.head + sub ? s.end - s.head - sub : 0;
-    r.load(static_cast<const TI *>(v.p) + place(v, s, sub), per * v.head_stride, slot, left, per);
-  };
   Batch s;
   s.group = static_cast<uint64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
   set_batch(a, s, first_groups, groups);
   if (!s.any) return;
-  HeadRows<TI, V, S, U> rows, next_rows;
-  load(rows, s);
-  uint64_t turned = ~0ull;  // the group whose angles are in cos and sin
-  uint32_t part = 2;        // whose weights are in wa and wb
-  float cos[S][V], sin[S][V], wa[S][V], wb[S][V];
-  while (true) {
+  const TI *x = static_cast<const TI *>(a.part[s.part].x.p) + place(a.part[s.part].x, s, sub);
+  uint64_t x_step = per * a.part[s.part].x.head_stride;
+  const auto left_of = [&](const Batch &s) { return s.end > s.head + sub ? s.end - s.head - sub : 0u; };
+  HeadRows<TI, V, U> even, odd;
+  even.clear();
+  odd.clear();
+  even.load(x, x_step, slot, left_of(s), per);
+  uint64_t turned = ~0ull;  // the token whose angles are in cos and sin
+  uint64_t of = ~0ull;      // the run that wa, wb and out are for
+  float cos[V], sin[V], wa[V], wb[V];
+  TO *out = nullptr;
+  uint64_t out_step = 0;
+  // one batch from `rows`, the next one into `next`; false behind the last
+  const auto work = [&](const HeadRows<TI, V, U> &rows, HeadRows<TI, V, U> &next) {
     Batch n = s;
-    next_batch(a, n, U * per, warps, first_groups, groups);
-    if (n.any) load(next_rows, n);
-    if (s.part != part) {
-      part = s.part;
-#pragma unroll
-      for (int i = 0; i < S; ++i) load_weights<V>(norm ? a.part[part].weight : nullptr, slot[i], wa[i], wb[i]);
+    if (next_batch(a, n, U * per, warps, first_groups, groups)) {
+      x += U * x_step;
+    } else if (n.any) {
+      x = static_cast<const TI *>(a.part[n.part].x.p) + place(a.part[n.part].x, n, sub);
+      x_step = per * a.part[n.part].x.head_stride;
     }
-    if (s.group != turned) {
-      turned = s.group;
-      angles<V, S>(a.frequencies, s.position, a.magnitude, at, lanes, a.rotary, cos, sin);
+    if (n.any) next.load(x, x_step, slot, left_of(n), per);
+    if (2 * s.group + s.part != of) {
+      of = 2 * s.group + s.part;
+      const RotaryPart &part = a.part[s.part];
+      if (s.token != turned) {
+        turned = s.token;
+        angles<V>(a.frequencies, s.position, a.magnitude, at, lanes, a.rotary, cos, sin);
+      }
+      if (NORM) load_weights<V>(part.weight, slot, wa, wb);
+      out = static_cast<TO *>(const_cast<void *>(part.out.p)) + place(part.out, s, sub);
+      out_step = per * part.out.head_stride;
     }
     float r[U];
-    if (norm) {
+    if (NORM) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        r[u] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < S; ++i) r[u] += rows.a[u][i].squares() + rows.b[u][i].squares();
-      }
+      for (int u = 0; u < U; ++u) r[u] = squares(rows.a[u], rows.b[u]);
       head_sums<U>(r, lanes);
     }
-    const tl_head_view &v = a.part[s.part].out;
-    TO *out = static_cast<TO *>(const_cast<void *>(v.p)) + place(v, s, sub);
-    const uint32_t left = s.end > s.head + sub ? s.end - s.head - sub : 0;
+    const uint32_t left = left_of(s);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int i = 0; i < S; ++i) {
-        float va[V], vb[V];
-        rows.a[u][i].get(va);
-        rows.b[u][i].get(vb);
-        if (norm) {
-          const float f = rsqrtf(fmaf(r[u], a.inv_d, a.eps));
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            va[e] *= f * wa[i][e];
-            vb[e] *= f * wb[i][e];
-          }
-        }
-        if (slot[i].turned) turn<V>(va, vb, cos[i], sin[i], inter);
-        Raw<TO, V> y;
-        if (u * per < left && slot[i].has_a) {
-          y.set(va);
-          y.store(out + u * (per * v.head_stride) + slot[i].a);
-        }
-        if (u * per < left && slot[i].has_b) {
-          y.set(vb);
-          y.store(out + u * (per * v.head_stride) + slot[i].b);
-        }
-      }
-    }
-    if (!n.any) return;
+    for (int u = 0; u < U; ++u)
+      finish_head<TI, TO, V>(rows.a[u], rows.b[u], slot, cos, sin, wa, wb, NORM ? rsqrtf(fmaf(r[u], a.inv_d, a.eps)) : 1.0f, NORM, INTER,
+                             u * per < left, out + u * out_step);
+    out += U * out_step;
     s = n;
-    rows = next_rows;
+    return n.any;
+  };
+  while (work(even, odd) && work(odd, even)) {
+  }
+}
+
+// A warp a head, by single elements.
+template <typename TI, typename TO> __global__ void __launch_bounds__(kThreads) rotate_elements_kernel(const RotaryArgs a) {
+  pdl_enter();
+  const uint64_t heads = a.part[0].heads + static_cast<uint64_t>(a.part[1].heads), items = a.tokens * heads;
+  const uint64_t warps = static_cast<uint64_t>(gridDim.x) * kWarps;
+  for (uint64_t item = static_cast<uint64_t>(blockIdx.x) * kWarps + threadIdx.x / 32; item < items; item += warps) {
+    const uint32_t token = static_cast<uint32_t>(item / heads), b = token / a.T, t = token - b * a.T;
+    uint32_t h = static_cast<uint32_t>(item - token * heads);
+    const RotaryPart &p = a.part[h >= a.part[0].heads];
+    if (h >= a.part[0].heads) h -= a.part[0].heads;
+    const TI *x = static_cast<const TI *>(p.x.p) + b * p.x.batch_stride + t * p.x.row_stride + h * p.x.head_stride;
+    TO *out = static_cast<TO *>(const_cast<void *>(p.out.p)) + b * p.out.batch_stride + t * p.out.row_stride + h * p.out.head_stride;
+    scalar_head<TI, TO>(x, out, a.D, a.rotary, a.frequencies, a.positions ? a.positions[token] : a.first_position + t,
+                        a.magnitude, p.weight, a.norm, a.interleaved, a.inv_d, a.eps);
   }
 }
 
 template <typename TI, typename TO> void launch_rotate(RotaryArgs &a, cudaStream_t s) {
-  constexpr int V = vector_of(sizeof(TI), sizeof(TO)), U = V == 8 ? 2 : 3;
+  constexpr int V = vector_of(sizeof(TI), sizeof(TO)), U = kRotateRows;
   if (!a.vectors) {
-    const unsigned grid = share_out(a, 1, false);
-    launch_pdl(rotate_kernel<TI, TO, 1, 4, 1, false, false>, grid, kThreads, 0, s, a);
+    const uint64_t heads = a.part[0].heads + static_cast<uint64_t>(a.part[1].heads);
+    launch_pdl(rotate_elements_kernel<TI, TO>, grid_for(a.tokens * heads, kWarps, 16), kThreads, 0, s, a);
     return;
   }
-  const unsigned grid = share_out(a, U, false);
+  const unsigned grid = share_out(a, U, kMaxCtas, false);
   if (a.norm) {
-    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, 1, U, true, true>, grid, kThreads, 0, s, a);
-    else launch_pdl(rotate_kernel<TI, TO, V, 1, U, true, false>, grid, kThreads, 0, s, a);
+    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, U, true, true>, grid, kThreads, 0, s, a);
+    else launch_pdl(rotate_kernel<TI, TO, V, U, true, false>, grid, kThreads, 0, s, a);
   } else {
-    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, 1, U, false, true>, grid, kThreads, 0, s, a);
-    else launch_pdl(rotate_kernel<TI, TO, V, 1, U, false, false>, grid, kThreads, 0, s, a);
+    if (a.interleaved) launch_pdl(rotate_kernel<TI, TO, V, U, false, true>, grid, kThreads, 0, s, a);
+    else launch_pdl(rotate_kernel<TI, TO, V, U, false, false>, grid, kThreads, 0, s, a);
   }
 }
 
@@ -213,7 +211,7 @@ int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryA
   return TL_OK;
 }
 
-unsigned share_out(RotaryArgs &a, uint32_t rows, bool apart) {
+unsigned share_out(RotaryArgs &a, uint32_t rows, uint32_t most, bool apart) {
   // A warp's run of a token's heads: all of them where the tokens alone keep two warps a
   // scheduler busy, shorter where they do not.
   const uint32_t per = 32 / a.lanes * rows, wanted = kNumSMs * 8;
@@ -229,14 +227,16 @@ unsigned share_out(RotaryArgs &a, uint32_t rows, bool apart) {
     groups += static_cast<uint64_t>(a.tokens) * p.chunks;
   }
   const auto fewest = [](uint64_t x, uint64_t y) { return static_cast<uint32_t>(x < y ? x : y); };
-  if (!apart) return fewest((groups + kWarps - 1) / kWarps, kMaxCtas);
+  a.whole = !apart && a.part[0].chunks <= 1 && a.part[1].chunks <= 1;
+  if (a.whole) groups = a.tokens;
+  if (!apart) return fewest((groups + kWarps - 1) / kWarps, most);
   const uint64_t heads = a.part[0].heads + static_cast<uint64_t>(a.part[1].heads);
-  uint32_t left = kMaxCtas;
+  uint32_t left = most;
   for (RotaryPart &p : a.part) {
     if (!p.heads) continue;
     const bool last = &p == &a.part[1] || !a.part[1].heads;
-    uint64_t share = last ? left : kMaxCtas * static_cast<uint64_t>(p.heads) / heads;
-    share = share < 1 ? 1 : share > kMaxCtas - 1 ? kMaxCtas - 1 : share;
+    uint64_t share = last ? left : most * static_cast<uint64_t>(p.heads) / heads;
+    share = share < 1 ? 1 : share > most - 1 ? most - 1 : share;
     p.ctas = fewest((static_cast<uint64_t>(a.tokens) * p.chunks + kWarps - 1) / kWarps, share);
     left -= p.ctas;
   }
