@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotate_kernel(const RotaryArgs a)
   HeadRows<TI, V, U> even, odd;
   even.clear();
   odd.clear();
-  even.load(x, x_step, slot, left_of(s), per);
+  even.template load<false>(x, x_step, slot, left_of(s), per);
   uint64_t turned = ~0ull;  // the token whose angles are in cos and sin
   uint64_t of = ~0ull;      // the run that wa, wb and out are for
   float cos[V], sin[V], wa[V], wb[V];
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotate_kernel(const RotaryArgs a)
       x = static_cast<const TI *>(a.part[n.part].x.p) + place(a.part[n.part].x, n, sub);
       x_step = per * a.part[n.part].x.head_stride;
     }
-    if (n.any) next.load(x, x_step, slot, left_of(n), per);
+    if (n.any) next.template load<false>(x, x_step, slot, left_of(n), per);
     if (2 * s.group + s.part != of) {
       of = 2 * s.group + s.part;
       const RotaryPart &part = a.part[s.part];

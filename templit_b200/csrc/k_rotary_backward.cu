@@ -60,8 +60,8 @@ __global__ void __launch_bounds__(kThreads, NORM ? kNormCtas : 4) rotate_backwar
     if (NORM) x = static_cast<const TI *>(part.x.p) + place(part.x, n, sub);
   };
   const auto load = [&](Rows &r, const Batch &n) {
-    r.g.load(g, g_step, slot, left_of(n), per);
-    if (NORM) r.x.load(x, x_step, slot, left_of(n), per);
+    r.g.template load<NORM>(g, g_step, slot, left_of(n), per);
+    if (NORM) r.x.template load<true>(x, x_step, slot, left_of(n), per);
   };
   Rows even, odd;
   even.g.clear();

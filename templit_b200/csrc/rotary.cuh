@@ -83,11 +83,12 @@ template <typename T, int V, int U> struct HeadRows {
 #pragma unroll
     for (int u = 0; u < U; ++u) a[u] = b[u] = Raw<T, V>{};
   }
-  // rows `step` apart; `left` heads, `per` at a time, are there (the others keep what
-  // they held, which goes nowhere)
-  __device__ __forceinline__ void load(const T *x, uint64_t step, const Slot &slot, uint32_t left, uint32_t per) {
+  // Rows `step` apart; `left` heads, `per` at a time, are there.  The others are 0
+  // (EMPTY: they add to sums over heads) or keep what they held, which goes nowhere.
+  template <bool EMPTY> __device__ __forceinline__ void load(const T *x, uint64_t step, const Slot &slot, uint32_t left, uint32_t per) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (EMPTY) a[u] = b[u] = Raw<T, V>{};
       if (u * per < left && slot.has_a) a[u].load(x + u * step + slot.a);
       if (u * per < left && slot.has_b) b[u].load(x + u * step + slot.b);
     }

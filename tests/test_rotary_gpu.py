@@ -263,10 +263,12 @@ def test_nan_stays_in_its_head(dev):
     assert bad[0, 2, 1].all() and bad.sum() == 64
 
 
-@pytest.mark.parametrize("B,T,hq,hk,D", [(4, 700, 12, 3, 128), (1, 5000, 1, 1, 64)])
-def test_many_tokens(dev, B, T, hq, hk, D):
-    """More work than one round of the grid: weight gradients over all of it."""
-    c = Case(dev, B, T, hq, hk, D, D, "bf16", norm=True)
+@pytest.mark.parametrize("B,T,hq,hk,D", [(4, 700, 12, 3, 128), (1, 5000, 1, 1, 64), (1, 4000, 13, 5, 128), (2, 3001, 9, 7, 96),
+                                         (1, 3500, 21, 10, 40)])
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+def test_many_tokens(dev, B, T, hq, hk, D, type):
+    """More work than one round of the grid, heads that do not fill a warp's last batch: weight gradients over all of it."""
+    c = Case(dev, B, T, hq, hk, D, D, type, norm=True)
     c.forward()
     c.backward()
 
