@@ -814,7 +814,7 @@ int tl_cache_append(const tl_cache_append_desc *desc, void *stream);
 typedef struct tl_paged_attention_desc {
   tl_paged_cache cache;
   tl_head_view q;       /* [tokens, q_heads, D] of the cache's type       */
-  tl_head_view out;     /* the same of out_type                           */
+  tl_head_view out;     /* the same of out_type; does not overlap q       */
   uint32_t q_heads;     /* a multiple of cache.heads: query head h reads
                            key head h / (q_heads / heads)                 */
   int32_t out_type;     /* the cache's type or TL_FLOAT32                 */

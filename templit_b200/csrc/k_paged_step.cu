@@ -376,10 +376,12 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
         const uint32_t row = (lane + 32 * i) / CH, ch = (lane + 32 * i) % CH;
         const int64_t place = __shfl_sync(0xffffffffu, from, row);
         const bool there = place >= 0 && ch * E < c.D;
-        const uint64_t e = there ? place + ch * E : 0;
+        // (a copy of nothing gets an address that exists too)
+        const T *const k_from = there ? kp + place + ch * E : static_cast<const T *>(a.q.p);
+        const T *const v_from = there ? vp + place + ch * E : static_cast<const T *>(a.q.p);
         const uint32_t spot = to + L::spot(row, ch);
-        copy16(spot, kp + e, there);
-        copy16(spot + kHalf, vp + e, there);
+        copy16(spot, k_from, there);
+        copy16(spot + kHalf, v_from, there);
       }
     };
     unsigned good[kStages];  // a bit for every key that is there
@@ -436,14 +438,18 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
 #pragma unroll
       for (int e = 0; e < DP / 32; ++e) nan = nan || (lane + 32 * e < c.D && acc[e] != acc[e]);
       if (uneven && ll == ll && __any_sync(0xffffffffu, nan)) {
-        // A value that other rows of the tile see, and this one does not, is not
+        // Where a value that other rows of the tile see, and this one does not, is not
         // finite (0 times it is NaN): the row's own keys one by one.
-        float again[kMaxHead / 32];
+        const uint32_t lo = max(all_from, w.block_lo * KEYS);
         seen(a, w.length, w.position(a, row), f, t);
-        const T *q = static_cast<const T *>(a.q.p) + token * a.q.row_stride + h * a.q.head_stride;
-        row_over_keys<T>(a, w.sequence, head, q, max(f, w.block_lo * KEYS), min(t, key_hi), lane, mm, ll, again);
+        if (any_infinite<T>(a, w.sequence, head, lo, min(f, key_hi), lane) ||
+            any_infinite<T>(a, w.sequence, head, max(t, lo), key_hi, lane)) {
+          float again[kMaxHead / 32];
+          const T *q = static_cast<const T *>(a.q.p) + token * a.q.row_stride + h * a.q.head_stride;
+          row_over_keys<T>(a, w.sequence, head, q, max(f, lo), min(t, key_hi), lane, mm, ll, again);
 #pragma unroll
-        for (int e = 0; e < DP / 32; ++e) acc[e] = again[e];
+          for (int e = 0; e < DP / 32; ++e) acc[e] = again[e];
+        }
       }
       if (w.opens && w.ends) {
         TO *out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;

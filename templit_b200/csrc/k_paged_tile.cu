@@ -331,7 +331,7 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Maps &maps, S
             const uint32_t row = (lane + 32 * i) / CH, ch = (lane + 32 * i) % CH;
             const int64_t from = __shfl_sync(0xffffffffu, at, row);
             const bool put = from >= 0 && ch * 8 < c.D;
-            copy16(to + spot(row, ch), base + (put ? from + ch * 8 : 0), put);
+            copy16(to + spot(row, ch), put ? base + from + ch * 8 : static_cast<const T *>(a.q.p), put);
           }
           by_rows |= 1u << (item & 31);
         }
@@ -467,22 +467,6 @@ __device__ __forceinline__ void multiply(const AttentionArgs &a, Shared &sh, uin
     item += 2 * most;
   }
   if (item) ptx::mma_commit(&sh.b.empty[item / 2 % kPairs]);
-}
-
-// Whether a value of the keys [from, to) is not finite, by a warp.
-template <typename T>
-__device__ __forceinline__ bool any_infinite(const AttentionArgs &a, uint32_t s, uint32_t head, uint32_t from, uint32_t to, uint32_t lane) {
-  const T *v = static_cast<const T *>(a.cache.v) + head * a.cache.head_stride;
-  bool found = false;
-  for (uint32_t j = from; j < to && !found; ++j) {
-    const int64_t at = key_offset(a, s, j);
-    for (uint32_t d = lane; at >= 0 && d < a.cache.D; d += 32) {
-      const float x = heads::element_of(v[at + d]);
-      found = found || x - x != 0.0f;
-    }
-    found = __any_sync(0xffffffffu, found);
-  }
-  return found;
 }
 
 // A warp's 32 rows of the output, 128 bytes of each at a time through its 4 KB
@@ -782,6 +766,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
   } else if (warp < 12) {
     load<T, DP>(a, maps, sh, queries, ring);
     await<0>();
+    if (*reinterpret_cast<volatile uint32_t *>(&sh.gave_up)) {
+      // TMA's copies may be on their way to this CTA's shared memory
+      const uint64_t t0 = ptx::global_timer_ns();
+      while (ptx::global_timer_ns() - t0 < 1000000) {
+      }
+    }
   } else if (warp == 12) {
     if (elect()) {
       multiply<T, DP>(a, sh, queries, ring);

@@ -102,6 +102,22 @@ __device__ __forceinline__ void row_over_keys(const AttentionArgs &a, uint32_t s
   }
 }
 
+// Whether a value of the keys [from, to) is not finite, by a warp.
+template <typename T>
+__device__ __forceinline__ bool any_infinite(const AttentionArgs &a, uint32_t s, uint32_t head, uint32_t from, uint32_t to, uint32_t lane) {
+  const T *v = static_cast<const T *>(a.cache.v) + head * a.cache.head_stride;
+  bool found = false;
+  for (uint32_t j = from; j < to && !found; ++j) {
+    const int64_t at = key_offset(a, s, j);
+    for (uint32_t d = lane; at >= 0 && d < a.cache.D; d += 32) {
+      const float x = heads::element_of(v[at + d]);
+      found = found || x - x != 0.0f;
+    }
+    found = __any_sync(0xffffffffu, found);
+  }
+  return found;
+}
+
 // How the work is shared out.  A job is one key head's query rows of one
 // sequence, `ROWS` rows at most (a tile; token by token, the group's heads of
 // a token side by side), over the keys that they see, in blocks of `KEYS`.

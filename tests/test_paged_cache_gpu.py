@@ -209,6 +209,49 @@ def test_long_chunks(dev, type, hq, hk, D, batch):
     check(dev, c, attend(dev, c, hq, sharp=2.0))
 
 
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hk,D,page", [(160, 1, 64, 16), (300, 2, 64, 24), (96, 3, 40, 8), (256, 2, 128, 32), (10, 10, 16, 40)])
+def test_many_heads_a_key_head(dev, type, hq, hk, D, page):
+    c = Cache(dev, [(3, 70), (1, 1), (17, 200)], hk, D, page, type)
+    check(dev, c, attend(dev, c, hq))
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_many_sequences(dev, type):
+    """More sequences than threads of a CTA, most of them short or empty, with and without hints."""
+    rng = np.random.default_rng(11)
+    batch = [(int(n), int(n + k)) for n, k in zip(rng.integers(0, 4, 1100), rng.integers(0, 40, 1100))]
+    batch[700] = (30, 900)
+    c = Cache(dev, batch, 1, 8, 8, type)
+    for kw in ({}, dict(max_length=900, max_new=30), dict(max_length=900, max_new=4)):
+        check(dev, c, attend(dev, c, 2, **kw))
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_cache_without_pages(dev, type, new):
+    """No page at all: no key is there, whatever the table says."""
+    c = Cache(dev, [(new, 50)], 2, 64, 16, type)
+    s = attend(dev, c, 4, prepare_only=True)
+    s["d"].cache.pages, s["d"].cache.k, s["d"].cache.v = 0, None, None
+    capi.check(dev.lib.tl_paged_attention(ctypes.byref(s["d"]), dev.stream), dev.lib)
+    dev.torch.cuda.synchronize()
+    assert (s["out"] == 0).all() and dev.torch.isneginf(s["lse"]).all()
+    assert dev.status() == capi.TL_FLAG_INDEX_RANGE
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [3, 200])
+def test_values_not_finite_that_all_rows_see(dev, type, new):
+    c = Cache(dev, [(new, 3000)], 1, 64, 16, type)
+    page, slot = c.places(0, 5, 6)
+    c.v[page, slot] = float("nan")
+    c.vals[0][5] = float("nan")
+    s = attend(dev, c, 4)
+    dev.torch.cuda.synchronize()
+    assert dev.torch.isnan(s["out"].float()).all() and dev.torch.isfinite(s["lse"]).all()
+
+
 @pytest.mark.parametrize("type", ["f16", "bf16"])
 def test_window_in_long_chunks(dev, type):
     for window in (1, 100, 128, 129, 500):
