@@ -46,7 +46,10 @@ int attention_args(const char *who, const tl_paged_attention_desc *d, AttentionA
 }
 
 // Many rows a key head go to the tensor cores' tiles (16-bit types; a scale
-// that is not positive would turn the order of the scores round there).
+// that is not positive would turn the order of the scores round there): more than the
+// 16 that read a sequence's keys once in the other kernel.  64 sequences of 8191 keys,
+// 8 key heads of 128 bf16: 16 rows take 429 us there and 382 in the other, 20 rows 424
+// and 708, 256 rows 586 and 4933.  (One sequence of them: 20 rows 44 us and 36.)
 bool tiled(const tl_paged_attention_desc *d, const AttentionArgs &a, uint32_t max_new) {
   return a.cache.type != TL_FLOAT32 && d->scale > 0.0f && static_cast<uint64_t>(max_new) * a.group > 16;
 }
@@ -69,7 +72,7 @@ size_t tl_paged_attention_workspace_size(const tl_paged_attention_desc *d) {
   bool nothing = false;
   if (attention_args("tl_paged_attention_workspace_size", d, a, &nothing) || nothing) return 0;
   const uint32_t n = most_new(d);
-  return plan_bytes(tiled(d, a, n) ? tile_plan(a, n) : step_plan(a, n));
+  return plan_bytes(tiled(d, a, n) ? tile_plan(a) : step_plan(a, n));
 }
 
 int tl_paged_attention(const tl_paged_attention_desc *d, void *stream) {
@@ -81,7 +84,7 @@ int tl_paged_attention(const tl_paged_attention_desc *d, void *stream) {
   if (nothing) return TL_OK;
   const uint32_t n = most_new(d);
   const bool tiles = tiled(d, a, n);
-  const Plan p = tiles ? tile_plan(a, n) : step_plan(a, n);
+  const Plan p = tiles ? tile_plan(a) : step_plan(a, n);
   const uint64_t bytes = plan_bytes(p);
   if (bytes) {
     if (!d->workspace || d->workspace_bytes < bytes) return fail(TL_ERR_INVALID, w + "workspace too small");

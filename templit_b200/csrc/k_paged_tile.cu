@@ -536,6 +536,9 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
     // rows behind the last one see everything: their scores go nowhere
     uint32_t from = 0, to = 0xffffffffu;
     if (there) seen(a, p.length, p.position(a, in_job), from, to);
+    // A warp without rows only passes its tile's turns on (what TMEM holds goes through
+    // the products to outputs that nobody reads).
+    const bool idle = t * kTile + (row & ~31u) > p.last;
     float m = -INFINITY, l = 0.0f;
     for (uint32_t j = 0; j < n; ++j) {
       // By halves of 64 keys, each with its scores' buffer; one copy of the code, which
@@ -543,6 +546,10 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
 #pragma unroll 1
       for (uint32_t h = 0; h < 2; ++h) {
         if (!wait_warp(sh, &sh.b.s_full[t][h], done & 1, a.status)) return;
+        if (idle) {
+          if (lane == 0) ptx::mbar_arrive(&sh.b.p_full[t][h]);
+          continue;
+        }
         ptx::tc_fence_after();
         const uint32_t key = (p.block_lo + j) * kKeys + h * 64, at = s_at + h * 64;
         const uint32_t *good = &sh.mask[(block_count + j) % kMasks][2 * h];
@@ -657,6 +664,13 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
       ++outputs;
       ptx::tc_fence_after();
     }
+    if (idle) {
+      if (lane == 0) {
+        if (n) ptx::mbar_arrive(&sh.b.o_free[t]);
+        release_job(sh, i_job);
+      }
+      continue;
+    }
     const uint32_t place = p.row0 + in_job, in_sequence = place / a.group;
     const uint64_t token = p.start + in_sequence;
     const uint32_t h = p.head * a.group + (place - in_sequence * a.group);
@@ -757,9 +771,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
     ptx::tmem_relinquish();
   }
   pdl_enter();
-  if (!a.whole && threadIdx.x == 13 * 32) a.joins[blockIdx.x] = Join{0xffffffffu, 0, 0, 0};
+  if (threadIdx.x == 13 * 32) a.joins[blockIdx.x] = Join{0xffffffffu, 0, 0, 0};
   ptx::tc_fence_before();
-  const Share share = share_of<kRows, kKeys, kThreads>(a, blockIdx.x, gridDim.x, a.whole ? 1 : 2 * kKeys);
+  const Share share = share_of<kRows, kKeys, kThreads>(a, blockIdx.x, gridDim.x, 2 * kKeys);
   ptx::tc_fence_after();
   if (warp < 8) {
     soften<T, TO, DP>(a, sh, staging);
@@ -827,15 +841,13 @@ template <typename T, typename TO, int DP> void launch(const AttentionArgs &a, c
   constexpr size_t smem = smem_bytes<DP>();
   (void)cudaFuncSetAttribute(tile_kernel<T, TO, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   launch_pdl(tile_kernel<T, TO, DP>, p.ctas, kThreads, smem, s, a, make_maps(a));
-  if (!p.whole) launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, kRows / 16), 128, 0, s, a);
+  launch_pdl(join_kernel<TO, kRows, DP>, dim3(p.ctas, kRows / 16), 128, 0, s, a);
 }
 
 }  // namespace
 
-Plan tile_plan(const AttentionArgs &a, uint32_t max_new) {
+Plan tile_plan(const AttentionArgs &a) {
   Plan p{};
-  (void)max_new;
-  p.whole = 0;
   p.ctas = kNumSMs;
   p.part_floats = kRows * (a.cache.D > 64 ? 128 : 64) + 2 * kRows;
   return p;

@@ -123,15 +123,16 @@ __device__ __forceinline__ bool any_infinite(const AttentionArgs &a, uint32_t s,
 // a token side by side), over the keys that they see, in blocks of `KEYS`.
 // The jobs lie in one line, sequence by sequence, tile by tile, head by head, each
 // as long as its keys (for causal tiles an even slope, at least what they see)
-// and kJob blocks more, about what starting and ending a job costs: with
-// shares of keys alone, 64 sequences of 16 to 8191 keys took 139 us where some
-// CTAs met many short ones.  The line is cut into equal shares; a share that starts or ends
+// and kJob more, about what starting and ending a job costs.  With 1, 2, 3, 5 and 8
+// blocks, 64 sequences of 16 to 8191 keys and a new token each took 148, 126, 112, 105
+// and 108 us, 8192 tokens of one prompt 893, 736, 609, 570 and 588, 24 chunks 113, 91,
+// 87, 89 and 95.  The line is cut into equal shares; a share that starts or ends
 // inside a job leaves a partial result (numerators' sum, maximum and sum of
 // the softmax), and join_kernel adds those up in the order of the keys.
 // Every CTA works its share out by itself from the lengths on the device, so
 // that a captured call follows them.
 template <uint32_t ROWS, uint32_t KEYS> struct Work {
-  static constexpr uint64_t kJob = 3 * KEYS;
+  static constexpr uint64_t kJob = 5 * KEYS;
   Sequence q;
   uint64_t tiles;
   uint64_t base, slope;  // line of tile t: base + slope t, for each head
@@ -306,14 +307,16 @@ template <uint32_t ROWS, int DP> constexpr uint32_t part_floats() { return ROWS 
 // The jobs that were cut, each where it ends: the partial results of a row are
 // added up in the order of the keys, a lane DP / 32 neighbouring elements.  Large
 // tiles are cut in two or three: a warp takes four rows, all their loads under
-// way at once (one row after another took 22 us for 147 joins of 256 rows).
+// way at once (one row after another took 22 us for 147 joins of 256 rows, so 15).
 // Small ones may be cut in many: four warps share a row's parts (37 parts of 8 jobs
-// of 4 rows: 40 us by one warp).
+// of 4 rows: 40 us by one warp, so 8).  The factors of 32 parts are worked out first, a
+// lane each, so that no load of outputs waits for one (19 parts of 8 jobs of 20 rows:
+// 33 us where each part's factor came before its outputs, so 15).
 template <typename TO, uint32_t ROWS, int DP>
 __global__ void __launch_bounds__(128) join_kernel(const AttentionArgs a) {
   constexpr bool kShare = ROWS <= 16;
   constexpr int R = kShare ? 1 : 4, E = DP / 32;
-  __shared__ float sums[kShare ? 4 : 1][DP + 1];
+  __shared__ float sums[kShare ? 4 : 1][DP];
   pdl_enter();
   const Join j = a.joins[blockIdx.x];
   if (j.first == 0xffffffffu) return;
@@ -339,37 +342,49 @@ __global__ void __launch_bounds__(128) join_kernel(const AttentionArgs a) {
       if (r0 + r < rows) mm[r] = fmaxf(mm[r], part(i)[ROWS * DP + r0 + r]);
 #pragma unroll
   for (int r = 0; r < R; ++r) mm[r] = warp_max(mm[r]);
-#pragma unroll 4
-  for (uint32_t i = j.first + (kShare ? warp : 0); i <= end; i += kShare ? 4 : 1) {
-    const float *const p = part(i);
+  // 32 parts at a time: their factors, a lane each, then their outputs
+  constexpr uint32_t kStep = kShare ? 4 : 1;
+  for (uint32_t i0 = j.first; i0 <= end; i0 += 32) {
+    const uint32_t i = i0 + lane, n = min(32u, end - i0 + 1);
+    float f[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (r0 + r >= rows) continue;
-      const uint32_t row = r0 + r;
-      const float wm = p[ROWS * DP + row], f = wm == -INFINITY ? 0.0f : ex2_approx(wm - mm[r]);
-      ll[r] = fmaf(f, p[ROWS * DP + ROWS + row], ll[r]);
-      float x[E];
-      if constexpr (E == 4) {
-        const float4 y = *reinterpret_cast<const float4 *>(p + row * DP + lane * E);
-        x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-      } else {
-        const float2 y = *reinterpret_cast<const float2 *>(p + row * DP + lane * E);
-        x[0] = y.x, x[1] = y.y;
-      }
+      f[r] = 0.0f;
+      if (r0 + r >= rows || i > end) continue;
+      const float wm = part(i)[ROWS * DP + r0 + r], wl = part(i)[ROWS * DP + ROWS + r0 + r];
+      f[r] = wm == -INFINITY ? 0.0f : ex2_approx(wm - mm[r]);
+      ll[r] = fmaf(f[r], wl, ll[r]);
+    }
+#pragma unroll 4
+    for (uint32_t k = kShare ? warp : 0; k < n; k += kStep) {
+      const float *const p = part(i0 + k);
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (f != 0.0f) acc[r][e] = fmaf(f, x[e], acc[r][e]);
+      for (int r = 0; r < R; ++r) {
+        const float by = __shfl_sync(0xffffffffu, f[r], k);
+        float x[E] = {};
+        if (r0 + r < rows) {
+          if constexpr (E == 4) {
+            const float4 y = *reinterpret_cast<const float4 *>(p + (r0 + r) * DP + lane * E);
+            x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+          } else {
+            const float2 y = *reinterpret_cast<const float2 *>(p + (r0 + r) * DP + lane * E);
+            x[0] = y.x, x[1] = y.y;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[r][e] = by != 0.0f ? fmaf(by, x[e], acc[r][e]) : acc[r][e];
+      }
     }
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r) ll[r] = warp_sum(ll[r]);
   if constexpr (kShare) {
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[0][e];
-    if (lane == 0) sums[warp][DP] = ll[0];
     __syncthreads();
     if (warp) return;
 #pragma unroll
     for (int w = 1; w < 4; ++w) {
-      ll[0] += sums[w][DP];
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[0][e] += sums[w][lane * E + e];
     }
@@ -409,7 +424,7 @@ inline uint64_t most_jobs(const AttentionArgs &a, uint32_t rows) {
 
 Plan step_plan(const AttentionArgs &a, uint32_t max_new);
 void launch_step(const AttentionArgs &a, const Plan &p, bool wide, cudaStream_t s);
-Plan tile_plan(const AttentionArgs &a, uint32_t max_new);
+Plan tile_plan(const AttentionArgs &a);
 void launch_tile(const AttentionArgs &a, const Plan &p, bool wide, cudaStream_t s);
 
 }  // namespace paged
