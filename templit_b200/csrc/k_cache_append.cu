@@ -5,6 +5,8 @@
 // Bound by memory, and by latency where there are few tokens: a warp finds its
 // token's sequence (one or two rounds of 32 starts), position and page, and
 // takes a run of the token's query, key or value heads, as in k_rotary.cu.
+// 64 tokens, one a sequence, 32 query and 8 key heads of 128 bf16: 7 us, a launch and that
+// chain of lookups; 24 chunks of up to 509 tokens: 22 us (4.6 TB/s).
 #include "paged_cache.cuh"
 
 #include <cmath>

@@ -1,14 +1,14 @@
 // Attention over a paged cache for many query rows a key head (chunks of a
 // prompt) in 16-bit types (include/templit_cuda.h: tl_paged_attention).
 //
-// Bound by the tensor cores and the softmax's exponentials: 128 x 128 scores
-// of 128 elements are 512 cycles of each product and 1024 of the 16
-// exponentials a cycle of an SM.  So a CTA, one an SM, holds two tiles of 128
+// Bound by the softmax's exponentials and the tensor cores: 128 x 128 scores of
+// 128 elements are 1024 cycles of the 16 exponentials a cycle of an SM and 512 of
+// each product.  So a CTA, one an SM, holds two tiles of 128
 // query rows (tokens, a token's heads of one key head side by side), and
 // while one is in the softmax the other is multiplied:
-//   warps 0-3, 4-7  softmax of tile 0 and 1, a row a thread: scores out of
-//                   TMEM, numerators rounded to the type back into the same
-//                   TMEM columns, where the second product takes them from;
+//   warps 0-3, 4-7  softmax of tile 0 and 1, a row a thread, 64 keys at a time: scores
+//                   out of TMEM, numerators rounded to the type back over them,
+//                   where the second product takes them from;
 //                   running maximum and sum in registers.  The output stays
 //                   in TMEM and is rescaled only when a row's maximum grew
 //                   by more than 2^8 (numerators then are at most 2^8, which
@@ -19,13 +19,26 @@
 //                   16 bytes a lane, which writes zeros for the keys that are
 //                   not there (3600 cycles of a warp for a block, more than its
 //                   products take; TMA's boxes are a few instructions)
-//   warp 13         one thread works out the CTA's pieces of jobs, ahead of the others
 //   warp 12         one thread issues S = Q K^T and O += P V (tcgen05.mma
 //                   kind::f16, fp32 in TMEM)
-// TMEM: 2 x 128 columns of scores (numerators over their second half), 2 x
-// 128 of outputs.  Every wait is bounded (2 s); where one gives up, the CTA
-// raises TL_FLAG_TIMEOUT, waits for what it issued and returns.  Shares of
-// the keys and their joining: paged_attention.cuh.
+//   warp 13         one thread works out the CTA's pieces of jobs, ahead of the others
+//   warps 14, 15    nothing (without them the compiler gives a thread 144 registers in
+//                   place of 128, and the prompt below took 556 us in place of 546)
+// TMEM: 2 x 2 buffers of 64 columns of scores, 2 x 128 of outputs.  With two buffers a
+// tile, the next scores are multiplied while the last ones are in the softmax; one of 128
+// leaves each waiting for the other (710 us where this takes 580), although scores of 64
+// keys take 48 cycles of a product of 32 (of 128 keys 64).  Every wait is bounded
+// (2 s); where one gives up, the CTA raises TL_FLAG_TIMEOUT, waits for what it issued
+// and returns.  Shares of the keys and their joining: paged_attention.cuh.
+//
+// 8192 tokens of one prompt, 8 key heads of 128 bf16, 4 query heads each, causal: 580 us,
+// 960 TFLOP/s of the 1650 of a large library product.  Both tiles' softmax warps share the
+// schedulers, two a scheduler: 2700 cycles for 2 x 128 x 128 scores, of which
+// the exponentials alone are 2048; the products are 2560.  A polynomial for some of the
+// exponentials gained nothing: the instructions that are issued then bound it.  A job's
+// end, 256 rows out of TMEM, is 8500 cycles more.  24 chunks of up to 509 tokens, 3 query
+// heads of 64 a key head, behind up to 4093 keys: 80 us; jobs are short there, their ends
+// and ragged first and last tiles are half of it.
 #include "paged_attention.cuh"
 #include "tc_ptx.cuh"
 

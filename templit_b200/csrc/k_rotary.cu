@@ -8,6 +8,10 @@
 // Bound by memory: every element is read once and written once.  A warp takes
 // one token (its angles are worked out once, shared by the lanes) and a run of
 // its heads, some side by side.
+//
+// 12288 x 12 heads of 64 fp32, rotation alone: 17 us (75 MB, 4.5 TB/s).  16384 x 40 heads of
+// 128 bf16, norm and rotation: 68 us (336 MB, 4.9 TB/s), where the instructions of an element
+// (issue 58 %) and loads share the time; 64 tokens of it 7 us, a launch.
 #include "rotary.cuh"
 
 #include <cmath>

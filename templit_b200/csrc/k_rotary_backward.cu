@@ -7,6 +7,10 @@
 // stays on the SMs; a CTA adds its heads' weight gradients up in registers,
 // then in shared memory, and leaves one row, which a second kernel sums over
 // the CTAs in a fixed order.
+//
+// 16384 x 40 heads of 128 bf16: 117 us (503 MB, 4.3 TB/s); the registers of the norm's sums
+// leave 12 warps an SM, whose instructions (issue 46 to 58 %) and loads share the time.  The
+// rotation alone, a quarter of each head turned, 16384 x 40 heads: 62 us.
 #include "rotary.cuh"
 
 namespace tl {
