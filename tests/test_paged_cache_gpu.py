@@ -145,7 +145,7 @@ def check(dev, c, s, causal=1, window=0):
         ok = np.isfinite(wlse)
         lerr = ds + longs + 2 * U * np.abs(wlse)
         off = np.abs(lse[at][ok] - wlse[ok])
-    assert (off <= lerr[ok]).all(), (i, off.max())
+        assert (off <= lerr[ok]).all(), (i, off.max())
     # rows of no sequence are as they were
     assert (out[~seen] == GUARD).all() and (lse[~seen] == GUARD).all()
     assert dev.status() == 0
