@@ -31,10 +31,11 @@
 // (2 s); where one gives up, the CTA raises TL_FLAG_TIMEOUT, waits for what it issued
 // and returns.  Shares of the keys and their joining: paged_attention.cuh.
 //
-// 8192 tokens of one prompt, 8 key heads of 128 bf16, 4 query heads each, causal: 580 us,
-// 960 TFLOP/s of the 1650 of a large library product.  Both tiles' softmax warps share the
+// 8192 tokens of one prompt, 8 key heads of 128 bf16, 4 query heads each, causal: 546 to
+// 580 us, 1000 TFLOP/s of the 1650 of a large library product; the tensor cores and the unit
+// for 2^x are half busy each.  Both tiles' softmax warps share the
 // schedulers, two a scheduler: 2700 cycles for 2 x 128 x 128 scores, of which
-// the exponentials alone are 2048; the products are 2560.  A polynomial for some of the
+// the exponentials alone are 2048; the products are 2560, and hand-overs come between.  A polynomial for some of the
 // exponentials gained nothing: the instructions that are issued then bound it.  A job's
 // end, 256 rows out of TMEM, is 8500 cycles more.  24 chunks of up to 509 tokens, 3 query
 // heads of 64 a key head, behind up to 4093 keys: 80 us; jobs are short there, their ends
