@@ -842,7 +842,9 @@ Maps make_maps(const AttentionArgs &a) {
     const cuuint32_t box[4] = {64, rows, 1, 1};
     if (encode(&m.k, c.type, c.k, 4, dims, strides, box) && encode(&m.v, c.type, c.v, 4, dims, strides, box)) m.rows = rows;
   }
-  if (a.group <= kTile && (a.group & (a.group - 1)) == 0) {
+  // (heads or tokens that lie on one another, broadcast queries, are copied row by row)
+  const bool apart = (a.q_heads == 1 || a.q.head_stride >= c.D) && (c.tokens == 1 || a.q.row_stride >= c.D);
+  if (apart && a.group <= kTile && (a.group & (a.group - 1)) == 0) {
     const cuuint64_t dims[3] = {c.D, a.q_heads, c.tokens};
     const uint64_t strides[2] = {a.q_heads > 1 ? a.q.head_stride : c.D * 2u, c.tokens > 1 ? a.q.row_stride : c.D * 2u};
     const cuuint32_t box[3] = {64, a.group, kTile / a.group};

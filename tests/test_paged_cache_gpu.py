@@ -378,6 +378,21 @@ def test_bad_pages_and_lengths(dev, type, new):
             assert (s["out"][2 * new:] == GUARD).all()
 
 
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("batch", [[(1, 70), (2, 5)], [(140, 200), (3, 64)]])
+@pytest.mark.parametrize("how", ["heads", "tokens", "both", "overlapping"])
+def test_broadcast_queries(dev, type, batch, how):
+    c = Cache(dev, batch, 2, 64, 16, type, seed=3)
+    shape = (1 if how in ("tokens", "both") else c.tokens, 1 if how in ("heads", "both") else 8, 64)
+    t = dev.torch
+    if how == "overlapping":  # a head starts 8 elements behind the one before, a token 16
+        q = t.from_numpy(c.rng.standard_normal(16 * c.tokens + 128)).to(dev.dev).to(torch_type(dev, type))
+        q = q.as_strided((c.tokens, 8, 64), (16, 8, 1))
+    else:
+        q = t.from_numpy(c.rng.standard_normal(shape)).to(dev.dev).to(torch_type(dev, type)).expand(c.tokens, 8, 64)
+    check(dev, c, attend(dev, c, 8, q=q))
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 def test_two_streams_at_once(dev, type):
     torch = dev.torch
