@@ -732,7 +732,7 @@ typedef struct tl_rotary_part {
 typedef struct tl_rotary_desc {
   uint32_t B, T, D;    /* D <= TL_HEAD_MAX_DIM                            */
   uint32_t rotary_dim; /* even, <= D; the elements behind it are not turned */
-  int32_t type, out_type; /* tl_float_type                                */
+  int32_t type, out_type; /* tl_float_type; not fp16 and bf16             */
   int32_t layout;      /* tl_rotary_layout                                */
   int32_t norm;        /* 1: y = x / sqrt(mean(x^2) + eps) * weight first */
   float eps;           /* >= 0, finite; 1e-6 in tl_rmsnorm_rows           */
@@ -807,7 +807,8 @@ typedef struct tl_cache_append_desc {
  * their queries alike into q_out, in one launch.  A token whose position would
  * be negative (more new tokens than keys) or behind the table, or whose page
  * id is out of range, is not written and raises TL_FLAG_INDEX_RANGE.  Two
- * tokens must not share a place in the cache.
+ * tokens must not share a place in the cache.  Rows of fp16 go into a bf16 cache
+ * and the reverse; q_out is of the cache's type there (TL_ERR_UNSUPPORTED).
  */
 int tl_cache_append(const tl_cache_append_desc *desc, void *stream);
 

@@ -175,7 +175,9 @@ int append(const char *who, AppendArgs a, int32_t type, int32_t out_type, bool a
     grid += p.ctas;
   }
 #define L(TI, TO) launch_append<TI, TO>(a, shape.vectors, grid, s)
-  TL_BY_TYPES(type, out_type, L)
+  if (type == TL_FLOAT16 && out_type == TL_BFLOAT16) L(__half, __nv_bfloat16);
+  else if (type == TL_BFLOAT16 && out_type == TL_FLOAT16) L(__nv_bfloat16, __half);
+  else TL_BY_TYPES(type, out_type, L)
 #undef L
   return launch_status(who);
 }
@@ -198,8 +200,10 @@ extern "C" int tl_cache_append(const tl_cache_append_desc *d, void *stream) {
   bool cache_aligned = false;
   if (int rc = check_cache(who, a.cache, &cache_aligned)) return rc;
   const tl_paged_cache &c = a.cache;
-  if (heads::mixed_halves(d->type, c.type) || (d->q_heads && heads::mixed_halves(d->type, d->q_out_type)))
-    return fail(TL_ERR_UNSUPPORTED, w + "fp16 and bf16 in one call");
+  // rows of one 16-bit type into a cache of the other, their queries to the type that the
+  // attention over it reads; other mixtures have no reader
+  if (d->q_heads && d->q_out_type != c.type && (heads::mixed_halves(d->type, c.type) || heads::mixed_halves(d->type, d->q_out_type)))
+    return fail(TL_ERR_UNSUPPORTED, w + "fp16 and bf16 in one call with q_out of another type than the cache");
   if (int rc = heads::check_turn(who, c.D, d->rotary_dim, d->layout, d->norm, d->eps, d->magnitude, d->frequencies))
     return rc;
   if (!c.tokens || !c.sequences) return TL_OK;
