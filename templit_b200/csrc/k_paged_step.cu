@@ -432,7 +432,8 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) {
         const float wm = sm_m[i][row];
-        if (wm == -INFINITY) continue;
+        // (a maximum passes NaN by: scores of nothing else leave it at -inf, their sum is NaN)
+        if (wm == -INFINITY && sm_l[i][row] == 0.0f) continue;
         const float f = ex2_approx(wm - mm);
         ll = fmaf(f, sm_l[i][row], ll);
 #pragma unroll

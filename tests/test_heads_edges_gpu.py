@@ -23,6 +23,38 @@ def dev():
     return Dev()
 
 
+# ------------------------------------------------------- NaN that a row sees
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("batch", [[(1, 1), (1, 60)], [(1, 5003), (2, 900)], [(40, 90), (1, 3)], [(40, 5003), (20, 20)]],
+                         ids=["steps", "cut_steps", "chunks", "cut_chunks"])
+def test_nan_queries(dev, type, batch):
+    """One NaN in a query makes all of that row's scores NaN, and its result, not the row of a token without keys."""
+    c = Cache(dev, batch, 2, 64, 16, type)
+    q = dev.torch.from_numpy(c.rng.standard_normal((c.tokens, 6, 64))).to(dev.dev).to(torch_type(dev, type))
+    q[0, 1, 5] = float("nan")
+    q[-1, 4, 63] = float("nan")
+    s = attend(dev, c, 6, q=q)
+    check(dev, c, s)
+    lse = s["lse"].cpu().numpy()
+    assert np.isnan(lse[0, 1]) and np.isnan(lse[-1, 4]) and np.isnan(lse).sum() == 2
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new,keys,bad", [(1, 1, 0), (1, 9, 8), (1, 17, 16), (2, 65, 63), (1, 65, 64), (1, 5003, 5002), (1, 4500, 2100),
+                                          (40, 40, 0), (40, 129, 128), (40, 5003, 5002), (40, 5003, 100)])
+def test_a_nan_key(dev, type, new, keys, bad):
+    """A NaN key reaches every row that sees it, alone in its warp's keys or not."""
+    c = Cache(dev, [(new, keys)], 1, 64, 16, type)
+    page, slot = c.places(0, bad, bad + 1)
+    c.k[page, slot] = float("nan")
+    c.keys[0][bad] = float("nan")
+    s = attend(dev, c, 3)
+    check(dev, c, s)
+    sees = np.arange(keys - new, keys) >= bad
+    assert (np.isnan(s["lse"].cpu().numpy()) == sees[:, None]).all()
+
+
 # --------------------------------------------------------------------- writer
 
 @pytest.mark.parametrize("type,cache_type", [("f16", "bf16"), ("bf16", "f16")])
