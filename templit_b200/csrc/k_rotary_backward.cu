@@ -121,7 +121,9 @@ __global__ void __launch_bounds__(kThreads, NORM ? kNormCtas : 4) rotate_backwar
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (NORM) {
-        const float r = rsqrtf(fmaf(both[2 * u], a.inv_d, a.eps)), dot = -(both[2 * u + 1] * r * a.inv_d) * r;
+        float r = rsqrtf(fmaf(both[2 * u], a.inv_d, a.eps));
+        if (s.head + sub + u * per >= s.end) r = 0.0f;  // not there: the norm of its zeros is none without an eps
+        const float dot = -(both[2 * u + 1] * r * a.inv_d) * r;
         const Pair r2 = pair(r, r), dot2 = pair(dot, dot);
         Pair va[V / 2], vb[V / 2];
         get_pairs(rows.x.a[u], va);

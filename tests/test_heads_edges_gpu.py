@@ -55,6 +55,36 @@ def test_a_nan_key(dev, type, new, keys, bad):
     assert (np.isnan(s["lse"].cpu().numpy()) == sees[:, None]).all()
 
 
+# ---------------------------------------------- the norm's gradient without eps
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads", [(3, 1), (6, 6), (13, 5)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("offset", [0, 1])  # vectors, single elements
+@pytest.mark.parametrize("T", [5, 1500])
+def test_norm_gradient_without_eps(dev, type, heads, D, offset, T):
+    """Heads that a warp's last batch lacks add nothing to the weights' gradients, with eps = 0 too."""
+    c = Case(dev, 2, T, *heads, D, D, type, norm=True, offset=offset)
+    c.d.eps = 0.0
+    ws = dev.ws(dev.lib.tl_rotary_heads_workspace_size(ctypes.byref(c.d)))
+    c.d.workspace, c.d.workspace_bytes = ws.data_ptr(), ws.numel()
+    dxs = []
+    for part, x, *_ in c.parts:
+        dxs.append(x.like())
+        part.dx = dxs[-1].c()
+    capi.check(dev.lib.tl_rotary_heads_backward(ctypes.byref(c.d), dev.stream), dev.lib)
+    for (part, x, g, w, dw), dx in zip(c.parts, dxs):
+        wh = w.double().cpu().numpy()
+        want, dweight = ops.heads_gradient(x.host, g.host, c.at, c.radians, False, c.mag, True, wh, eps=0.0)
+        size = pair_size(g.host, len(c.radians), False, c.mag)
+        rms = np.sqrt((x.host ** 2).mean(-1, keepdims=True))
+        y, t = np.abs(x.host / rms), size * np.abs(wh)
+        err = (t + 3 * y * (t * y).mean(-1, keepdims=True)) / rms * 2 * NORM + np.abs(want) * 1.01 * ROUND[type] + TINY[type]
+        assert (np.abs(dx.get() - want) <= err).all()
+        n, total = want[..., 0].size, (size * y).reshape(-1, D).sum(0)
+        assert (np.abs(dw.double().cpu().numpy() - dweight) <= total * (2 * NORM + (n / 32 + 64) * U)).all()
+
+
 # --------------------------------------------------------------------- writer
 
 @pytest.mark.parametrize("type,cache_type", [("f16", "bf16"), ("bf16", "f16")])
