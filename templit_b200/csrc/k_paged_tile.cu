@@ -78,6 +78,8 @@ struct Shared {
   Barriers b;
   Job jobs[kJobs];
   uint32_t tmem, gave_up;
+  uint32_t not_finite;  // rows may ask for mend_rows()
+  Share share;
   uint32_t mask[kMasks][4];  // a bit for every key of a block that is there
 };
 template <int DP> constexpr size_t smem_bytes() {
@@ -709,41 +711,60 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
         part[kRows * DP + kRows + in_job] = l;
       }
     }
-    // NaN from finite sums: where a value that other rows of the tile see, and this one
-    // does not, is not finite (0 times it is NaN), the row's own keys one by one.
-    unsigned rows = __ballot_sync(0xffffffffu, there && nan && l == l);
-    const uint32_t lo = p.block_lo * kKeys, hi = (p.block_lo + n) * kKeys;
-    while (rows) {
-      const int r = __ffs(rows) - 1;
-      rows &= rows - 1;
-      const uint32_t r_from = __shfl_sync(0xffffffffu, from, r), r_to = __shfl_sync(0xffffffffu, to, r);
-      if (!any_infinite<T>(a, p.sequence, p.head, max(lo, p.from), min(r_from, min(hi, p.to)), lane) &&
-          !any_infinite<T>(a, p.sequence, p.head, max(r_to, max(lo, p.from)), min(hi, p.to), lane))
+    if (there && nan && l == l) *reinterpret_cast<volatile uint32_t *>(&sh.not_finite) = 1;
+    __syncwarp();
+    if (lane == 0) release_job(sh, i_job);
+  }
+}
+
+// NaN from finite sums: where a value that other rows of the tile see, and this one does
+// not, is not finite (0 times it is NaN), the row's own keys one by one.  By all warps of the
+// CTA when its pieces are done: a row of 200000 keys takes tens of milliseconds, for which
+// no wait of the pipeline is made.
+template <typename T, typename TO, int DP> __device__ __forceinline__ void mend_rows(const AttentionArgs &a, const Share &share) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, D = a.cache.D;
+  Walk<kRows, kKeys> walk;
+  Piece p;
+  walk.start(a, share);
+  while (walk.next(a, share, p)) {
+    const bool complete = p.opens && p.ends;
+    float *const part = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (p.opens ? 1 : 0)) * part_floats<kRows, DP>();
+    for (uint32_t row = warp; row <= p.last; row += kThreads / 32) {
+      const uint32_t lo = max(p.block_lo * kKeys, p.from);
+      const uint32_t hi = min((p.block_lo + tile_blocks(a, p, row / kTile)) * kKeys, p.to);
+      uint32_t from, to;
+      seen(a, p.length, p.position(a, row), from, to);
+      if (lo >= hi || (from <= lo && to >= hi)) continue;
+      const uint32_t place = p.row0 + row, h = p.head * a.group + place % a.group;
+      const uint64_t token = p.start + static_cast<uint64_t>(place / a.group);
+      TO *const out = static_cast<TO *>(const_cast<void *>(a.out.p)) + token * a.out.row_stride + h * a.out.head_stride;
+      bool nan = false;
+      for (uint32_t d = lane; d < D; d += 32) {
+        const float y = complete ? heads::element_of(out[d]) : part[row * DP + d];
+        nan = nan || y != y;
+      }
+      if (!__any_sync(0xffffffffu, nan)) continue;
+      if (!any_infinite<T>(a, p.sequence, p.head, lo, min(from, hi), lane) &&
+          !any_infinite<T>(a, p.sequence, p.head, max(to, lo), hi, lane))
         continue;
-      const uint32_t r_job = __shfl_sync(0xffffffffu, in_job, r);
-      const uint32_t r_place = p.row0 + r_job, r_h = p.head * a.group + r_place % a.group;
-      const uint64_t r_token = p.start + r_place / a.group;
-      float acc[kMaxHead / 32], rm, rl;
-      const T *q = static_cast<const T *>(a.q.p) + r_token * a.q.row_stride + r_h * a.q.head_stride;
-      row_over_keys<T>(a, p.sequence, p.head, q, max(r_from, lo), min(r_to, min(hi, p.to)), lane, rm, rl, acc);
-      TO *const r_out = static_cast<TO *>(const_cast<void *>(a.out.p)) + r_token * a.out.row_stride + r_h * a.out.head_stride;
+      float acc[kMaxHead / 32], m, l;
+      const T *q = static_cast<const T *>(a.q.p) + token * a.q.row_stride + h * a.q.head_stride;
+      row_over_keys<T>(a, p.sequence, p.head, q, max(from, lo), min(to, hi), lane, m, l, acc);
       __syncwarp();
 #pragma unroll
       for (int e = 0; e < static_cast<int>(kMaxHead) / 32; ++e) {
-        if (lane + 32 * e >= cache.D) continue;
-        if (complete) heads::set_element(r_out[lane + 32 * e], rl == 0.0f ? 0.0f : acc[e] / rl);
-        else part[r_job * DP + lane + 32 * e] = acc[e];
+        if (lane + 32 * e >= D) continue;
+        if (complete) heads::set_element(out[lane + 32 * e], l == 0.0f ? 0.0f : acc[e] / l);
+        else part[row * DP + lane + 32 * e] = acc[e];
       }
       if (lane == 0) {
-        if (complete) put_lse<TO>(a, r_token, r_h, rm, rl);
+        if (complete) put_lse<TO>(a, token, h, m, l);
         else {
-          part[kRows * DP + r_job] = rm;
-          part[kRows * DP + kRows + r_job] = rl;
+          part[kRows * DP + row] = m;
+          part[kRows * DP + kRows + row] = l;
         }
       }
     }
-    __syncwarp();
-    if (lane == 0) release_job(sh, i_job);
   }
 }
 
@@ -778,6 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
     }
     ptx::mbar_init(&sh.b.drained, 1);
     sh.gave_up = 0;
+    sh.not_finite = 0;
     ptx::fence_barrier_init();
   }
   if (warp == 12) {
@@ -788,6 +810,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
   if (threadIdx.x == 13 * 32) a.joins[blockIdx.x] = Join{0xffffffffu, 0, 0, 0};
   ptx::tc_fence_before();
   const Share share = share_of<kRows, kKeys, kThreads>(a, blockIdx.x, gridDim.x, 2 * kKeys);
+  if (threadIdx.x == 0) sh.share = share;  // for mend_rows, behind the last barrier
   ptx::tc_fence_after();
   if (warp < 8) {
     soften<T, TO, DP>(a, sh, staging);
@@ -815,6 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const AttentionArgs a
   __syncthreads();
   ptx::tc_fence_after();
   if (warp == 12) ptx::tmem_dealloc(sh.tmem, 512);
+  if (sh.not_finite && !sh.gave_up) mend_rows<T, TO, DP>(a, sh.share);
 }
 
 bool encode(CUtensorMap *map, int32_t type, const void *base, uint32_t rank, const cuuint64_t *dims, const uint64_t *strides,

@@ -55,6 +55,53 @@ def test_a_nan_key(dev, type, new, keys, bad):
     assert (np.isnan(s["lse"].cpu().numpy()) == sees[:, None]).all()
 
 
+# --------------------------------- values that are not finite, of later tokens
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("out_type", [None, "f32"])
+@pytest.mark.parametrize("window", [0, 50])
+def test_unseen_values_in_many_sequences(dev, type, out_type, window):
+    """Several pieces a CTA, cut and whole, with rows that do not see a value that is not finite."""
+    rng = np.random.default_rng(4)
+    batch = [(int(n), int(n + k)) for n, k in zip(rng.integers(20, 90, 160), rng.integers(0, 900, 160))]
+    batch[3] = (50, 30000)
+    c = Cache(dev, batch, 2, 64, 16, type)
+    for i, (new, keys) in enumerate(batch):
+        for bad, back in ((np.nan, 1), (np.inf, 7), (-np.inf, new), (np.nan, new + 60)):
+            if rng.random() < 0.5 and 0 <= keys - back:
+                page, slot = c.places(i, keys - back, keys - back + 1)
+                c.v[page, slot, :, 5 + back % 40] = float(bad)
+                c.vals[i][keys - back, :, 5 + back % 40] = bad
+    check(dev, c, attend(dev, c, 4, 1, window, out_type), 1, window)
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_unseen_values_in_long_caches(dev, type):
+    """Hundreds of thousands of keys a row, of rows that all have to be worked out again: nothing gives up."""
+    t, n, new, keys, D = dev.torch, 300, 40, 200003, 64
+    c = Cache(dev, [(new, keys)], 1, D, 64, type)
+    page, slot = c.places(0, keys - 1, keys)
+    c.v[page, slot] = float("inf")
+    c.vals[0][keys - 1] = np.inf
+    # every sequence reads the same pages
+    c.table, c.tokens, c.batch = np.repeat(c.table, n, 0), n * new, [(new, keys)] * n
+    c.c_table, c.c_starts, c.c_lengths = (dev.t(x, np.uint32) for x in (c.table, np.arange(n + 1) * new, np.full(n, keys)))
+    q = t.from_numpy(c.rng.standard_normal((new, 1, D))).to(dev.dev).to(torch_type(dev, type)).repeat(n, 1, 1)
+    s = attend(dev, c, 1, q=q)
+    got, lse = (s[x].double().cpu().numpy().reshape(n, new, -1) for x in ("out", "lse"))
+    assert dev.status() == 0
+    q = q[:new].double().cpu().numpy()
+    want, wlse, size = ops.attention(q, c.keys[0], c.vals[0], s["d"].scale)
+    products = s["d"].scale * (np.abs(q) * np.abs(c.keys[0]).max(0)).sum(-1)
+    ds, longs = products * (D * U + 3 * U), 2.0 ** -20 + (keys / 64 + 64) * U
+    with np.errstate(invalid="ignore"):
+        err = (size * (2 * ds + longs + ROUND[type])[..., None] + np.abs(want) * ROUND[type] + TINY[type])[:, 0]
+        worst = (np.abs(got - want[:, 0]) / err)[:, :-1]
+    assert worst.max() <= 1, worst.max()
+    assert (got[:, -1] == np.inf).all()
+    assert (np.abs(lse - wlse) <= ds + longs + 2 * U * np.abs(wlse)).all()
+
+
 # ---------------------------------------------- the norm's gradient without eps
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
