@@ -431,11 +431,11 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
       for (int e = 0; e < DP / 32; ++e) acc[e] = 0.0f;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) {
-        const float wm = sm_m[i][row];
-        // (a maximum passes NaN by: scores of nothing else leave it at -inf, their sum is NaN)
-        if (wm == -INFINITY && sm_l[i][row] == 0.0f) continue;
-        const float f = ex2_approx(wm - mm);
-        ll = fmaf(f, sm_l[i][row], ll);
+        // nothing seen: a sum of 0 (a maximum passes NaN by: of nothing else it is -inf too)
+        const float wl = sm_l[i][row];
+        if (wl == 0.0f) continue;
+        const float f = ex2_approx(sm_m[i][row] - mm);
+        ll = fmaf(f, wl, ll);
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) acc[e] = fmaf(f, outs[(i * kRows + row) * DP + lane + 32 * e], acc[e]);
       }

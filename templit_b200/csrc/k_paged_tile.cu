@@ -719,8 +719,8 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
 
 // NaN from finite sums: where a value that other rows of the tile see, and this one does
 // not, is not finite (0 times it is NaN), the row's own keys one by one.  By all warps of the
-// CTA when its pieces are done: a row of 200000 keys takes tens of milliseconds, for which
-// no wait of the pipeline is made.
+// CTA when its pieces are done: a row of 200003 keys takes 0.1 s, for which no wait of the
+// pipeline is made (300 sequences of 40 such rows 872 ms, without infinite values 4.3).
 template <typename T, typename TO, int DP> __device__ __forceinline__ void mend_rows(const AttentionArgs &a, const Share &share) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, D = a.cache.D;
   Walk<kRows, kKeys> walk;

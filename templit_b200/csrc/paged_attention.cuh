@@ -78,16 +78,7 @@ __device__ __forceinline__ void row_over_keys(const AttentionArgs &a, uint32_t s
     float x = -INFINITY;
     if (at >= 0) {
       x = 0.0f;
-      for (uint32_t d = 0; d < c.D; d += 8) {
-        heads::Raw<T, 8> rq, rk;
-        float fq[8], fk[8];
-        rq.load(q + d);
-        rk.load(k + at + d);
-        rq.get(fq);
-        rk.get(fk);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x = fmaf(fq[i], fk[i], x);
-      }
+      for (uint32_t d = 0; d < c.D; ++d) x = fmaf(heads::element_of(q[d]), heads::element_of(k[at + d]), x);
       x *= scale;
     }
     float top = x;
@@ -99,14 +90,14 @@ __device__ __forceinline__ void row_over_keys(const AttentionArgs &a, uint32_t s
     m = to_m;
 #pragma unroll
     for (int i = 0; i < static_cast<int>(kMaxHead) / 32; ++i) acc[i] *= f;
-#pragma unroll 8
-    for (uint32_t i = 0; i < 32; ++i) {
+    for (uint32_t i = 0; i < 32 && j0 + i < to; ++i) {
       const float w = __shfl_sync(0xffffffffu, p, i);
-      const int64_t place = __shfl_sync(0xffffffffu, x == -INFINITY ? -1 : at, i);
-      // (w is 0 where nothing is loaded)
+      const int64_t place = __shfl_sync(0xffffffffu, at, i);
+      const float score = __shfl_sync(0xffffffffu, x, i);
+      if (place < 0 || score == -INFINITY) continue;
 #pragma unroll
       for (int e = 0; e < static_cast<int>(kMaxHead) / 32; ++e)
-        acc[e] = fmaf(w, place >= 0 && lane + 32 * e < c.D ? heads::element_of(v[place + lane + 32 * e]) : 0.0f, acc[e]);
+        if (lane + 32 * e < c.D) acc[e] = fmaf(w, heads::element_of(v[place + lane + 32 * e]), acc[e]);
     }
   }
 }
