@@ -150,7 +150,7 @@ template <uint32_t ROWS, uint32_t KEYS> struct Work {
     if (a.window) base = min(base, static_cast<uint64_t>(a.window) + step + KEYS);
     else if (a.causal) {
       slope = step;
-      base = (q.length > q.count ? q.length - q.count : 0) + step;
+      base = (q.total > q.count ? min(q.total - q.count, q.length) : 0) + step;
     }
     base += kJob;
   }
@@ -267,7 +267,7 @@ template <uint32_t ROWS, uint32_t KEYS> struct Walk {
       p.row0 = static_cast<uint32_t>(lo) * ROWS;
       p.last = min(ROWS, w.q.count * a.group - p.row0) - 1;
       p.length = w.q.length;
-      p.position0 = static_cast<int64_t>(w.q.length) - w.q.count;
+      p.position0 = static_cast<int64_t>(w.q.total) - w.q.count;
       uint32_t unused;
       seen(a, w.q.length, p.position(a, 0), p.from, unused);
       seen(a, w.q.length, p.position(a, p.last), unused, p.to);

@@ -17,11 +17,12 @@ int check_cache(const char *who, tl_paged_cache &c, bool *aligned);
 struct Sequence {
   uint32_t start, count;  // rows of its new tokens
   uint32_t length;        // keys
+  uint32_t total;         // keys before they were clipped, which the positions go by
   bool bad;               // something was clipped
 };
 __device__ __forceinline__ Sequence sequence_of(const tl_paged_cache &c, uint32_t s, uint64_t most) {
   const uint32_t start = c.starts[s], end = c.starts[s + 1], length = c.lengths[s];
-  Sequence q{start, end - start, length, false};
+  Sequence q{start, end - start, length, length, false};
   if (end < start || end > c.tokens) {
     q.bad = true;
     q.count = 0;

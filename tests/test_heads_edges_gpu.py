@@ -132,6 +132,33 @@ def test_norm_gradient_without_eps(dev, type, heads, D, offset, T):
         assert (np.abs(dw.double().cpu().numpy() - dweight) <= total * (2 * NORM + (n / 32 + 64) * U)).all()
 
 
+# ------------------------------------------------------ sequences that are cut
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new,keys,cut", [(1, 100, 90), (3, 100, 98), (3, 100, 90), (40, 100, 80), (200, 300, 150), (3, 5000, 4999)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_cut_sequences_keep_their_positions(dev, type, new, keys, cut, window):
+    """The keys behind max_length are not there; the tokens' positions are as they were."""
+    c = Cache(dev, [(new, keys), (1, 30)], 2, 64, 16, type)
+    s = attend(dev, c, 4, 1, window, max_length=cut)
+    dev.torch.cuda.synchronize()
+    assert dev.status() == capi.TL_FLAG_INDEX_RANGE
+    q, out, lse = (s[n].double().cpu().numpy() for n in ("q", "out", "lse"))
+    for i in range(new):
+        p = keys - new + i
+        b = min(p + 1, cut)
+        a = min(max(0, p + 1 - window), b) if window else 0
+        want, wlse, size = (x[0] for x in ops.attention(q[i:i + 1], c.keys[0][a:b], c.vals[0][a:b], s["d"].scale, causal=False))
+        most = np.abs(c.keys[0]).max(0).repeat(2, 0)  # a key head for two query heads
+        ds = s["d"].scale * (np.abs(q[i]) * most).sum(-1) * (64 * U + 3 * U)
+        longs = 2.0 ** -20 + (keys / 64 + 64) * U
+        err = size * (2 * ds + longs + (0 if type == "f32" else ROUND[type]))[:, None] + np.abs(want) * ROUND[type] + TINY[type]
+        assert (np.abs(out[i] - want) <= err).all(), i
+        none = np.isneginf(wlse)
+        assert (np.isneginf(lse[i]) == none).all() and (out[i][none] == 0).all()
+        assert (np.abs(lse[i][~none] - wlse[~none]) <= (ds + longs + 2 * U * np.abs(wlse))[~none]).all(), i
+
+
 # --------------------------------------------------------------------- writer
 
 @pytest.mark.parametrize("type,cache_type", [("f16", "bf16"), ("bf16", "f16")])
