@@ -64,6 +64,7 @@ struct AppendArgs {
   tl_paged_cache cache;
   AppendPart part[3];  // queries, keys, values
   uint32_t parts, rotary, lanes;
+  uint32_t checks;  // CTAs behind the parts' that look the sequences over
   bool interleaved, norm;
   float eps, inv_d, magnitude;
   const uint64_t *frequencies;
@@ -74,12 +75,18 @@ struct AppendArgs {
 template <typename TI, typename TO, int V>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
   pdl_enter();
+  const tl_paged_cache &c = a.cache;
+  const uint64_t most = table_keys(c);
   uint32_t cta = blockIdx.x, which = 0;
+  if (cta >= gridDim.x - a.checks) {
+    // also sequences that no row leads to
+    for (uint32_t s = (gridDim.x - 1 - cta) * kThreads + threadIdx.x; s < c.sequences; s += a.checks * kThreads)
+      if (sequence_of(c, s, most).bad) raise_flag(a.status, TL_FLAG_INDEX_RANGE);
+    return;
+  }
   while (which + 1 < a.parts && cta >= a.part[which].ctas) cta -= a.part[which++].ctas;
   const AppendPart &part = a.part[which];
-  const tl_paged_cache &c = a.cache;
   const uint32_t lane = threadIdx.x & 31, lanes = a.lanes, at = lane & (lanes - 1), sub = lane / lanes, per = 32 / lanes;
-  const uint64_t most = table_keys(c);
   const bool norm = a.norm && part.turned;
   const uint64_t items = static_cast<uint64_t>(c.tokens) * part.chunks;
   const uint64_t warps = static_cast<uint64_t>(part.ctas) * kWarps;
@@ -174,6 +181,8 @@ int append(const char *who, AppendArgs a, int32_t type, int32_t out_type, bool a
     p.ctas = static_cast<uint32_t>(ctas < kNumSMs * 256ull ? ctas : kNumSMs * 256ull);
     grid += p.ctas;
   }
+  a.checks = a.cache.sequences / 1024 + 1 < kNumSMs ? a.cache.sequences / 1024 + 1 : kNumSMs;
+  grid += a.checks;
 #define L(TI, TO) launch_append<TI, TO>(a, shape.vectors, grid, s)
   if (type == TL_FLOAT16 && out_type == TL_BFLOAT16) L(__half, __nv_bfloat16);
   else if (type == TL_BFLOAT16 && out_type == TL_FLOAT16) L(__nv_bfloat16, __half);

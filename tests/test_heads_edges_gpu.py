@@ -173,3 +173,25 @@ def test_append_to_the_other_16_bit_type(dev, type, cache_type, D, rotary, inter
         s = append(dev, c, 5, rotary, type, None, interleaved, norm, pad, queries=queries)
         check_append(dev, c, s, k, v, queries=queries)
         assert dev.status() == 0
+
+
+@pytest.mark.parametrize("what", ["backwards", "behind", "all_behind", "length", "empty_length"])
+def test_append_raises_the_flag_for_every_bad_sequence(dev, what):
+    """Also for those that no row of the call leads to; the others are written."""
+    c = Cache(dev, [(3, 50)] if what == "backwards" else [(2, 40), (0, 30), (3, 50)], 2, 64, 16, "bf16", extra=5)
+    if what == "backwards":       # rows 5 .. 3
+        skip, starts = (0,), [5, 3]
+    elif what == "behind":        # the last one's rows end behind the tensors
+        skip, starts = (2,), [0, 2, 2, c.tokens + 1]
+    elif what == "all_behind":    # they lie behind the tensors altogether
+        skip, starts = (2,), [0, 2, c.tokens, c.tokens + 3]
+        c.batch[1] = (c.tokens - 2, 30)
+    else:                         # more keys than a row of the table holds, with and without new tokens
+        skip, starts = (2 if what == "length" else 1,), [0, 2, 2, 5]
+        c.c_lengths[skip[0]] = c.table.shape[1] * c.page + 1
+    c.c_starts = dev.t(starts, np.uint32)
+    k, v = c.k.clone(), c.v.clone()
+    s = append(dev, c, 2, 64, "bf16")
+    dev.torch.cuda.synchronize()
+    assert dev.status() == capi.TL_FLAG_INDEX_RANGE
+    check_append(dev, c, s, k, v, skip=skip)
