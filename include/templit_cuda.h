@@ -804,11 +804,12 @@ typedef struct tl_cache_append_desc {
 /*
  * The new tokens' keys, normed and turned by their positions as in
  * tl_rotary_heads, and their values into the cache, rounded once to its type;
- * their queries alike into q_out, in one launch.  A token whose position would
- * be negative (more new tokens than keys) or behind the table, or whose page
- * id is out of range, is not written and raises TL_FLAG_INDEX_RANGE.  Two
- * tokens must not share a place in the cache.  Rows of fp16 go into a bf16 cache
- * and the reverse; q_out is of the cache's type there (TL_ERR_UNSUPPORTED).
+ * their queries alike into q_out, in one launch (two where q_out's type is not
+ * the cache's).  A token whose position is behind the table, or whose page id
+ * is out of range, is not written and raises TL_FLAG_INDEX_RANGE; nor is any of
+ * a sequence with more new tokens than keys.  Two tokens must not share a place
+ * in the cache.  Rows of fp16 go into a bf16 cache and the reverse; q_out is of
+ * the cache's type there (else TL_ERR_UNSUPPORTED).
  */
 int tl_cache_append(const tl_cache_append_desc *desc, void *stream);
 
@@ -826,7 +827,8 @@ typedef struct tl_paged_attention_desc {
   uint32_t max_new;     /* no sequence has more new tokens; 0: `tokens`.  Both
                            only choose how the work is split: a longer chunk
                            gives the same result, a longer sequence is cut
-                           and raises TL_FLAG_INDEX_RANGE                 */
+                           (the keys behind it are not there; positions
+                           stay) and raises TL_FLAG_INDEX_RANGE           */
   uint32_t reserved;
   float *lse;           /* [tokens, q_heads], optional: ln sum_j e^(s_j)  */
   void *workspace;      /* tl_paged_attention_workspace_size() bytes      */
@@ -837,7 +839,10 @@ typedef struct tl_paged_attention_desc {
  * the cache.  fp32 caches: fp32 products.  16-bit caches: products of 16-bit
  * numbers summed in fp32, the softmax in fp32, its numerators rounded to the
  * cache's type for the second product.  A row that sees no key (or only
- * scores of -inf) is 0 with lse -inf.  What lies in slots behind a sequence's
+ * scores of -inf) is 0 with lse -inf.  Of a sequence with more new tokens than
+ * keys the first have negative positions and, causal, see none; the others see
+ * the keys that its length gives it, although tl_cache_append writes none of
+ * them (and raises the flag).  What lies in slots behind a sequence's
  * length, and keys and values that a row does not see, do not reach it, NaN
  * and infinities included.
  * D a multiple of 8, at most 128; rows 16-byte aligned (pointers and strides),
