@@ -37,6 +37,8 @@ int check_cache(const char *who, tl_paged_cache &c, bool *aligned) {
     if (!c.starts || !c.lengths) return fail(TL_ERR_INVALID, w + "null starts or lengths");
     if (c.table_stride && !c.table) return fail(TL_ERR_INVALID, w + "null table");
     if (c.pages && (!c.k || !c.v)) return fail(TL_ERR_INVALID, w + "null cache");
+    if ((reinterpret_cast<uintptr_t>(c.starts) | reinterpret_cast<uintptr_t>(c.lengths) | reinterpret_cast<uintptr_t>(c.table)) % 4)
+      return fail(TL_ERR_INVALID, w + "starts, lengths or table not aligned");
     if (reinterpret_cast<uintptr_t>(c.k) % e || reinterpret_cast<uintptr_t>(c.v) % e)
       return fail(TL_ERR_INVALID, w + "the cache is not aligned to its type");
   }
@@ -218,6 +220,8 @@ extern "C" int tl_cache_append(const tl_cache_append_desc *d, void *stream) {
   if (!c.tokens || !c.sequences) return TL_OK;
   if (int rc = heads::check_view(who, "k", d->k, d->type, 1, c.tokens, c.heads, c.D, false)) return rc;
   if (int rc = heads::check_view(who, "v", d->v, d->type, 1, c.tokens, c.heads, c.D, false)) return rc;
+  if ((reinterpret_cast<uintptr_t>(d->q_weight) | reinterpret_cast<uintptr_t>(d->k_weight)) % 4)
+    return fail(TL_ERR_INVALID, w + "a weight is not aligned");
   bool q_aligned = true;
   if (d->q_heads) {
     if (int rc = heads::check_view(who, "q", d->q, d->type, 1, c.tokens, d->q_heads, c.D, false)) return rc;

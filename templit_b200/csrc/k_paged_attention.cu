@@ -32,6 +32,7 @@ int attention_args(const char *who, const tl_paged_attention_desc *d, AttentionA
   if (d->out.p == d->q.p) return fail(TL_ERR_INVALID, w + "out is q");
   if (!aligned || !heads::aligned_view(d->q, c.type, false, 8) || !heads::aligned_view(d->out, d->out_type, false, 8))
     return fail(TL_ERR_UNSUPPORTED, w + "rows are not 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(d->lse) % 4) return fail(TL_ERR_INVALID, w + "lse not aligned");
   a.q = d->q;
   a.out = d->out;
   a.q_heads = d->q_heads;

@@ -163,6 +163,7 @@ int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryA
     return rc;
   const uint64_t tokens = static_cast<uint64_t>(d->B) * d->T;
   if (tokens >> 32) return fail(TL_ERR_RANGE, w + "more than 2^32 - 1 tokens");
+  if (reinterpret_cast<uintptr_t>(d->positions) % 4) return fail(TL_ERR_INVALID, w + "positions not aligned");
   if (!d->q.heads && !d->k.heads) return fail(TL_ERR_INVALID, w + "no heads");
   a.D = d->D;
   a.T = d->T;
@@ -184,6 +185,8 @@ int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryA
     RotaryPart &r = a.part[i];
     r.heads = p.heads;
     if (!p.heads) continue;
+    if ((reinterpret_cast<uintptr_t>(p.weight) | reinterpret_cast<uintptr_t>(p.dweight)) % 4)
+      return fail(TL_ERR_INVALID, w + "weight or dweight not aligned");
     const auto view = [&](const char *name, const tl_head_view &v, int32_t type, bool written) {
       aligned = aligned && aligned_view(v, type, d->B > 1, V);
       return check_view(who, name, v, type, d->B, d->T, p.heads, d->D, written);

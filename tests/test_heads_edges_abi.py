@@ -1,0 +1,30 @@
+"""More refusals of the rotation, cache and paged attention entry points,
+without a GPU: what would fault there, or write a place twice."""
+import pytest
+
+from templit_b200 import capi
+from tests.test_heads_abi import BAD, NOT, RANGE, SOME, append, attend, refused, rotary, view  # noqa: F401
+
+WORK = dict(workspace=SOME, workspace_bytes=1 << 30)
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+@pytest.mark.parametrize("name,make,fields,word", [
+    ("tl_rotary_heads", rotary, dict(positions=SOME), b"positions"),
+    ("tl_rotary_heads", rotary, dict(norm=1, q__weight=SOME), b"weight"),
+    ("tl_rotary_heads_backward", rotary, dict(positions=SOME), b"positions"),
+    ("tl_rotary_heads_backward", rotary, dict(norm=1, k__weight=SOME), b"weight"),
+    ("tl_rotary_heads_backward", rotary, dict(norm=1, q__dweight=SOME, **WORK), b"dweight"),
+    ("tl_cache_append", append, dict(norm=1, q_weight=SOME), b"weight"),
+    ("tl_cache_append", append, dict(norm=1, k_weight=SOME), b"weight"),
+    ("tl_cache_append", append, dict(cache__table=SOME), b"table"),
+    ("tl_cache_append", append, dict(cache__starts=SOME), b"starts"),
+    ("tl_cache_append", append, dict(cache__lengths=SOME), b"lengths"),
+    ("tl_paged_attention", attend, dict(cache__table=SOME), b"table"),
+    ("tl_paged_attention", attend, dict(cache__starts=SOME), b"starts"),
+    ("tl_paged_attention", attend, dict(cache__lengths=SOME), b"lengths"),
+    ("tl_paged_attention", attend, dict(lse=SOME), b"lse"),
+])
+def test_pointers_to_words_are_aligned(name, make, fields, word, off):
+    *rest, last = [f for f in fields if f not in ("norm", *WORK)]
+    refused(name, make(**{**fields, last: SOME + off}), BAD, word)
