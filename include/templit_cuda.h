@@ -727,7 +727,8 @@ typedef struct tl_rotary_part {
   tl_head_view d_out;  /* backward: gradient of out, `out_type`           */
   tl_head_view dx;     /* backward: gradient of x, `type`; may be d_out   */
   const float *weight; /* [D], optional: the norm's weights               */
-  float *dweight;      /* [D], optional, backward: their gradient (set)   */
+  float *dweight;      /* [D], optional, backward: their gradient (set; q
+                          and k that share weights add theirs up after)   */
 } tl_rotary_part;
 typedef struct tl_rotary_desc {
   uint32_t B, T, D;    /* D <= TL_HEAD_MAX_DIM                            */

@@ -212,6 +212,10 @@ int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryA
     r.weight = p.weight;
     r.dweight = backward ? p.dweight : nullptr;
   }
+  if (a.part[0].dweight && a.part[1].dweight) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.part[0].dweight), y = reinterpret_cast<uintptr_t>(a.part[1].dweight);
+    if ((x < y ? y - x : x - y) < d->D * sizeof(float)) return fail(TL_ERR_INVALID, w + "q and k share a dweight, which each sets");
+  }
   const Shape shape = shape_for(d->D, d->rotary_dim, V, aligned);
   a.lanes = shape.lanes;
   a.vectors = shape.vectors;

@@ -28,3 +28,9 @@ WORK = dict(workspace=SOME, workspace_bytes=1 << 30)
 def test_pointers_to_words_are_aligned(name, make, fields, word, off):
     *rest, last = [f for f in fields if f not in ("norm", *WORK)]
     refused(name, make(**{**fields, last: SOME + off}), BAD, word)
+
+
+@pytest.mark.parametrize("apart", [0, 4, -252])
+def test_weight_gradients_are_apart(apart):
+    """Queries' and keys' are each set, not added to."""
+    refused("tl_rotary_heads_backward", rotary(norm=1, q__dweight=SOME, k__dweight=SOME + apart, **WORK), BAD, b"dweight")
