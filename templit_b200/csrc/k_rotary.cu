@@ -164,6 +164,8 @@ int rotary_args(const char *who, const tl_rotary_desc *d, bool backward, RotaryA
   const uint64_t tokens = static_cast<uint64_t>(d->B) * d->T;
   if (tokens >> 32) return fail(TL_ERR_RANGE, w + "more than 2^32 - 1 tokens");
   if (reinterpret_cast<uintptr_t>(d->positions) % 4) return fail(TL_ERR_INVALID, w + "positions not aligned");
+  if (!d->positions && d->T && d->first_position > UINT32_MAX - (d->T - 1))
+    return fail(TL_ERR_RANGE, w + "positions behind 2^32 - 1");
   if (!d->q.heads && !d->k.heads) return fail(TL_ERR_INVALID, w + "no heads");
   a.D = d->D;
   a.T = d->T;

@@ -34,3 +34,9 @@ def test_pointers_to_words_are_aligned(name, make, fields, word, off):
 def test_weight_gradients_are_apart(apart):
     """Queries' and keys' are each set, not added to."""
     refused("tl_rotary_heads_backward", rotary(norm=1, q__dweight=SOME, k__dweight=SOME + apart, **WORK), BAD, b"dweight")
+
+
+@pytest.mark.parametrize("name", ["tl_rotary_heads", "tl_rotary_heads_backward"])
+@pytest.mark.parametrize("first,T", [((1 << 32) - 1, 2), ((1 << 32) - 2, 3), (1 << 31, (1 << 31) + 1)])
+def test_positions_stay_in_32_bits(name, first, T):
+    refused(name, rotary(first_position=first, T=T, B=1), RANGE, b"positions")
