@@ -22,7 +22,7 @@ int attention_args(const char *who, const tl_paged_attention_desc *d, AttentionA
   if (d->out_type != c.type && d->out_type != TL_FLOAT32) return fail(TL_ERR_INVALID, w + "out_type is the cache's or fp32");
   if (d->causal != 0 && d->causal != 1) return fail(TL_ERR_INVALID, w + "causal is 0 or 1");
   if (d->window && !d->causal) return fail(TL_ERR_INVALID, w + "a window needs causal");
-  if (!std::isfinite(d->scale)) return fail(TL_ERR_INVALID, w + "scale is finite");
+  if (!std::isfinite(d->scale * kLog2e)) return fail(TL_ERR_INVALID, w + "scale / ln 2 is finite");
   if (static_cast<uint64_t>(c.tokens) * d->q_heads >> 32) return fail(TL_ERR_RANGE, w + "more than 2^32 - 1 query rows");
   *nothing = !c.tokens || !c.sequences;
   if (*nothing) return TL_OK;

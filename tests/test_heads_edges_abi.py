@@ -40,3 +40,8 @@ def test_weight_gradients_are_apart(apart):
 @pytest.mark.parametrize("first,T", [((1 << 32) - 1, 2), ((1 << 32) - 2, 3), (1 << 31, (1 << 31) + 1)])
 def test_positions_stay_in_32_bits(name, first, T):
     refused(name, rotary(first_position=first, T=T, B=1), RANGE, b"positions")
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -2.4e38, 3.4e38])
+def test_scales_that_powers_of_two_cannot_hold(scale):
+    refused("tl_paged_attention", attend(scale=scale), BAD, b"scale")
