@@ -378,7 +378,8 @@ inline bool aligned_view(const tl_head_view &v, int32_t type, bool batches, uint
 int check_turn(const char *who, uint32_t D, uint32_t rotary_dim, int32_t layout, int32_t norm, float eps,
                float magnitude, const uint64_t *frequencies);
 // A view of [batches, rows, heads, D] of `type`: pointer, alignment, extent;
-// one that is written has no two rows in one place.
+// no stride of one that is written is 0 or below D (whether larger ones meet is not
+// worked out: a caller's).
 int check_view(const char *who, const char *name, const tl_head_view &v, int32_t type, uint64_t batches,
                uint64_t rows, uint64_t heads, uint32_t D, bool written);
 // In place or apart: one pointer means one layout and one type.

@@ -159,6 +159,32 @@ def test_cut_sequences_keep_their_positions(dev, type, new, keys, cut, window):
         assert (np.abs(lse[i][~none] - wlse[~none]) <= (ds + longs + 2 * U * np.abs(wlse))[~none]).all(), i
 
 
+# --------------------------------------------------------- fp32 products
+
+@pytest.mark.parametrize("D", [64, 128, 40])
+@pytest.mark.parametrize("batch", [[(1, 1), (3, 3), (1, 16)], [(40, 200), (1, 900)]])
+@pytest.mark.parametrize("sharp", [1.0, 20.0])
+def test_fp32_attention_in_fp32(dev, D, batch, sharp):
+    """fp32 caches by fp32 products alone: a score is four lanes' four sums of D / 16 products, added up in four
+    steps, so within S = (D / 16 + 4) u scale sum |q k| of itself, with each row's own sum; log2(e), the maximum and
+    their difference round it by 4 u |s|, an exponential by 2^-22 of itself, numerators and sum alike.  The sums over
+    keys and the warps' and parts' joins are chains of at most L / 32 + 24 roundings."""
+    c = Cache(dev, batch, 2, D, 16, "f32")
+    s = attend(dev, c, 4, sharp=sharp)
+    out, lse, q = (s[n].double().cpu().numpy() for n in ("out", "lse", "q"))
+    steps = (64 if D <= 64 else 128) / 16 + 4
+    for i, (new, keys) in enumerate(batch):
+        at = slice(int(c.starts[i]), int(c.starts[i]) + new)
+        want, wlse, size = ops.attention(q[at], c.keys[i], c.vals[i], s["d"].scale)
+        for r in range(new):
+            k = c.keys[i][:keys - new + r + 1].repeat(2, 1)
+            products = s["d"].scale * np.einsum("hd,lhd->hl", np.abs(q[at][r]), np.abs(k)).max(-1)
+            ds, longs = (steps + 4) * U * products, 2.0 ** -22 + (keys / 32 + 24) * U
+            err = size[r] * 2 * (ds + longs)[:, None] + 2 * U * np.abs(want[r])
+            assert (np.abs(out[at][r] - want[r]) <= err).all(), (i, r)
+            assert (np.abs(lse[at][r] - wlse[r]) <= ds + longs + 2 * U * np.abs(wlse[r])).all(), (i, r)
+
+
 # --------------------------------------------------------------------- writer
 
 @pytest.mark.parametrize("type,cache_type", [("f16", "bf16"), ("bf16", "f16")])
