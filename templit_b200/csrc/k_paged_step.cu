@@ -37,12 +37,6 @@ template <typename T, int DP> constexpr size_t smem_bytes() {
          (sizeof(T) == 4 ? (kRows * DP + kWarps * kRows * 8) * sizeof(float) : 0);
 }
 
-__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ void load_matrices(uint32_t at, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -463,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 2) step_kernel(const AttentionArgs a
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e)
           if (lane + 32 * e < c.D) heads::set_element(out[lane + 32 * e], ll == 0.0f ? 0.0f : acc[e] / ll);
-        if (lane == 0) put_lse<TO>(a, token, h, mm, ll);
+        if (lane == 0) put_lse(a, token, h, mm, ll);
       } else {
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) part[row * DP + lane + 32 * e] = acc[e];

@@ -86,12 +86,6 @@ template <int DP> constexpr size_t smem_bytes() {
   return 1024 + 2 * tile_bytes<DP>() + stages<DP>() * static_cast<size_t>(tile_bytes<DP>()) + kStaging + sizeof(Shared);
 }
 
-__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Waits for a phase; false where it gave up, here or elsewhere in the CTA.  The
 // first look is inline, a few instructions; the rest is not.
 __device__ __noinline__ bool wait_longer(Shared &sh, uint64_t *bar, uint32_t parity, uint32_t *status) {
@@ -178,23 +172,10 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uin
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Two fp32 in a register pair: one issued instruction for both.
-typedef unsigned long long Pair;
-__device__ __forceinline__ Pair pair(uint32_t lo, uint32_t hi) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(lo), "r"(hi));
-  return p;
-}
-__device__ __forceinline__ float2 halves(Pair p) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-  return f;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
+using heads::fma2;
+using heads::halves;
+using heads::Pair;
+__device__ __forceinline__ Pair pair(uint32_t lo, uint32_t hi) { return heads::pair(__uint_as_float(lo), __uint_as_float(hi)); }
 __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   Pair d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -705,7 +686,7 @@ __device__ __forceinline__ void soften(const AttentionArgs &a, Shared &sh, uint8
       if (lane == 0) ptx::mbar_arrive(&sh.b.o_free[t]);
     }
     if (there) {
-      if (complete) put_lse<TO>(a, token, h, m, l);
+      if (complete) put_lse(a, token, h, m, l);
       else {
         part[kRows * DP + in_job] = m;
         part[kRows * DP + kRows + in_job] = l;
@@ -758,7 +739,7 @@ template <typename T, typename TO, int DP> __device__ __forceinline__ void mend_
         else part[row * DP + lane + 32 * e] = acc[e];
       }
       if (lane == 0) {
-        if (complete) put_lse<TO>(a, token, h, m, l);
+        if (complete) put_lse(a, token, h, m, l);
         else {
           part[kRows * DP + row] = m;
           part[kRows * DP + kRows + row] = l;

@@ -11,6 +11,13 @@ constexpr uint32_t kMaxHead = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// 16 bytes into shared memory, zeros where they are not there
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void await() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // A job that is cut over several CTAs, written by the one that ends it: its
 // first CTA (none: UINT32_MAX) and which rows it is.
 struct Join {
@@ -296,7 +303,6 @@ template <uint32_t ROWS, uint32_t KEYS> struct Walk {
 };
 
 // One row's result: the whole of it, or a part in the workspace.
-template <typename TO>
 __device__ __forceinline__ void put_lse(const AttentionArgs &a, uint64_t token, uint32_t h, float m, float l) {
   if (a.lse) a.lse[token * a.q_heads + h] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
 }
@@ -399,7 +405,7 @@ __global__ void __launch_bounds__(128) join_kernel(const AttentionArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (lane * E + e < a.cache.D) heads::set_element(out[lane * E + e], ll[r] == 0.0f ? 0.0f : acc[r][e] / ll[r]);
-    if (lane == 0) put_lse<TO>(a, token, h, mm[r], ll[r]);
+    if (lane == 0) put_lse(a, token, h, mm[r], ll[r]);
   }
 }
 
