@@ -383,6 +383,13 @@ __device__ __forceinline__ void load(const AttentionArgs &a, const Maps &maps, S
       page = next_page;
       slot = next_slot;
     }
+    if (n == 0) {
+      // A piece without keys: the last copies before it go on here, as they do with a
+      // piece's first keys.  Kept back over several such pieces, they would hold up the
+      // piece that waits for them, and with it the next one's place in the jobs' ring.
+      await<0>();
+      hand_over(item);
+    }
     __syncwarp();
     if (lane == 0) release_job(sh, i_job);
   }

@@ -132,6 +132,18 @@ def test_norm_gradient_without_eps(dev, type, heads, D, offset, T):
         assert (np.abs(dw.double().cpu().numpy() - dweight) <= total * (2 * NORM + (n / 32 + 64) * U)).all()
 
 
+# ------------------------------------------------- sequences without any keys
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("page,D", [(5, 64), (16, 128)])
+@pytest.mark.parametrize("empty", [(1, 0), (3, 0), (20, 1)])
+def test_runs_of_sequences_without_keys(dev, type, page, D, empty):
+    """Tiles without keys, eight in a row and more than four a CTA, behind one with a last block that is not whole."""
+    batch = ([(2, 134), (1, 60)] + [empty] * 4) * 70
+    c = Cache(dev, batch, 2, D, page, type)
+    check(dev, c, attend(dev, c, 66, max_new=20))
+
+
 # ------------------------------------------------------ sequences that are cut
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
