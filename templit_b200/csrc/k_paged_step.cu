@@ -13,7 +13,9 @@
 //
 // 8 key heads of 128 bf16, 4 query heads each: one token over 200003 keys 135 us
 // (819 MB, 6.1 TB/s); 64 sequences of 16 to 8191 keys 92 us (5.0 TB/s), where a CTA's
-// jobs' starts and ends, between which its loads pause, are what is left.
+// jobs' starts and ends, between which its loads pause, are what is left.  Chunks in fp32 read
+// a sequence's keys once for 16 rows: 64 sequences of 192 tokens, 6 heads of 64: 433 us; one
+// prompt of 2048: 508 us (6.4 TFLOP/s).
 #include "paged_attention.cuh"
 
 namespace tl {

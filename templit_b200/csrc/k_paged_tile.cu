@@ -23,23 +23,25 @@
 //                   kind::f16, fp32 in TMEM)
 //   warp 13         one thread works out the CTA's pieces of jobs, ahead of the others
 //   warps 14, 15    nothing (without them the compiler gives a thread 144 registers in
-//                   place of 128, and the prompt below took 556 us in place of 546)
+//                   place of 128, and the prompt below took 556 us in place of 546, both in the first calls)
 // TMEM: 2 x 2 buffers of 64 columns of scores, 2 x 128 of outputs.  With two buffers a
 // tile, the next scores are multiplied while the last ones are in the softmax; one of 128
-// leaves each waiting for the other (710 us where this takes 580), although scores of 64
+// leaves each waiting for the other (710 us where this took 580), although scores of 64
 // keys take 48 cycles of a product of 32 (of 128 keys 64).  Every wait is bounded
 // (2 s); where one gives up, the CTA raises TL_FLAG_TIMEOUT, waits for what it issued
 // and returns.  Shares of the keys and their joining: paged_attention.cuh.
 //
-// 8192 tokens of one prompt, 8 key heads of 128 bf16, 4 query heads each, causal: 546 to
-// 580 us, 1000 TFLOP/s of the 1650 of a large library product; the tensor cores and the unit
-// for 2^x are half busy each.  Both tiles' softmax warps share the
-// schedulers, two a scheduler: 2700 cycles for 2 x 128 x 128 scores, of which
-// the exponentials alone are 2048; the products are 2560, and hand-overs come between.  A polynomial for some of the
-// exponentials gained nothing: the instructions that are issued then bound it.  A job's
-// end, 256 rows out of TMEM, is 8500 cycles more.  24 chunks of up to 509 tokens, 3 query
-// heads of 64 a key head, behind up to 4093 keys: 80 us; jobs are short there, their ends
-// and ragged first and last tiles are half of it.
+// 8192 tokens of one prompt, 8 key heads of 128 bf16, 4 query heads each, causal: 538 us in
+// the first calls, at 1965 MHz; 608 to 620 (900 to 915 TFLOP/s of the 1372 of a large library
+// product that is as long under way) repeated, where the power limit leaves 1710 MHz.  980000
+// cycles of the tile kernel are 225 blocks of 2 x 128 x 128 scores an SM and 7 jobs' ends
+// of 8500 (256 rows out of TMEM): 4100 cycles a block, of which the exponentials take the
+// unit for 2^x 2048 and the products the tensor cores 2200, half each.  Both tiles' softmax
+// warps share the schedulers, two a scheduler, and hand-overs come between.  A polynomial
+// for some of the exponentials gained nothing: the instructions that are issued then
+// bound it.  24 chunks of up to 509 tokens, 3 query heads of 64 a key head, behind up to
+// 4093 keys: 80 us; jobs are short there, their ends and ragged first and last tiles are
+// half of it.
 #include "paged_attention.cuh"
 #include "tc_ptx.cuh"
 

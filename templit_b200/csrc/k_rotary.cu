@@ -11,7 +11,7 @@
 //
 // 12288 x 12 heads of 64 fp32, rotation alone: 17 us (75 MB, 4.5 TB/s).  16384 x 40 heads of
 // 128 bf16, norm and rotation: 68 us (336 MB, 4.9 TB/s), where the instructions of an element
-// (issue 58 %) and loads share the time; 64 tokens of it 7 us, a launch.
+// (issue 61 %) and loads (memory 54 %) share the time; 64 tokens of it 7 us, a launch.
 #include "rotary.cuh"
 
 #include <cmath>

@@ -8,9 +8,10 @@
 // then in shared memory, and leaves one row, which a second kernel sums over
 // the CTAs in a fixed order.
 //
-// 16384 x 40 heads of 128 bf16: 117 us (503 MB, 4.3 TB/s); the registers of the norm's sums
-// leave 12 warps an SM, whose instructions (issue 46 to 58 %) and loads share the time.  The
-// rotation alone, a quarter of each head turned, 16384 x 40 heads: 62 us.
+// 16384 x 40 heads of 128 bf16: 118 us (503 MB, 4.25 TB/s); the registers of the norm's sums
+// leave 12 warps an SM, too few to cover what each waits for: a warp issues every 5.8 cycles,
+// of which 1.6 are its own operands, 1.0 loads and 0.6 shuffles, so that issue (48 %) and
+// memory (50 %) are half busy each; the sum of the CTAs' rows is 7 us more.  The rotation alone, a quarter of each head turned, 16384 x 40 heads: 62 us.
 #include "rotary.cuh"
 
 namespace tl {
