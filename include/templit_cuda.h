@@ -843,7 +843,8 @@ typedef struct tl_paged_attention_desc {
  * scores of -inf) is 0 with lse -inf.  Of a sequence with more new tokens than
  * keys the first have negative positions and, causal, see none; the others see
  * the keys that its length gives it, although tl_cache_append writes none of
- * them (and raises the flag).  What lies in slots behind a sequence's
+ * them (and raises the flag).  A key that is seen with a score of -inf has no
+ * weight (where its value is not finite, the row is NaN or without it).  What lies in slots behind a sequence's
  * length, and keys and values that a row does not see, do not reach it, NaN
  * and infinities included.
  * D a multiple of 8, at most 128; rows 16-byte aligned (pointers and strides),
