@@ -144,6 +144,110 @@ def test_runs_of_sequences_without_keys(dev, type, page, D, empty):
     check(dev, c, attend(dev, c, 66, max_new=20))
 
 
+# ------------------------------------------- captured, far apart, very many
+
+def captured(dev, call):
+    """`call(stream)` captured into a graph; replay() launches it and waits."""
+    t = dev.torch
+    side, graph = t.cuda.Stream(), ctypes.c_void_p()
+    stream = ctypes.c_void_p(side.cuda_stream)
+    t.cuda.synchronize()
+    capi.check(dev.lib.tl_graph_capture_begin(stream), dev.lib)
+    call(stream)
+    capi.check(dev.lib.tl_graph_capture_end(stream, ctypes.byref(graph)), dev.lib)
+
+    def replay():
+        t.cuda.synchronize()
+        capi.check(dev.lib.tl_graph_launch(graph, stream), dev.lib)
+        t.cuda.synchronize()
+
+    return replay, lambda: capi.check(dev.lib.tl_graph_destroy(graph), dev.lib)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+def test_a_captured_chunk_follows_values_that_are_not_finite(dev, type):
+    """A replayed call sees a later token's infinite value come and go, and lengths that shrink."""
+    c = Cache(dev, [(70, 600), (40, 300)], 2, 64, 16, type)
+    s = attend(dev, c, 6, prepare_only=True)
+    replay, close = captured(dev, lambda st: capi.check(dev.lib.tl_paged_attention(ctypes.byref(s["d"]), st), dev.lib))
+    page, slot = c.places(0, 590, 591)
+    good, kept = c.v[page, slot].clone(), c.vals[0][590].copy()
+    full = c.batch, c.keys, c.vals
+    for bad, keys in ((None, (600, 300)), (float("inf"), (600, 300)), (None, (600, 300)), (float("nan"), (595, 40)), (None, (70, 41))):
+        c.v[page, slot] = good if bad is None else bad
+        full[2][0][590] = kept if bad is None else bad
+        c.c_lengths.copy_(dev.torch.tensor(keys).to(dev.torch.int32).view(c.c_lengths.dtype))
+        c.batch = [(70, keys[0]), (40, keys[1])]
+        c.keys, c.vals = ([x[i][:n] for i, n in enumerate(keys)] for x in full[1:])
+        replay()
+        check(dev, c, s)
+    close()
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_a_captured_append_follows_the_lengths(dev, type):
+    c = Cache(dev, [(3, 3), (1, 2), (20, 20)], 2, 64, 16, type)
+    k, v = c.k.clone(), c.v.clone()
+    s = append(dev, c, 4, 64, type, norm=True)  # once outside, for the oracle's numbers
+    replay, close = captured(dev, lambda st: capi.check(dev.lib.tl_cache_append(ctypes.byref(s["d"]), st), dev.lib))
+    for lengths in ((3, 2, 20), (9, 7, 31), (16, 1, 32)):
+        c.k.copy_(k)
+        c.v.copy_(v)
+        s["q_out"].fill_(GUARD)
+        c.c_lengths.copy_(dev.torch.tensor(lengths).to(dev.torch.int32).view(c.c_lengths.dtype))
+        c.batch = [(n, length) for (n, _), length in zip(c.batch, lengths)]
+        replay()
+        check_append(dev, c, s, k, v)
+        assert dev.status() == 0
+    close()
+
+
+@pytest.mark.parametrize("type,new", [("bf16", 2), ("bf16", 30), ("f32", 2)])
+def test_queries_and_outputs_behind_32_bits(dev, type, new):
+    """Rows of queries and outputs farther apart than 2^32 elements in all."""
+    t = dev.torch
+    c = Cache(dev, [(new, 90)], 1, 64, 16, type)
+    stride = ((1 << 32) // new + 64) // 64 * 64
+    rows = [t.empty(stride * (new - 1) + 128, dtype=torch_type(dev, type), device=dev.dev).as_strided((new, 2, 64), (stride, 64, 1))
+            for _ in range(2)]
+    rows[0].copy_(t.from_numpy(c.rng.standard_normal((new, 2, 64))))
+    rows[1].fill_(GUARD)
+    s = attend(dev, c, 2, q=rows[0], prepare_only=True)
+    s["out"] = rows[1]
+    s["d"].out = capi.TlHeadView(rows[1].data_ptr(), 0, 64, stride)
+    capi.check(dev.lib.tl_paged_attention(ctypes.byref(s["d"]), dev.stream), dev.lib)
+    check(dev, c, s)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("max_new", [0, 2])
+def test_a_hundred_thousand_sequences(dev, type, max_new):
+    """One page each, most with one new token: the whole batch against the same sums by torch in 64 bits."""
+    t, n, D = dev.torch, 100003, 8
+    c = Cache(dev, [(1, 1)], 1, D, 4, type)
+    rng = np.random.default_rng(8)
+    new = rng.choice([0, 1, 1, 1, 2], n)
+    keys = new + rng.integers(0, 3, n)
+    c.k, c.v = (t.from_numpy(rng.standard_normal((n, 4, 1, D))).to(dev.dev).to(torch_type(dev, type)) for _ in range(2))
+    c.pages, c.table, starts = n, rng.permutation(n)[:, None].astype(np.uint32), np.concatenate(([0], np.cumsum(new)))
+    c.tokens, c.batch = int(starts[-1]), [(1, 1)] * n
+    c.c_table, c.c_starts, c.c_lengths = (dev.t(x, np.uint32) for x in (c.table, starts, keys))
+    s = attend(dev, c, 9, max_new=max_new)
+    of = np.repeat(np.arange(n), new)
+    position = keys[of] - new[of] + np.arange(c.tokens) - starts[of]
+    at = t.from_numpy(c.table[of, 0].astype(np.int64)).to(dev.dev)
+    k, v, q = c.k[at, :, 0].double(), c.v[at, :, 0].double(), s["q"].double()
+    x = t.einsum("thd,tsd->ths", q, k) * s["d"].scale
+    x = x.masked_fill((t.arange(4)[None] > t.from_numpy(position)[:, None]).to(dev.dev)[:, None], -math.inf)
+    p, size = x.softmax(-1), t.einsum("ths,tsd->thd", x.softmax(-1), v.abs())
+    products = s["d"].scale * t.einsum("thd,tsd->ths", q.abs(), k.abs()).amax(-1)
+    rel = 2 * products * (D * U + 3 * U) + 2.0 ** -20 + 64 * U + (0 if type == "f32" else ROUND[type])
+    want = t.einsum("ths,tsd->thd", p, v)
+    assert ((s["out"].double() - want).abs() <= size * rel[..., None] + want.abs() * ROUND[type] + TINY[type]).all()
+    assert ((s["lse"].double() - x.logsumexp(-1)).abs() <= rel + 2 * U * x.abs().nan_to_num(posinf=0).amax(-1)).all()
+    assert dev.status() == 0
+
+
 # ------------------------------------------------------ sequences that are cut
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
