@@ -824,7 +824,8 @@ typedef struct tl_paged_attention_desc {
   int32_t causal;       /* 1: a token sees no key behind its position     */
   uint32_t window;      /* > 0: only the last `window` keys up to its position */
   float scale;          /* finite, / ln 2 too; 1 / sqrt(D) as a rule      */
-  uint32_t max_length;  /* no sequence has more keys; 0: what the table holds */
+  uint32_t max_length;  /* no sequence has more keys; 0: what the table holds
+                           (above 2^26, chunks take a slower kernel)      */
   uint32_t max_new;     /* no sequence has more new tokens; 0: `tokens`.  Both
                            only choose how the work is split: a longer chunk
                            gives the same result, a longer sequence is cut

@@ -53,8 +53,11 @@ int attention_args(const char *who, const tl_paged_attention_desc *d, AttentionA
 // and 708, 256 rows 586 and 4933.  (One sequence of them: 20 rows 44 us and 36.)
 // One choice for the whole call: of 64 sequences of 16 to 8191 keys with one token and 4
 // query heads a key head each, 91 us in the other kernel, 122 here where max_new is not given.
+// The tiles' waits end after 2 s, and a job is waited for as a whole: 2^26 keys take 1.1 s
+// there (2.1 us for 128), so that sequences which may be longer stay with the other kernel,
+// whose warps wait for nothing but their own copies.
 bool tiled(const tl_paged_attention_desc *d, const AttentionArgs &a, uint32_t max_new) {
-  return a.cache.type != TL_FLOAT32 && d->scale > 0.0f && static_cast<uint64_t>(max_new) * a.group > 16;
+  return a.cache.type != TL_FLOAT32 && d->scale > 0.0f && static_cast<uint64_t>(max_new) * a.group > 16 && a.most <= 1u << 26;
 }
 
 uint32_t most_new(const tl_paged_attention_desc *d) {

@@ -1,5 +1,7 @@
 """More refusals of the rotation, cache and paged attention entry points,
 without a GPU: what would fault there, or write a place twice."""
+import ctypes
+
 import pytest
 
 from templit_b200 import capi
@@ -45,3 +47,15 @@ def test_positions_stay_in_32_bits(name, first, T):
 @pytest.mark.parametrize("scale", [2.4e38, -2.4e38, 3.4e38])
 def test_scales_that_powers_of_two_cannot_hold(scale):
     refused("tl_paged_attention", attend(scale=scale), BAD, b"scale")
+
+
+def test_very_long_sequences_are_not_waited_for():
+    """Chunks of sequences that may have more than 2^26 keys go to the kernel without timed waits: its workspace."""
+    lib = capi.cuda_lib()
+    size = lambda **f: lib.tl_paged_attention_workspace_size(ctypes.byref(attend(  # noqa: E731
+        cache__type=capi.TL_BFLOAT16, out_type=capi.TL_BFLOAT16, cache__tokens=64, cache__page_size=1 << 20, **f)))
+    tiles, steps = size(cache__table_stride=64), size(cache__table_stride=64, max_new=1)
+    assert tiles != steps
+    assert size(cache__table_stride=65) == steps
+    assert size(cache__table_stride=65, max_length=1 << 26) == tiles
+    assert size(cache__table_stride=65, max_length=(1 << 26) + 1) == steps

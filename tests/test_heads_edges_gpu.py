@@ -248,6 +248,15 @@ def test_a_hundred_thousand_sequences(dev, type, max_new):
     assert dev.status() == 0
 
 
+@pytest.mark.parametrize("width", [64, 65, 300])
+def test_chunks_with_room_for_very_long_sequences(dev, width):
+    """Pages of 2^20 slots and tables for 2^26 keys and more."""
+    c = Cache(dev, [(70, 300), (2, 40)], 1, 8, 1 << 20, "bf16", spare=0)
+    c.table = np.concatenate([c.table[:, :1], np.full((2, width - 1), 0xffffffff, np.uint32)], 1)
+    c.c_table = dev.t(c.table, np.uint32)
+    check(dev, c, attend(dev, c, 4))
+
+
 # ------------------------------------------------------ sequences that are cut
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
