@@ -32,7 +32,7 @@
 // and returns.  Shares of the keys and their joining: paged_attention.cuh.
 //
 // 8192 tokens of one prompt, 8 key heads of 128 bf16, 4 query heads each, causal: 538 us in
-// the first calls, at 1965 MHz; 608 to 620 (900 to 915 TFLOP/s of the 1372 of a large library
+// the first calls, at 1965 MHz; 604 to 620 (897 to 920 TFLOP/s of the 1372 of a large library
 // product that is as long under way) repeated, where the power limit leaves 1710 MHz.  980000
 // cycles of the tile kernel are 225 blocks of 2 x 128 x 128 scores an SM and 7 jobs' ends
 // of 8500 (256 rows out of TMEM): 4100 cycles a block, of which the exponentials take the
